@@ -906,6 +906,102 @@ typedef struct uzu_side_attention_args {
 } uzu_side_attention_args;
 UZU_API void uzu_side_attention_encode(uzu_command_buffer* cmd, const uzu_side_attention_args* args);
 
+/* ---- State space mixer and routed experts of a few tokens (extensions) -------------------------------------------------------------------------
+ * What a hybrid model's layer runs between its projections. All four entries take rows that may be slices of wider ones (strides in elements), read and
+ * write nothing of rows that belong to no sequence, accumulate in f32 and record UZU_ERROR_INVALID_ARGUMENT (the same that the _validate call returns,
+ * which needs no device) for arguments they do not take. Buffers of one call do not overlap but for what is said to be updated in place.
+ *
+ * Rows [first_row, first_row + rows) of a pass are one sequence, in token order; `slot` names its state. Sequences of one call have rows and slots of
+ * their own (checked). fresh != 0: it starts from a state of zeros, whatever the slot holds. rows = 0: a fresh slot is zeroed, any other kept. */
+typedef struct uzu_row_sequence { uint32_t first_row, rows, slot, fresh; } uzu_row_sequence;
+
+/* Short causal convolution per channel over packed sequences, for prompts and for single rows:
+ *   output[t, c] = act(bias[c] + sum_j weights[c, j] * u[t - taps + 1 + j, c])
+ * where u are the sequence's rows behind the taps - 1 inputs that its slot holds, oldest first; the slot takes the last taps - 1 inputs. One rounding, of
+ * the output. Channels, strides and pointers of whole 16-byte groups take vector loads, others single ones. */
+typedef struct uzu_causal_conv_args {
+    uint64_t input, output;        /* data_type [rows, channels] */
+    uint64_t weights, bias;        /* f32 [channels, taps], optional f32 [channels] */
+    uint64_t state;                /* data_type [slots, taps - 1, channels], updated in place (0 with taps = 1) */
+    const uzu_row_sequence* sequences;   /* HOST pointer, copied into the launch */
+    uint32_t sequence_count, rows, slots, channels, taps /* 1 .. 8 */, input_stride, output_stride;
+    uint32_t activation;           /* UZU_ACT_SILU | UZU_ACT_IDENTITY */
+    uint32_t data_type;            /* UZU_DT_BF16 | UZU_DT_F32 | UZU_DT_F16 */
+    uint32_t reserved0;
+} uzu_causal_conv_args;
+UZU_API void uzu_causal_conv_encode(uzu_command_buffer* cmd, const uzu_causal_conv_args* args);
+UZU_API uzu_status uzu_causal_conv_validate(const uzu_causal_conv_args* args);
+
+/* Selective state space scan over packed sequences: one decay per head and token, head h reads group h / (heads / groups) of b and c. With
+ *   step = dt + dt_bias[h];  dt_softplus: step <- softplus(step);  step <- min(max(step, dt_min), dt_max)
+ *   S_t = exp(step a[h]) S_(t-1) + step x_t b_t^T   (per head [head_dim, state_size]);   y_t = S_t c_t + d[h] x_t;   out = y * silu(z)  (z optional)
+ * The state f32 [slots, heads, head_dim, state_size] is read and written back per sequence. a is negative in a model (decays below 1); nothing checks it.
+ * dt_min >= 0.
+ * scratch: of uzu_state_space_scan_scratch_bytes() bytes, 16-byte aligned, content free before and after; with none (0), or less, long sequences are not
+ * cut into parts, which costs time only. Calls that may run at the same time do not share it. */
+typedef struct uzu_state_space_scan_args {
+    uint64_t x, dt, b, c, z;       /* data_type [rows, heads * head_dim], [rows, heads], [rows, groups * state_size] twice, optional [rows, heads * head_dim] */
+    uint64_t a, d, dt_bias;        /* f32 [heads]; d and dt_bias optional */
+    uint64_t state, out;           /* f32 in place; data_type [rows, heads * head_dim] */
+    uint64_t scratch, scratch_bytes;
+    const uzu_row_sequence* sequences;   /* HOST pointer, copied into the launch */
+    uint32_t sequence_count, rows, slots, heads, groups, head_dim /* 1 .. 256 */, state_size /* 1 .. 256 */;
+    uint32_t x_stride, dt_stride, b_stride, c_stride, z_stride, out_stride;
+    float dt_min, dt_max;
+    uint32_t dt_softplus, data_type;
+    uint32_t reserved0;
+} uzu_state_space_scan_args;
+UZU_API void uzu_state_space_scan_encode(uzu_command_buffer* cmd, const uzu_state_space_scan_args* args);
+UZU_API uzu_status uzu_state_space_scan_validate(const uzu_state_space_scan_args* args);
+UZU_API size_t uzu_state_space_scan_scratch_bytes(uzu_context* ctx, const uzu_state_space_scan_args* args);
+
+/* One token of `rows` running sequences through the mixer between its projections, in one launch: the convolution (silu or identity) of xbc = [x: heads *
+ * head_dim | b: groups * state_size | c: groups * state_size], the scan of one token and the gate, as the two entries above but with nothing rounded
+ * between them. Row r uses state and conv_state slot slots[r] (r without a list); a slot number that is not below slot_count leaves the row out (a padded
+ * batch: its output is kept too), and so does one that an earlier row of the call names. The list is read on the device: a captured call follows it.
+ * tickets: u32 [rows * groups], zero before the first use and again after every call; calls that may run at the same time do not share them. */
+typedef struct uzu_state_space_step_args {
+    uint64_t xbc, dt, z;           /* data_type rows; z optional */
+    uint64_t conv_weights, conv_bias;    /* f32 [channels, taps], optional f32 [channels] */
+    uint64_t conv_state;           /* data_type [slot_count, taps - 1, channels], in place (0 with taps = 1) */
+    uint64_t a, d, dt_bias;        /* f32 [heads]; d and dt_bias optional */
+    uint64_t state, out;           /* f32 [slot_count, heads, head_dim, state_size] in place; data_type [rows, heads * head_dim] */
+    uint64_t slots, tickets;       /* optional u32 [rows] (DEVICE); u32 [rows * groups] */
+    uint32_t rows, slot_count, heads, groups, head_dim /* 1 .. 256 */, state_size /* 1 .. 256 */, taps /* 1 .. 8 */;
+    uint32_t xbc_stride, dt_stride, z_stride, out_stride;
+    float dt_min, dt_max;
+    uint32_t dt_softplus, activation, data_type;
+} uzu_state_space_step_args;
+UZU_API void uzu_state_space_step_encode(uzu_command_buffer* cmd, const uzu_state_space_step_args* args);
+UZU_API uzu_status uzu_state_space_step_validate(const uzu_state_space_step_args* args);
+
+/* A whole layer of routed experts for 1 .. 64 tokens in one launch: router, choice, the chosen experts' gated units, the shared experts, the weighted sum.
+ *   logits = x router^T + router_bias.  score 0: the `top` largest logits, weights = softmax over them; 1: s = softmax over all logits, the `top` largest s,
+ *   weights = s; 2: s = sigmoid(logits), the `top` largest s, weights = s.  renormalise: weights / their sum;  weights * weight_scale. The lower index wins
+ *   a tie; a logit that is NaN comes last.
+ *   out[t] = sum_k weights[t, k] E_(ids[t, k])(x_t) + sum over shared experts E(x_t),   E(x) = down (act(gate) * up),  [up | gate] = up_gate x
+ * x and out are bf16 or f32 rows, the weights bf16. f32 rows and hidden values enter the products as two bf16 parts, of bf16 rows the hidden values as one;
+ * products and sums are f32, summed in an order that only the shapes and the choice set. width and ff are multiples of 8, weights 16-byte aligned.
+ * scratch: of uzu_expert_layer_scratch_bytes() bytes, 256-byte aligned, its first 16 KB zero before the first use; every call leaves it ready for the next,
+ * of any sizes. Calls that may run at the same time do not share it. */
+typedef enum uzu_expert_score { UZU_EXPERT_SCORE_CHOSEN = 0, UZU_EXPERT_SCORE_ALL = 1, UZU_EXPERT_SCORE_SIGMOID = 2 } uzu_expert_score;
+typedef struct uzu_expert_layer_args {
+    uint64_t x, out;               /* data_type [rows, width] */
+    uint64_t router, router_bias;  /* bf16 [experts, width], optional f32 [experts] */
+    uint64_t up_gate, down;        /* bf16 [experts + shared, 2 * ff, width] (ff up rows, then ff gate rows), [experts + shared, width, ff] */
+    uint64_t ids, weights;         /* optional results: u32 [rows, top], f32 [rows, top] */
+    uint64_t scratch, scratch_bytes;
+    uint32_t rows, width, ff, experts /* 1 .. 512 */, top /* 1 .. 16 */, shared /* 0 .. 16 */, x_stride, out_stride;
+    uint32_t score, renormalise;
+    float weight_scale;
+    uint32_t activation;           /* uzu_activation_type, of the gate */
+    uint32_t data_type;            /* UZU_DT_BF16 | UZU_DT_F32 */
+    uint32_t reserved0;
+} uzu_expert_layer_args;
+UZU_API void uzu_expert_layer_encode(uzu_command_buffer* cmd, const uzu_expert_layer_args* args);
+UZU_API uzu_status uzu_expert_layer_validate(const uzu_expert_layer_args* args);
+UZU_API size_t uzu_expert_layer_scratch_bytes(const uzu_expert_layer_args* args);
+
 /* ---- Host engine (C++ mirror of the reference's backend-agnostic Rust host code) ---------- *
  * No Rust toolchain exists in the build image, so the layer above the kernels -- Engine /
  * LanguageModel / LanguageModelStream / Decoder / Transformer / TransformerLayer (engine/mod.rs:15-43,

@@ -48,6 +48,9 @@ pub const UZU_ACTIVATION_TRANSFORM_INPUT_RHT: u32 = 0;
 pub const UZU_ACTIVATION_TRANSFORM_OUTPUT_RHT: u32 = 1;
 pub const UZU_ACTIVATION_TRANSFORM_QUANTIZE: u32 = 2;
 pub const UZU_ACTIVATION_TRANSFORM_QUANTIZE_WITH_GROUP_SUMS: u32 = 3;
+pub const UZU_EXPERT_SCORE_CHOSEN: u32 = 0;
+pub const UZU_EXPERT_SCORE_ALL: u32 = 1;
+pub const UZU_EXPERT_SCORE_SIGMOID: u32 = 2;
 pub const UZU_SAMPLING_GREEDY: u32 = 0;
 pub const UZU_SAMPLING_STOCHASTIC: u32 = 1;
 
@@ -948,6 +951,135 @@ pub struct uzu_side_attention_args {
     pub norm: uzu_head_norm_gate_args,
 }
 
+/// 16 bytes
+#[repr(C)] #[derive(Default, Clone, Copy)]
+pub struct uzu_row_sequence {
+    pub first_row: u32,
+    pub rows: u32,
+    pub slot: u32,
+    pub fresh: u32,
+}
+
+/// 88 bytes
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct uzu_causal_conv_args {
+    pub input: u64,
+    pub output: u64,
+    pub weights: u64,
+    pub bias: u64,
+    pub state: u64,
+    pub sequences: *const uzu_row_sequence,
+    pub sequence_count: u32,
+    pub rows: u32,
+    pub slots: u32,
+    pub channels: u32,
+    pub taps: u32,
+    pub input_stride: u32,
+    pub output_stride: u32,
+    pub activation: u32,
+    pub data_type: u32,
+    pub reserved0: u32,
+}
+
+/// 176 bytes
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct uzu_state_space_scan_args {
+    pub x: u64,
+    pub dt: u64,
+    pub b: u64,
+    pub c: u64,
+    pub z: u64,
+    pub a: u64,
+    pub d: u64,
+    pub dt_bias: u64,
+    pub state: u64,
+    pub out: u64,
+    pub scratch: u64,
+    pub scratch_bytes: u64,
+    pub sequences: *const uzu_row_sequence,
+    pub sequence_count: u32,
+    pub rows: u32,
+    pub slots: u32,
+    pub heads: u32,
+    pub groups: u32,
+    pub head_dim: u32,
+    pub state_size: u32,
+    pub x_stride: u32,
+    pub dt_stride: u32,
+    pub b_stride: u32,
+    pub c_stride: u32,
+    pub z_stride: u32,
+    pub out_stride: u32,
+    pub dt_min: f32,
+    pub dt_max: f32,
+    pub dt_softplus: u32,
+    pub data_type: u32,
+    pub reserved0: u32,
+}
+
+/// 168 bytes
+#[repr(C)] #[derive(Default, Clone, Copy)]
+pub struct uzu_state_space_step_args {
+    pub xbc: u64,
+    pub dt: u64,
+    pub z: u64,
+    pub conv_weights: u64,
+    pub conv_bias: u64,
+    pub conv_state: u64,
+    pub a: u64,
+    pub d: u64,
+    pub dt_bias: u64,
+    pub state: u64,
+    pub out: u64,
+    pub slots: u64,
+    pub tickets: u64,
+    pub rows: u32,
+    pub slot_count: u32,
+    pub heads: u32,
+    pub groups: u32,
+    pub head_dim: u32,
+    pub state_size: u32,
+    pub taps: u32,
+    pub xbc_stride: u32,
+    pub dt_stride: u32,
+    pub z_stride: u32,
+    pub out_stride: u32,
+    pub dt_min: f32,
+    pub dt_max: f32,
+    pub dt_softplus: u32,
+    pub activation: u32,
+    pub data_type: u32,
+}
+
+/// 136 bytes
+#[repr(C)] #[derive(Default, Clone, Copy)]
+pub struct uzu_expert_layer_args {
+    pub x: u64,
+    pub out: u64,
+    pub router: u64,
+    pub router_bias: u64,
+    pub up_gate: u64,
+    pub down: u64,
+    pub ids: u64,
+    pub weights: u64,
+    pub scratch: u64,
+    pub scratch_bytes: u64,
+    pub rows: u32,
+    pub width: u32,
+    pub ff: u32,
+    pub experts: u32,
+    pub top: u32,
+    pub shared: u32,
+    pub x_stride: u32,
+    pub out_stride: u32,
+    pub score: u32,
+    pub renormalise: u32,
+    pub weight_scale: f32,
+    pub activation: u32,
+    pub data_type: u32,
+    pub reserved0: u32,
+}
+
 /// 56 bytes
 #[repr(C)] #[derive(Default, Clone, Copy)]
 pub struct uzu_engine_options {
@@ -1041,6 +1173,11 @@ pub const STRUCT_SIZES: &[(&str, usize)] = &[
     ("uzu_window_attention_args", std::mem::size_of::<uzu_window_attention_args>()),
     ("uzu_side_step_args", std::mem::size_of::<uzu_side_step_args>()),
     ("uzu_side_attention_args", std::mem::size_of::<uzu_side_attention_args>()),
+    ("uzu_row_sequence", std::mem::size_of::<uzu_row_sequence>()),
+    ("uzu_causal_conv_args", std::mem::size_of::<uzu_causal_conv_args>()),
+    ("uzu_state_space_scan_args", std::mem::size_of::<uzu_state_space_scan_args>()),
+    ("uzu_state_space_step_args", std::mem::size_of::<uzu_state_space_step_args>()),
+    ("uzu_expert_layer_args", std::mem::size_of::<uzu_expert_layer_args>()),
     ("uzu_engine_options", std::mem::size_of::<uzu_engine_options>()),
     ("uzu_sampling_method", std::mem::size_of::<uzu_sampling_method>()),
     ("uzu_model_info", std::mem::size_of::<uzu_model_info>()),
@@ -1168,6 +1305,16 @@ extern "C" {
     pub fn uzu_window_attention_encode(cmd: *mut uzu_command_buffer, args: *const uzu_window_attention_args);
     pub fn uzu_side_step_encode(cmd: *mut uzu_command_buffer, args: *const uzu_side_step_args);
     pub fn uzu_side_attention_encode(cmd: *mut uzu_command_buffer, args: *const uzu_side_attention_args);
+    pub fn uzu_causal_conv_encode(cmd: *mut uzu_command_buffer, args: *const uzu_causal_conv_args);
+    pub fn uzu_causal_conv_validate(args: *const uzu_causal_conv_args) -> c_int;
+    pub fn uzu_state_space_scan_encode(cmd: *mut uzu_command_buffer, args: *const uzu_state_space_scan_args);
+    pub fn uzu_state_space_scan_validate(args: *const uzu_state_space_scan_args) -> c_int;
+    pub fn uzu_state_space_scan_scratch_bytes(ctx: *mut uzu_context, args: *const uzu_state_space_scan_args) -> usize;
+    pub fn uzu_state_space_step_encode(cmd: *mut uzu_command_buffer, args: *const uzu_state_space_step_args);
+    pub fn uzu_state_space_step_validate(args: *const uzu_state_space_step_args) -> c_int;
+    pub fn uzu_expert_layer_encode(cmd: *mut uzu_command_buffer, args: *const uzu_expert_layer_args);
+    pub fn uzu_expert_layer_validate(args: *const uzu_expert_layer_args) -> c_int;
+    pub fn uzu_expert_layer_scratch_bytes(args: *const uzu_expert_layer_args) -> usize;
     pub fn uzu_engine_create(ctx: *mut uzu_context, model_dir: *const c_char, opts: *const uzu_engine_options, out: *mut *mut uzu_engine) -> c_int;
     pub fn uzu_engine_destroy(e: *mut uzu_engine);
     pub fn uzu_engine_info(e: *const uzu_engine, out: *mut uzu_model_info) -> c_int;

@@ -1,0 +1,289 @@
+"""The state space mixer's entries against their definitions in float64: packed prompts, single tokens, a run of them together."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from tests import state_space_plain as P
+from uzu_b200 import binding as B
+
+pytestmark = pytest.mark.gpu
+
+SENTINEL = 0x5A      # bytes of what a call leaves alone
+
+
+def _np(dt):
+    return {P.BF16: np.uint16, P.F32: np.float32, P.F16: np.float16}[dt]
+
+
+class _Rows:
+    """rows of `width` elements, `stride` apart, `shift` elements into a buffer of their own"""
+
+    def __init__(self, ctx, values, dt, stride=0, shift=0):
+        rows, width = values.shape
+        self.stride, self.shift, self.width, self.rows, self.dt = stride or width, shift, width, rows, dt
+        flat = np.frombuffer(bytes([SENTINEL]) * ((rows * self.stride + shift + 8) * np.dtype(_np(dt)).itemsize), _np(dt)).copy()
+        self.view(flat)[:, :width] = P.to_kept(values, dt)
+        self.buf = ctx.upload(flat)
+        self.ptr = self.buf.ptr + shift * flat.itemsize
+        self.n = flat.size
+
+    def view(self, flat):
+        return flat[self.shift:self.shift + self.rows * self.stride].reshape(self.rows, self.stride)
+
+    def raw(self):
+        return self.view(self.buf.numpy(_np(self.dt), (self.n,)))
+
+    def get(self):
+        """float64 values, and whether everything beside the rows is as it was"""
+        raw = self.raw()
+        return P.of_kept(raw[:, :self.width], self.dt), raw
+
+
+def _kept(values, dt):
+    return P.of_kept(P.to_kept(values, dt), dt)
+
+
+def _table(seqs):
+    return (B.RowSequence * max(1, len(seqs)))(*[B.RowSequence(*s) for s in seqs])
+
+
+def _check(got, ref, bound, dt, what):
+    """within a rounding of the reference and `bound`"""
+    assert np.isfinite(got).all(), what
+    tol = P.HALF_STEP[dt] * (np.abs(ref) + bound) + P.TINY[dt] + bound
+    worst = (np.abs(got - ref) / tol).max(initial=0)
+    assert worst <= 1, (what, float(worst))
+
+
+# ---- convolution ----------------------------------------------------------------------------------------------------------------------------------
+def _conv(ctx, dt, channels, taps, seqs, rows, slots, act=True, stride=0, shift=0, bias=True, seed=0):
+    rng = np.random.default_rng(seed)
+    u, w = rng.standard_normal((rows, channels)), rng.standard_normal((channels, taps)).astype(np.float32)
+    b = rng.standard_normal(channels).astype(np.float32) if bias else np.zeros(channels, np.float32)
+    st = rng.standard_normal((slots, max(taps - 1, 1), channels))
+    covered = np.zeros(rows, bool)
+    for f, n, _, _ in seqs:
+        covered[f:f + n] = True
+    u[~covered] = np.nan                     # rows of no sequence are not read into any
+    x = _Rows(ctx, u, dt, stride, shift)
+    out = _Rows(ctx, np.zeros((rows, channels)), dt, stride, shift)
+    before = out.raw().copy()
+    sb = ctx.upload(P.to_kept(st, dt))
+    wb, bb = ctx.upload(w), ctx.upload(b)
+    t = _table(seqs)
+    a = B.CausalConvArgs(input=x.ptr, output=out.ptr, weights=wb.ptr, bias=bb.ptr if bias else 0, state=sb.ptr if taps > 1 else 0, sequences=C.addressof(t), sequence_count=len(seqs), rows=rows,
+                         slots=slots, channels=channels, taps=taps, input_stride=x.stride, output_stride=out.stride, activation=B.ACT_SILU if act else B.ACT_IDENTITY, data_type=dt)
+    with ctx.command_buffer("conv") as cmd:
+        cmd.encode("uzu_causal_conv_encode", C.byref(a))
+    ref, state, mag = P.conv(_kept(u, dt), w.astype(np.float64), b.astype(np.float64), _kept(st, dt)[:, :taps - 1], seqs, act)
+    got, raw = out.get()
+    # taps + 1 additions in 32 bits; the gate: an exponential of a value of up to `mag` and a division, its slope below 1.1
+    bound = 1.1 * (taps + 2) * 2.0 ** -24 * mag + (2.0 ** -21 + 2.0 ** -22 * mag) * np.abs(np.nan_to_num(ref))
+    _check(got[covered], ref[covered], bound[covered], dt, "out")
+    assert np.array_equal(raw[~covered], before[~covered]) and np.array_equal(raw[:, channels:], before[:, channels:])
+    if taps > 1:
+        assert np.array_equal(sb.numpy(_np(dt), (slots, taps - 1, channels)), P.to_kept(state, dt))
+
+
+RAGGED = [(0, 9, 3, 0), (9, 1, 0, 1), (10, 0, 1, 0), (10, 130, 4, 0), (140, 2, 2, 0), (142, 3, 5, 1), (146, 70, 6, 0), (220, 0, 7, 1)]
+
+
+@pytest.mark.parametrize("dt", [P.BF16, P.F32, P.F16])
+@pytest.mark.parametrize("taps", [1, 2, 3, 4, 5, 8])
+def test_conv_ragged(ctx, dt, taps):
+    _conv(ctx, dt, 72, taps, RAGGED, 223, 9)
+
+
+@pytest.mark.parametrize("channels,stride,shift", [(8, 0, 0), (1, 0, 0), (63, 0, 0), (64, 72, 8), (64, 65, 0), (64, 0, 1), (1032, 0, 0)])
+@pytest.mark.parametrize("act", [True, False])
+def test_conv_layouts(ctx, channels, stride, shift, act):
+    _conv(ctx, P.BF16, channels, 4, [(0, 40, 1, 0), (40, 7, 0, 1)], 48, 2, act, stride, shift, bias=act)
+
+
+def test_conv_many_sequences(ctx):
+    """more than one launch takes"""
+    seqs = [(3 * i, 1 + i % 3, i, i % 2) for i in range(300)]
+    _conv(ctx, P.BF16, 16, 4, seqs, 900, 300)
+
+
+def test_conv_empty(ctx):
+    _conv(ctx, P.BF16, 16, 4, [], 5, 1)
+
+
+def test_conv_long(ctx):
+    _conv(ctx, P.BF16, 2048, 4, [(0, 3001, 0, 0), (3001, 1096, 1, 0)], 4097, 2)
+
+
+# ---- scan ------------------------------------------------------------------------------------------------------------------------------------------
+def _scan_inputs(rng, rows, heads, groups, dim, n, dt):
+    x, z = rng.standard_normal((rows, heads * dim)), rng.standard_normal((rows, heads * dim))
+    b, c = rng.standard_normal((rows, groups * n)), rng.standard_normal((rows, groups * n))
+    d = rng.standard_normal((rows, heads))
+    a = -(1 + 15 * rng.random(heads)).astype(np.float32)
+    skip = (1 + 0.2 * rng.standard_normal(heads)).astype(np.float32)
+    size = np.exp(np.log(1e-3) + rng.random(heads) * np.log(100.0))
+    bias = (size + np.log(-np.expm1(-size))).astype(np.float32)
+    return x, z, b, c, d, a, skip, bias
+
+
+def _scan(ctx, dt, heads, groups, dim, n, seqs, rows, slots, gate=True, pad=0, seed=0, softplus=True, lo=0.0, hi=float("inf"), scratch=True, chunks=False, skip_d=True, scale_dt=1.0):
+    rng = np.random.default_rng(seed)
+    x, z, b, c, d, a, skip, bias = _scan_inputs(rng, rows, heads, groups, dim, n, dt)
+    d = d * scale_dt
+    if not softplus:
+        d, bias = np.abs(d) * 0.05, np.zeros_like(bias)
+    covered = np.zeros(rows, bool)
+    for f, m, _, _ in seqs:
+        covered[f:f + m] = True
+    for v in (x, z, b, c, d):
+        v[~covered] = np.nan
+    st = rng.standard_normal((slots, heads, dim, n)).astype(np.float32)
+    bufs = [_Rows(ctx, v, dt, v.shape[1] + pad if pad else 0) for v in (x, z, b, c, d)]
+    xb, zb, bb, cb, db = bufs
+    out = _Rows(ctx, np.zeros((rows, heads * dim)), dt, heads * dim + pad if pad else 0)
+    before = out.raw().copy()
+    f32 = [ctx.upload(v) for v in (a, skip, bias, st)]
+    t = _table(seqs)
+    args = B.StateSpaceScanArgs(x=xb.ptr, dt=db.ptr, b=bb.ptr, c=cb.ptr, z=zb.ptr if gate else 0, a=f32[0].ptr, d=f32[1].ptr if skip_d else 0, dt_bias=f32[2].ptr if softplus else 0,
+                                state=f32[3].ptr, out=out.ptr, sequences=C.addressof(t), sequence_count=len(seqs), rows=rows, slots=slots, heads=heads, groups=groups, head_dim=dim, state_size=n,
+                                x_stride=xb.stride, dt_stride=db.stride, b_stride=bb.stride, c_stride=cb.stride, z_stride=zb.stride, out_stride=out.stride, dt_min=lo, dt_max=hi,
+                                dt_softplus=int(softplus), data_type=dt)
+    if scratch:
+        args.scratch_bytes = ctx.lib.uzu_state_space_scan_scratch_bytes(ctx.h, C.byref(args))
+        sc = ctx.buffer(max(16, args.scratch_bytes), B.BUFFER_DEVICE)
+        args.scratch = sc.ptr
+    with ctx.command_buffer("scan") as cmd:
+        cmd.encode("uzu_state_space_scan_encode", C.byref(args))
+    k = lambda v, *s: np.nan_to_num(_kept(v, dt)).reshape(rows, *s)
+    a64, s64 = a.astype(np.float64), (skip if skip_d else 0 * skip).astype(np.float64)
+    step = P.steps(k(d, heads), bias.astype(np.float64), softplus, lo, hi)
+    ref, state, mag, smag = P.scan(k(x, heads, dim), step, k(b, groups, n), k(c, groups, n), k(z, heads, dim) if gate else None, a64, s64, st.astype(np.float64), seqs)
+    got, raw = out.get()
+    longest = max([m for _, m, _, _ in seqs], default=0)
+    # in 32 bits: two roundings a token of the state, a decay that is off by 3 steps of its own and |step a| of the step's four, n + 2 of a read-out
+    unit = 2.0 ** -24 * (longest * (5 + 4 * float(np.abs(step * a64).max(initial=0))) + n + 8)
+    # in chunks: scores and the state that is read out rounded to bf16, decayed inputs to two of them
+    y_unit, s_unit = (unit + 2.0 ** -8, unit + 2.0 ** -16) if chunks else (unit, unit)
+    bound = y_unit * mag
+    if gate:
+        zz = k(z, heads, dim)
+        bound = bound * np.abs(P.silu(zz)) + (2.0 ** -21 + 2.0 ** -22 * np.abs(zz)) * np.abs(np.nan_to_num(ref))
+    cov = covered
+    _check(got.reshape(rows, heads, dim)[cov], ref[cov], bound[cov], dt, "out")
+    assert np.array_equal(raw[~cov], before[~cov]) and np.array_equal(raw[:, heads * dim:], before[:, heads * dim:])
+    _check(f32[3].numpy(np.float32, st.shape).astype(np.float64), state, s_unit * smag, P.F32, "state")
+    named = {s for _, _, s, _ in seqs}
+    for s in range(slots):
+        if s not in named:
+            assert np.array_equal(f32[3].numpy(np.float32, st.shape)[s], st[s])
+
+
+@pytest.mark.parametrize("dt", [P.BF16, P.F32, P.F16])
+@pytest.mark.parametrize("heads,groups,dim,n", [(4, 2, 16, 16), (2, 1, 33, 7), (3, 3, 1, 1), (2, 1, 40, 65), (2, 2, 70, 130), (1, 1, 256, 256)])
+def test_scan_shapes(ctx, dt, heads, groups, dim, n):
+    _scan(ctx, dt, heads, groups, dim, n, RAGGED, 223, 9)
+
+
+@pytest.mark.parametrize("over", [dict(gate=False), dict(pad=3), dict(softplus=False), dict(lo=0.01, hi=0.02), dict(skip_d=False), dict(scratch=False), dict(scale_dt=30.0)])
+def test_scan_forms(ctx, over):
+    _scan(ctx, P.F32, 4, 1, 32, 32, RAGGED, 223, 9, **over)
+
+
+def test_scan_many_sequences(ctx):
+    _scan(ctx, P.F32, 2, 1, 8, 8, [(3 * i, 1 + i % 3, i, i % 2) for i in range(300)], 900, 300)
+
+
+def test_scan_empty(ctx):
+    _scan(ctx, P.F32, 2, 1, 8, 8, [], 4, 1)
+
+
+# ---- one token ------------------------------------------------------------------------------------------------------------------------------------
+def _step_case(ctx, dt, heads, groups, dim, n, taps, slots, slot_count, gate=True, act=True, seed=0, calls=1, pad=0, graph=False):
+    rng = np.random.default_rng(seed)
+    rows, inner, ch = len(slots), heads * dim, heads * dim + 2 * groups * n
+    order = list(range(rows)) if slots is None else slots
+    w, cbias = rng.standard_normal((ch, taps)).astype(np.float32), rng.standard_normal(ch).astype(np.float32)
+    conv0, st0 = rng.standard_normal((slot_count, max(1, taps - 1), ch)), rng.standard_normal((slot_count, heads, dim, n)).astype(np.float32)
+    a = -(1 + 15 * rng.random(heads)).astype(np.float32)
+    skip, bias = rng.standard_normal(heads).astype(np.float32), (rng.standard_normal(heads) - 3).astype(np.float32)
+    conv_b, st_b, tick = ctx.upload(P.to_kept(conv0, dt)), ctx.upload(st0), ctx.upload(np.zeros(rows * groups, np.uint32))
+    f32 = [ctx.upload(v) for v in (w, cbias, a, skip, bias)]
+    sl = ctx.upload(np.array(slots, np.uint32))
+    conv, st = _kept(conv0, dt)[:, :taps - 1], st0.astype(np.float64)
+    seen, live = set(), []
+    for r, s in enumerate(slots):
+        if s < slot_count and s not in seen:
+            seen.add(s)
+            live.append(r)
+    smag = np.abs(st)
+    for call in range(calls):
+        xbc, z, d = rng.standard_normal((rows, ch)), rng.standard_normal((rows, inner)), rng.standard_normal((rows, heads))
+        X, Z, Dt = (_Rows(ctx, v, dt, v.shape[1] + pad if pad else 0) for v in (xbc, z, d))
+        out = _Rows(ctx, np.zeros((rows, inner)), dt, inner + pad if pad else 0)
+        before = out.raw().copy()
+        args = B.StateSpaceStepArgs(xbc=X.ptr, dt=Dt.ptr, z=Z.ptr if gate else 0, conv_weights=f32[0].ptr, conv_bias=f32[1].ptr, conv_state=conv_b.ptr if taps > 1 else 0, a=f32[2].ptr, d=f32[3].ptr,
+                                    dt_bias=f32[4].ptr, state=st_b.ptr, out=out.ptr, slots=sl.ptr, tickets=tick.ptr, rows=rows, slot_count=slot_count, heads=heads, groups=groups, head_dim=dim,
+                                    state_size=n, taps=taps, xbc_stride=X.stride, dt_stride=Dt.stride, z_stride=Z.stride, out_stride=out.stride, dt_min=0.0, dt_max=float("inf"), dt_softplus=1,
+                                    activation=B.ACT_SILU if act else B.ACT_IDENTITY, data_type=dt)
+        with ctx.command_buffer("step") as cmd:
+            cmd.encode("uzu_state_space_step_encode", C.byref(args))
+        assert cmd.launches == 1
+        got, raw = out.get()
+        xk, zk, dk = (_kept(v, dt) for v in (xbc, z, d))
+        for r in live:
+            s = slots[r]
+            seq = [(0, 1, 0, 0)]
+            v, cs, mag = P.conv(xk[r:r + 1], w.astype(np.float64), cbias.astype(np.float64), conv[s:s + 1], seq, act)
+            conv[s] = cs[0]
+            off = 1.1 * (taps + 2) * 2.0 ** -24 * mag[0] + (2.0 ** -21 + 2.0 ** -22 * mag[0]) * np.abs(v[0])      # of the convolution
+            x, b, c = v[0, :inner].reshape(1, heads, dim), v[0, inner:inner + groups * n].reshape(1, groups, n), v[0, inner + groups * n:].reshape(1, groups, n)
+            step = P.steps(dk[r:r + 1], bias.astype(np.float64))
+            prev = smag[s].copy()
+            y, s1, ymag, _ = P.scan(x, step, b, c, zk[r:r + 1].reshape(1, heads, dim) if gate else None, a.astype(np.float64), skip.astype(np.float64), st[s:s + 1], seq)
+            ox, ob, oc = off[:inner].reshape(heads, dim), np.repeat(off[inner:inner + groups * n].reshape(groups, n), heads // groups, 0), np.repeat(off[inner + groups * n:].reshape(groups, n), heads // groups, 0)
+            bb, cc = np.repeat(np.abs(b[0]), heads // groups, 0), np.repeat(np.abs(c[0]), heads // groups, 0)
+            add = step[0][:, None, None] * (ox[:, :, None] * (bb + ob)[:, None, :] + np.abs(x[0])[:, :, None] * ob[:, None, :])
+            unit = 2.0 ** -24 * (8 + 8 * float(np.abs(step * a).max()))
+            f = np.exp(step[0] * a)[:, None, None]
+            mags = f * prev + np.abs(step[0][:, None, None] * x[0][:, :, None] * bb[:, None, :])
+            s_bound = (unit * (call + 1) * mags + add * 1.01) + (call > 0) * 0.0
+            err = np.abs(st_b.numpy(np.float32, st0.shape)[s].astype(np.float64) - s1[0])
+            assert (err <= s_bound + (0 if call == 0 else carried[s] * f) + 2.0 ** -24 * np.abs(s1[0])).all(), ("state", r, call)
+            carried = {} if call == 0 and r == live[0] else carried
+            carried[s] = s_bound + (0 if call == 0 else carried[s] * f) + 2.0 ** -24 * np.abs(s1[0])
+            y_bound = (carried[s] * cc[:, None, :] + (np.abs(s1[0]) + carried[s]) * oc[:, None, :]).sum(-1) + (n + 4) * 2.0 ** -24 * (ymag[0] + 1e-30) + np.abs(skip)[:, None] * ox
+            ref = y[0]
+            if gate:
+                zz = zk[r].reshape(heads, dim)
+                y_bound = y_bound * np.abs(P.silu(zz)) + (2.0 ** -21 + 2.0 ** -22 * np.abs(zz)) * np.abs(ref)
+            _check(got[r].reshape(heads, dim), ref, y_bound, dt, ("out", r, call))
+            st[s], smag[s] = s1[0], mags
+        left = [r for r in range(rows) if r not in live]
+        assert np.array_equal(raw[left], before[left]) and np.array_equal(raw[:, inner:], before[:, inner:])
+        if taps > 1:
+            assert np.array_equal(conv_b.numpy(_np(dt), (slot_count, taps - 1, ch)), P.to_kept(conv, dt))
+        assert not tick.numpy(np.uint32, (rows * groups,)).any()
+        for s in range(slot_count):
+            if s not in seen:
+                assert np.array_equal(st_b.numpy(np.float32, st0.shape)[s], st0[s])
+
+
+@pytest.mark.parametrize("dt", [P.BF16, P.F32, P.F16])
+@pytest.mark.parametrize("heads,groups,dim,n", [(4, 2, 64, 128), (2, 1, 33, 7), (3, 3, 1, 1), (2, 1, 128, 64), (2, 2, 70, 130), (8, 1, 256, 256), (4, 4, 16, 20), (2, 1, 65, 40)])
+def test_step_shapes(ctx, dt, heads, groups, dim, n):
+    _step_case(ctx, dt, heads, groups, dim, n, 4, [2, 0, 5], 6)
+
+
+@pytest.mark.parametrize("taps", [1, 2, 3, 5, 8])
+def test_step_taps(ctx, taps):
+    _step_case(ctx, P.BF16, 4, 1, 32, 16, taps, [1, 0], 3, act=taps != 2, gate=taps != 3, calls=3)
+
+
+def test_step_rows_left_out(ctx):
+    """padded rows, and rows that name a slot again"""
+    _step_case(ctx, P.BF16, 4, 2, 64, 64, 4, [3, 0xFFFFFFFF, 1, 3, 7, 1, 0], 7, calls=2, pad=5)
+
+
+def test_step_many_rows(ctx):
+    _step_case(ctx, P.BF16, 2, 1, 8, 8, 4, list(np.random.default_rng(1).permutation(400)[:391]), 400)

@@ -17,7 +17,7 @@ LIB_PATH = Path(os.environ.get("UZU_B200_LIB") or Path(__file__).resolve().paren
 u32, u64, f32 = C.c_uint32, C.c_uint64, C.c_float
 
 # enums (include/uzu_b200.h)
-DT_BF16, DT_F32 = 0, 1
+DT_BF16, DT_F32, DT_F16 = 0, 1, 2
 QMODE_U4, QMODE_I8, QMODE_U8 = 0, 1, 2
 QMETHOD_SCALE_BIAS, QMETHOD_SCALE_ZERO_POINT, QMETHOD_SCALE_SYMMETRIC = 0, 1, 2
 B_FULL_PRECISION, B_SCALE_BIAS, B_SCALE_ZERO_POINT, B_SCALE_SYMMETRIC = 0, 1, 2, 3
@@ -257,9 +257,36 @@ GatedDeltaArgs = _struct("uzu_gated_delta_args", [("prep", DeltaPrepareArgs), ("
 GatedDeltaStepArgs = _struct("uzu_gated_delta_step_args", [
     ("prep", DeltaPrepareArgs), ("state", u64), ("norm", u64), ("out", u64), ("gate_offset", u32), ("epsilon", f32)])
 
+RowSequence = _struct("uzu_row_sequence", [("first_row", u32), ("rows", u32), ("slot", u32), ("fresh", u32)])
+
+# `sequences` is the address of a RowSequence array in host memory
+CausalConvArgs = _struct("uzu_causal_conv_args", [
+    ("input", u64), ("output", u64), ("weights", u64), ("bias", u64), ("state", u64), ("sequences", u64), ("sequence_count", u32), ("rows", u32),
+    ("slots", u32), ("channels", u32), ("taps", u32), ("input_stride", u32), ("output_stride", u32), ("activation", u32), ("data_type", u32),
+    ("reserved0", u32)])
+
+StateSpaceScanArgs = _struct("uzu_state_space_scan_args", [
+    ("x", u64), ("dt", u64), ("b", u64), ("c", u64), ("z", u64), ("a", u64), ("d", u64), ("dt_bias", u64), ("state", u64), ("out", u64),
+    ("scratch", u64), ("scratch_bytes", u64), ("sequences", u64), ("sequence_count", u32), ("rows", u32), ("slots", u32), ("heads", u32),
+    ("groups", u32), ("head_dim", u32), ("state_size", u32), ("x_stride", u32), ("dt_stride", u32), ("b_stride", u32), ("c_stride", u32),
+    ("z_stride", u32), ("out_stride", u32), ("dt_min", f32), ("dt_max", f32), ("dt_softplus", u32), ("data_type", u32), ("reserved0", u32)])
+
+StateSpaceStepArgs = _struct("uzu_state_space_step_args", [
+    ("xbc", u64), ("dt", u64), ("z", u64), ("conv_weights", u64), ("conv_bias", u64), ("conv_state", u64), ("a", u64), ("d", u64),
+    ("dt_bias", u64), ("state", u64), ("out", u64), ("slots", u64), ("tickets", u64), ("rows", u32), ("slot_count", u32), ("heads", u32),
+    ("groups", u32), ("head_dim", u32), ("state_size", u32), ("taps", u32), ("xbc_stride", u32), ("dt_stride", u32), ("z_stride", u32),
+    ("out_stride", u32), ("dt_min", f32), ("dt_max", f32), ("dt_softplus", u32), ("activation", u32), ("data_type", u32)])
+
+EXPERT_SCORE_CHOSEN, EXPERT_SCORE_ALL, EXPERT_SCORE_SIGMOID = 0, 1, 2
+ExpertLayerArgs = _struct("uzu_expert_layer_args", [
+    ("x", u64), ("out", u64), ("router", u64), ("router_bias", u64), ("up_gate", u64), ("down", u64), ("ids", u64), ("weights", u64),
+    ("scratch", u64), ("scratch_bytes", u64), ("rows", u32), ("width", u32), ("ff", u32), ("experts", u32), ("top", u32), ("shared", u32),
+    ("x_stride", u32), ("out_stride", u32), ("score", u32), ("renormalise", u32), ("weight_scale", f32), ("activation", u32),
+    ("data_type", u32), ("reserved0", u32)])
+
 MAIN_SLOT = 0xFFFFFFFF
 
-ABI_STRUCTS = [SideStepArgs, SideAttentionArgs, EmbeddingF32Args, GluArgs, StreamMixArgs, DeltaPrepareArgs, GatedDeltaArgs, GatedDeltaStepArgs, ExpGatesArgs, NormAddArgs, TokenGateArgs, MinGruArgs, RetentionArgs, WindowAttentionPrepareArgs, WindowAttentionArgs, TopkRouteArgs, RoutedCombineArgs, SigmoidAttentionPrepareArgs, SigmoidAttentionArgs, DenseLinearArgs, GroupRmsNormArgs, TableRouteArgs, GeneralDeltaArgs, HeadNormGateArgs, LatentPrepareArgs, LatentAttentionArgs,
+ABI_STRUCTS = [RowSequence, CausalConvArgs, StateSpaceScanArgs, StateSpaceStepArgs, ExpertLayerArgs, SideStepArgs, SideAttentionArgs, EmbeddingF32Args, GluArgs, StreamMixArgs, DeltaPrepareArgs, GatedDeltaArgs, GatedDeltaStepArgs, ExpGatesArgs, NormAddArgs, TokenGateArgs, MinGruArgs, RetentionArgs, WindowAttentionPrepareArgs, WindowAttentionArgs, TopkRouteArgs, RoutedCombineArgs, SigmoidAttentionPrepareArgs, SigmoidAttentionArgs, DenseLinearArgs, GroupRmsNormArgs, TableRouteArgs, GeneralDeltaArgs, HeadNormGateArgs, LatentPrepareArgs, LatentAttentionArgs,
                DeltaNetFusedUpdateArgs, QkNormConfig, AttentionPrepareNormArgs, FusedLinearArgs, RingParams, TrieNode, KvCopy, MatmulArgs, NormalizationArgs, QkvNormArgs, AttentionPrepareArgs, AttentionArgs,
                AttentionTwoPass2Args, KvCacheUpdateArgs, GatedActMulArgs, QuantizedEmbeddingLookupArgs, UnifiedSamplingArgs,
                DeltaNetConvUpdateArgs, DeltaNetUpdateArgs, EngineOptions, SamplingMethod, ModelInfo, TpAllGatherArgs]
@@ -294,7 +321,9 @@ uzu_silu_glu_encode uzu_topk_route_encode uzu_routed_combine_gated_encode uzu_si
 uzu_engine_slot_acquire uzu_engine_slot_release uzu_engine_forward_rows uzu_engine_debug_layer_outputs uzu_debug_dense_umma_error uzu_debug_set_wait_error uzu_debug_decode_attention_encode uzu_debug_fused_linear_encode
 uzu_min_gru_encode uzu_retention_encode uzu_window_attention_prepare_encode uzu_window_attention_encode
 uzu_exp_gates_encode uzu_norm_add_encode uzu_token_gate_encode uzu_embedding_f32_scaled_encode uzu_rows_to_bf16_encode
-uzu_side_step_encode uzu_side_attention_encode uzu_embedding_f32_position_encode uzu_glu_encode uzu_stream_mix_encode uzu_delta_prepare_encode uzu_gated_delta_encode uzu_gated_delta_step_encode""".split()
+uzu_side_step_encode uzu_side_attention_encode uzu_embedding_f32_position_encode uzu_glu_encode uzu_stream_mix_encode uzu_delta_prepare_encode uzu_gated_delta_encode uzu_gated_delta_step_encode
+uzu_causal_conv_encode uzu_causal_conv_validate uzu_state_space_scan_encode uzu_state_space_scan_validate uzu_state_space_scan_scratch_bytes
+uzu_state_space_step_encode uzu_state_space_step_validate uzu_expert_layer_encode uzu_expert_layer_validate uzu_expert_layer_scratch_bytes""".split()
 
 _lib = None
 
@@ -460,6 +489,16 @@ def load() -> C.CDLL:
         "uzu_delta_prepare_encode": (None, [vp, C.POINTER(DeltaPrepareArgs)]),
         "uzu_gated_delta_encode": (None, [vp, C.POINTER(GatedDeltaArgs)]),
         "uzu_gated_delta_step_encode": (None, [vp, C.POINTER(GatedDeltaStepArgs)]),
+        "uzu_causal_conv_encode": (None, [vp, C.POINTER(CausalConvArgs)]),
+        "uzu_causal_conv_validate": (C.c_int, [C.POINTER(CausalConvArgs)]),
+        "uzu_state_space_scan_encode": (None, [vp, C.POINTER(StateSpaceScanArgs)]),
+        "uzu_state_space_scan_validate": (C.c_int, [C.POINTER(StateSpaceScanArgs)]),
+        "uzu_state_space_scan_scratch_bytes": (C.c_size_t, [vp, C.POINTER(StateSpaceScanArgs)]),
+        "uzu_state_space_step_encode": (None, [vp, C.POINTER(StateSpaceStepArgs)]),
+        "uzu_state_space_step_validate": (C.c_int, [C.POINTER(StateSpaceStepArgs)]),
+        "uzu_expert_layer_encode": (None, [vp, C.POINTER(ExpertLayerArgs)]),
+        "uzu_expert_layer_validate": (C.c_int, [C.POINTER(ExpertLayerArgs)]),
+        "uzu_expert_layer_scratch_bytes": (C.c_size_t, [C.POINTER(ExpertLayerArgs)]),
         "uzu_token_gate_encode": (None, [vp, C.POINTER(TokenGateArgs)]),
         "uzu_rows_to_bf16_encode": (None, [vp, u64, u32, u64, u32, u32]),
         "uzu_embedding_f32_scaled_encode": (None, [vp, u64, u64, u32, u64, u32, u32, u32, f32]),

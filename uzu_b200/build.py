@@ -54,6 +54,9 @@ SOURCES = {
     "linear_recurrence.cu": [],
     "retention_chunked.cu": [],
     "gated_delta.cu": [],
+    "causal_conv.cu": [],
+    "state_space.cu": [],
+    "expert_layer.cu": [],
     "engine.cu": [],
 }
 

@@ -1,0 +1,177 @@
+// Short causal convolution over packed sequences: y[t, c] = act(bias[c] + sum_j w[c, j] u[t - taps + 1 + j, c]).
+//
+// Bound by memory: a value is read and written once, 2 taps flops each. A thread has 16 bytes of channels (8 of 16 bits, 4 of 32) and walks a strip of a sequence's
+// rows with the last taps - 1 of them in registers, eight rows of loads under way at a time; a strip reads taps - 1 rows of the one before it again (from L2). The
+// strip that starts a sequence reads the slot's inputs and then writes the new ones: nobody else touches these channels of the slot, so the order is its own.
+#include "state_space.cuh"
+
+namespace uzu {
+
+namespace {
+
+constexpr uint32_t CC_THREADS = 128;
+
+struct ConvParams {
+    uzu_causal_conv_args a;
+    uint32_t strip;      // rows
+    SequenceTable table;
+};
+
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) ConvVec {
+    T v[VEC];
+};
+
+template <typename T, int VEC, int TAPS>
+__global__ void __launch_bounds__(CC_THREADS) causal_conv_kernel(const __grid_constant__ ConvParams p) {
+    using V = ConvVec<T, VEC>;
+    constexpr int BATCH = 8;
+    const uzu_causal_conv_args& a = p.a;
+    const uint32_t c = (blockIdx.y * CC_THREADS + threadIdx.x) * VEC;
+    if (c >= a.channels) return;
+    const uint32_t tile = blockIdx.x, q = ss_find(p.table, tile);
+    const PackedSequence s = p.table.s[q];
+    const uint32_t t0 = (tile - s.tile0) * p.strip, t1 = min(t0 + p.strip, s.rows), kept = a.taps - 1;
+    const T* in = reinterpret_cast<const T*>(a.input) + (size_t)s.first * a.input_stride + c;
+    T* out = reinterpret_cast<T*>(a.output) + (size_t)s.first * a.output_stride + c;
+    T* state = reinterpret_cast<T*>(a.state) + (size_t)s.slot() * kept * a.channels + c;
+
+    float w[TAPS][VEC], bias[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+        bias[i] = a.bias ? reinterpret_cast<const float*>(a.bias)[c + i] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < TAPS; ++j) {      // fewer taps than the kernel has: the oldest ones are zero
+            const int k = j - (TAPS - (int)a.taps);
+            w[j][i] = k >= 0 ? reinterpret_cast<const float*>(a.weights)[(size_t)(c + i) * a.taps + k] : 0.0f;
+        }
+    }
+    // the inputs before the strip, oldest first
+    V past[TAPS > 1 ? TAPS - 1 : 1];
+#pragma unroll
+    for (int j = 0; j < TAPS - 1; ++j) {
+        const int k = j - (TAPS - 1 - (int)kept);      // of the slot's inputs
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) past[j].v[i] = ss_t<T>(0.0f);
+        if (k < 0) continue;
+        if (t0) past[j] = *reinterpret_cast<const V*>(in + (size_t)(t0 - kept + k) * a.input_stride);
+        else if (!s.fresh()) past[j] = *reinterpret_cast<const V*>(state + (size_t)k * a.channels);
+    }
+    if (t0 == 0) {      // the last `kept` of (slot, rows)
+#pragma unroll
+        for (int j = 0; j < TAPS - 1; ++j) {
+            const int k = j - (TAPS - 1 - (int)kept);
+            if (k < 0) continue;
+            V v = past[j];
+            if (s.rows + k >= kept) v = *reinterpret_cast<const V*>(in + (size_t)(s.rows + k - kept) * a.input_stride);
+            else {
+#pragma unroll
+                for (int o = j + 1; o < TAPS - 1; ++o)
+                    if (o == j + (int)s.rows) v = past[o];
+            }
+            *reinterpret_cast<V*>(state + (size_t)k * a.channels) = v;
+        }
+    }
+    float u[TAPS][VEC];      // u[TAPS - 1]: the row at hand
+#pragma unroll
+    for (int j = 0; j < TAPS - 1; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) u[j][i] = ss_f(past[j].v[i]);
+
+    for (uint32_t t = t0; t < t1; t += BATCH) {
+        V rows[BATCH];
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b)
+            if (t + b < t1) rows[b] = *reinterpret_cast<const V*>(in + (size_t)(t + b) * a.input_stride);
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+            if (t + b >= t1) break;
+            V o;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                u[TAPS - 1][i] = ss_f(rows[b].v[i]);
+                float y = bias[i];
+#pragma unroll
+                for (int j = 0; j < TAPS; ++j) y = fmaf(w[j][i], u[j][i], y);
+                if (a.activation == UZU_ACT_SILU) y = ss_silu(y);
+                o.v[i] = ss_t<T>(y);
+#pragma unroll
+                for (int j = 0; j < TAPS - 1; ++j) u[j][i] = u[j + 1][i];
+            }
+            *reinterpret_cast<V*>(out + (size_t)(t + b) * a.output_stride) = o;
+        }
+    }
+}
+
+const char* conv_check(const uzu_causal_conv_args* a) {
+    if (!a) return "null arguments";
+    if (!ss_data_type(a->data_type)) return "data_type must be bf16, f32 or f16";
+    if (a->activation != UZU_ACT_SILU && a->activation != UZU_ACT_IDENTITY) return "the activation must be silu or identity";
+    if (a->taps == 0 || a->taps > 8) return "taps must be in 1 .. 8";
+    if (a->channels == 0 || a->channels > 65535 * CC_THREADS) return "channels must be in 1 .. 8388480";
+    if (a->input_stride < a->channels || a->output_stride < a->channels) return "a row is shorter than its channels";
+    if (const char* e = check_sequences(a->sequences, a->sequence_count, a->rows, a->slots)) return e;
+    if (a->sequence_count == 0) return nullptr;
+    if (!a->input || !a->output || !a->weights || (a->taps > 1 && !a->state)) return "null operand";
+    const uint64_t size = ss_size(a->data_type);
+    if ((a->input | a->output | (a->taps > 1 ? a->state : 0)) % size || (a->weights | a->bias) % 4) return "an operand is not aligned to its elements";
+    if (rows_overlap(a->input, a->input_stride, a->channels, a->output, a->output_stride, a->channels, a->rows, size)) return "input and output overlap";
+    const uint64_t state_bytes = (uint64_t)a->slots * (a->taps - 1) * a->channels * size;
+    if (bytes_overlap(a->state, state_bytes, a->input, rows_extent(a->rows, a->input_stride, a->channels, size)) ||
+        bytes_overlap(a->state, state_bytes, a->output, rows_extent(a->rows, a->output_stride, a->channels, size)))
+        return "the state overlaps rows";
+    return nullptr;
+}
+
+template <typename T, int VEC>
+void conv_launch(uzu_command_buffer* cmd, const ConvParams& p) {
+    const dim3 grid(p.table.tiles, (p.a.channels + CC_THREADS * VEC - 1) / (CC_THREADS * VEC));
+    auto go = [&](auto kernel) { launch(cmd, "causal_conv_kernel", kernel, grid, dim3(CC_THREADS), 0, p); };
+    if (p.a.taps <= 2) go(causal_conv_kernel<T, VEC, 2>);
+    else if (p.a.taps == 3) go(causal_conv_kernel<T, VEC, 3>);
+    else if (p.a.taps == 4) go(causal_conv_kernel<T, VEC, 4>);
+    else go(causal_conv_kernel<T, VEC, 8>);
+}
+template <typename T>
+void conv_by_alignment(uzu_command_buffer* cmd, const ConvParams& p) {
+    constexpr int VEC = 16 / sizeof(T);
+    const uzu_causal_conv_args& a = p.a;
+    const bool wide = a.channels % VEC == 0 && a.input_stride % VEC == 0 && a.output_stride % VEC == 0 && ((a.input | a.output | a.state) & 15u) == 0;
+    if (wide) conv_launch<T, VEC>(cmd, p);
+    else conv_launch<T, 1>(cmd, p);
+}
+
+}  // namespace
+}  // namespace uzu
+
+using namespace uzu;
+
+extern "C" {
+
+uzu_status uzu_causal_conv_validate(const uzu_causal_conv_args* a) {
+    const char* e = conv_check(a);
+    return e ? fail(UZU_ERROR_INVALID_ARGUMENT, std::string("causal_conv: ") + e) : UZU_OK;
+}
+
+void uzu_causal_conv_encode(uzu_command_buffer* cmd, const uzu_causal_conv_args* a) {
+    if (!encodable(cmd, "causal_conv")) return;
+    if (const char* e = conv_check(a)) {
+        cmd->record_error(UZU_ERROR_INVALID_ARGUMENT, std::string("causal_conv: ") + e);
+        return;
+    }
+    ConvParams p{};
+    p.a = *a;
+    // the longest strips that still give every SM a dozen warps: a strip reads taps - 1 rows again
+    const uint64_t threads = (uint64_t)a->channels * ss_size(a->data_type) / 16 + 1;
+    p.strip = 64;
+    while (p.strip > 8 && threads * (a->rows / p.strip + 1) < (uint64_t)cmd->ctx->sm_count * 384) p.strip /= 2;
+    for (uint32_t begin = 0; begin < a->sequence_count;) {
+        auto tiles_of = [&](uint32_t rows) { return std::max(1u, (uint32_t)(((uint64_t)rows + p.strip - 1) / p.strip)); };
+        begin = fill_sequences(p.table, a->sequences, a->sequence_count, begin, tiles_of);
+        if (a->data_type == UZU_DT_F32) conv_by_alignment<float>(cmd, p);
+        else if (a->data_type == UZU_DT_F16) conv_by_alignment<__half>(cmd, p);
+        else conv_by_alignment<__nv_bfloat16>(cmd, p);
+    }
+}
+
+}  // extern "C"

@@ -1,0 +1,569 @@
+// A whole layer of routed experts for 1 .. 64 tokens in one cooperative launch, one CTA an SM: router, choice, the chosen experts' gated units, the weighted sum.
+//
+// Bound by the chosen experts' weights, each read once: a warp streams them by TMA into a ring of 32 KB stages (32 rows of 512 columns) and never waits for anything but
+// room, over the units and over the phases, so that the wait of all CTAs for the hidden values is spent filling the ring with rows of `down`. Eight warps multiply:
+// warp w has columns [64 w, 64 w + 64) of a stage, weights as operand A of m16n8k16, up to eight tokens as operand B from L2; which column of a chunk a thread has does
+// not matter to a sum, so a thread reads 16-byte chunks (2 t + i of a row of eight: no two of a phase share banks). The warps' sums are added in order in shared memory.
+//   1  logits: an (expert, four tokens) pair a warp, or a CTA where there are fewer pairs than CTAs; rows are copied as bf16 planes (f32 rows: value and remainder).
+//   2  every CTA makes the choice for itself from the logits (waiting for one to do it would cost more), lists the chosen experts and their tokens.
+//   3  up: a unit is 16 rows of an expert's up and the 16 of its gate; hidden values, times the routing weight, go to scratch as bf16 planes.
+//   4  down: all stages of all 32-row tiles over all chosen experts, cut evenly over the CTAs; a tile that several have is summed by the last of them, in their order.
+// Two waits for all CTAs, behind phases 1 and 3. They and the ring's barriers are bounded (wait_errors.h).
+#include <algorithm>
+
+#include "umma.cuh"
+
+namespace uzu {
+
+namespace {
+
+constexpr uint32_t XL_WARPS = 8, XL_THREADS = 32 * XL_WARPS + 32, XL_STAGE = 32 * 1024, XL_COLS = 512, XL_BOX = 4096;
+constexpr uint32_t XL_MAX_TOKENS = 64, XL_MAX_EXPERTS = 528, XL_MAX_TOP = 16, XL_MAX_PAIRS = 64 * 32, XL_CTAS = 148, XL_MAX_WIDTH = 65536;
+
+// where what lies in the scratch; the counters and tickets are zero between calls
+struct XlScratch {
+    uint64_t logits, rows, hidden, partials, total;
+    static constexpr uint64_t TICKETS = 256, FIXED = 16384;
+};
+inline XlScratch xl_scratch(const uzu_expert_layer_args& a) {
+    auto up = [](uint64_t v) { return (v + 255) & ~255ull; };
+    const uint64_t planes = a.data_type == UZU_DT_F32 ? 2 : 1;
+    XlScratch s;
+    s.logits = up(XlScratch::FIXED);
+    s.rows = up(s.logits + (uint64_t)a.rows * a.experts * 4);
+    s.hidden = up(s.rows + planes * a.rows * a.width * 2);
+    s.partials = up(s.hidden + planes * a.rows * (a.top + a.shared) * a.ff * 2);
+    s.total = up(s.partials + (uint64_t)XL_CTAS * 2 * 32 * a.rows * 4);
+    return s;
+}
+
+static_assert(XlScratch::TICKETS + XL_MAX_WIDTH / 32 * 4 <= XlScratch::FIXED, "a ticket for every tile");
+
+struct XlParams {
+    uzu_expert_layer_args a;
+    XlScratch s;
+    unsigned int* error;
+};
+
+template <int NT, int PLANES>
+struct XlShape {
+    static constexpr uint32_t RED = XL_WARPS * 32 * NT * 8 * 4, STAGES = NT <= 2 ? 6 : NT == 4 ? 5 : 4;
+    static constexpr size_t SMEM = STAGES * XL_STAGE + RED + 1024;
+};
+
+__device__ __forceinline__ void xl_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 xl_lds(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ float xl_x(const uzu_expert_layer_args& a, uint32_t t, uint32_t c) {
+    return a.data_type == UZU_DT_F32 ? reinterpret_cast<const float*>(a.x)[(size_t)t * a.x_stride + c] : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.x)[(size_t)t * a.x_stride + c]);
+}
+
+// all CTAs of the launch; false: not within about a second
+__device__ __noinline__ bool xl_all(unsigned int* counter, volatile uint32_t* gave_up, unsigned int* error, uint32_t code) {
+    __threadfence();
+    atomicAdd(counter, 1u);
+    const uint64_t t0 = um_now();
+    for (uint32_t n = 1;; ++n) {
+        unsigned int v;
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(counter) : "memory");
+        if (v >= gridDim.x) return true;
+        if ((n & 63u) == 0) {
+            if (*gave_up) return false;
+            if (um_now() - t0 > 1000000000ull) {
+                *gave_up = 1;
+                report_wait_error(error, code);
+                return false;
+            }
+        }
+    }
+}
+
+struct XlLists {
+    uint32_t mask[XL_MAX_EXPERTS][2];      // tokens of an expert
+    uint16_t expert[XL_MAX_EXPERTS];       // the chosen ones, ascending
+    uint16_t base[XL_MAX_EXPERTS + 1];     // their pairs, in that order
+    uint8_t token[XL_MAX_PAIRS];
+    uint16_t id[XL_MAX_TOKENS][XL_MAX_TOP];
+    float weight[XL_MAX_TOKENS][XL_MAX_TOP];
+    uint32_t chosen;
+};
+
+// the choice for one token by a warp
+__device__ void xl_choose(const uzu_expert_layer_args& a, const float* logits, uint32_t t, XlLists& l, bool write) {
+    constexpr int PER = 16;
+    const uint32_t lane = threadIdx.x & 31u;
+    float v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const uint32_t e = lane + 32 * i;
+        v[i] = e < a.experts ? __ldcg(logits + (size_t)t * a.experts + e) : -INFINITY;
+        if (v[i] != v[i]) v[i] = -INFINITY;
+    }
+    if (a.score == UZU_EXPERT_SCORE_SIGMOID) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[i] = lane + 32 * i < a.experts ? 1.0f / (1.0f + expf(-v[i])) : -INFINITY;
+    } else if (a.score == UZU_EXPERT_SCORE_ALL) {
+        float most = v[0], sum = 0.0f;
+#pragma unroll
+        for (int i = 1; i < PER; ++i) most = fmaxf(most, v[i]);
+        most = warp_max(most);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            v[i] = lane + 32 * i < a.experts ? expf(v[i] - most) : -INFINITY;
+            if (lane + 32 * i < a.experts) sum += v[i];
+        }
+        sum = warp_sum(sum);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[i] /= sum;
+    }
+    uint32_t taken = 0;
+    float mine = 0.0f, first = 0.0f;      // lane k: the score of choice k
+    uint32_t mine_id = 0;
+    for (uint32_t k = 0; k < a.top; ++k) {
+        float best = -INFINITY;
+        uint32_t at = 0xffffffffu;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const uint32_t e = lane + 32 * i;
+            if (e < a.experts && !(taken >> i & 1u) && (at == 0xffffffffu || v[i] > best)) { best = v[i]; at = e; }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const float ob = __shfl_xor_sync(0xffffffffu, best, o);
+            const uint32_t oa = __shfl_xor_sync(0xffffffffu, at, o);
+            if (oa != 0xffffffffu && (at == 0xffffffffu || ob > best || (ob == best && oa < at))) { best = ob; at = oa; }
+        }
+        if ((at & 31u) == lane) taken |= 1u << (at >> 5);
+        if (k == 0) first = best;
+        if (lane == k) { mine = best; mine_id = at; }
+    }
+    float w = lane < a.top ? mine : 0.0f;
+    if (a.score == UZU_EXPERT_SCORE_CHOSEN) {
+        w = lane < a.top ? expf(mine - first) : 0.0f;
+        w /= warp_sum(w);
+    }
+    if (a.renormalise) w /= warp_sum(w);
+    w *= a.weight_scale;
+    if (lane < a.top) {
+        l.id[t][lane] = (uint16_t)mine_id;
+        l.weight[t][lane] = w;
+        atomicOr(&l.mask[mine_id][t >> 5], 1u << (t & 31u));
+        if (write && a.ids) reinterpret_cast<uint32_t*>(a.ids)[(size_t)t * a.top + lane] = mine_id;
+        if (write && a.weights) reinterpret_cast<float*>(a.weights)[(size_t)t * a.top + lane] = w;
+    }
+}
+
+}  // namespace
+
+template <int NT, int PLANES>
+__global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __grid_constant__ CUtensorMap map_up, const __grid_constant__ CUtensorMap map_down, const __grid_constant__ XlParams p) {
+    using S = XlShape<NT, PLANES>;
+    constexpr uint32_t TOK = NT * 8;
+    extern __shared__ uint8_t xl_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * S::STAGES];
+    __shared__ volatile uint32_t gave_up;
+    __shared__ uint32_t last;
+    __shared__ XlLists l;
+    const uzu_expert_layer_args& a = p.a;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), g = lane >> 2, t4 = lane & 3u;
+    const uint32_t ring = (um_smem(xl_raw) + 1023u) & ~1023u, bar0 = um_smem(bars);
+    float* red = reinterpret_cast<float*>(xl_raw + (ring - um_smem(xl_raw)) + S::STAGES * XL_STAGE);
+    uint8_t* scratch = reinterpret_cast<uint8_t*>(a.scratch);
+    unsigned int* counters = reinterpret_cast<unsigned int*>(scratch);
+    unsigned int* tickets = reinterpret_cast<unsigned int*>(scratch + XlScratch::TICKETS);
+    float* logits = reinterpret_cast<float*>(scratch + p.s.logits);
+    __nv_bfloat16* rows = reinterpret_cast<__nv_bfloat16*>(scratch + p.s.rows);
+    __nv_bfloat16* hidden = reinterpret_cast<__nv_bfloat16*>(scratch + p.s.hidden);
+    float* partials = reinterpret_cast<float*>(scratch + p.s.partials);
+    const uint32_t T = a.rows, D = a.width, F = a.ff, E = a.experts, all = E + a.shared, ctas = gridDim.x, cta = blockIdx.x;
+    const size_t row_plane = (size_t)T * D, hidden_plane = (size_t)T * (a.top + a.shared) * F;
+    auto full = [&](uint32_t s) { return bar0 + 8u * s; };
+    auto empty = [&](uint32_t s) { return bar0 + 8u * (S::STAGES + s); };
+
+    if (tid == 0) {
+        for (uint32_t s = 0; s < S::STAGES; ++s) { um_init(full(s), 1); um_init(empty(s), XL_WARPS); }
+        gave_up = 0;
+        um_fence_init();
+    }
+    for (uint32_t e = tid; e < all; e += XL_THREADS) {      // shared experts have every token
+        l.mask[e][0] = e < E ? 0u : T >= 32 ? 0xffffffffu : (1u << T) - 1u;
+        l.mask[e][1] = e < E || T <= 32 ? 0u : T >= 64 ? 0xffffffffu : (1u << (T - 32)) - 1u;
+    }
+    pdl_wait();
+
+    // ---- 1: rows as planes, logits ----
+    for (uint32_t i = cta * XL_THREADS + tid; i < T * D; i += ctas * XL_THREADS) {
+        const float v = xl_x(a, i / D, i % D);
+        const __nv_bfloat16 hi = __float2bfloat16_rn(v);
+        rows[i] = hi;
+        // (not of what is no number or infinite: the product shows it by the first part alone)
+        if (PLANES == 2) rows[row_plane + i] = __float2bfloat16_rn(fabsf(v) < INFINITY ? v - __bfloat162float(hi) : 0.0f);
+    }
+    {
+        const uint32_t quads = (T + 3) / 4, pairs = E * quads;
+        const bool split = pairs <= ctas;      // the CTA's warps share the columns
+        const __nv_bfloat16* router = reinterpret_cast<const __nv_bfloat16*>(a.router);
+        for (uint32_t i = split ? cta : cta * XL_WARPS + warp; i < pairs && (split || warp < XL_WARPS); i += split ? ctas : ctas * XL_WARPS) {
+            const uint32_t e = i / quads, tk = i % quads * 4;
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (warp < XL_WARPS) {
+                for (uint32_t c = (split ? warp * 256 : 0) + lane * 8; c < D; c += split ? XL_WARPS * 256 : 256) {
+                    const uint4 w = ldg_stream_u4(router + (size_t)e * D + c);
+                    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k)
+                        if (tk + k < T) {
+#pragma unroll
+                            for (uint32_t j = 0; j < 4; ++j) sum[k] = fmaf(um_hi(ws[j]), xl_x(a, tk + k, c + 2 * j + 1), fmaf(um_lo(ws[j]), xl_x(a, tk + k, c + 2 * j), sum[k]));
+                        }
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) sum[k] = warp_sum(sum[k]);
+            }
+            const float bias = a.router_bias ? reinterpret_cast<const float*>(a.router_bias)[e] : 0.0f;
+            if (split) {
+                if (warp < XL_WARPS && lane < 4) red[warp * 4 + lane] = lane == 0 ? sum[0] : lane == 1 ? sum[1] : lane == 2 ? sum[2] : sum[3];
+                __syncthreads();
+                if (tid < 4 && tk + tid < T) {
+                    float v = bias;
+                    for (uint32_t w = 0; w < XL_WARPS; ++w) v += red[w * 4 + tid];
+                    logits[(size_t)(tk + tid) * E + e] = v;
+                }
+                __syncthreads();
+            } else if (lane < 4 && tk + lane < T) logits[(size_t)(tk + lane) * E + e] = bias + (lane == 0 ? sum[0] : lane == 1 ? sum[1] : lane == 2 ? sum[2] : sum[3]);
+        }
+    }
+    __syncthreads();
+    if (tid == 0) xl_all(counters, &gave_up, p.error, 0x601u);
+    __syncthreads();
+    bool ok = !gave_up;
+
+    // ---- 2: the choice ----
+    if (ok) {
+        for (uint32_t t = warp; t < T; t += XL_THREADS / 32) xl_choose(a, logits, t, l, cta == 0);
+        __syncthreads();
+        if (warp == 0) {
+            uint32_t count = 0, pairs = 0;
+            for (uint32_t e0 = 0; e0 < all; e0 += 32) {
+                const uint32_t e = e0 + lane, n = e < all ? __popc(l.mask[e][0]) + __popc(l.mask[e][1]) : 0u, there = __ballot_sync(0xffffffffu, n != 0);
+                uint32_t before = n;      // pairs of the experts below, this one's included
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t v = __shfl_up_sync(0xffffffffu, before, o);
+                    if (lane >= o) before += v;
+                }
+                if (n) {
+                    const uint32_t at = count + __popc(there & ((1u << lane) - 1u));
+                    uint32_t pair = pairs + before - n;
+                    l.expert[at] = (uint16_t)e;
+                    l.base[at] = (uint16_t)pair;
+                    for (uint32_t half = 0; half < 2; ++half)
+                        for (uint32_t m = l.mask[e][half]; m; m &= m - 1) l.token[pair++] = (uint8_t)(half * 32 + __ffs(m) - 1);
+                }
+                count += __popc(there);
+                pairs += __shfl_sync(0xffffffffu, before, 31);
+            }
+            if (lane == 0) {
+                l.base[count] = (uint16_t)pairs;
+                l.chosen = count;
+            }
+        }
+        __syncthreads();
+    }
+    const uint32_t chosen = ok ? l.chosen : 0, f_tiles = (F + 15) / 16, units = chosen * f_tiles, up_stages = (D + XL_COLS - 1) / XL_COLS;
+    const uint32_t d_tiles = (D + 31) / 32, f_stages = (F + XL_COLS - 1) / XL_COLS, tile_stages = chosen * f_stages;
+    const uint64_t work = (uint64_t)d_tiles * tile_stages, parts = min((uint64_t)ctas, work), begin = cta < parts ? work * cta / parts : work, end = cta < parts ? work * (cta + 1) / parts : work;
+    uint32_t it = 0;      // stages so far
+
+    if (warp == XL_WARPS) {
+        // ---- weights by TMA ----
+        auto stage = [&](const CUtensorMap* map, uint32_t col, uint32_t width, uint32_t row_a, uint32_t row_b) {
+            const uint32_t s = it % S::STAGES;
+            if (ok) ok = um_wait(empty(s), (it / S::STAGES & 1u) ^ 1u, &gave_up, p.error, 0x602u);
+            if (!ok) return;
+            if (um_elect()) {
+                const uint32_t boxes = min(XL_WARPS, (width - col + 63) / 64);
+                um_expect(full(s), boxes * XL_BOX);
+                for (uint32_t b = 0; b < boxes; ++b) {
+                    um_tma(ring + s * XL_STAGE + b * XL_BOX, map, col + b * 64, row_a, full(s));
+                    um_tma(ring + s * XL_STAGE + b * XL_BOX + XL_BOX / 2, map, col + b * 64, row_b, full(s));
+                }
+            }
+            __syncwarp();
+            ++it;
+        };
+        for (uint32_t u = cta; u < units && ok; u += ctas) {
+            const uint32_t row = l.expert[u / f_tiles] * 2 * F + u % f_tiles * 16;
+            for (uint32_t s = 0; s < up_stages && ok; ++s) stage(&map_up, s * XL_COLS, D, row, row + F);
+        }
+        for (uint64_t w = begin; w < end && ok; ++w) {
+            const uint32_t tile = (uint32_t)(w / tile_stages), at = (uint32_t)(w % tile_stages), row = l.expert[at / f_stages] * D + tile * 32;
+            stage(&map_down, at % f_stages * XL_COLS, F, row, row + 16);
+        }
+        if (!ok)      // copies on their way end before the CTA does
+            for (uint32_t n = 1; n <= S::STAGES && n <= it; ++n) um_settle(full((it - n) % S::STAGES), (it - n) / S::STAGES & 1u);
+    } else {
+        // ---- products ----
+        float acc[2][NT][4];
+        auto clear = [&]() {
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[m][n][j] = 0.0f;
+        };
+        // This warp's columns of a stage: operand B of tile n, a token's row from `src(n)` (null: no token), a plane `plane` elements behind the one before.
+        auto multiply = [&](uint32_t col, uint32_t width, size_t plane, uint32_t live, auto src) {
+            const uint32_t s = it % S::STAGES, c0 = col + warp * 64;
+            const bool there = c0 < width;
+            constexpr bool AHEAD = NT * PLANES <= 4;      // registers for B before the weights are there
+            uint4 b[AHEAD ? NT : 1][PLANES][2];
+            auto fetch = [&](int n, uint4 (&v)[PLANES][2]) {
+                const __nv_bfloat16* at = src(n);
+#pragma unroll
+                for (int pl = 0; pl < PLANES; ++pl)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t c = c0 + (2 * t4 + i) * 8;
+                        v[pl][i] = at && c < width ? __ldcg(reinterpret_cast<const uint4*>(at + pl * plane + c)) : make_uint4(0, 0, 0, 0);
+                    }
+            };
+            if (AHEAD && there) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    if (live >> n & 1u) fetch(n, b[n]);
+            }
+            if (ok) ok = um_wait(full(s), it / S::STAGES & 1u, &gave_up, p.error, 0x603u);
+            if (!ok) return;
+            if (there) {
+                const uint32_t box = ring + s * XL_STAGE + warp * XL_BOX + g * 128;
+                uint4 w[2][4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) w[i][q] = xl_lds(box + q * 1024 + (((2 * t4 + i) ^ g) << 4));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    if (!(live >> n & 1u)) continue;
+                    uint4 here[PLANES][2];
+                    if (!AHEAD) fetch(n, here);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int pl = PLANES - 1; pl >= 0; --pl) {
+                            const uint4 v = AHEAD ? b[AHEAD ? n : 0][pl][i] : here[pl][i];
+#pragma unroll
+                            for (int m = 0; m < 2; ++m) {
+                                xl_mma(acc[m][n], w[i][2 * m].x, w[i][2 * m + 1].x, w[i][2 * m].y, w[i][2 * m + 1].y, v.x, v.y);
+                                xl_mma(acc[m][n], w[i][2 * m].z, w[i][2 * m + 1].z, w[i][2 * m].w, w[i][2 * m + 1].w, v.z, v.w);
+                            }
+                        }
+                }
+            }
+            um_arrive(empty(s));
+            ++it;
+        };
+        auto meet = [&]() {
+            __syncwarp();
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+        };
+        // the warps' sums side by side: red[warp][row][token]
+        auto share = [&]() {
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        *reinterpret_cast<float2*>(&red[(warp * 32 + m * 16 + j * 8 + g) * TOK + n * 8 + 2 * t4]) = make_float2(acc[m][n][2 * j], acc[m][n][2 * j + 1]);
+            meet();
+        };
+        auto total = [&](uint32_t row, uint32_t tok) {
+            float v = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < XL_WARPS; ++w) v += red[(w * 32 + row) * TOK + tok];
+            return v;
+        };
+
+        // ---- 3: up ----
+        for (uint32_t u = cta; u < units; u += ctas) {
+            const uint32_t at = u / f_tiles, f0 = u % f_tiles * 16, base = l.base[at], count = l.base[at + 1] - base, e = l.expert[at];
+            const uint32_t live = (1u << ((count + 7) / 8)) - 1u;
+            clear();
+            for (uint32_t s = 0; s < up_stages && ok; ++s)
+                multiply(s * XL_COLS, D, row_plane, live, [&](int n) { return n * 8 + g < count ? rows + (size_t)l.token[base + n * 8 + g] * D : nullptr; });
+            share();      // (also where a wait ran out: nobody is left waiting)
+            for (uint32_t i = tid; i < count * 16; i += 256) {
+                const uint32_t f = i & 15u, k = i >> 4, tok = l.token[base + k];
+                if (f0 + f >= F) continue;
+                float w = 1.0f;
+                if (e < E)
+                    for (uint32_t j = 0; j < a.top; ++j)
+                        if (l.id[tok][j] == e) w = l.weight[tok][j];
+                const float v = act_f32(a.activation, total(16 + f, k)) * total(f, k) * w;
+                const __nv_bfloat16 hi = __float2bfloat16_rn(v);
+                __nv_bfloat16* to = hidden + (size_t)(base + k) * F + f0 + f;
+                to[0] = hi;
+                if (PLANES == 2) to[hidden_plane] = __float2bfloat16_rn(fabsf(v) < INFINITY ? v - __bfloat162float(hi) : 0.0f);
+            }
+            meet();
+        }
+        if (tid == 0) xl_all(counters + 1, &gave_up, p.error, 0x604u);
+        meet();
+        ok = ok && !gave_up;
+
+        // ---- 4: down ----
+        auto cta_of = [&](uint64_t w) { return (uint32_t)(((w + 1) * parts - 1) / work); };
+        auto store = [&](uint32_t d, uint32_t tok, float v) {
+            if (a.data_type == UZU_DT_F32) reinterpret_cast<float*>(a.out)[(size_t)tok * a.out_stride + d] = v;
+            else reinterpret_cast<__nv_bfloat16*>(a.out)[(size_t)tok * a.out_stride + d] = __float2bfloat16_rn(v);
+        };
+        for (uint64_t w = begin; w < end;) {
+            const uint32_t tile = (uint32_t)(w / tile_stages);
+            const uint64_t tile0 = (uint64_t)tile * tile_stages, tile1 = tile0 + tile_stages, stop = min(tile1, end);
+            const bool whole = w == tile0 && stop == tile1;
+            const uint32_t slot = begin > tile0 ? 0u : 1u;      // of this CTA's two tiles in parts
+            clear();
+            for (; w < stop && ok; ++w) {
+                const uint32_t at = (uint32_t)(w - tile0) / f_stages, s = (uint32_t)(w - tile0) % f_stages, base = l.base[at], e = l.expert[at];
+                const uint64_t mask = (uint64_t)l.mask[e][1] << 32 | l.mask[e][0];
+                uint32_t live = 0;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) live |= (mask >> (8 * n) & 0xffu) ? 1u << n : 0u;
+                multiply(s * XL_COLS, F, hidden_plane, live, [&](int n) {
+                    const uint32_t tok = n * 8 + g;
+                    return mask >> tok & 1u ? hidden + (size_t)(base + __popcll(mask & ((1ull << tok) - 1u))) * F : nullptr;
+                });
+            }
+            w = stop;
+            share();
+            if (whole) {
+                if (ok)
+                    for (uint32_t i = tid; i < 32 * T; i += 256)
+                        if (tile * 32 + (i & 31u) < D) store(tile * 32 + (i & 31u), i >> 5, total(i & 31u, i >> 5));
+            } else {
+                float* part = partials + ((size_t)cta * 2 + slot) * 32 * T;
+                for (uint32_t i = tid; i < 32 * T; i += 256) part[i] = total(i & 31u, i >> 5);
+                __threadfence();
+                meet();
+                const uint32_t from = cta_of(tile0), to = cta_of(tile1 - 1);
+                if (tid == 0) {
+                    last = atomicAdd(&tickets[tile], 1u) == to - from;
+                    if (last) tickets[tile] = 0;
+                    __threadfence();
+                }
+                meet();
+                if (last && ok)
+                    for (uint32_t i = tid; i < 32 * T; i += 256) {
+                        if (tile * 32 + (i & 31u) >= D) continue;
+                        float v = 0.0f;
+                        for (uint32_t c = from; c <= to; ++c) v += __ldcg(partials + ((size_t)c * 2 + (work * c / parts > tile0 ? 0u : 1u)) * 32 * T + i);
+                        store(tile * 32 + (i & 31u), i >> 5, v);
+                    }
+            }
+            meet();
+        }
+    }
+    __syncthreads();
+    if (tid == 0 && atomicAdd(counters + 2, 1u) == ctas - 1) {      // the last one out: for the next call
+        counters[0] = counters[1] = counters[2] = 0;
+        __threadfence();
+    }
+}
+
+namespace {
+
+const char* xl_check(const uzu_expert_layer_args* a, bool run) {
+    if (!a) return "null arguments";
+    if (a->data_type != UZU_DT_BF16 && a->data_type != UZU_DT_F32) return "data_type must be bf16 or f32";
+    if (a->rows > XL_MAX_TOKENS) return "at most 64 rows";
+    if (a->width == 0 || a->width > XL_MAX_WIDTH || a->ff == 0 || a->ff > XL_MAX_WIDTH || a->width % 8 || a->ff % 8) return "width and ff must be multiples of 8 up to 65536";
+    if (a->experts == 0 || a->experts > 512 || a->shared > 16) return "experts must be in 1 .. 512, shared in 0 .. 16";
+    if (a->top == 0 || a->top > XL_MAX_TOP || a->top > a->experts) return "top must be in 1 .. 16 and not above experts";
+    if (a->score > UZU_EXPERT_SCORE_SIGMOID || a->activation > UZU_ACT_SOFTPLUS) return "unknown score or activation";
+    if ((uint64_t)(a->experts + a->shared) * std::max(2ull * a->ff, (unsigned long long)a->width) >> 31) return "too many rows of weights";
+    if (a->x_stride < a->width || a->out_stride < a->width) return "a row is shorter than width";
+    if (!run || a->rows == 0) return nullptr;
+    if (!a->x || !a->out || !a->router || !a->up_gate || !a->down || !a->scratch) return "null operand";
+    const uint64_t size = a->data_type == UZU_DT_F32 ? 4 : 2;
+    if ((a->x | a->out) % size || (a->router | a->up_gate | a->down) % 16 || (a->router_bias | a->ids | a->weights) % 4) return "an operand is not aligned";
+    if (a->scratch % 256 || a->scratch_bytes < xl_scratch(*a).total) return "the scratch is too small or not 256-byte aligned";
+    const uint64_t x_bytes = ((uint64_t)(a->rows - 1) * a->x_stride + a->width) * size, out_bytes = ((uint64_t)(a->rows - 1) * a->out_stride + a->width) * size;
+    if (a->x < a->out + out_bytes && a->out < a->x + x_bytes) return "x and out overlap";
+    return nullptr;
+}
+
+template <int NT, int PLANES>
+void xl_launch(uzu_command_buffer* cmd, const XlParams& p, const CUtensorMap& up, const CUtensorMap& down) {
+    static std::atomic<uint64_t> opted{0};
+    opt_in_dynamic_smem(cmd, expert_layer_kernel<NT, PLANES>, (int)XlShape<NT, PLANES>::SMEM, opted);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(std::min<uint32_t>(cmd->ctx->sm_count, XL_CTAS));
+    cfg.blockDim = dim3(XL_THREADS);
+    cfg.dynamicSmemBytes = XlShape<NT, PLANES>::SMEM;
+    cfg.stream = cmd->ctx->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeCooperative;      // all CTAs run together, or the launch fails
+    attr[0].val.cooperative = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, expert_layer_kernel<NT, PLANES>, up, down, p);
+    if (e != cudaSuccess) {
+        cmd->record_error(UZU_ERROR_CUDA, std::string("expert_layer_kernel: ") + cudaGetErrorString(e));
+        cudaGetLastError();
+    }
+    cmd->launches++;
+}
+
+}  // namespace
+}  // namespace uzu
+
+using namespace uzu;
+
+extern "C" {
+
+uzu_status uzu_expert_layer_validate(const uzu_expert_layer_args* a) {
+    const char* e = xl_check(a, true);
+    return e ? fail(UZU_ERROR_INVALID_ARGUMENT, std::string("expert_layer: ") + e) : UZU_OK;
+}
+
+size_t uzu_expert_layer_scratch_bytes(const uzu_expert_layer_args* a) { return xl_check(a, false) ? 0 : xl_scratch(*a).total; }
+
+void uzu_expert_layer_encode(uzu_command_buffer* cmd, const uzu_expert_layer_args* a) {
+    if (!encodable(cmd, "expert_layer")) return;
+    if (const char* e = xl_check(a, true)) {
+        cmd->record_error(UZU_ERROR_INVALID_ARGUMENT, std::string("expert_layer: ") + e);
+        return;
+    }
+    if (a->rows == 0) return;
+    XlParams p{};
+    p.a = *a;
+    p.s = xl_scratch(*a);
+    p.error = cmd->ctx->wait_errors.device_word;
+    CUtensorMap up, down;
+    const uint64_t all = a->experts + a->shared;
+    if (!um_map(&up, a->up_gate, a->width, all * 2 * a->ff, a->width, 16) || !um_map(&down, a->down, a->ff, all * a->width, a->ff, 16)) {
+        cmd->record_error(UZU_ERROR_CUDA, "expert_layer: cuTensorMapEncodeTiled failed");
+        return;
+    }
+    // token tiles of eight: the smallest kernel that holds the rows (a larger one's ring is shorter)
+    auto go = [&](auto planes) {
+        constexpr int PL = decltype(planes)::value;
+        if (a->rows <= 8) xl_launch<1, PL>(cmd, p, up, down);
+        else if (a->rows <= 16) xl_launch<2, PL>(cmd, p, up, down);
+        else if (a->rows <= 32) xl_launch<4, PL>(cmd, p, up, down);
+        else xl_launch<8, PL>(cmd, p, up, down);
+    };
+    if (a->data_type == UZU_DT_F32) go(std::integral_constant<int, 2>{});
+    else go(std::integral_constant<int, 1>{});
+}
+
+}  // extern "C"

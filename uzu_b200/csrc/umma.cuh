@@ -1,0 +1,99 @@
+// Barriers with bounded waits, tiled copies, tcgen05 products and tensor memory, as the kernels of the state space scan and of the experts' layer use them.
+// A wait that runs out (about a second) reports its code to the context (wait_errors.h) and makes every role of the CTA leave.
+#pragma once
+
+#include <cuda.h>
+
+#include "common.cuh"
+
+namespace uzu {
+
+#ifdef __CUDACC__
+__device__ __forceinline__ uint32_t um_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void um_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void um_fence_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
+// (a whole warp, for all its lanes)
+__device__ __forceinline__ void um_arrive(uint32_t bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31u) == 0) asm volatile("{ .reg .b64 st; mbarrier.arrive.shared::cta.b64 st, [%0]; }" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool um_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }" : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
+    return ok != 0;
+}
+// after a wait that ran out: what is in flight ends before the CTA does
+__device__ __forceinline__ void um_settle(uint32_t bar, uint32_t parity) {
+    for (uint32_t n = 0; n < 4096 && !um_try(bar, parity); ++n) {}
+}
+__device__ __forceinline__ uint64_t um_now() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+// false: the phase did not complete within about a second, or another role of the CTA has given up
+__device__ __noinline__ inline bool um_wait_long(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up, unsigned int* error, uint32_t code) {
+    const uint64_t t0 = um_now();
+    for (uint32_t tries = 1;; ++tries) {
+        if (um_try(bar, parity)) return true;
+        if (tries & 15u) continue;
+        if (*gave_up) return false;
+        if (um_now() - t0 > 1000000000ull) {
+            *gave_up = 1;
+            report_wait_error(error, code);
+            return false;
+        }
+    }
+}
+__device__ __forceinline__ bool um_wait(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up, unsigned int* error, uint32_t code) {      // by whole warps
+    if (__all_sync(0xffffffffu, um_try(bar, parity))) return true;
+    return __all_sync(0xffffffffu, um_wait_long(bar, parity, gave_up, error, code));
+}
+__device__ __forceinline__ bool um_elect() {
+    uint32_t p = 0;
+    asm volatile("{ .reg .pred q; .reg .b32 r; elect.sync r|q, 0xffffffff; @q mov.u32 %0, 1; }" : "+r"(p));
+    return p != 0;
+}
+__device__ __forceinline__ void um_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("{ .reg .b64 st; mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1; }" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void um_tma(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void um_commit(uint32_t bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void um_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void um_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void um_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void um_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void um_fence_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ uint32_t um_pack(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float um_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float um_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+#endif
+
+inline decltype(&cuTensorMapEncodeTiled) um_encoder() {
+    static decltype(&cuTensorMapEncodeTiled) fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
+        cudaGetLastError();
+        return (decltype(&cuTensorMapEncodeTiled))f;
+    }();
+    return fn;
+}
+// rows of bf16, `pitch` elements apart, in boxes of 64 elements (128-byte swizzled rows) by `box_rows`
+inline bool um_map(CUtensorMap* map, uint64_t addr, uint64_t width, uint64_t rows, uint64_t pitch, uint32_t box_rows) {
+    const cuuint64_t dims[2] = {width, rows}, strides[1] = {pitch * 2};
+    const cuuint32_t box[2] = {64, box_rows}, steps[2] = {1, 1};
+    return um_encoder() && um_encoder()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (void*)addr, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace uzu
