@@ -936,7 +936,10 @@ UZU_API uzu_status uzu_causal_conv_validate(const uzu_causal_conv_args* args);
  *   step = dt + dt_bias[h];  dt_softplus: step <- softplus(step);  step <- min(max(step, dt_min), dt_max)
  *   S_t = exp(step a[h]) S_(t-1) + step x_t b_t^T   (per head [head_dim, state_size]);   y_t = S_t c_t + d[h] x_t;   out = y * silu(z)  (z optional)
  * The state f32 [slots, heads, head_dim, state_size] is read and written back per sequence. a is negative in a model (decays below 1); nothing checks it.
- * dt_min >= 0.
+ * dt_min >= 0. bf16 rows with head_dim a multiple of 64, state_size 64 or 128 and pointers and strides of whole 16-byte groups run in chunks of 128 tokens on
+ * the tensor cores (csrc/state_space_umma.cu): states, decays and sums are f32 there too, decayed inputs enter the state as two bf16 parts (16 bits), scores
+ * and the state that is read out are rounded to bf16. An input that is not finite leaves NaN or infinity in what depends on it and in nothing else; which of the
+ * two is not said. Everything else runs token by token.
  * scratch: of uzu_state_space_scan_scratch_bytes() bytes, 16-byte aligned, content free before and after; with none (0), or less, long sequences are not
  * cut into parts, which costs time only. Calls that may run at the same time do not share it. */
 typedef struct uzu_state_space_scan_args {

@@ -198,6 +198,32 @@ def test_scan_empty(ctx):
     _scan(ctx, P.F32, 2, 1, 8, 8, [], 4, 1)
 
 
+# heads of whole chunks' shapes in bf16: on the tensor cores
+CHUNKED = [(0, 1, 3, 0), (1, 127, 0, 1), (128, 128, 1, 0), (256, 129, 4, 0), (390, 300, 2, 0), (690, 0, 5, 1), (690, 0, 6, 0), (700, 64, 7, 1)]
+
+
+@pytest.mark.parametrize("heads,groups,dim,n", [(2, 1, 64, 128), (2, 2, 64, 64), (2, 1, 128, 64), (2, 1, 128, 128), (1, 1, 192, 128)])
+@pytest.mark.parametrize("over", [dict(), dict(gate=False, pad=8), dict(scale_dt=30.0), dict(skip_d=False, lo=0.5, hi=20.0)])
+def test_scan_chunks(ctx, heads, groups, dim, n, over):
+    _scan(ctx, P.BF16, heads, groups, dim, n, CHUNKED, 770, 9, chunks=True, **over)
+
+
+@pytest.mark.parametrize("scratch", [True, False])
+@pytest.mark.parametrize("rows,seqs", [(2500, [(0, 2500, 1, 0)]), (2049, [(0, 1025, 0, 1), (1025, 1024, 1, 0)]), (1100, [(3, 1090, 0, 0)])])
+def test_scan_in_parts(ctx, rows, seqs, scratch):
+    """few heads: long sequences are cut, with a scratch"""
+    _scan(ctx, P.BF16, 2, 1, 64, 128, seqs, rows, 2, chunks=True, scratch=scratch)
+
+
+def test_scan_parts_and_whole_agree(ctx):
+    """parts start from the sums of the parts before them: the state differs by roundings only (checked against float64 above); whole sequences give the same bits twice"""
+    _scan(ctx, P.BF16, 4, 4, 64, 64, [(0, 1500, 0, 0), (1500, 40, 1, 1)], 1540, 3, chunks=True)
+
+
+def test_scan_many_sequences_in_chunks(ctx):
+    _scan(ctx, P.BF16, 1, 1, 64, 64, [(3 * i, 1 + i % 3, i, i % 2) for i in range(300)], 900, 300, chunks=True)
+
+
 # ---- one token ------------------------------------------------------------------------------------------------------------------------------------
 def _step_case(ctx, dt, heads, groups, dim, n, taps, slots, slot_count, gate=True, act=True, seed=0, calls=1, pad=0, graph=False):
     rng = np.random.default_rng(seed)

@@ -56,6 +56,7 @@ SOURCES = {
     "gated_delta.cu": [],
     "causal_conv.cu": [],
     "state_space.cu": [],
+    "state_space_umma.cu": [],
     "expert_layer.cu": [],
     "engine.cu": [],
 }

@@ -26,6 +26,8 @@ template <typename T, int VEC, int TAPS>
 __global__ void __launch_bounds__(CC_THREADS) causal_conv_kernel(const __grid_constant__ ConvParams p) {
     using V = ConvVec<T, VEC>;
     constexpr int BATCH = 8;
+    pdl_launch_dependents();
+    pdl_wait();
     const uzu_causal_conv_args& a = p.a;
     const uint32_t c = (blockIdx.y * CC_THREADS + threadIdx.x) * VEC;
     if (c >= a.channels) return;

@@ -38,6 +38,8 @@ __global__ void __launch_bounds__(SS_THREADS) state_space_scan_kernel(const __gr
     constexpr uint32_t COLS = 16 * GROUPS, PER = SS_BATCH * COLS / SS_THREADS, XPER = SS_BATCH * SS_ROWS / SS_THREADS;
     __shared__ __align__(16) float bs[SS_BATCH][COLS], cs[SS_BATCH][COLS];
     __shared__ float xs[SS_BATCH][SS_ROWS], ys[SS_BATCH][SS_ROWS], decay[SS_BATCH], step[SS_BATCH];
+    pdl_launch_dependents();
+    pdl_wait();
     const uzu_state_space_scan_args& a = p.a;
     const uint32_t tid = threadIdx.x, h = blockIdx.y, p0 = blockIdx.x * SS_ROWS, part = tid & 3u, pl = tid >> 2, N = a.state_size, P = a.head_dim;
     const PackedSequence s = p.table.s[blockIdx.z];
@@ -199,6 +201,8 @@ __global__ void __launch_bounds__(SS_THREADS) state_space_step_kernel(const __gr
     __shared__ __align__(16) float bs[COLS], cs[COLS];
     __shared__ float xs[ROWS], ys[ROWS];
     __shared__ uint32_t last;
+    pdl_launch_dependents();
+    pdl_wait();
     const uint32_t tid = threadIdx.x, lane = tid & 31u, part = tid % L, P = a.head_dim, N = a.state_size, slices = (P + ROWS - 1) / ROWS;
     const uint32_t row = blockIdx.y, h = blockIdx.x / slices, p0 = blockIdx.x % slices * ROWS, per_group = a.heads / a.groups, g = h / per_group;
     const uint32_t* slots = reinterpret_cast<const uint32_t*>(a.slots);
@@ -382,7 +386,9 @@ uzu_status uzu_state_space_scan_validate(const uzu_state_space_scan_args* a) {
     return e ? fail(UZU_ERROR_INVALID_ARGUMENT, std::string("state_space_scan: ") + e) : UZU_OK;
 }
 
-size_t uzu_state_space_scan_scratch_bytes(uzu_context* ctx, const uzu_state_space_scan_args* a) { return 0; }
+size_t uzu_state_space_scan_scratch_bytes(uzu_context* ctx, const uzu_state_space_scan_args* a) {
+    return ctx && a && a->sequences && ss_data_type(a->data_type) && a->heads && a->groups && scan_umma_applicable(*a) ? scan_umma_scratch_bytes(ctx, *a) : 0;
+}
 
 void uzu_state_space_scan_encode(uzu_command_buffer* cmd, const uzu_state_space_scan_args* a) {
     if (!encodable(cmd, "state_space_scan")) return;
@@ -390,6 +396,8 @@ void uzu_state_space_scan_encode(uzu_command_buffer* cmd, const uzu_state_space_
         cmd->record_error(UZU_ERROR_INVALID_ARGUMENT, std::string("state_space_scan: ") + e);
         return;
     }
+    if (a->sequence_count == 0) return;
+    if (scan_umma_applicable(*a) && encode_scan_umma(cmd, *a)) return;
     ScanParams p{};
     p.a = *a;
     for (uint32_t begin = 0; begin < a->sequence_count;) {

@@ -1,0 +1,575 @@
+// The selective state space scan of prompts on the 5th-generation tensor cores, in chunks of 128 tokens. With L_t the sum of step a up to token t of the chunk (log2):
+//   y_i = sum_(j <= i) 2^(L_i - L_j) step_j (c_i . b_j) x_j  +  2^(L_i) S c_i  +  d x_i,      S' = 2^(L_end) S + sum_j 2^(L_end - L_j) step_j x_j b_j^T
+// A CTA walks one sequence (or a part of it) for 64 rows of one head:
+//   copy     x, b and c of a chunk by TMA, two stages
+//   steps    one warp: step sizes, sums of logarithms from the front and from the end (each accurate where its weights are not small)
+//   scores   c b^T out of tensor memory, times 2^(L_i - L_j) step_j, back as bf16 operand A. Below the diagonal's 32 x 32 blocks the factor is a product of a row's and
+//            a column's, both relative to the row block's start, so that neither overflows (decays are at most 1) and no exponential is taken per element.
+//   state    x times its weight as two bf16 parts (16 bits: the state keeps what f32 sums need) for the state's sum, the state in registers, f32, its bf16 copy as operand
+//   output   the two sums, d x and the gate
+//   issue    scores c b^T (128 x 128), their product with x (64), c S (64), b^T [x hi | x lo] (128 columns, both parts at one reading of b)
+// Rows past the sequence's end are zeroed in shared memory (what another sequence or nobody left there may be no number).
+// An input x that is not finite is taken out of the product with the scores, where its zero weights would make NaN of earlier tokens; rows from it on become NaN.
+// Few heads: a sequence is cut into parts; a first pass leaves each part's state from zero (the first's from its start), a second one starts from the sums of those.
+// Every barrier wait is bounded (wait_errors.h).
+#include "state_space.cuh"
+#include "umma.cuh"
+
+namespace uzu {
+
+namespace {
+
+constexpr uint32_t SU_Q = 128, SU_P = 64, SU_THREADS = 480, SU_BLOCK = SU_Q * 128;      // tokens of a chunk, rows of the state, bytes of 64 columns of a chunk
+constexpr uint32_t SU_STAGE = 5 * SU_BLOCK, SU_WX = 2 * SU_STAGE, SU_S = SU_WX + 2 * SU_BLOCK;
+constexpr size_t SU_SMEM = SU_S + SU_BLOCK + 1024;
+// tensor memory
+constexpr uint32_t SU_G = 0, SU_SCORES = 128, SU_YI = 192, SU_YX = 256, SU_U = 320, SU_COLUMNS = 512;
+
+struct ScanUmmaParams {
+    uzu_state_space_scan_args a;
+    unsigned int* error;
+    float* ends;       // of the parts: [tile][head][64 rows][state_size]
+    float* logs;       // [tile][head]
+    SequenceTable table;
+};
+
+__device__ __forceinline__ float su_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float2 su_mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return d;
+}
+__device__ __forceinline__ uint4 su_lds(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void su_sts(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+}  // namespace
+
+// N: state_size, 64 or 128. STATE: only the state at the end of every part but the last
+template <int N, bool STATE>
+__global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c, const __grid_constant__ ScanUmmaParams p) {
+    extern __shared__ uint8_t su_raw[];
+    __shared__ __align__(8) uint64_t bars[18];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile uint32_t gave_up;
+    __shared__ __align__(16) float steps[2][SU_Q], front[2][SU_Q], back[2][SU_Q];      // [stage][token]: step, log2 of the decays up to it, behind it
+    __shared__ __align__(16) float column[4][96];                                      // of a warp of scores: step_j 2^(L_ref - L_j)
+    __shared__ uint32_t odd_rows[2][4];                                                // rows with an x that is not finite
+    const uzu_state_space_scan_args& a = p.a;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const uint32_t base = (um_smem(su_raw) + 1023u) & ~1023u, bar0 = um_smem(bars);
+    auto x_full = [&](uint32_t s) { return bar0 + 8u * s; };
+    auto x_empty = [&](uint32_t s) { return bar0 + 8u * (2 + s); };
+    auto d_full = [&](uint32_t s) { return bar0 + 8u * (4 + s); };
+    auto d_empty = [&](uint32_t s) { return bar0 + 8u * (6 + s); };
+    auto o_full = [&](uint32_t s) { return bar0 + 8u * (16 + s); };      // odd_rows
+    const uint32_t g_full = bar0 + 64, g_empty = bar0 + 72, p_full = bar0 + 80, w_full = bar0 + 88, s_full = bar0 + 96, y_full = bar0 + 104, y_empty = bar0 + 112, u_full = bar0 + 120;
+    __shared__ __align__(8) uint64_t last_bar;
+    const uint32_t last_products = um_smem(&last_bar);
+
+    const uint32_t slices = a.head_dim / SU_P, h = blockIdx.x / slices, slice = blockIdx.x % slices, group = h / (a.heads / a.groups);
+    const uint32_t tile = blockIdx.y, q = ss_find(p.table, tile);
+    const PackedSequence s_ = p.table.s[q];
+    const uint32_t parts = (q + 1 < p.table.count ? p.table.s[q + 1].tile0 : p.table.tiles) - s_.tile0, part = tile - s_.tile0;
+    const uint32_t all = (s_.rows + SU_Q - 1) / SU_Q, per = (all + parts - 1) / parts, chunk0 = min(all, part * per), chunks = min(all, chunk0 + per) - chunk0;
+    if (STATE && part + 1 == parts) return;
+    const uint32_t row0 = s_.first + chunk0 * SU_Q, rows = min(s_.rows - chunk0 * SU_Q, chunks * SU_Q);      // of this CTA (chunk0 * SU_Q <= rows + 127; 0 chunks: not used)
+
+    if (warp == 0) {
+        if (lane == 0) {
+            for (uint32_t s = 0; s < 2; ++s) {
+                um_init(x_full(s), 1); um_init(x_empty(s), STATE ? 1 : 5); um_init(d_full(s), 1); um_init(d_empty(s), STATE ? 4 : 12); um_init(o_full(s), 4);
+            }
+            um_init(g_full, 1); um_init(g_empty, 4); um_init(p_full, 4); um_init(w_full, 4); um_init(s_full, 4); um_init(y_full, 1); um_init(y_empty, 4); um_init(u_full, 1);
+            um_init(last_products, 1);
+            gave_up = 0;
+            um_fence_init();
+        }
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(um_smem(&tmem_slot)), "r"(SU_COLUMNS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    um_fence_before();
+    __syncthreads();
+    um_fence_after();
+    const uint32_t tmem = tmem_slot, lanes = (warp & 3u) << 21;
+    pdl_launch_dependents();
+    pdl_wait();
+    bool ok = true;
+
+    if (warp < 4) {
+        // ================================ scores ================================
+        if (!STATE) {
+            const uint32_t w = warp;
+            uint32_t zero[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) zero[i] = 0;
+            for (uint32_t jb = w + 1; jb < 4; ++jb) um_st16(tmem + lanes + SU_SCORES + jb * 16, zero);      // tokens behind the row's: once for all chunks
+            um_wait_st();
+            for (uint32_t c = 0; c < chunks; ++c) {
+                const uint32_t s = c & 1u;
+                ok = um_wait(d_full(s), c >> 1 & 1u, &gave_up, p.error, 0x701u);
+                if (!ok) break;
+                const float mine = front[s][tid], ref = w ? front[s][32 * w - 1] : 0.0f;
+                for (uint32_t jb = 0; jb < w; ++jb) column[w][jb * 32 + lane] = steps[s][jb * 32 + lane] * su_exp2(ref - front[s][jb * 32 + lane]);
+                __syncwarp();
+                const float r = su_exp2(mine - ref);
+                ok = um_wait(g_full, c & 1u, &gave_up, p.error, 0x702u);
+                if (ok && c) ok = um_wait(y_full, (c - 1) & 1u, &gave_up, p.error, 0x703u);      // the scores before are read
+                if (!ok) break;
+                um_fence_after();
+                const float2 r2 = make_float2(r, r);
+#pragma unroll 1
+                for (uint32_t jb = 0; jb < w; ++jb) {
+                    uint32_t v[32], o[16];
+                    um_ld32(tmem + lanes + SU_G + jb * 32, v);
+                    um_wait_ld(v);
+#pragma unroll
+                    for (uint32_t j = 0; j < 32; j += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(&column[w][jb * 32 + j]);
+                        const float2 e0 = su_mul2(su_mul2(make_float2(f.x, f.y), r2), make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])));
+                        const float2 e1 = su_mul2(su_mul2(make_float2(f.z, f.w), r2), make_float2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])));
+                        o[j / 2] = um_pack(e0.x, e0.y);
+                        o[j / 2 + 1] = um_pack(e1.x, e1.y);
+                    }
+                    um_st16(tmem + lanes + SU_SCORES + jb * 16, o);
+                }
+                {
+                    uint32_t v[32], o[16];
+                    um_ld32(tmem + lanes + SU_G + w * 32, v);
+                    um_wait_ld(v);
+                    um_fence_before();
+                    um_arrive(g_empty);
+#pragma unroll
+                    for (uint32_t j = 0; j < 32; j += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(&front[s][w * 32 + j]), st = *reinterpret_cast<const float4*>(&steps[s][w * 32 + j]);
+                        const float e[4] = {st.x * su_exp2(mine - f.x), st.y * su_exp2(mine - f.y), st.z * su_exp2(mine - f.z), st.w * su_exp2(mine - f.w)};
+                        float t[4];
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) t[i] = j + i <= lane ? e[i] * __uint_as_float(v[j + i]) : 0.0f;
+                        o[j / 2] = um_pack(t[0], t[1]);
+                        o[j / 2 + 1] = um_pack(t[2], t[3]);
+                    }
+                    um_st16(tmem + lanes + SU_SCORES + w * 16, o);
+                }
+                um_wait_st();
+                um_fence_before();
+                um_arrive(p_full);
+                um_arrive(d_empty(s));
+            }
+        }
+    } else if (warp < 8) {
+        // ================================ state ================================
+        const uint32_t t = tid - 128, n = t, heads = a.heads * slices;
+        const size_t at = (((size_t)s_.slot() * a.heads + h) * a.head_dim + slice * SU_P) * N + n;
+        float* slot = reinterpret_cast<float*>(a.state) + at;
+        auto end_of = [&](uint32_t k) { return p.ends + ((size_t)(s_.tile0 + k) * heads + blockIdx.x) * SU_P * N + n; };      // (the last part's place: a copy of the start)
+        float S[SU_P];
+#pragma unroll
+        for (uint32_t i = 0; i < SU_P; ++i) S[i] = 0.0f;
+        if (n < N) {
+            if (STATE) {
+                if (part == 0) {
+                    float* copy = end_of(parts - 1);
+#pragma unroll
+                    for (uint32_t i = 0; i < SU_P; ++i) {
+                        if (!s_.fresh()) S[i] = slot[i * N];
+                        copy[i * N] = S[i];
+                    }
+                }
+            } else if (parts == 1) {
+                if (!s_.fresh()) {
+#pragma unroll
+                    for (uint32_t i = 0; i < SU_P; ++i) S[i] = slot[i * N];
+                }
+            } else if (part == 0) {
+                const float* copy = end_of(parts - 1);
+#pragma unroll
+                for (uint32_t i = 0; i < SU_P; ++i) S[i] = copy[i * N];
+            } else {
+                for (uint32_t k = 0; k < part; ++k) {      // the parts before, in order
+                    const float f = k ? su_exp2(p.logs[(size_t)(s_.tile0 + k) * heads + blockIdx.x]) : 0.0f;
+                    const float* end = end_of(k);
+#pragma unroll
+                    for (uint32_t i = 0; i < SU_P; ++i) S[i] = k ? fmaf(f, S[i], end[i * N]) : end[i * N];
+                }
+            }
+        }
+        auto store = [&]() {      // row n of the operand: its 64 rows of the state
+            if (!STATE) {
+                if (n < N) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i)
+                        su_sts(base + SU_S + n * 128 + ((i ^ (n & 7u)) << 4), um_pack(S[8 * i], S[8 * i + 1]), um_pack(S[8 * i + 2], S[8 * i + 3]), um_pack(S[8 * i + 4], S[8 * i + 5]), um_pack(S[8 * i + 6], S[8 * i + 7]));
+                }
+                um_fence_proxy();
+                um_arrive(s_full);
+            }
+        };
+        if (chunks) store();
+        float total = 0.0f;
+        for (uint32_t c = 0; c < chunks; ++c) {
+            const uint32_t s = c & 1u, x0 = base + s * SU_STAGE, b0 = x0 + SU_BLOCK, valid = min(SU_Q, rows - c * SU_Q);
+            ok = um_wait(d_full(s), c >> 1 & 1u, &gave_up, p.error, 0x704u);
+            if (ok) ok = um_wait(x_full(s), c >> 1 & 1u, &gave_up, p.error, 0x705u);
+            if (!ok) break;
+            // (the products that read the parts of chunk c - 1 are done: u_full was waited for)
+            const float weight = steps[s][t] * su_exp2(back[s][t]), end = front[s][SU_Q - 1];
+            const float2 w2 = make_float2(weight, weight);
+            total += end;
+            bool odd = false;
+            if (t < valid) {
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) {
+                    const uint32_t o = t * 128 + ((i ^ (t & 7u)) << 4);
+                    const uint4 v = su_lds(x0 + o);
+                    const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) {
+                        odd |= (in[k] & 0x7f80u) == 0x7f80u || (in[k] & 0x7f800000u) == 0x7f800000u;
+                        const float2 y = su_mul2(make_float2(um_lo(in[k]), um_hi(in[k])), w2);
+                        hi[k] = um_pack(y.x, y.y);
+                        lo[k] = um_pack(y.x - um_lo(hi[k]), y.y - um_hi(hi[k]));
+                    }
+                    su_sts(base + SU_WX + o, hi[0], hi[1], hi[2], hi[3]);
+                    su_sts(base + SU_WX + SU_BLOCK + o, lo[0], lo[1], lo[2], lo[3]);
+                }
+                if (odd) {      // not finite: not in the product with the scores
+                    for (uint32_t i = 0; i < 8; ++i) {
+                        const uint32_t o = x0 + t * 128 + ((i ^ (t & 7u)) << 4);
+                        const uint4 v = su_lds(o);
+                        uint32_t in[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k) {
+                            if ((in[k] & 0x7f80u) == 0x7f80u) in[k] &= 0xffff0000u;
+                            if ((in[k] & 0x7f800000u) == 0x7f800000u) in[k] &= 0xffffu;
+                        }
+                        su_sts(o, in[0], in[1], in[2], in[3]);
+                    }
+                }
+            } else {            // behind the sequence
+                for (uint32_t i = 0; i < 8; ++i) {
+                    const uint32_t o = t * 128 + (i << 4);
+                    su_sts(x0 + o, 0, 0, 0, 0);
+                    su_sts(b0 + o, 0, 0, 0, 0);
+                    if (N == 128) su_sts(b0 + SU_BLOCK + o, 0, 0, 0, 0);
+                    su_sts(base + SU_WX + o, 0, 0, 0, 0);
+                    su_sts(base + SU_WX + SU_BLOCK + o, 0, 0, 0, 0);
+                }
+            }
+            const uint32_t odds = __ballot_sync(0xffffffffu, odd);
+            if (lane == 0) odd_rows[s][warp - 4] = odds;
+            um_fence_proxy();
+            um_arrive(w_full);
+            um_arrive(o_full(s));
+            um_arrive(d_empty(s));
+
+            const float f = su_exp2(end);
+            ok = um_wait(u_full, c & 1u, &gave_up, p.error, 0x706u);
+            if (!ok) break;
+            um_fence_after();
+#pragma unroll
+            for (uint32_t i = 0; i < SU_P; ++i) S[i] *= f;
+#pragma unroll
+            for (uint32_t half = 0; half < 4; ++half) {
+                uint32_t v[32];
+                um_ld32(tmem + lanes + SU_U + half * 32, v);
+                um_wait_ld(v);
+#pragma unroll
+                for (uint32_t j = 0; j < 32; ++j) S[(half & 1u) * 32 + j] += __uint_as_float(v[j]);
+            }
+            um_fence_before();
+            if (c + 1 < chunks) {
+                if (!STATE) ok = um_wait(y_full, c & 1u, &gave_up, p.error, 0x707u);      // the operand before is read
+                if (!ok) break;
+                store();
+            }
+        }
+        if (ok && n < N) {
+            float* to = STATE ? end_of(part) : slot;
+            if ((STATE || part + 1 == parts) && (chunks || s_.fresh())) {
+#pragma unroll
+                for (uint32_t i = 0; i < SU_P; ++i) to[i * N] = S[i];
+            }
+            if (STATE && n == 0) p.logs[(size_t)tile * heads + blockIdx.x] = total;
+        }
+    } else if (warp < 12) {
+        // ================================ output ================================
+        if (!STATE) {
+            const uint32_t t = tid - 256, c0 = h * a.head_dim + slice * SU_P;
+            const float skip = a.d ? reinterpret_cast<const float*>(a.d)[h] : 0.0f;
+            const bool gated = a.z != 0;
+            const __nv_bfloat16* z = reinterpret_cast<const __nv_bfloat16*>(a.z) + (size_t)row0 * a.z_stride + c0;
+            __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)row0 * a.out_stride + c0;
+            for (uint32_t c = 0; c < chunks; ++c) {
+                const uint32_t s = c & 1u, x0 = base + s * SU_STAGE, valid = min(SU_Q, rows - c * SU_Q), r = c * SU_Q + t;
+                uint4 zv[8], xv[8];
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) zv[i] = gated && t < valid ? *reinterpret_cast<const uint4*>(z + (size_t)r * a.z_stride + 8 * i) : make_uint4(0, 0, 0, 0);
+                ok = um_wait(x_full(s), c >> 1 & 1u, &gave_up, p.error, 0x708u);
+                if (!ok) break;
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) xv[i] = su_lds(x0 + t * 128 + ((i ^ (t & 7u)) << 4));
+                um_arrive(x_empty(s));
+                ok = um_wait(d_full(s), c >> 1 & 1u, &gave_up, p.error, 0x709u);
+                if (ok) ok = um_wait(o_full(s), c >> 1 & 1u, &gave_up, p.error, 0x70au);
+                if (ok) ok = um_wait(y_full, c & 1u, &gave_up, p.error, 0x70bu);
+                if (!ok) break;
+                um_fence_after();
+                const float f = su_exp2(front[s][t]);
+                const uint32_t odd = odd_rows[s][0] | odd_rows[s][1] | odd_rows[s][2] | odd_rows[s][3];
+#pragma unroll
+                for (uint32_t half = 0; half < 2; ++half) {
+                    uint32_t vi[32], vx[32];
+                    um_ld32(tmem + lanes + SU_YI + half * 32, vi);
+                    um_ld32(tmem + lanes + SU_YX + half * 32, vx);
+                    um_wait_ld(vi);
+                    um_wait_ld(vx);
+                    if (half == 1) {
+                        um_fence_before();
+                        um_arrive(y_empty);
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        const uint4 xx = xv[half * 4 + i], zz = zv[half * 4 + i];
+                        const uint32_t xs[4] = {xx.x, xx.y, xx.z, xx.w}, zs[4] = {zz.x, zz.y, zz.z, zz.w};
+                        float y[8];
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k) {
+                            const uint32_t j = i * 8 + 2 * k;
+                            y[2 * k] = fmaf(skip, um_lo(xs[k]), fmaf(f, __uint_as_float(vx[j]), __uint_as_float(vi[j])));
+                            y[2 * k + 1] = fmaf(skip, um_hi(xs[k]), fmaf(f, __uint_as_float(vx[j + 1]), __uint_as_float(vi[j + 1])));
+                            if (gated) {
+                                y[2 * k] *= ss_silu(um_lo(zs[k]));
+                                y[2 * k + 1] *= ss_silu(um_hi(zs[k]));
+                            }
+                        }
+                        if (odd) {      // columns whose x was not finite at this token or before it in the chunk
+                            const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x) + (size_t)(row0 + c * SU_Q) * a.x_stride + c0 + half * 32 + i * 8;
+                            for (uint32_t j = 0; j <= t; ++j)
+                                if (odd_rows[s][j >> 5] >> (j & 31u) & 1u) {
+#pragma unroll
+                                    for (uint32_t k = 0; k < 8; ++k)
+                                        if (!(fabsf(__bfloat162float(x[(size_t)j * a.x_stride + k])) < INFINITY)) y[k] = __int_as_float(0x7fc00000);
+                                }
+                        }
+                        if (t < valid)
+                            *reinterpret_cast<uint4*>(out + (size_t)r * a.out_stride + half * 32 + i * 8) = make_uint4(um_pack(y[0], y[1]), um_pack(y[2], y[3]), um_pack(y[4], y[5]), um_pack(y[6], y[7]));
+                    }
+                }
+                um_arrive(d_empty(s));
+            }
+        }
+    } else if (warp == 12) {
+        // ================================ x, b and c by TMA ================================
+        uint32_t asked = 0;
+        for (uint32_t c = 0; c < chunks; ++c) {
+            const uint32_t s = c & 1u, x0 = base + s * SU_STAGE;
+            ok = um_wait(x_empty(s), (c >> 1 & 1u) ^ 1u, &gave_up, p.error, 0x70cu);
+            if (!ok) break;
+            if (um_elect()) {
+                const uint32_t row = row0 + c * SU_Q;
+                um_expect(x_full(s), SU_BLOCK * (1 + (STATE ? 1 : 2) * (N / 64)));
+                um_tma(x0, &map_x, h * a.head_dim + slice * SU_P, row, x_full(s));
+                for (uint32_t i = 0; i < N / 64; ++i) {
+                    um_tma(x0 + SU_BLOCK * (1 + i), &map_b, group * N + i * 64, row, x_full(s));
+                    if (!STATE) um_tma(x0 + SU_BLOCK * (3 + i), &map_c, group * N + i * 64, row, x_full(s));
+                }
+            }
+            __syncwarp();
+            ++asked;
+        }
+        if (!ok)      // copies that are on their way end before the CTA does
+            for (uint32_t n = 1; n <= 2 && n <= asked; ++n) um_settle(x_full((asked - n) & 1u), (asked - n) >> 1 & 1u);
+    } else if (warp == 13) {
+        // ================================ products ================================
+        // shared-memory descriptors: 128-byte swizzle, 1024 bytes between groups of 8 rows, SU_BLOCK between blocks of 64 columns
+        constexpr uint64_t desc = (uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32, k_major = desc | (1u << 16), wide = desc | ((uint64_t)(SU_BLOCK >> 4) << 16);
+        constexpr uint32_t common = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24), a_wide = 1u << 15, b_wide = 1u << 16;
+        constexpr uint32_t i_scores = common | ((128u >> 3) << 17), i_y = common | b_wide | ((64u >> 3) << 17), i_u = common | a_wide | b_wide | ((128u >> 3) << 17);
+        auto scores = [&](uint32_t c) {
+            const uint32_t s = c & 1u, b0 = base + s * SU_STAGE + SU_BLOCK, c0 = b0 + 2 * SU_BLOCK;
+            ok = um_wait(x_full(s), c >> 1 & 1u, &gave_up, p.error, 0x70du);
+            if (ok && c) ok = um_wait(g_empty, (c - 1) & 1u, &gave_up, p.error, 0x70eu);
+            if (!ok) return;
+            um_fence_after();
+            if (um_elect()) {
+#pragma unroll
+                for (uint32_t kk = 0; kk < N / 16; ++kk) {
+                    const uint32_t o = (kk >> 2) * SU_BLOCK + (kk & 3u) * 32u;
+                    um_mma_ss(tmem + SU_G, k_major | ((c0 + o) >> 4), k_major | ((b0 + o) >> 4), i_scores, kk != 0);
+                }
+                um_commit(g_full);
+            }
+            __syncwarp();
+        };
+        if (!STATE && chunks) scores(0);
+        for (uint32_t c = 0; c < chunks && ok; ++c) {
+            const uint32_t s = c & 1u, x0 = base + s * SU_STAGE, b0 = x0 + SU_BLOCK, c0 = b0 + 2 * SU_BLOCK;
+            if (!STATE) {
+                if (c + 1 < chunks) scores(c + 1);
+                if (ok) ok = um_wait(p_full, c & 1u, &gave_up, p.error, 0x70fu);
+                if (ok) ok = um_wait(s_full, c & 1u, &gave_up, p.error, 0x710u);
+                if (ok && c) ok = um_wait(y_empty, (c - 1) & 1u, &gave_up, p.error, 0x711u);
+            } else if (ok) ok = um_wait(x_full(s), c >> 1 & 1u, &gave_up, p.error, 0x712u);
+            if (ok) ok = um_wait(w_full, c & 1u, &gave_up, p.error, 0x713u);
+            if (!ok) break;
+            um_fence_after();
+            if (um_elect()) {
+                if (!STATE) {
+#pragma unroll
+                    for (uint32_t kk = 0; kk < SU_Q / 16; ++kk) um_mma_ts(tmem + SU_YI, tmem + SU_SCORES + kk * 8u, wide | ((x0 + kk * 2048u) >> 4), i_y, kk != 0);
+#pragma unroll
+                    for (uint32_t kk = 0; kk < N / 16; ++kk)
+                        um_mma_ss(tmem + SU_YX, k_major | ((c0 + (kk >> 2) * SU_BLOCK + (kk & 3u) * 32u) >> 4), wide | ((base + SU_S + kk * 2048u) >> 4), i_y, kk != 0);
+                    um_commit(y_full);
+                }
+                // (64 columns: operand A's second block is whatever lies behind; the sums' lanes 64 .. 127 are not read)
+#pragma unroll
+                for (uint32_t kk = 0; kk < SU_Q / 16; ++kk) um_mma_ss(tmem + SU_U, wide | ((b0 + kk * 2048u) >> 4), wide | ((base + SU_WX + kk * 2048u) >> 4), i_u, kk != 0);
+                um_commit(u_full);
+                um_commit(x_empty(s));
+            }
+            __syncwarp();
+        }
+        if (!ok) {
+            if (um_elect()) um_commit(last_products);
+            __syncwarp();
+            um_settle(last_products, 0);                                 // none in flight when tensor memory is given back
+        }
+    } else {
+        // ================================ steps: four tokens a lane ================================
+        const float rate = reinterpret_cast<const float*>(a.a)[h] * 1.4426950408889634f, bias = a.dt_bias ? reinterpret_cast<const float*>(a.dt_bias)[h] : 0.0f;
+        const __nv_bfloat16* dt = reinterpret_cast<const __nv_bfloat16*>(a.dt) + (size_t)row0 * a.dt_stride + h;
+        __nv_bfloat16 next[4];
+        auto fetch = [&](uint32_t c) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint32_t r = c * SU_Q + 4 * lane + i;
+                next[i] = r < rows ? dt[(size_t)r * a.dt_stride] : __float2bfloat16_rn(0.0f);
+            }
+        };
+        if (chunks) fetch(0);
+        for (uint32_t c = 0; c < chunks; ++c) {
+            const uint32_t s = c & 1u;
+            float step[4], l[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const bool there = c * SU_Q + 4 * lane + i < rows;
+                step[i] = there ? ss_step(__bfloat162float(next[i]), bias, a.dt_softplus, a.dt_min, a.dt_max) : 0.0f;
+                l[i] = there ? step[i] * rate : 0.0f;
+                l[i] = l[i] < -256.0f ? -256.0f : l[i];      // (nothing is left of a state then; sums stay fine)
+            }
+            if (c + 1 < chunks) fetch(c + 1);
+            const float f0 = l[0], f1 = f0 + l[1], f2 = f1 + l[2], f3 = f2 + l[3], b2 = l[3], b1 = b2 + l[2], b0 = b1 + l[1];
+            float up = f3, down = b0 + l[0];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const float u = __shfl_up_sync(0xffffffffu, up, o), d = __shfl_down_sync(0xffffffffu, down, o);
+                if (lane >= o) up += u;
+                if (lane + o < 32) down += d;
+            }
+            float before = __shfl_up_sync(0xffffffffu, up, 1), behind = __shfl_down_sync(0xffffffffu, down, 1);
+            if (lane == 0) before = 0.0f;
+            if (lane == 31) behind = 0.0f;
+            ok = um_wait(d_empty(s), (c >> 1 & 1u) ^ 1u, &gave_up, p.error, 0x714u);
+            if (!ok) break;
+            *reinterpret_cast<float4*>(&steps[s][4 * lane]) = make_float4(step[0], step[1], step[2], step[3]);
+            *reinterpret_cast<float4*>(&front[s][4 * lane]) = make_float4(before + f0, before + f1, before + f2, before + f3);
+            *reinterpret_cast<float4*>(&back[s][4 * lane]) = make_float4(behind + b0, behind + b1, behind + b2, behind);
+            um_arrive(d_full(s));
+        }
+    }
+
+    __syncthreads();
+    um_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        um_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(SU_COLUMNS) : "memory");
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------------------------------------
+// how many parts a sequence of `chunks` chunks is cut into, where `ctas` CTAs would run without cutting: two passes cost 1.6 times the one, so three parts pay and two do not
+static uint32_t su_parts(uint32_t chunks, uint64_t ctas, uint32_t sms) {
+    const uint64_t room = sms / std::max<uint64_t>(1, ctas);
+    if (room < 3 || chunks < 8) return 1;
+    const uint32_t want = (uint32_t)std::min<uint64_t>(room, chunks / 2), per = (chunks + want - 1) / want;
+    return (chunks + per - 1) / per;
+}
+static uint64_t su_ctas(const uzu_state_space_scan_args& a) { return (uint64_t)a.sequence_count * a.heads * (a.head_dim / SU_P); }
+static uint64_t su_tiles(const uzu_state_space_scan_args& a, uint32_t sms) {
+    uint64_t n = 0;
+    for (uint32_t i = 0; i < a.sequence_count; ++i) n += su_parts((uint32_t)(((uint64_t)a.sequences[i].rows + SU_Q - 1) / SU_Q), su_ctas(a), sms);
+    return n;
+}
+
+// shapes, types and alignment (of arguments that scan_check takes)
+bool scan_umma_applicable(const uzu_state_space_scan_args& a) {
+    return a.data_type == UZU_DT_BF16 && a.head_dim % SU_P == 0 && (a.state_size == 64 || a.state_size == 128) && ((a.x | a.b | a.c | a.z | a.out) & 15u) == 0 && a.x_stride % 8 == 0 && a.b_stride % 8 == 0 &&
+           a.c_stride % 8 == 0 && (a.z == 0 || a.z_stride % 8 == 0) && a.out_stride % 8 == 0 && um_encoder() != nullptr;
+}
+
+size_t scan_umma_scratch_bytes(const uzu_context* ctx, const uzu_state_space_scan_args& a) {
+    const uint64_t tiles = su_tiles(a, ctx->sm_count), heads = (uint64_t)a.heads * (a.head_dim / SU_P);
+    return tiles == a.sequence_count ? 0 : tiles * heads * (SU_P * a.state_size + 4) * 4;
+}
+
+template <int N, bool STATE>
+static void su_launch(uzu_command_buffer* cmd, const CUtensorMap& mx, const CUtensorMap& mb, const CUtensorMap& mc, const ScanUmmaParams& p) {
+    static std::atomic<uint64_t> opted{0};
+    opt_in_dynamic_smem(cmd, scan_umma_kernel<N, STATE>, (int)SU_SMEM, opted);
+    launch(cmd, "scan_umma_kernel", scan_umma_kernel<N, STATE>, dim3(p.a.heads * (p.a.head_dim / SU_P), p.table.tiles), dim3(SU_THREADS), SU_SMEM, mx, mb, mc, p);
+}
+
+bool encode_scan_umma(uzu_command_buffer* cmd, const uzu_state_space_scan_args& a) {
+    CUtensorMap mx, mb, mc;
+    if (!um_map(&mx, a.x, (uint64_t)a.heads * a.head_dim, a.rows, a.x_stride, SU_Q) || !um_map(&mb, a.b, (uint64_t)a.groups * a.state_size, a.rows, a.b_stride, SU_Q) ||
+        !um_map(&mc, a.c, (uint64_t)a.groups * a.state_size, a.rows, a.c_stride, SU_Q))
+        return false;
+    // the longest first: the last CTAs to start are short ones
+    std::vector<uzu_row_sequence> order;
+    try {
+        order.assign(a.sequences, a.sequences + a.sequence_count);
+        std::sort(order.begin(), order.end(), [](const uzu_row_sequence& x, const uzu_row_sequence& y) { return x.rows != y.rows ? x.rows > y.rows : x.slot < y.slot; });
+    } catch (const std::bad_alloc&) {
+        cmd->record_error(UZU_ERROR_OUT_OF_MEMORY, "state_space_scan: out of host memory");
+        return true;
+    }
+    const uint32_t sms = cmd->ctx->sm_count;
+    const size_t need = scan_umma_scratch_bytes(cmd->ctx, a);
+    const bool cut = need && a.scratch && a.scratch_bytes >= need;
+    const uint64_t heads = (uint64_t)a.heads * (a.head_dim / SU_P);
+    ScanUmmaParams p{};
+    p.a = a;
+    p.error = cmd->ctx->wait_errors.device_word;
+    for (uint32_t begin = 0; begin < a.sequence_count;) {
+        begin = fill_sequences(p.table, order.data(), a.sequence_count, begin, [&](uint32_t rows) { return cut ? su_parts((uint32_t)(((uint64_t)rows + SU_Q - 1) / SU_Q), su_ctas(a), sms) : 1u; });
+        // (one launch behind the other: the next may use the same scratch)
+        p.ends = reinterpret_cast<float*>(a.scratch);
+        p.logs = p.ends + (uint64_t)p.table.tiles * heads * SU_P * a.state_size;
+        if (a.state_size == 128) {
+            if (p.table.tiles > p.table.count) su_launch<128, true>(cmd, mx, mb, mc, p);
+            su_launch<128, false>(cmd, mx, mb, mc, p);
+        } else {
+            if (p.table.tiles > p.table.count) su_launch<64, true>(cmd, mx, mb, mc, p);
+            su_launch<64, false>(cmd, mx, mb, mc, p);
+        }
+    }
+    return true;
+}
+
+}  // namespace uzu
