@@ -56,11 +56,6 @@ __device__ __forceinline__ void xl_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint4 xl_lds(uint32_t at) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
-    return v;
-}
 __device__ __forceinline__ float xl_x(const uzu_expert_layer_args& a, uint32_t t, uint32_t c) {
     return a.data_type == UZU_DT_F32 ? reinterpret_cast<const float*>(a.x)[(size_t)t * a.x_stride + c] : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.x)[(size_t)t * a.x_stride + c]);
 }
@@ -343,13 +338,17 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
             }
             if (ok) ok = um_wait(full(s), it / S::STAGES & 1u, &gave_up, p.error, 0x603u);
             if (!ok) return;
+            uint32_t seen = 0;
             if (there) {
                 const uint32_t box = ring + s * XL_STAGE + warp * XL_BOX + g * 128;
                 uint4 w[2][4];
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) w[i][q] = xl_lds(box + q * 1024 + (((2 * t4 + i) ^ g) << 4));
+                    for (int q = 0; q < 4; ++q) {
+                        w[i][q] = um_lds(box + q * 1024 + (((2 * t4 + i) ^ g) << 4));
+                        seen ^= w[i][q].x;
+                    }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     if (!(live >> n & 1u)) continue;
@@ -368,7 +367,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
                         }
                 }
             }
-            um_arrive(empty(s));
+            um_arrive_after(empty(s), seen, a.reserved0);
             ++it;
         };
         auto meet = [&]() {
@@ -546,6 +545,7 @@ void uzu_expert_layer_encode(uzu_command_buffer* cmd, const uzu_expert_layer_arg
     if (a->rows == 0) return;
     XlParams p{};
     p.a = *a;
+    p.a.reserved0 = 0;      // (um_arrive_after)
     p.s = xl_scratch(*a);
     p.error = cmd->ctx->wait_errors.device_word;
     CUtensorMap up, down;

@@ -43,11 +43,6 @@ __device__ __forceinline__ float2 su_mul2(float2 a, float2 b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
     return d;
 }
-__device__ __forceinline__ uint4 su_lds(uint32_t at) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-    return v;
-}
 __device__ __forceinline__ void su_sts(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
@@ -63,7 +58,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
     __shared__ volatile uint32_t gave_up;
     __shared__ __align__(16) float steps[2][SU_Q], front[2][SU_Q], back[2][SU_Q];      // [stage][token]: step, log2 of the decays up to it, behind it
     __shared__ __align__(16) float column[4][96];                                      // of a warp of scores: step_j 2^(L_ref - L_j)
-    __shared__ uint32_t odd_rows[2][4];                                                // rows with an x that is not finite
+    __shared__ volatile uint32_t odd_rows[2][4];                                              // rows with an x that is not finite
     const uzu_state_space_scan_args& a = p.a;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const uint32_t base = (um_smem(su_raw) + 1023u) & ~1023u, bar0 = um_smem(bars);
@@ -119,8 +114,8 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                 const uint32_t s = c & 1u;
                 ok = um_wait(d_full(s), c >> 1 & 1u, &gave_up, p.error, 0x701u);
                 if (!ok) break;
-                const float mine = front[s][tid], ref = w ? front[s][32 * w - 1] : 0.0f;
-                for (uint32_t jb = 0; jb < w; ++jb) column[w][jb * 32 + lane] = steps[s][jb * 32 + lane] * su_exp2(ref - front[s][jb * 32 + lane]);
+                const float mine = um_ldf(&front[s][tid]), ref = w ? um_ldf(&front[s][32 * w - 1]) : 0.0f;
+                for (uint32_t jb = 0; jb < w; ++jb) column[w][jb * 32 + lane] = um_ldf(&steps[s][jb * 32 + lane]) * su_exp2(ref - um_ldf(&front[s][jb * 32 + lane]));
                 __syncwarp();
                 const float r = su_exp2(mine - ref);
                 ok = um_wait(g_full, c & 1u, &gave_up, p.error, 0x702u);
@@ -132,7 +127,6 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                 for (uint32_t jb = 0; jb < w; ++jb) {
                     uint32_t v[32], o[16];
                     um_ld32(tmem + lanes + SU_G + jb * 32, v);
-                    um_wait_ld(v);
 #pragma unroll
                     for (uint32_t j = 0; j < 32; j += 4) {
                         const float4 f = *reinterpret_cast<const float4*>(&column[w][jb * 32 + j]);
@@ -146,12 +140,11 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                 {
                     uint32_t v[32], o[16];
                     um_ld32(tmem + lanes + SU_G + w * 32, v);
-                    um_wait_ld(v);
                     um_fence_before();
                     um_arrive(g_empty);
 #pragma unroll
                     for (uint32_t j = 0; j < 32; j += 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(&front[s][w * 32 + j]), st = *reinterpret_cast<const float4*>(&steps[s][w * 32 + j]);
+                        const float4 f = um_ldf4(&front[s][w * 32 + j]), st = um_ldf4(&steps[s][w * 32 + j]);
                         const float e[4] = {st.x * su_exp2(mine - f.x), st.y * su_exp2(mine - f.y), st.z * su_exp2(mine - f.z), st.w * su_exp2(mine - f.w)};
                         float t[4];
 #pragma unroll
@@ -223,7 +216,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             if (ok) ok = um_wait(x_full(s), c >> 1 & 1u, &gave_up, p.error, 0x705u);
             if (!ok) break;
             // (the products that read the parts of chunk c - 1 are done: u_full was waited for)
-            const float weight = steps[s][t] * su_exp2(back[s][t]), end = front[s][SU_Q - 1];
+            const float weight = um_ldf(&steps[s][t]) * su_exp2(um_ldf(&back[s][t])), end = um_ldf(&front[s][SU_Q - 1]);
             const float2 w2 = make_float2(weight, weight);
             total += end;
             bool odd = false;
@@ -231,7 +224,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i) {
                     const uint32_t o = t * 128 + ((i ^ (t & 7u)) << 4);
-                    const uint4 v = su_lds(x0 + o);
+                    const uint4 v = um_lds(x0 + o);
                     const uint32_t in[4] = {v.x, v.y, v.z, v.w};
                     uint32_t hi[4], lo[4];
 #pragma unroll
@@ -247,7 +240,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                 if (odd) {      // not finite: not in the product with the scores
                     for (uint32_t i = 0; i < 8; ++i) {
                         const uint32_t o = x0 + t * 128 + ((i ^ (t & 7u)) << 4);
-                        const uint4 v = su_lds(o);
+                        const uint4 v = um_lds(o);
                         uint32_t in[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                         for (uint32_t k = 0; k < 4; ++k) {
@@ -284,7 +277,6 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             for (uint32_t half = 0; half < 4; ++half) {
                 uint32_t v[32];
                 um_ld32(tmem + lanes + SU_U + half * 32, v);
-                um_wait_ld(v);
 #pragma unroll
                 for (uint32_t j = 0; j < 32; ++j) S[(half & 1u) * 32 + j] += __uint_as_float(v[j]);
             }
@@ -319,22 +311,19 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                 ok = um_wait(x_full(s), c >> 1 & 1u, &gave_up, p.error, 0x708u);
                 if (!ok) break;
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) xv[i] = su_lds(x0 + t * 128 + ((i ^ (t & 7u)) << 4));
-                um_arrive(x_empty(s));
+                for (uint32_t i = 0; i < 8; ++i) xv[i] = um_lds(x0 + t * 128 + ((i ^ (t & 7u)) << 4));
+                um_arrive_after(x_empty(s), (xv[0].x ^ xv[1].x) ^ (xv[2].x ^ xv[3].x) ^ (xv[4].x ^ xv[5].x) ^ (xv[6].x ^ xv[7].x), a.reserved0);
                 ok = um_wait(d_full(s), c >> 1 & 1u, &gave_up, p.error, 0x709u);
                 if (ok) ok = um_wait(o_full(s), c >> 1 & 1u, &gave_up, p.error, 0x70au);
                 if (ok) ok = um_wait(y_full, c & 1u, &gave_up, p.error, 0x70bu);
                 if (!ok) break;
                 um_fence_after();
-                const float f = su_exp2(front[s][t]);
+                const float f = su_exp2(um_ldf(&front[s][t]));
                 const uint32_t odd = odd_rows[s][0] | odd_rows[s][1] | odd_rows[s][2] | odd_rows[s][3];
 #pragma unroll
                 for (uint32_t half = 0; half < 2; ++half) {
                     uint32_t vi[32], vx[32];
-                    um_ld32(tmem + lanes + SU_YI + half * 32, vi);
-                    um_ld32(tmem + lanes + SU_YX + half * 32, vx);
-                    um_wait_ld(vi);
-                    um_wait_ld(vx);
+                    um_ld32x2(tmem + lanes + SU_YI + half * 32, tmem + lanes + SU_YX + half * 32, vi, vx);
                     if (half == 1) {
                         um_fence_before();
                         um_arrive(y_empty);
@@ -555,6 +544,7 @@ bool encode_scan_umma(uzu_command_buffer* cmd, const uzu_state_space_scan_args& 
     const uint64_t heads = (uint64_t)a.heads * (a.head_dim / SU_P);
     ScanUmmaParams p{};
     p.a = a;
+    p.a.reserved0 = 0;      // (um_arrive_after)
     p.error = cmd->ctx->wait_errors.device_word;
     for (uint32_t begin = 0; begin < a.sequence_count;) {
         begin = fill_sequences(p.table, order.data(), a.sequence_count, begin, [&](uint32_t rows) { return cut ? su_parts((uint32_t)(((uint64_t)rows + SU_Q - 1) / SU_Q), su_ctas(a), sms) : 1u; });

@@ -17,6 +17,24 @@ __device__ __forceinline__ void um_arrive(uint32_t bar) {
     __syncwarp();
     if ((threadIdx.x & 31u) == 0) asm volatile("{ .reg .b64 st; mbarrier.arrive.shared::cta.b64 st, [%0]; }" ::"r"(bar) : "memory");
 }
+// ... once what was loaded into `seen` is there. An arrival takes another way than loads from shared memory and does not wait for them: behind many global accesses
+// they came back after the place had been given away (rows of x two chunks on were found). `zero` is 0, which the compiler does not know: the barrier's address then
+// depends on the loads, and a warp issues in order.
+__device__ __forceinline__ void um_arrive_after(uint32_t bar, uint32_t seen, uint32_t zero) {
+    __syncwarp();
+    if ((threadIdx.x & 31u) == 0) asm volatile("{ .reg .b64 st; mbarrier.arrive.shared::cta.b64 st, [%0]; }" ::"r"(bar + (seen & zero)) : "memory");
+}
+__device__ __forceinline__ uint4 um_lds(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.volatile.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 um_ldf4(const float* p) {
+    float4 v;
+    asm volatile("ld.volatile.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(um_smem(p)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float um_ldf(const float* p) { return *reinterpret_cast<const volatile float*>(p); }
 __device__ __forceinline__ bool um_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }" : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
@@ -70,27 +88,35 @@ __device__ __forceinline__ void um_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
 __device__ __forceinline__ void um_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void um_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void um_fence_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// 32 columns of the warp's lanes. The wait is part of it: between a load and its wait the registers hold nothing, and the compiler may move or spill what it takes for a value.
 __device__ __forceinline__ void um_ld32(uint32_t taddr, uint32_t (&v)[32]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-          "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]),
-          "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(taddr)
+        : "memory");
+}
+// twice 32 columns under way together
+__device__ __forceinline__ void um_ld32x2(uint32_t taddr0, uint32_t taddr1, uint32_t (&v0)[32], uint32_t (&v1)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n\ttcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=&r"(v0[0]), "=&r"(v0[1]), "=&r"(v0[2]), "=&r"(v0[3]), "=&r"(v0[4]), "=&r"(v0[5]), "=&r"(v0[6]), "=&r"(v0[7]),
+          "=&r"(v0[8]), "=&r"(v0[9]), "=&r"(v0[10]), "=&r"(v0[11]), "=&r"(v0[12]), "=&r"(v0[13]), "=&r"(v0[14]), "=&r"(v0[15]),
+          "=&r"(v0[16]), "=&r"(v0[17]), "=&r"(v0[18]), "=&r"(v0[19]), "=&r"(v0[20]), "=&r"(v0[21]), "=&r"(v0[22]), "=&r"(v0[23]),
+          "=&r"(v0[24]), "=&r"(v0[25]), "=&r"(v0[26]), "=&r"(v0[27]), "=&r"(v0[28]), "=&r"(v0[29]), "=&r"(v0[30]), "=&r"(v0[31]),
+          "=&r"(v1[0]), "=&r"(v1[1]), "=&r"(v1[2]), "=&r"(v1[3]), "=&r"(v1[4]), "=&r"(v1[5]), "=&r"(v1[6]), "=&r"(v1[7]),
+          "=&r"(v1[8]), "=&r"(v1[9]), "=&r"(v1[10]), "=&r"(v1[11]), "=&r"(v1[12]), "=&r"(v1[13]), "=&r"(v1[14]), "=&r"(v1[15]),
+          "=&r"(v1[16]), "=&r"(v1[17]), "=&r"(v1[18]), "=&r"(v1[19]), "=&r"(v1[20]), "=&r"(v1[21]), "=&r"(v1[22]), "=&r"(v1[23]),
+          "=&r"(v1[24]), "=&r"(v1[25]), "=&r"(v1[26]), "=&r"(v1[27]), "=&r"(v1[28]), "=&r"(v1[29]), "=&r"(v1[30]), "=&r"(v1[31])
+        : "r"(taddr0), "r"(taddr1)
         : "memory");
 }
 __device__ __forceinline__ void um_st16(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
                  "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-                 : "memory");
-}
-// nothing that uses what was asked for is done before the wait
-__device__ __forceinline__ void um_wait_ld(uint32_t (&v)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
-                   "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]),
-                   "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
-                 :
                  : "memory");
 }
 __device__ __forceinline__ void um_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
