@@ -19,7 +19,7 @@ namespace uzu {
 
 namespace {
 
-constexpr uint32_t SU_Q = 128, SU_P = 64, SU_THREADS = 480, SU_BLOCK = SU_Q * 128;      // tokens of a chunk, rows of the state, bytes of 64 columns of a chunk
+constexpr uint32_t SU_Q = 128, SU_P = 64, SU_THREADS = 27 * 32, SU_BLOCK = SU_Q * 128;      // tokens of a chunk, rows of the state, bytes of 64 columns of a chunk
 constexpr uint32_t SU_STAGE = 5 * SU_BLOCK, SU_WX = 2 * SU_STAGE, SU_S = SU_WX + 2 * SU_BLOCK;
 constexpr size_t SU_SMEM = SU_S + SU_BLOCK + 1024;
 // tensor memory
@@ -43,6 +43,11 @@ __device__ __forceinline__ float2 su_mul2(float2 a, float2 b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
     return d;
 }
+__device__ __forceinline__ float2 su_fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+    return d;
+}
 __device__ __forceinline__ void su_sts(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
@@ -51,25 +56,30 @@ __device__ __forceinline__ void su_sts(uint32_t at, uint32_t x, uint32_t y, uint
 
 // N: state_size, 64 or 128. STATE: only the state at the end of every part but the last
 template <int N, bool STATE>
-__global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c, const __grid_constant__ ScanUmmaParams p) {
+__global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c,
+                                                                  const __grid_constant__ CUtensorMap map_out, const __grid_constant__ ScanUmmaParams p) {
     extern __shared__ uint8_t su_raw[];
-    __shared__ __align__(8) uint64_t bars[18];
+    __shared__ __align__(8) uint64_t bars[41];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t gave_up;
-    __shared__ __align__(16) float steps[2][SU_Q], front[2][SU_Q], back[2][SU_Q];      // [stage][token]: step, log2 of the decays up to it, behind it
-    __shared__ __align__(16) float column[4][96];                                      // of a warp of scores: step_j 2^(L_ref - L_j)
-    __shared__ volatile uint32_t odd_rows[2][4];                                              // rows with an x that is not finite
+    __shared__ __align__(16) float steps[4][SU_Q], front[4][SU_Q], back[4][SU_Q];      // [chunk & 3][token]: step, log2 of the decays up to it, behind it
+    __shared__ __align__(16) float column[4][96];                                      // of a row block of scores: step_j 2^(L_ref - L_j)
+    __shared__ volatile uint32_t odd_rows[4][8];                                       // [chunk & 3][half, row block]: rows with an x that is not finite
     const uzu_state_space_scan_args& a = p.a;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const uint32_t base = (um_smem(su_raw) + 1023u) & ~1023u, bar0 = um_smem(bars);
-    auto x_full = [&](uint32_t s) { return bar0 + 8u * s; };
-    auto x_empty = [&](uint32_t s) { return bar0 + 8u * (2 + s); };
-    auto d_full = [&](uint32_t s) { return bar0 + 8u * (4 + s); };
-    auto d_empty = [&](uint32_t s) { return bar0 + 8u * (6 + s); };
-    auto o_full = [&](uint32_t s) { return bar0 + 8u * (16 + s); };      // odd_rows
-    const uint32_t g_full = bar0 + 64, g_empty = bar0 + 72, p_full = bar0 + 80, w_full = bar0 + 88, s_full = bar0 + 96, y_full = bar0 + 104, y_empty = bar0 + 112, u_full = bar0 + 120;
-    __shared__ __align__(8) uint64_t last_bar;
-    const uint32_t last_products = um_smem(&last_bar);
+    auto x_full = [&](uint32_t c) { return bar0 + 8u * (c & 1u); };
+    auto x_empty = [&](uint32_t c) { return bar0 + 8u * (2 + (c & 1u)); };
+    auto bc_full = [&](uint32_t c) { return bar0 + 8u * (4 + (c & 1u)); };
+    auto bc_empty = [&](uint32_t c) { return bar0 + 8u * (6 + (c & 1u)); };
+    auto d_full = [&](uint32_t c) { return bar0 + 8u * (8 + (c & 3u)); };
+    auto d_empty = [&](uint32_t c) { return bar0 + 8u * (12 + (c & 3u)); };
+    auto o_full = [&](uint32_t c) { return bar0 + 8u * (16 + (c & 3u)); };             // odd_rows
+    auto out_full = [&](uint32_t c, uint32_t block) { return bar0 + 8u * (20 + (c & 1u) * 4 + block); };      // both halves of 32 rows of output
+    const uint32_t g_full = bar0 + 8u * 28, g_empty = bar0 + 8u * 29, p_full = bar0 + 8u * 30, w_full = bar0 + 8u * 31, s_full = bar0 + 8u * 32, y_full = bar0 + 8u * 33, y_empty = bar0 + 8u * 34,
+                   u_full = bar0 + 8u * 35, last_products = bar0 + 8u * 36;
+    auto two = [](uint32_t c) { return c >> 1 & 1u; };      // parities of rings of two and four
+    auto four = [](uint32_t c) { return c >> 2 & 1u; };
 
     const uint32_t slices = a.head_dim / SU_P, h = blockIdx.x / slices, slice = blockIdx.x % slices, group = h / (a.heads / a.groups);
     const uint32_t tile = blockIdx.y, q = ss_find(p.table, tile);
@@ -77,14 +87,16 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
     const uint32_t parts = (q + 1 < p.table.count ? p.table.s[q + 1].tile0 : p.table.tiles) - s_.tile0, part = tile - s_.tile0;
     const uint32_t all = (s_.rows + SU_Q - 1) / SU_Q, per = (all + parts - 1) / parts, chunk0 = min(all, part * per), chunks = min(all, chunk0 + per) - chunk0;
     if (STATE && part + 1 == parts) return;
-    const uint32_t row0 = s_.first + chunk0 * SU_Q, rows = min(s_.rows - chunk0 * SU_Q, chunks * SU_Q);      // of this CTA (chunk0 * SU_Q <= rows + 127; 0 chunks: not used)
+    const uint32_t row0 = s_.first + chunk0 * SU_Q, rows = min(s_.rows - chunk0 * SU_Q, chunks * SU_Q), col0 = h * a.head_dim + slice * SU_P;      // of this CTA
 
     if (warp == 0) {
         if (lane == 0) {
             for (uint32_t s = 0; s < 2; ++s) {
-                um_init(x_full(s), 1); um_init(x_empty(s), STATE ? 1 : 5); um_init(d_full(s), 1); um_init(d_empty(s), STATE ? 4 : 12); um_init(o_full(s), 4);
+                um_init(x_full(s), 1); um_init(x_empty(s), STATE ? 1 : 4); um_init(bc_full(s), 1); um_init(bc_empty(s), 1);
+                for (uint32_t k = 0; k < 4; ++k) um_init(out_full(s, k), 2);
             }
-            um_init(g_full, 1); um_init(g_empty, 4); um_init(p_full, 4); um_init(w_full, 4); um_init(s_full, 4); um_init(y_full, 1); um_init(y_empty, 4); um_init(u_full, 1);
+            for (uint32_t s = 0; s < 4; ++s) { um_init(d_full(s), 1); um_init(d_empty(s), STATE ? 8 : 24); um_init(o_full(s), 8); }
+            um_init(g_full, 1); um_init(g_empty, 8); um_init(p_full, 8); um_init(w_full, 8); um_init(s_full, 8); um_init(y_full, 1); um_init(y_empty, 8); um_init(u_full, 1);
             um_init(last_products, 1);
             gave_up = 0;
             um_fence_init();
@@ -96,85 +108,87 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
     um_fence_before();
     __syncthreads();
     um_fence_after();
-    const uint32_t tmem = tmem_slot, lanes = (warp & 3u) << 21;
+    const uint32_t tmem = tmem_slot, w = warp & 3u, half = warp >> 2 & 1u, t = w * 32 + lane, lanes = w << 21;      // of the first 24 warps: block of 32 rows, which of its two warps
     pdl_launch_dependents();
     pdl_wait();
     bool ok = true;
 
-    if (warp < 4) {
+    if (warp < 8) {
         // ================================ scores ================================
         if (!STATE) {
-            const uint32_t w = warp;
-            uint32_t zero[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) zero[i] = 0;
-            for (uint32_t jb = w + 1; jb < 4; ++jb) um_st16(tmem + lanes + SU_SCORES + jb * 16, zero);      // tokens behind the row's: once for all chunks
-            um_wait_st();
+            // Blocks of 32 tokens up to the row block's own, the diagonal one: one warp has that and, of four, the one before it; the other one the rest.
+            const uint32_t own = w == 3 ? 2 : w, jb0 = half ? own : 0, jb1 = half ? w : own;      // off the diagonal
+            if (!half) {
+                const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                for (uint32_t k = 2 * (w + 1); k < 8; ++k) um_st8(tmem + lanes + SU_SCORES + k * 8, zero);      // tokens behind the row's: once for all chunks
+                um_wait_st();
+            }
             for (uint32_t c = 0; c < chunks; ++c) {
-                const uint32_t s = c & 1u;
-                ok = um_wait(d_full(s), c >> 1 & 1u, &gave_up, p.error, 0x701u);
+                const float *st = steps[c & 3u], *fr = front[c & 3u];
+                ok = um_wait(d_full(c), four(c), &gave_up, p.error, 0x701u);
                 if (!ok) break;
-                const float mine = um_ldf(&front[s][tid]), ref = w ? um_ldf(&front[s][32 * w - 1]) : 0.0f;
-                for (uint32_t jb = 0; jb < w; ++jb) column[w][jb * 32 + lane] = um_ldf(&steps[s][jb * 32 + lane]) * su_exp2(ref - um_ldf(&front[s][jb * 32 + lane]));
+                const float mine = um_ldf(&fr[t]), ref = w ? um_ldf(&fr[32 * w - 1]) : 0.0f;
+                for (uint32_t jb = jb0; jb < jb1; ++jb) column[w][jb * 32 + lane] = um_ldf(&st[jb * 32 + lane]) * su_exp2(ref - um_ldf(&fr[jb * 32 + lane]));
                 __syncwarp();
                 const float r = su_exp2(mine - ref);
+                const float2 r2 = make_float2(r, r);
                 ok = um_wait(g_full, c & 1u, &gave_up, p.error, 0x702u);
                 if (ok && c) ok = um_wait(y_full, (c - 1) & 1u, &gave_up, p.error, 0x703u);      // the scores before are read
                 if (!ok) break;
                 um_fence_after();
-                const float2 r2 = make_float2(r, r);
-#pragma unroll 1
-                for (uint32_t jb = 0; jb < w; ++jb) {
-                    uint32_t v[32], o[16];
-                    um_ld32(tmem + lanes + SU_G + jb * 32, v);
+                for (uint32_t k = 2 * jb0; k < 2 * jb1; ++k) {
+                    uint32_t v[16], o[8];
+                    um_ld16(tmem + lanes + SU_G + k * 16, v);
 #pragma unroll
-                    for (uint32_t j = 0; j < 32; j += 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(&column[w][jb * 32 + j]);
+                    for (uint32_t j = 0; j < 16; j += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(&column[w][k * 16 + j]);
                         const float2 e0 = su_mul2(su_mul2(make_float2(f.x, f.y), r2), make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])));
                         const float2 e1 = su_mul2(su_mul2(make_float2(f.z, f.w), r2), make_float2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])));
                         o[j / 2] = um_pack(e0.x, e0.y);
                         o[j / 2 + 1] = um_pack(e1.x, e1.y);
                     }
-                    um_st16(tmem + lanes + SU_SCORES + jb * 16, o);
+                    um_st8(tmem + lanes + SU_SCORES + k * 8, o);
                 }
-                {
-                    uint32_t v[32], o[16];
-                    um_ld32(tmem + lanes + SU_G + w * 32, v);
-                    um_fence_before();
-                    um_arrive(g_empty);
+                if (half) {
 #pragma unroll
-                    for (uint32_t j = 0; j < 32; j += 4) {
-                        const float4 f = um_ldf4(&front[s][w * 32 + j]), st = um_ldf4(&steps[s][w * 32 + j]);
-                        const float e[4] = {st.x * su_exp2(mine - f.x), st.y * su_exp2(mine - f.y), st.z * su_exp2(mine - f.z), st.w * su_exp2(mine - f.w)};
-                        float t[4];
+                    for (uint32_t k = 0; k < 2; ++k) {
+                        uint32_t v[16], o[8];
+                        um_ld16(tmem + lanes + SU_G + w * 32 + k * 16, v);
 #pragma unroll
-                        for (uint32_t i = 0; i < 4; ++i) t[i] = j + i <= lane ? e[i] * __uint_as_float(v[j + i]) : 0.0f;
-                        o[j / 2] = um_pack(t[0], t[1]);
-                        o[j / 2 + 1] = um_pack(t[2], t[3]);
+                        for (uint32_t j = 0; j < 16; j += 4) {
+                            const float4 f = um_ldf4(&fr[w * 32 + k * 16 + j]), sj = um_ldf4(&st[w * 32 + k * 16 + j]);
+                            const float e[4] = {sj.x * su_exp2(mine - f.x), sj.y * su_exp2(mine - f.y), sj.z * su_exp2(mine - f.z), sj.w * su_exp2(mine - f.w)};
+                            float x[4];
+#pragma unroll
+                            for (uint32_t i = 0; i < 4; ++i) x[i] = k * 16 + j + i <= lane ? e[i] * __uint_as_float(v[j + i]) : 0.0f;
+                            o[j / 2] = um_pack(x[0], x[1]);
+                            o[j / 2 + 1] = um_pack(x[2], x[3]);
+                        }
+                        um_st8(tmem + lanes + SU_SCORES + w * 16 + k * 8, o);
                     }
-                    um_st16(tmem + lanes + SU_SCORES + w * 16, o);
                 }
                 um_wait_st();
                 um_fence_before();
+                um_arrive(g_empty);
                 um_arrive(p_full);
-                um_arrive(d_empty(s));
+                um_arrive(d_empty(c));
             }
         }
-    } else if (warp < 8) {
-        // ================================ state ================================
-        const uint32_t t = tid - 128, n = t, heads = a.heads * slices;
-        const size_t at = (((size_t)s_.slot() * a.heads + h) * a.head_dim + slice * SU_P) * N + n;
+    } else if (warp < 16) {
+        // ================================ state: column n = t, rows [32 half, 32 half + 32) ================================
+        const uint32_t n = t, heads = a.heads * slices;
+        const size_t at = (((size_t)s_.slot() * a.heads + h) * a.head_dim + slice * SU_P + half * 32) * N + n;
         float* slot = reinterpret_cast<float*>(a.state) + at;
-        auto end_of = [&](uint32_t k) { return p.ends + ((size_t)(s_.tile0 + k) * heads + blockIdx.x) * SU_P * N + n; };      // (the last part's place: a copy of the start)
-        float S[SU_P];
+        auto end_of = [&](uint32_t k) { return p.ends + (((size_t)(s_.tile0 + k) * heads + blockIdx.x) * SU_P + half * 32) * N + n; };      // (the last part's place: a copy of the start)
+        float S[32];
 #pragma unroll
-        for (uint32_t i = 0; i < SU_P; ++i) S[i] = 0.0f;
+        for (uint32_t i = 0; i < 32; ++i) S[i] = 0.0f;
         if (n < N) {
             if (STATE) {
                 if (part == 0) {
                     float* copy = end_of(parts - 1);
 #pragma unroll
-                    for (uint32_t i = 0; i < SU_P; ++i) {
+                    for (uint32_t i = 0; i < 32; ++i) {
                         if (!s_.fresh()) S[i] = slot[i * N];
                         copy[i * N] = S[i];
                     }
@@ -182,27 +196,28 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             } else if (parts == 1) {
                 if (!s_.fresh()) {
 #pragma unroll
-                    for (uint32_t i = 0; i < SU_P; ++i) S[i] = slot[i * N];
+                    for (uint32_t i = 0; i < 32; ++i) S[i] = slot[i * N];
                 }
             } else if (part == 0) {
                 const float* copy = end_of(parts - 1);
 #pragma unroll
-                for (uint32_t i = 0; i < SU_P; ++i) S[i] = copy[i * N];
+                for (uint32_t i = 0; i < 32; ++i) S[i] = copy[i * N];
             } else {
                 for (uint32_t k = 0; k < part; ++k) {      // the parts before, in order
                     const float f = k ? su_exp2(p.logs[(size_t)(s_.tile0 + k) * heads + blockIdx.x]) : 0.0f;
                     const float* end = end_of(k);
 #pragma unroll
-                    for (uint32_t i = 0; i < SU_P; ++i) S[i] = k ? fmaf(f, S[i], end[i * N]) : end[i * N];
+                    for (uint32_t i = 0; i < 32; ++i) S[i] = k ? fmaf(f, S[i], end[i * N]) : end[i * N];
                 }
             }
         }
-        auto store = [&]() {      // row n of the operand: its 64 rows of the state
+        auto chunk_of = [&](uint32_t row, uint32_t i) { return row * 128 + (((half * 4 + i) ^ (row & 7u)) << 4); };      // 16 bytes of a swizzled row, of this warp's half
+        auto store = [&]() {      // row n of the operand: its rows of the state
             if (!STATE) {
                 if (n < N) {
 #pragma unroll
-                    for (uint32_t i = 0; i < 8; ++i)
-                        su_sts(base + SU_S + n * 128 + ((i ^ (n & 7u)) << 4), um_pack(S[8 * i], S[8 * i + 1]), um_pack(S[8 * i + 2], S[8 * i + 3]), um_pack(S[8 * i + 4], S[8 * i + 5]), um_pack(S[8 * i + 6], S[8 * i + 7]));
+                    for (uint32_t i = 0; i < 4; ++i)
+                        su_sts(base + SU_S + chunk_of(n, i), um_pack(S[8 * i], S[8 * i + 1]), um_pack(S[8 * i + 2], S[8 * i + 3]), um_pack(S[8 * i + 4], S[8 * i + 5]), um_pack(S[8 * i + 6], S[8 * i + 7]));
                 }
                 um_fence_proxy();
                 um_arrive(s_full);
@@ -211,74 +226,77 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
         if (chunks) store();
         float total = 0.0f;
         for (uint32_t c = 0; c < chunks; ++c) {
-            const uint32_t s = c & 1u, x0 = base + s * SU_STAGE, b0 = x0 + SU_BLOCK, valid = min(SU_Q, rows - c * SU_Q);
-            ok = um_wait(d_full(s), c >> 1 & 1u, &gave_up, p.error, 0x704u);
-            if (ok) ok = um_wait(x_full(s), c >> 1 & 1u, &gave_up, p.error, 0x705u);
+            const uint32_t x0 = base + (c & 1u) * SU_STAGE, b0 = x0 + SU_BLOCK, valid = min(SU_Q, rows - c * SU_Q);
+            ok = um_wait(d_full(c), four(c), &gave_up, p.error, 0x704u);
+            if (ok) ok = um_wait(x_full(c), two(c), &gave_up, p.error, 0x705u);
+            if (ok && valid < SU_Q) ok = um_wait(bc_full(c), two(c), &gave_up, p.error, 0x717u);      // (b's rows are there)
             if (!ok) break;
             // (the products that read the parts of chunk c - 1 are done: u_full was waited for)
-            const float weight = um_ldf(&steps[s][t]) * su_exp2(um_ldf(&back[s][t])), end = um_ldf(&front[s][SU_Q - 1]);
+            const float weight = um_ldf(&steps[c & 3u][t]) * su_exp2(um_ldf(&back[c & 3u][t])), end = um_ldf(&front[c & 3u][SU_Q - 1]);
             const float2 w2 = make_float2(weight, weight);
             total += end;
             bool odd = false;
             if (t < valid) {
+                uint4 in[4];
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) {
-                    const uint32_t o = t * 128 + ((i ^ (t & 7u)) << 4);
-                    const uint4 v = um_lds(x0 + o);
-                    const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+                for (uint32_t i = 0; i < 4; ++i) in[i] = um_lds(x0 + chunk_of(t, i));
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint32_t v[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
                     uint32_t hi[4], lo[4];
 #pragma unroll
                     for (uint32_t k = 0; k < 4; ++k) {
-                        odd |= (in[k] & 0x7f80u) == 0x7f80u || (in[k] & 0x7f800000u) == 0x7f800000u;
-                        const float2 y = su_mul2(make_float2(um_lo(in[k]), um_hi(in[k])), w2);
+                        odd |= (v[k] & 0x7f80u) == 0x7f80u || (v[k] & 0x7f800000u) == 0x7f800000u;
+                        const float2 y = su_mul2(make_float2(um_lo(v[k]), um_hi(v[k])), w2);
                         hi[k] = um_pack(y.x, y.y);
                         lo[k] = um_pack(y.x - um_lo(hi[k]), y.y - um_hi(hi[k]));
                     }
-                    su_sts(base + SU_WX + o, hi[0], hi[1], hi[2], hi[3]);
-                    su_sts(base + SU_WX + SU_BLOCK + o, lo[0], lo[1], lo[2], lo[3]);
+                    su_sts(base + SU_WX + chunk_of(t, i), hi[0], hi[1], hi[2], hi[3]);
+                    su_sts(base + SU_WX + SU_BLOCK + chunk_of(t, i), lo[0], lo[1], lo[2], lo[3]);
                 }
                 if (odd) {      // not finite: not in the product with the scores
-                    for (uint32_t i = 0; i < 8; ++i) {
-                        const uint32_t o = x0 + t * 128 + ((i ^ (t & 7u)) << 4);
-                        const uint4 v = um_lds(o);
-                        uint32_t in[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        uint32_t v[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
 #pragma unroll
                         for (uint32_t k = 0; k < 4; ++k) {
-                            if ((in[k] & 0x7f80u) == 0x7f80u) in[k] &= 0xffff0000u;
-                            if ((in[k] & 0x7f800000u) == 0x7f800000u) in[k] &= 0xffffu;
+                            if ((v[k] & 0x7f80u) == 0x7f80u) v[k] &= 0xffff0000u;
+                            if ((v[k] & 0x7f800000u) == 0x7f800000u) v[k] &= 0xffffu;
                         }
-                        su_sts(o, in[0], in[1], in[2], in[3]);
+                        su_sts(x0 + chunk_of(t, i), v[0], v[1], v[2], v[3]);
                     }
                 }
             } else {            // behind the sequence
-                for (uint32_t i = 0; i < 8; ++i) {
-                    const uint32_t o = t * 128 + (i << 4);
-                    su_sts(x0 + o, 0, 0, 0, 0);
-                    su_sts(b0 + o, 0, 0, 0, 0);
-                    if (N == 128) su_sts(b0 + SU_BLOCK + o, 0, 0, 0, 0);
-                    su_sts(base + SU_WX + o, 0, 0, 0, 0);
-                    su_sts(base + SU_WX + SU_BLOCK + o, 0, 0, 0, 0);
+                for (uint32_t i = 0; i < 4; ++i) {
+                    su_sts(x0 + chunk_of(t, i), 0, 0, 0, 0);
+                    su_sts(b0 + chunk_of(t, i), 0, 0, 0, 0);
+                    if (N == 128) su_sts(b0 + SU_BLOCK + chunk_of(t, i), 0, 0, 0, 0);
+                    su_sts(base + SU_WX + chunk_of(t, i), 0, 0, 0, 0);
+                    su_sts(base + SU_WX + SU_BLOCK + chunk_of(t, i), 0, 0, 0, 0);
                 }
             }
             const uint32_t odds = __ballot_sync(0xffffffffu, odd);
-            if (lane == 0) odd_rows[s][warp - 4] = odds;
+            if (lane == 0) odd_rows[c & 3u][warp - 8] = odds;
             um_fence_proxy();
             um_arrive(w_full);
-            um_arrive(o_full(s));
-            um_arrive(d_empty(s));
+            um_arrive(o_full(c));
+            um_arrive(d_empty(c));
 
             const float f = su_exp2(end);
+            const float2 f2 = make_float2(f, f);
             ok = um_wait(u_full, c & 1u, &gave_up, p.error, 0x706u);
             if (!ok) break;
             um_fence_after();
 #pragma unroll
-            for (uint32_t i = 0; i < SU_P; ++i) S[i] *= f;
+            for (uint32_t k = 0; k < 2; ++k) {
+                uint32_t hi[16], lo[16];
+                um_ld16x2(tmem + lanes + SU_U + half * 32 + k * 16, tmem + lanes + SU_U + 64 + half * 32 + k * 16, hi, lo);
 #pragma unroll
-            for (uint32_t half = 0; half < 4; ++half) {
-                uint32_t v[32];
-                um_ld32(tmem + lanes + SU_U + half * 32, v);
-#pragma unroll
-                for (uint32_t j = 0; j < 32; ++j) S[(half & 1u) * 32 + j] += __uint_as_float(v[j]);
+                for (uint32_t j = 0; j < 16; j += 2) {
+                    const float2 old = su_fma2(f2, make_float2(S[k * 16 + j], S[k * 16 + j + 1]), make_float2(__uint_as_float(hi[j]), __uint_as_float(hi[j + 1])));
+                    S[k * 16 + j] = old.x + __uint_as_float(lo[j]);
+                    S[k * 16 + j + 1] = old.y + __uint_as_float(lo[j + 1]);
+                }
             }
             um_fence_before();
             if (c + 1 < chunks) {
@@ -291,105 +309,127 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             float* to = STATE ? end_of(part) : slot;
             if ((STATE || part + 1 == parts) && (chunks || s_.fresh())) {
 #pragma unroll
-                for (uint32_t i = 0; i < SU_P; ++i) to[i * N] = S[i];
+                for (uint32_t i = 0; i < 32; ++i) to[i * N] = S[i];
             }
-            if (STATE && n == 0) p.logs[(size_t)tile * heads + blockIdx.x] = total;
+            if (STATE && n == 0 && half == 0) p.logs[(size_t)tile * heads + blockIdx.x] = total;
         }
-    } else if (warp < 12) {
-        // ================================ output ================================
+    } else if (warp < 24) {
+        // ================================ output: row t, columns [32 half, 32 half + 32) ================================
         if (!STATE) {
-            const uint32_t t = tid - 256, c0 = h * a.head_dim + slice * SU_P;
             const float skip = a.d ? reinterpret_cast<const float*>(a.d)[h] : 0.0f;
             const bool gated = a.z != 0;
-            const __nv_bfloat16* z = reinterpret_cast<const __nv_bfloat16*>(a.z) + (size_t)row0 * a.z_stride + c0;
-            __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)row0 * a.out_stride + c0;
+            const __nv_bfloat16* z = reinterpret_cast<const __nv_bfloat16*>(a.z) + (size_t)row0 * a.z_stride + col0 + half * 32;
+            __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)row0 * a.out_stride + col0 + half * 32;
             for (uint32_t c = 0; c < chunks; ++c) {
-                const uint32_t s = c & 1u, x0 = base + s * SU_STAGE, valid = min(SU_Q, rows - c * SU_Q), r = c * SU_Q + t;
-                uint4 zv[8], xv[8];
+                const uint32_t x0 = base + (c & 1u) * SU_STAGE, valid = min(SU_Q, rows - c * SU_Q), r = c * SU_Q + t;
+                const bool whole = w * 32 + 32 <= valid;      // all rows of the block are the sequence's
+                uint4 zv[4];
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) zv[i] = gated && t < valid ? *reinterpret_cast<const uint4*>(z + (size_t)r * a.z_stride + 8 * i) : make_uint4(0, 0, 0, 0);
-                ok = um_wait(x_full(s), c >> 1 & 1u, &gave_up, p.error, 0x708u);
-                if (!ok) break;
-#pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) xv[i] = um_lds(x0 + t * 128 + ((i ^ (t & 7u)) << 4));
-                um_arrive_after(x_empty(s), (xv[0].x ^ xv[1].x) ^ (xv[2].x ^ xv[3].x) ^ (xv[4].x ^ xv[5].x) ^ (xv[6].x ^ xv[7].x), a.reserved0);
-                ok = um_wait(d_full(s), c >> 1 & 1u, &gave_up, p.error, 0x709u);
-                if (ok) ok = um_wait(o_full(s), c >> 1 & 1u, &gave_up, p.error, 0x70au);
+                for (uint32_t i = 0; i < 4; ++i) zv[i] = gated && t < valid ? *reinterpret_cast<const uint4*>(z + (size_t)r * a.z_stride + 8 * i) : make_uint4(0, 0, 0, 0);
+                if (c && half == 0) {      // the rows stored from x's place a chunk ago are read: x may come there
+                    um_store_read();
+                    um_arrive(x_empty(c - 1));
+                }
+                ok = um_wait(x_full(c), two(c), &gave_up, p.error, 0x708u);
+                if (ok) ok = um_wait(d_full(c), four(c), &gave_up, p.error, 0x709u);
+                if (ok) ok = um_wait(o_full(c), four(c), &gave_up, p.error, 0x70au);
                 if (ok) ok = um_wait(y_full, c & 1u, &gave_up, p.error, 0x70bu);
                 if (!ok) break;
                 um_fence_after();
-                const float f = su_exp2(um_ldf(&front[s][t]));
-                const uint32_t odd = odd_rows[s][0] | odd_rows[s][1] | odd_rows[s][2] | odd_rows[s][3];
+                const float f = su_exp2(um_ldf(&front[c & 3u][t]));
+                uint32_t odd = 0;
 #pragma unroll
-                for (uint32_t half = 0; half < 2; ++half) {
-                    uint32_t vi[32], vx[32];
-                    um_ld32x2(tmem + lanes + SU_YI + half * 32, tmem + lanes + SU_YX + half * 32, vi, vx);
-                    if (half == 1) {
+                for (uint32_t i = 0; i < 4; ++i) odd |= odd_rows[c & 3u][half * 4 + i];
+#pragma unroll
+                for (uint32_t k = 0; k < 2; ++k) {
+                    uint32_t vi[16], vx[16];
+                    um_ld16x2(tmem + lanes + SU_YI + half * 32 + k * 16, tmem + lanes + SU_YX + half * 32 + k * 16, vi, vx);
+                    if (k == 1) {
                         um_fence_before();
                         um_arrive(y_empty);
                     }
 #pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
-                        const uint4 xx = xv[half * 4 + i], zz = zv[half * 4 + i];
+                    for (uint32_t i = 0; i < 2; ++i) {
+                        const uint32_t chunk = x0 + t * 128 + (((half * 4 + k * 2 + i) ^ (t & 7u)) << 4);
+                        const uint4 xx = um_lds(chunk), zz = zv[k * 2 + i];
                         const uint32_t xs[4] = {xx.x, xx.y, xx.z, xx.w}, zs[4] = {zz.x, zz.y, zz.z, zz.w};
                         float y[8];
 #pragma unroll
-                        for (uint32_t k = 0; k < 4; ++k) {
-                            const uint32_t j = i * 8 + 2 * k;
-                            y[2 * k] = fmaf(skip, um_lo(xs[k]), fmaf(f, __uint_as_float(vx[j]), __uint_as_float(vi[j])));
-                            y[2 * k + 1] = fmaf(skip, um_hi(xs[k]), fmaf(f, __uint_as_float(vx[j + 1]), __uint_as_float(vi[j + 1])));
+                        for (uint32_t e = 0; e < 4; ++e) {
+                            const uint32_t j = i * 8 + 2 * e;
+                            y[2 * e] = fmaf(skip, um_lo(xs[e]), fmaf(f, __uint_as_float(vx[j]), __uint_as_float(vi[j])));
+                            y[2 * e + 1] = fmaf(skip, um_hi(xs[e]), fmaf(f, __uint_as_float(vx[j + 1]), __uint_as_float(vi[j + 1])));
                             if (gated) {
-                                y[2 * k] *= ss_silu(um_lo(zs[k]));
-                                y[2 * k + 1] *= ss_silu(um_hi(zs[k]));
+                                y[2 * e] *= ss_silu(um_lo(zs[e]));
+                                y[2 * e + 1] *= ss_silu(um_hi(zs[e]));
                             }
                         }
                         if (odd) {      // columns whose x was not finite at this token or before it in the chunk
-                            const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x) + (size_t)(row0 + c * SU_Q) * a.x_stride + c0 + half * 32 + i * 8;
+                            const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x) + (size_t)(row0 + c * SU_Q) * a.x_stride + col0 + half * 32 + k * 16 + i * 8;
                             for (uint32_t j = 0; j <= t; ++j)
-                                if (odd_rows[s][j >> 5] >> (j & 31u) & 1u) {
+                                if (odd_rows[c & 3u][half * 4 + (j >> 5)] >> (j & 31u) & 1u) {
 #pragma unroll
-                                    for (uint32_t k = 0; k < 8; ++k)
-                                        if (!(fabsf(__bfloat162float(x[(size_t)j * a.x_stride + k])) < INFINITY)) y[k] = __int_as_float(0x7fc00000);
+                                    for (uint32_t e = 0; e < 8; ++e)
+                                        if (!(fabsf(__bfloat162float(x[(size_t)j * a.x_stride + e])) < INFINITY)) y[e] = __int_as_float(0x7fc00000);
                                 }
                         }
-                        if (t < valid)
-                            *reinterpret_cast<uint4*>(out + (size_t)r * a.out_stride + half * 32 + i * 8) = make_uint4(um_pack(y[0], y[1]), um_pack(y[2], y[3]), um_pack(y[4], y[5]), um_pack(y[6], y[7]));
+                        const uint4 o = make_uint4(um_pack(y[0], y[1]), um_pack(y[2], y[3]), um_pack(y[4], y[5]), um_pack(y[6], y[7]));
+                        if (whole) su_sts(chunk, o.x, o.y, o.z, o.w);      // over x, which nobody needs any more
+                        else if (t < valid) *reinterpret_cast<uint4*>(out + (size_t)r * a.out_stride + k * 16 + i * 8) = o;
                     }
                 }
-                um_arrive(d_empty(s));
+                if (whole) um_fence_proxy();
+                um_arrive(out_full(c, w));
+                um_arrive(d_empty(c));
+                if (half == 0) {
+                    ok = um_wait(out_full(c, w), two(c), &gave_up, p.error, 0x70cu);
+                    if (!ok) break;
+                    if (whole && lane == 0) um_tma_store(&map_out, x0 + w * 4096, col0, row0 + c * SU_Q + w * 32);
+                    __syncwarp();
+                }
             }
+            um_store_done();
         }
-    } else if (warp == 12) {
+    } else if (warp == 24) {
         // ================================ x, b and c by TMA ================================
-        uint32_t asked = 0;
+        uint32_t asked = 0, asked_x = 0;
         for (uint32_t c = 0; c < chunks; ++c) {
-            const uint32_t s = c & 1u, x0 = base + s * SU_STAGE;
-            ok = um_wait(x_empty(s), (c >> 1 & 1u) ^ 1u, &gave_up, p.error, 0x70cu);
+            const uint32_t x0 = base + (c & 1u) * SU_STAGE, row = row0 + c * SU_Q;
+            ok = um_wait(bc_empty(c), two(c) ^ 1u, &gave_up, p.error, 0x70du);
             if (!ok) break;
             if (um_elect()) {
-                const uint32_t row = row0 + c * SU_Q;
-                um_expect(x_full(s), SU_BLOCK * (1 + (STATE ? 1 : 2) * (N / 64)));
-                um_tma(x0, &map_x, h * a.head_dim + slice * SU_P, row, x_full(s));
+                um_expect(bc_full(c), SU_BLOCK * (STATE ? 1 : 2) * (N / 64));
                 for (uint32_t i = 0; i < N / 64; ++i) {
-                    um_tma(x0 + SU_BLOCK * (1 + i), &map_b, group * N + i * 64, row, x_full(s));
-                    if (!STATE) um_tma(x0 + SU_BLOCK * (3 + i), &map_c, group * N + i * 64, row, x_full(s));
+                    um_tma(x0 + SU_BLOCK * (1 + i), &map_b, group * N + i * 64, row, bc_full(c));
+                    if (!STATE) um_tma(x0 + SU_BLOCK * (3 + i), &map_c, group * N + i * 64, row, bc_full(c));
                 }
             }
             __syncwarp();
             ++asked;
+            ok = um_wait(x_empty(c), two(c) ^ 1u, &gave_up, p.error, 0x70eu);
+            if (!ok) break;
+            if (um_elect()) {
+                um_expect(x_full(c), SU_BLOCK);
+                um_tma(x0, &map_x, col0, row, x_full(c));
+            }
+            __syncwarp();
+            ++asked_x;
         }
         if (!ok)      // copies that are on their way end before the CTA does
-            for (uint32_t n = 1; n <= 2 && n <= asked; ++n) um_settle(x_full((asked - n) & 1u), (asked - n) >> 1 & 1u);
-    } else if (warp == 13) {
+            for (uint32_t n = 1; n <= 2; ++n) {
+                if (n <= asked) um_settle(bc_full(asked - n), two(asked - n));
+                if (n <= asked_x) um_settle(x_full(asked_x - n), two(asked_x - n));
+            }
+    } else if (warp == 25) {
         // ================================ products ================================
         // shared-memory descriptors: 128-byte swizzle, 1024 bytes between groups of 8 rows, SU_BLOCK between blocks of 64 columns
         constexpr uint64_t desc = (uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32, k_major = desc | (1u << 16), wide = desc | ((uint64_t)(SU_BLOCK >> 4) << 16);
         constexpr uint32_t common = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24), a_wide = 1u << 15, b_wide = 1u << 16;
         constexpr uint32_t i_scores = common | ((128u >> 3) << 17), i_y = common | b_wide | ((64u >> 3) << 17), i_u = common | a_wide | b_wide | ((128u >> 3) << 17);
         auto scores = [&](uint32_t c) {
-            const uint32_t s = c & 1u, b0 = base + s * SU_STAGE + SU_BLOCK, c0 = b0 + 2 * SU_BLOCK;
-            ok = um_wait(x_full(s), c >> 1 & 1u, &gave_up, p.error, 0x70du);
-            if (ok && c) ok = um_wait(g_empty, (c - 1) & 1u, &gave_up, p.error, 0x70eu);
+            const uint32_t b0 = base + (c & 1u) * SU_STAGE + SU_BLOCK, c0 = b0 + 2 * SU_BLOCK;
+            ok = um_wait(bc_full(c), two(c), &gave_up, p.error, 0x70fu);
+            if (ok && c) ok = um_wait(g_empty, (c - 1) & 1u, &gave_up, p.error, 0x710u);
             if (!ok) return;
             um_fence_after();
             if (um_elect()) {
@@ -404,14 +444,14 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
         };
         if (!STATE && chunks) scores(0);
         for (uint32_t c = 0; c < chunks && ok; ++c) {
-            const uint32_t s = c & 1u, x0 = base + s * SU_STAGE, b0 = x0 + SU_BLOCK, c0 = b0 + 2 * SU_BLOCK;
+            const uint32_t x0 = base + (c & 1u) * SU_STAGE, b0 = x0 + SU_BLOCK, c0 = b0 + 2 * SU_BLOCK;
             if (!STATE) {
                 if (c + 1 < chunks) scores(c + 1);
-                if (ok) ok = um_wait(p_full, c & 1u, &gave_up, p.error, 0x70fu);
-                if (ok) ok = um_wait(s_full, c & 1u, &gave_up, p.error, 0x710u);
-                if (ok && c) ok = um_wait(y_empty, (c - 1) & 1u, &gave_up, p.error, 0x711u);
-            } else if (ok) ok = um_wait(x_full(s), c >> 1 & 1u, &gave_up, p.error, 0x712u);
-            if (ok) ok = um_wait(w_full, c & 1u, &gave_up, p.error, 0x713u);
+                if (ok) ok = um_wait(p_full, c & 1u, &gave_up, p.error, 0x711u);
+                if (ok) ok = um_wait(s_full, c & 1u, &gave_up, p.error, 0x712u);
+                if (ok && c) ok = um_wait(y_empty, (c - 1) & 1u, &gave_up, p.error, 0x713u);
+            } else if (ok) ok = um_wait(bc_full(c), two(c), &gave_up, p.error, 0x714u);
+            if (ok) ok = um_wait(w_full, c & 1u, &gave_up, p.error, 0x715u);
             if (!ok) break;
             um_fence_after();
             if (um_elect()) {
@@ -427,7 +467,8 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
 #pragma unroll
                 for (uint32_t kk = 0; kk < SU_Q / 16; ++kk) um_mma_ss(tmem + SU_U, wide | ((b0 + kk * 2048u) >> 4), wide | ((base + SU_WX + kk * 2048u) >> 4), i_u, kk != 0);
                 um_commit(u_full);
-                um_commit(x_empty(s));
+                um_commit(bc_empty(c));
+                if (STATE) um_commit(x_empty(c));
             }
             __syncwarp();
         }
@@ -450,7 +491,6 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
         };
         if (chunks) fetch(0);
         for (uint32_t c = 0; c < chunks; ++c) {
-            const uint32_t s = c & 1u;
             float step[4], l[4];
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
@@ -471,12 +511,12 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             float before = __shfl_up_sync(0xffffffffu, up, 1), behind = __shfl_down_sync(0xffffffffu, down, 1);
             if (lane == 0) before = 0.0f;
             if (lane == 31) behind = 0.0f;
-            ok = um_wait(d_empty(s), (c >> 1 & 1u) ^ 1u, &gave_up, p.error, 0x714u);
+            ok = um_wait(d_empty(c), four(c) ^ 1u, &gave_up, p.error, 0x716u);
             if (!ok) break;
-            *reinterpret_cast<float4*>(&steps[s][4 * lane]) = make_float4(step[0], step[1], step[2], step[3]);
-            *reinterpret_cast<float4*>(&front[s][4 * lane]) = make_float4(before + f0, before + f1, before + f2, before + f3);
-            *reinterpret_cast<float4*>(&back[s][4 * lane]) = make_float4(behind + b0, behind + b1, behind + b2, behind);
-            um_arrive(d_full(s));
+            *reinterpret_cast<float4*>(&steps[c & 3u][4 * lane]) = make_float4(step[0], step[1], step[2], step[3]);
+            *reinterpret_cast<float4*>(&front[c & 3u][4 * lane]) = make_float4(before + f0, before + f1, before + f2, before + f3);
+            *reinterpret_cast<float4*>(&back[c & 3u][4 * lane]) = make_float4(behind + b0, behind + b1, behind + b2, behind);
+            um_arrive(d_full(c));
         }
     }
 
@@ -518,16 +558,16 @@ size_t scan_umma_scratch_bytes(const uzu_context* ctx, const uzu_state_space_sca
 }
 
 template <int N, bool STATE>
-static void su_launch(uzu_command_buffer* cmd, const CUtensorMap& mx, const CUtensorMap& mb, const CUtensorMap& mc, const ScanUmmaParams& p) {
+static void su_launch(uzu_command_buffer* cmd, const CUtensorMap& mx, const CUtensorMap& mb, const CUtensorMap& mc, const CUtensorMap& mo, const ScanUmmaParams& p) {
     static std::atomic<uint64_t> opted{0};
     opt_in_dynamic_smem(cmd, scan_umma_kernel<N, STATE>, (int)SU_SMEM, opted);
-    launch(cmd, "scan_umma_kernel", scan_umma_kernel<N, STATE>, dim3(p.a.heads * (p.a.head_dim / SU_P), p.table.tiles), dim3(SU_THREADS), SU_SMEM, mx, mb, mc, p);
+    launch(cmd, "scan_umma_kernel", scan_umma_kernel<N, STATE>, dim3(p.a.heads * (p.a.head_dim / SU_P), p.table.tiles), dim3(SU_THREADS), SU_SMEM, mx, mb, mc, mo, p);
 }
 
 bool encode_scan_umma(uzu_command_buffer* cmd, const uzu_state_space_scan_args& a) {
-    CUtensorMap mx, mb, mc;
+    CUtensorMap mx, mb, mc, mo;
     if (!um_map(&mx, a.x, (uint64_t)a.heads * a.head_dim, a.rows, a.x_stride, SU_Q) || !um_map(&mb, a.b, (uint64_t)a.groups * a.state_size, a.rows, a.b_stride, SU_Q) ||
-        !um_map(&mc, a.c, (uint64_t)a.groups * a.state_size, a.rows, a.c_stride, SU_Q))
+        !um_map(&mc, a.c, (uint64_t)a.groups * a.state_size, a.rows, a.c_stride, SU_Q) || !um_map(&mo, a.out, (uint64_t)a.heads * a.head_dim, a.rows, a.out_stride, 32))
         return false;
     // the longest first: the last CTAs to start are short ones
     std::vector<uzu_row_sequence> order;
@@ -544,7 +584,6 @@ bool encode_scan_umma(uzu_command_buffer* cmd, const uzu_state_space_scan_args& 
     const uint64_t heads = (uint64_t)a.heads * (a.head_dim / SU_P);
     ScanUmmaParams p{};
     p.a = a;
-    p.a.reserved0 = 0;      // (um_arrive_after)
     p.error = cmd->ctx->wait_errors.device_word;
     for (uint32_t begin = 0; begin < a.sequence_count;) {
         begin = fill_sequences(p.table, order.data(), a.sequence_count, begin, [&](uint32_t rows) { return cut ? su_parts((uint32_t)(((uint64_t)rows + SU_Q - 1) / SU_Q), su_ctas(a), sms) : 1u; });
@@ -552,11 +591,11 @@ bool encode_scan_umma(uzu_command_buffer* cmd, const uzu_state_space_scan_args& 
         p.ends = reinterpret_cast<float*>(a.scratch);
         p.logs = p.ends + (uint64_t)p.table.tiles * heads * SU_P * a.state_size;
         if (a.state_size == 128) {
-            if (p.table.tiles > p.table.count) su_launch<128, true>(cmd, mx, mb, mc, p);
-            su_launch<128, false>(cmd, mx, mb, mc, p);
+            if (p.table.tiles > p.table.count) su_launch<128, true>(cmd, mx, mb, mc, mo, p);
+            su_launch<128, false>(cmd, mx, mb, mc, mo, p);
         } else {
-            if (p.table.tiles > p.table.count) su_launch<64, true>(cmd, mx, mb, mc, p);
-            su_launch<64, false>(cmd, mx, mb, mc, p);
+            if (p.table.tiles > p.table.count) su_launch<64, true>(cmd, mx, mb, mc, mo, p);
+            su_launch<64, false>(cmd, mx, mb, mc, mo, p);
         }
     }
     return true;

@@ -78,6 +78,12 @@ __device__ __forceinline__ void um_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void um_tma(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
+// rows of shared memory to global memory; the group of them is read when um_store_read returns
+__device__ __forceinline__ void um_tma_store(const CUtensorMap* map, uint32_t src, uint32_t x, uint32_t y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n\tcp.async.bulk.commit_group;" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
+}
+__device__ __forceinline__ void um_store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void um_store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void um_commit(uint32_t bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void um_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
@@ -88,36 +94,28 @@ __device__ __forceinline__ void um_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
 __device__ __forceinline__ void um_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void um_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void um_fence_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// 32 columns of the warp's lanes. The wait is part of it: between a load and its wait the registers hold nothing, and the compiler may move or spill what it takes for a value.
-__device__ __forceinline__ void um_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+// 16 columns of the warp's lanes. The wait is part of it: between a load and its wait the registers hold nothing, and the compiler may move or spill what it takes for a value.
+__device__ __forceinline__ void um_ld16(uint32_t taddr0, uint32_t (&v0)[16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
-          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-        : "r"(taddr)
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=&r"(v0[0]), "=&r"(v0[1]), "=&r"(v0[2]), "=&r"(v0[3]), "=&r"(v0[4]), "=&r"(v0[5]), "=&r"(v0[6]), "=&r"(v0[7]), 
+          "=&r"(v0[8]), "=&r"(v0[9]), "=&r"(v0[10]), "=&r"(v0[11]), "=&r"(v0[12]), "=&r"(v0[13]), "=&r"(v0[14]), "=&r"(v0[15])
+        : "r"(taddr0)
         : "memory");
 }
-// twice 32 columns under way together
-__device__ __forceinline__ void um_ld32x2(uint32_t taddr0, uint32_t taddr1, uint32_t (&v0)[32], uint32_t (&v1)[32]) {
+// twice 16 columns under way together
+__device__ __forceinline__ void um_ld16x2(uint32_t taddr0, uint32_t taddr1, uint32_t (&v0)[16], uint32_t (&v1)[16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n\ttcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n\ttcgen05.wait::ld.sync.aligned;"
-        : "=&r"(v0[0]), "=&r"(v0[1]), "=&r"(v0[2]), "=&r"(v0[3]), "=&r"(v0[4]), "=&r"(v0[5]), "=&r"(v0[6]), "=&r"(v0[7]),
-          "=&r"(v0[8]), "=&r"(v0[9]), "=&r"(v0[10]), "=&r"(v0[11]), "=&r"(v0[12]), "=&r"(v0[13]), "=&r"(v0[14]), "=&r"(v0[15]),
-          "=&r"(v0[16]), "=&r"(v0[17]), "=&r"(v0[18]), "=&r"(v0[19]), "=&r"(v0[20]), "=&r"(v0[21]), "=&r"(v0[22]), "=&r"(v0[23]),
-          "=&r"(v0[24]), "=&r"(v0[25]), "=&r"(v0[26]), "=&r"(v0[27]), "=&r"(v0[28]), "=&r"(v0[29]), "=&r"(v0[30]), "=&r"(v0[31]),
-          "=&r"(v1[0]), "=&r"(v1[1]), "=&r"(v1[2]), "=&r"(v1[3]), "=&r"(v1[4]), "=&r"(v1[5]), "=&r"(v1[6]), "=&r"(v1[7]),
-          "=&r"(v1[8]), "=&r"(v1[9]), "=&r"(v1[10]), "=&r"(v1[11]), "=&r"(v1[12]), "=&r"(v1[13]), "=&r"(v1[14]), "=&r"(v1[15]),
-          "=&r"(v1[16]), "=&r"(v1[17]), "=&r"(v1[18]), "=&r"(v1[19]), "=&r"(v1[20]), "=&r"(v1[21]), "=&r"(v1[22]), "=&r"(v1[23]),
-          "=&r"(v1[24]), "=&r"(v1[25]), "=&r"(v1[26]), "=&r"(v1[27]), "=&r"(v1[28]), "=&r"(v1[29]), "=&r"(v1[30]), "=&r"(v1[31])
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\ttcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=&r"(v0[0]), "=&r"(v0[1]), "=&r"(v0[2]), "=&r"(v0[3]), "=&r"(v0[4]), "=&r"(v0[5]), "=&r"(v0[6]), "=&r"(v0[7]), 
+          "=&r"(v0[8]), "=&r"(v0[9]), "=&r"(v0[10]), "=&r"(v0[11]), "=&r"(v0[12]), "=&r"(v0[13]), "=&r"(v0[14]), "=&r"(v0[15]), 
+          "=&r"(v1[0]), "=&r"(v1[1]), "=&r"(v1[2]), "=&r"(v1[3]), "=&r"(v1[4]), "=&r"(v1[5]), "=&r"(v1[6]), "=&r"(v1[7]), 
+          "=&r"(v1[8]), "=&r"(v1[9]), "=&r"(v1[10]), "=&r"(v1[11]), "=&r"(v1[12]), "=&r"(v1[13]), "=&r"(v1[14]), "=&r"(v1[15])
         : "r"(taddr0), "r"(taddr1)
         : "memory");
 }
-__device__ __forceinline__ void um_st16(uint32_t taddr, const uint32_t (&v)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-                 : "memory");
+__device__ __forceinline__ void um_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 __device__ __forceinline__ void um_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t um_pack(float a, float b) {
