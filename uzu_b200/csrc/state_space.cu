@@ -20,18 +20,6 @@ struct ScanParams {
     SequenceTable table;
 };
 
-// pairs of f32 in one instruction
-__device__ __forceinline__ float2 ss_fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
-    return d;
-}
-__device__ __forceinline__ float2 ss_mul2(float2 a, float2 b) {
-    float2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-    return d;
-}
-
 // GROUPS: of four columns a thread; columns past state_size are zeros
 template <typename T, int GROUPS>
 __global__ void __launch_bounds__(SS_THREADS) state_space_scan_kernel(const __grid_constant__ ScanParams p) {

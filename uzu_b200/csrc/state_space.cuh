@@ -29,8 +29,40 @@ __device__ __forceinline__ __half ss_t<__half>(float v) { return __float2half_rn
 template <>
 __device__ __forceinline__ float ss_t<float>(float v) { return v; }
 
-// x sigmoid(x), to about 2^-21 of its value
-__device__ __forceinline__ float ss_silu(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
+// 2^x, 1 / x: to a few 2^-24 of the value, below 2^-126 zero
+__device__ __forceinline__ float ss_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float ss_rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// pairs of f32 in one instruction
+__device__ __forceinline__ float2 ss_fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 ss_mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 ss_add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return d;
+}
+// x sigmoid(x), to about 2^-21 of its value (the exponent's rounding: 2^-24 |x| more)
+__device__ __forceinline__ float ss_silu(float x) { return x * ss_rcp(1.0f + ss_exp2(-1.4426950408889634f * x)); }
+__device__ __forceinline__ float2 ss_silu2(float2 x) {
+    const float2 e = ss_mul2(x, make_float2(-1.4426950408889634f, -1.4426950408889634f));
+    const float2 d = ss_add2(make_float2(ss_exp2(e.x), ss_exp2(e.y)), make_float2(1.0f, 1.0f));
+    return ss_mul2(x, make_float2(ss_rcp(d.x), ss_rcp(d.y)));
+}
 // a token's step (log1p: steps of 1e-3 keep their digits); not a number stays so
 __device__ __forceinline__ float ss_step(float dt, float bias, uint32_t softplus, float lo, float hi) {
     float s = dt + bias;

@@ -19,7 +19,7 @@ namespace uzu {
 
 namespace {
 
-constexpr uint32_t SU_Q = 128, SU_P = 64, SU_THREADS = 27 * 32, SU_BLOCK = SU_Q * 128;      // tokens of a chunk, rows of the state, bytes of 64 columns of a chunk
+constexpr uint32_t SU_Q = 128, SU_P = 64, SU_THREADS = 28 * 32, SU_BLOCK = SU_Q * 128;      // tokens of a chunk, rows of the state, bytes of 64 columns of a chunk
 constexpr uint32_t SU_STAGE = 5 * SU_BLOCK, SU_WX = 2 * SU_STAGE, SU_S = SU_WX + 2 * SU_BLOCK;
 constexpr size_t SU_SMEM = SU_S + SU_BLOCK + 1024;
 // tensor memory
@@ -33,21 +33,6 @@ struct ScanUmmaParams {
     SequenceTable table;
 };
 
-__device__ __forceinline__ float su_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float2 su_mul2(float2 a, float2 b) {
-    float2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-    return d;
-}
-__device__ __forceinline__ float2 su_fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
-    return d;
-}
 __device__ __forceinline__ void su_sts(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
@@ -57,7 +42,7 @@ __device__ __forceinline__ void su_sts(uint32_t at, uint32_t x, uint32_t y, uint
 // N: state_size, 64 or 128. STATE: only the state at the end of every part but the last
 template <int N, bool STATE>
 __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c,
-                                                                  const __grid_constant__ CUtensorMap map_out, const __grid_constant__ ScanUmmaParams p) {
+                                                                  const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_z, const __grid_constant__ ScanUmmaParams p) {
     extern __shared__ uint8_t su_raw[];
     __shared__ __align__(8) uint64_t bars[41];
     __shared__ uint32_t tmem_slot;
@@ -128,9 +113,9 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                 ok = um_wait(d_full(c), four(c), &gave_up, p.error, 0x701u);
                 if (!ok) break;
                 const float mine = um_ldf(&fr[t]), ref = w ? um_ldf(&fr[32 * w - 1]) : 0.0f;
-                for (uint32_t jb = jb0; jb < jb1; ++jb) column[w][jb * 32 + lane] = um_ldf(&st[jb * 32 + lane]) * su_exp2(ref - um_ldf(&fr[jb * 32 + lane]));
+                for (uint32_t jb = jb0; jb < jb1; ++jb) column[w][jb * 32 + lane] = um_ldf(&st[jb * 32 + lane]) * ss_exp2(ref - um_ldf(&fr[jb * 32 + lane]));
                 __syncwarp();
-                const float r = su_exp2(mine - ref);
+                const float r = ss_exp2(mine - ref);
                 const float2 r2 = make_float2(r, r);
                 ok = um_wait(g_full, c & 1u, &gave_up, p.error, 0x702u);
                 if (ok && c) ok = um_wait(y_full, (c - 1) & 1u, &gave_up, p.error, 0x703u);      // the scores before are read
@@ -142,8 +127,8 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
 #pragma unroll
                     for (uint32_t j = 0; j < 16; j += 4) {
                         const float4 f = *reinterpret_cast<const float4*>(&column[w][k * 16 + j]);
-                        const float2 e0 = su_mul2(su_mul2(make_float2(f.x, f.y), r2), make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])));
-                        const float2 e1 = su_mul2(su_mul2(make_float2(f.z, f.w), r2), make_float2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])));
+                        const float2 e0 = ss_mul2(ss_mul2(make_float2(f.x, f.y), r2), make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])));
+                        const float2 e1 = ss_mul2(ss_mul2(make_float2(f.z, f.w), r2), make_float2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])));
                         o[j / 2] = um_pack(e0.x, e0.y);
                         o[j / 2 + 1] = um_pack(e1.x, e1.y);
                     }
@@ -157,7 +142,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
 #pragma unroll
                         for (uint32_t j = 0; j < 16; j += 4) {
                             const float4 f = um_ldf4(&fr[w * 32 + k * 16 + j]), sj = um_ldf4(&st[w * 32 + k * 16 + j]);
-                            const float e[4] = {sj.x * su_exp2(mine - f.x), sj.y * su_exp2(mine - f.y), sj.z * su_exp2(mine - f.z), sj.w * su_exp2(mine - f.w)};
+                            const float e[4] = {sj.x * ss_exp2(mine - f.x), sj.y * ss_exp2(mine - f.y), sj.z * ss_exp2(mine - f.z), sj.w * ss_exp2(mine - f.w)};
                             float x[4];
 #pragma unroll
                             for (uint32_t i = 0; i < 4; ++i) x[i] = k * 16 + j + i <= lane ? e[i] * __uint_as_float(v[j + i]) : 0.0f;
@@ -204,7 +189,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                 for (uint32_t i = 0; i < 32; ++i) S[i] = copy[i * N];
             } else {
                 for (uint32_t k = 0; k < part; ++k) {      // the parts before, in order
-                    const float f = k ? su_exp2(p.logs[(size_t)(s_.tile0 + k) * heads + blockIdx.x]) : 0.0f;
+                    const float f = k ? ss_exp2(p.logs[(size_t)(s_.tile0 + k) * heads + blockIdx.x]) : 0.0f;
                     const float* end = end_of(k);
 #pragma unroll
                     for (uint32_t i = 0; i < 32; ++i) S[i] = k ? fmaf(f, S[i], end[i * N]) : end[i * N];
@@ -232,10 +217,11 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             if (ok && valid < SU_Q) ok = um_wait(bc_full(c), two(c), &gave_up, p.error, 0x717u);      // (b's rows are there)
             if (!ok) break;
             // (the products that read the parts of chunk c - 1 are done: u_full was waited for)
-            const float weight = um_ldf(&steps[c & 3u][t]) * su_exp2(um_ldf(&back[c & 3u][t])), end = um_ldf(&front[c & 3u][SU_Q - 1]);
+            const float weight = um_ldf(&steps[c & 3u][t]) * ss_exp2(um_ldf(&back[c & 3u][t])), end = um_ldf(&front[c & 3u][SU_Q - 1]);
             const float2 w2 = make_float2(weight, weight);
             total += end;
             bool odd = false;
+            float2 check = make_float2(0.0f, 0.0f);      // stays 0 while all are finite
             if (t < valid) {
                 uint4 in[4];
 #pragma unroll
@@ -246,14 +232,16 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                     uint32_t hi[4], lo[4];
 #pragma unroll
                     for (uint32_t k = 0; k < 4; ++k) {
-                        odd |= (v[k] & 0x7f80u) == 0x7f80u || (v[k] & 0x7f800000u) == 0x7f800000u;
-                        const float2 y = su_mul2(make_float2(um_lo(v[k]), um_hi(v[k])), w2);
+                        const float2 x = make_float2(um_lo(v[k]), um_hi(v[k])), y = ss_mul2(x, w2);
+                        check = ss_fma2(x, make_float2(0.0f, 0.0f), check);
                         hi[k] = um_pack(y.x, y.y);
-                        lo[k] = um_pack(y.x - um_lo(hi[k]), y.y - um_hi(hi[k]));
+                        const float2 rest = ss_fma2(make_float2(um_lo(hi[k]), um_hi(hi[k])), make_float2(-1.0f, -1.0f), y);
+                        lo[k] = um_pack(rest.x, rest.y);
                     }
                     su_sts(base + SU_WX + chunk_of(t, i), hi[0], hi[1], hi[2], hi[3]);
                     su_sts(base + SU_WX + SU_BLOCK + chunk_of(t, i), lo[0], lo[1], lo[2], lo[3]);
                 }
+                odd = !(check.x + check.y == 0.0f);
                 if (odd) {      // not finite: not in the product with the scores
 #pragma unroll
                     for (uint32_t i = 0; i < 4; ++i) {
@@ -282,7 +270,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             um_arrive(o_full(c));
             um_arrive(d_empty(c));
 
-            const float f = su_exp2(end);
+            const float f = ss_exp2(end);
             const float2 f2 = make_float2(f, f);
             ok = um_wait(u_full, c & 1u, &gave_up, p.error, 0x706u);
             if (!ok) break;
@@ -293,7 +281,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                 um_ld16x2(tmem + lanes + SU_U + half * 32 + k * 16, tmem + lanes + SU_U + 64 + half * 32 + k * 16, hi, lo);
 #pragma unroll
                 for (uint32_t j = 0; j < 16; j += 2) {
-                    const float2 old = su_fma2(f2, make_float2(S[k * 16 + j], S[k * 16 + j + 1]), make_float2(__uint_as_float(hi[j]), __uint_as_float(hi[j + 1])));
+                    const float2 old = ss_fma2(f2, make_float2(S[k * 16 + j], S[k * 16 + j + 1]), make_float2(__uint_as_float(hi[j]), __uint_as_float(hi[j + 1])));
                     S[k * 16 + j] = old.x + __uint_as_float(lo[j]);
                     S[k * 16 + j + 1] = old.y + __uint_as_float(lo[j + 1]);
                 }
@@ -336,47 +324,44 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                 if (ok) ok = um_wait(y_full, c & 1u, &gave_up, p.error, 0x70bu);
                 if (!ok) break;
                 um_fence_after();
-                const float f = su_exp2(um_ldf(&front[c & 3u][t]));
+                const float f = ss_exp2(um_ldf(&front[c & 3u][t]));
+                const float2 f2 = make_float2(f, f), skip2 = make_float2(skip, skip);
                 uint32_t odd = 0;
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) odd |= odd_rows[c & 3u][half * 4 + i];
 #pragma unroll
-                for (uint32_t k = 0; k < 2; ++k) {
-                    uint32_t vi[16], vx[16];
-                    um_ld16x2(tmem + lanes + SU_YI + half * 32 + k * 16, tmem + lanes + SU_YX + half * 32 + k * 16, vi, vx);
-                    if (k == 1) {
+                for (uint32_t i = 0; i < 4; ++i) {
+                    uint32_t vi[8], vx[8];
+                    um_ld8x2(tmem + lanes + SU_YI + half * 32 + i * 8, tmem + lanes + SU_YX + half * 32 + i * 8, vi, vx);
+                    if (i == 3) {
                         um_fence_before();
                         um_arrive(y_empty);
                     }
+                    const uint32_t chunk = x0 + t * 128 + (((half * 4 + i) ^ (t & 7u)) << 4);
+                    const uint4 xx = um_lds(chunk), zz = zv[i];
+                    const uint32_t xs[4] = {xx.x, xx.y, xx.z, xx.w}, zs[4] = {zz.x, zz.y, zz.z, zz.w};
+                    float2 y[4];
 #pragma unroll
-                    for (uint32_t i = 0; i < 2; ++i) {
-                        const uint32_t chunk = x0 + t * 128 + (((half * 4 + k * 2 + i) ^ (t & 7u)) << 4);
-                        const uint4 xx = um_lds(chunk), zz = zv[k * 2 + i];
-                        const uint32_t xs[4] = {xx.x, xx.y, xx.z, xx.w}, zs[4] = {zz.x, zz.y, zz.z, zz.w};
-                        float y[8];
-#pragma unroll
-                        for (uint32_t e = 0; e < 4; ++e) {
-                            const uint32_t j = i * 8 + 2 * e;
-                            y[2 * e] = fmaf(skip, um_lo(xs[e]), fmaf(f, __uint_as_float(vx[j]), __uint_as_float(vi[j])));
-                            y[2 * e + 1] = fmaf(skip, um_hi(xs[e]), fmaf(f, __uint_as_float(vx[j + 1]), __uint_as_float(vi[j + 1])));
-                            if (gated) {
-                                y[2 * e] *= ss_silu(um_lo(zs[e]));
-                                y[2 * e + 1] *= ss_silu(um_hi(zs[e]));
-                            }
-                        }
-                        if (odd) {      // columns whose x was not finite at this token or before it in the chunk
-                            const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x) + (size_t)(row0 + c * SU_Q) * a.x_stride + col0 + half * 32 + k * 16 + i * 8;
-                            for (uint32_t j = 0; j <= t; ++j)
-                                if (odd_rows[c & 3u][half * 4 + (j >> 5)] >> (j & 31u) & 1u) {
-#pragma unroll
-                                    for (uint32_t e = 0; e < 8; ++e)
-                                        if (!(fabsf(__bfloat162float(x[(size_t)j * a.x_stride + e])) < INFINITY)) y[e] = __int_as_float(0x7fc00000);
-                                }
-                        }
-                        const uint4 o = make_uint4(um_pack(y[0], y[1]), um_pack(y[2], y[3]), um_pack(y[4], y[5]), um_pack(y[6], y[7]));
-                        if (whole) su_sts(chunk, o.x, o.y, o.z, o.w);      // over x, which nobody needs any more
-                        else if (t < valid) *reinterpret_cast<uint4*>(out + (size_t)r * a.out_stride + k * 16 + i * 8) = o;
+                    for (uint32_t e = 0; e < 4; ++e) {
+                        y[e] = ss_fma2(f2, make_float2(__uint_as_float(vx[2 * e]), __uint_as_float(vx[2 * e + 1])), make_float2(__uint_as_float(vi[2 * e]), __uint_as_float(vi[2 * e + 1])));
+                        y[e] = ss_fma2(skip2, make_float2(um_lo(xs[e]), um_hi(xs[e])), y[e]);
                     }
+                    if (gated) {
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e) y[e] = ss_mul2(y[e], ss_silu2(make_float2(um_lo(zs[e]), um_hi(zs[e]))));
+                    }
+                    if (odd) {      // columns whose x was not finite at this token or before it in the chunk
+                        const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x) + (size_t)(row0 + c * SU_Q) * a.x_stride + col0 + half * 32 + i * 8;
+                        for (uint32_t j = 0; j <= t; ++j)
+                            if (odd_rows[c & 3u][half * 4 + (j >> 5)] >> (j & 31u) & 1u) {
+#pragma unroll
+                                for (uint32_t e = 0; e < 8; ++e)
+                                    if (!(fabsf(__bfloat162float(x[(size_t)j * a.x_stride + e])) < INFINITY)) (e & 1u ? y[e / 2].y : y[e / 2].x) = __int_as_float(0x7fc00000);
+                            }
+                    }
+                    const uint4 o = make_uint4(um_pack(y[0].x, y[0].y), um_pack(y[1].x, y[1].y), um_pack(y[2].x, y[2].y), um_pack(y[3].x, y[3].y));
+                    if (whole) su_sts(chunk, o.x, o.y, o.z, o.w);      // over x, which nobody needs any more
+                    else if (t < valid) *reinterpret_cast<uint4*>(out + (size_t)r * a.out_stride + i * 8) = o;
                 }
                 if (whole) um_fence_proxy();
                 um_arrive(out_full(c, w));
@@ -390,36 +375,33 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             }
             um_store_done();
         }
-    } else if (warp == 24) {
-        // ================================ x, b and c by TMA ================================
-        uint32_t asked = 0, asked_x = 0;
+    } else if (warp == 24 || warp == 27) {
+        // ================================ b and c by TMA, x by another warp (its place is free later) ================================
+        const bool is_x = warp == 27;
+        auto full = [&](uint32_t c) { return is_x ? x_full(c) : bc_full(c); };
+        uint32_t asked = 0;
         for (uint32_t c = 0; c < chunks; ++c) {
             const uint32_t x0 = base + (c & 1u) * SU_STAGE, row = row0 + c * SU_Q;
-            ok = um_wait(bc_empty(c), two(c) ^ 1u, &gave_up, p.error, 0x70du);
+            ok = um_wait(is_x ? x_empty(c) : bc_empty(c), two(c) ^ 1u, &gave_up, p.error, is_x ? 0x70eu : 0x70du);
             if (!ok) break;
             if (um_elect()) {
-                um_expect(bc_full(c), SU_BLOCK * (STATE ? 1 : 2) * (N / 64));
-                for (uint32_t i = 0; i < N / 64; ++i) {
-                    um_tma(x0 + SU_BLOCK * (1 + i), &map_b, group * N + i * 64, row, bc_full(c));
-                    if (!STATE) um_tma(x0 + SU_BLOCK * (3 + i), &map_c, group * N + i * 64, row, bc_full(c));
+                if (is_x) {
+                    um_expect(x_full(c), SU_BLOCK);
+                    um_tma(x0, &map_x, col0, row, x_full(c));
+                    if (!STATE && a.z) um_tma_prefetch(&map_z, col0, row);      // (read by the threads themselves, a chunk and more later)
+                } else {
+                    um_expect(bc_full(c), SU_BLOCK * (STATE ? 1 : 2) * (N / 64));
+                    for (uint32_t i = 0; i < N / 64; ++i) {
+                        um_tma(x0 + SU_BLOCK * (1 + i), &map_b, group * N + i * 64, row, bc_full(c));
+                        if (!STATE) um_tma(x0 + SU_BLOCK * (3 + i), &map_c, group * N + i * 64, row, bc_full(c));
+                    }
                 }
             }
             __syncwarp();
             ++asked;
-            ok = um_wait(x_empty(c), two(c) ^ 1u, &gave_up, p.error, 0x70eu);
-            if (!ok) break;
-            if (um_elect()) {
-                um_expect(x_full(c), SU_BLOCK);
-                um_tma(x0, &map_x, col0, row, x_full(c));
-            }
-            __syncwarp();
-            ++asked_x;
         }
         if (!ok)      // copies that are on their way end before the CTA does
-            for (uint32_t n = 1; n <= 2; ++n) {
-                if (n <= asked) um_settle(bc_full(asked - n), two(asked - n));
-                if (n <= asked_x) um_settle(x_full(asked_x - n), two(asked_x - n));
-            }
+            for (uint32_t n = 1; n <= 2 && n <= asked; ++n) um_settle(full(asked - n), two(asked - n));
     } else if (warp == 25) {
         // ================================ products ================================
         // shared-memory descriptors: 128-byte swizzle, 1024 bytes between groups of 8 rows, SU_BLOCK between blocks of 64 columns
@@ -558,17 +540,19 @@ size_t scan_umma_scratch_bytes(const uzu_context* ctx, const uzu_state_space_sca
 }
 
 template <int N, bool STATE>
-static void su_launch(uzu_command_buffer* cmd, const CUtensorMap& mx, const CUtensorMap& mb, const CUtensorMap& mc, const CUtensorMap& mo, const ScanUmmaParams& p) {
+static void su_launch(uzu_command_buffer* cmd, const CUtensorMap& mx, const CUtensorMap& mb, const CUtensorMap& mc, const CUtensorMap& mo, const CUtensorMap& mz, const ScanUmmaParams& p) {
     static std::atomic<uint64_t> opted{0};
     opt_in_dynamic_smem(cmd, scan_umma_kernel<N, STATE>, (int)SU_SMEM, opted);
-    launch(cmd, "scan_umma_kernel", scan_umma_kernel<N, STATE>, dim3(p.a.heads * (p.a.head_dim / SU_P), p.table.tiles), dim3(SU_THREADS), SU_SMEM, mx, mb, mc, mo, p);
+    launch(cmd, "scan_umma_kernel", scan_umma_kernel<N, STATE>, dim3(p.a.heads * (p.a.head_dim / SU_P), p.table.tiles), dim3(SU_THREADS), SU_SMEM, mx, mb, mc, mo, mz, p);
 }
 
 bool encode_scan_umma(uzu_command_buffer* cmd, const uzu_state_space_scan_args& a) {
-    CUtensorMap mx, mb, mc, mo;
+    CUtensorMap mx, mb, mc, mo, mz;
     if (!um_map(&mx, a.x, (uint64_t)a.heads * a.head_dim, a.rows, a.x_stride, SU_Q) || !um_map(&mb, a.b, (uint64_t)a.groups * a.state_size, a.rows, a.b_stride, SU_Q) ||
         !um_map(&mc, a.c, (uint64_t)a.groups * a.state_size, a.rows, a.c_stride, SU_Q) || !um_map(&mo, a.out, (uint64_t)a.heads * a.head_dim, a.rows, a.out_stride, 32))
         return false;
+    mz = mo;
+    if (a.z && !um_map(&mz, a.z, (uint64_t)a.heads * a.head_dim, a.rows, a.z_stride, SU_Q)) return false;
     // the longest first: the last CTAs to start are short ones
     std::vector<uzu_row_sequence> order;
     try {
@@ -591,11 +575,11 @@ bool encode_scan_umma(uzu_command_buffer* cmd, const uzu_state_space_scan_args& 
         p.ends = reinterpret_cast<float*>(a.scratch);
         p.logs = p.ends + (uint64_t)p.table.tiles * heads * SU_P * a.state_size;
         if (a.state_size == 128) {
-            if (p.table.tiles > p.table.count) su_launch<128, true>(cmd, mx, mb, mc, mo, p);
-            su_launch<128, false>(cmd, mx, mb, mc, mo, p);
+            if (p.table.tiles > p.table.count) su_launch<128, true>(cmd, mx, mb, mc, mo, mz, p);
+            su_launch<128, false>(cmd, mx, mb, mc, mo, mz, p);
         } else {
-            if (p.table.tiles > p.table.count) su_launch<64, true>(cmd, mx, mb, mc, mo, p);
-            su_launch<64, false>(cmd, mx, mb, mc, mo, p);
+            if (p.table.tiles > p.table.count) su_launch<64, true>(cmd, mx, mb, mc, mo, mz, p);
+            su_launch<64, false>(cmd, mx, mb, mc, mo, mz, p);
         }
     }
     return true;

@@ -78,6 +78,10 @@ __device__ __forceinline__ void um_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void um_tma(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
+// asked into L2
+__device__ __forceinline__ void um_tma_prefetch(const CUtensorMap* map, uint32_t x, uint32_t y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
 // rows of shared memory to global memory; the group of them is read when um_store_read returns
 __device__ __forceinline__ void um_tma_store(const CUtensorMap* map, uint32_t src, uint32_t x, uint32_t y) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n\tcp.async.bulk.commit_group;" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
@@ -103,7 +107,7 @@ __device__ __forceinline__ void um_ld16(uint32_t taddr0, uint32_t (&v0)[16]) {
         : "r"(taddr0)
         : "memory");
 }
-// twice 16 columns under way together
+// twice 16 (8) columns under way together
 __device__ __forceinline__ void um_ld16x2(uint32_t taddr0, uint32_t taddr1, uint32_t (&v0)[16], uint32_t (&v1)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\ttcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\ttcgen05.wait::ld.sync.aligned;"
@@ -111,6 +115,14 @@ __device__ __forceinline__ void um_ld16x2(uint32_t taddr0, uint32_t taddr1, uint
           "=&r"(v0[8]), "=&r"(v0[9]), "=&r"(v0[10]), "=&r"(v0[11]), "=&r"(v0[12]), "=&r"(v0[13]), "=&r"(v0[14]), "=&r"(v0[15]), 
           "=&r"(v1[0]), "=&r"(v1[1]), "=&r"(v1[2]), "=&r"(v1[3]), "=&r"(v1[4]), "=&r"(v1[5]), "=&r"(v1[6]), "=&r"(v1[7]), 
           "=&r"(v1[8]), "=&r"(v1[9]), "=&r"(v1[10]), "=&r"(v1[11]), "=&r"(v1[12]), "=&r"(v1[13]), "=&r"(v1[14]), "=&r"(v1[15])
+        : "r"(taddr0), "r"(taddr1)
+        : "memory");
+}
+__device__ __forceinline__ void um_ld8x2(uint32_t taddr0, uint32_t taddr1, uint32_t (&v0)[8], uint32_t (&v1)[8]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%16];\n\ttcgen05.ld.sync.aligned.32x32b.x8.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%17];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=&r"(v0[0]), "=&r"(v0[1]), "=&r"(v0[2]), "=&r"(v0[3]), "=&r"(v0[4]), "=&r"(v0[5]), "=&r"(v0[6]), "=&r"(v0[7]), 
+          "=&r"(v1[0]), "=&r"(v1[1]), "=&r"(v1[2]), "=&r"(v1[3]), "=&r"(v1[4]), "=&r"(v1[5]), "=&r"(v1[6]), "=&r"(v1[7])
         : "r"(taddr0), "r"(taddr1)
         : "memory");
 }
