@@ -61,19 +61,18 @@ __device__ __forceinline__ float xl_x(const uzu_expert_layer_args& a, uint32_t t
 }
 
 // all CTAs of the launch; false: not within about a second
-__device__ __noinline__ bool xl_all(unsigned int* counter, volatile uint32_t* gave_up, unsigned int* error, uint32_t code) {
+__device__ __noinline__ bool xl_all(unsigned int* counter, volatile uint32_t* gave_up, uint32_t code) {
     __threadfence();
     atomicAdd(counter, 1u);
-    const uint64_t t0 = um_now();
+    const uint64_t until = um_now() + 1000000000ull;
     for (uint32_t n = 1;; ++n) {
         unsigned int v;
         asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(counter) : "memory");
         if (v >= gridDim.x) return true;
         if ((n & 63u) == 0) {
             if (*gave_up) return false;
-            if (um_now() - t0 > 1000000000ull) {
-                *gave_up = 1;
-                report_wait_error(error, code);
+            if (um_now() > until) {
+                *gave_up = code;
                 return false;
             }
         }
@@ -236,7 +235,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
         }
     }
     __syncthreads();
-    if (tid == 0) xl_all(counters, &gave_up, p.error, 0x601u);
+    if (tid == 0) xl_all(counters, &gave_up, 0x601u);
     __syncthreads();
     bool ok = !gave_up;
 
@@ -281,7 +280,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
         // ---- weights by TMA ----
         auto stage = [&](const CUtensorMap* map, uint32_t col, uint32_t width, uint32_t row_a, uint32_t row_b) {
             const uint32_t s = it % S::STAGES;
-            if (ok) ok = um_wait(empty(s), (it / S::STAGES & 1u) ^ 1u, &gave_up, p.error, 0x602u);
+            if (ok) ok = um_wait(empty(s), (it / S::STAGES & 1u) ^ 1u, &gave_up, 0x602u);
             if (!ok) return;
             if (um_elect()) {
                 const uint32_t boxes = min(XL_WARPS, (width - col + 63) / 64);
@@ -336,7 +335,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
                 for (int n = 0; n < NT; ++n)
                     if (live >> n & 1u) fetch(n, b[n]);
             }
-            if (ok) ok = um_wait(full(s), it / S::STAGES & 1u, &gave_up, p.error, 0x603u);
+            if (ok) ok = um_wait(full(s), it / S::STAGES & 1u, &gave_up, 0x603u);
             if (!ok) return;
             uint32_t seen = 0;
             if (there) {
@@ -415,7 +414,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
             }
             meet();
         }
-        if (tid == 0) xl_all(counters + 1, &gave_up, p.error, 0x604u);
+        if (tid == 0) xl_all(counters + 1, &gave_up, 0x604u);
         meet();
         ok = ok && !gave_up;
 
@@ -472,6 +471,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
         }
     }
     __syncthreads();
+    if (tid == 0) um_report(&gave_up, p.error);
     if (tid == 0 && atomicAdd(counters + 2, 1u) == ctas - 1) {      // the last one out: for the next call
         counters[0] = counters[1] = counters[2] = 0;
         __threadfence();

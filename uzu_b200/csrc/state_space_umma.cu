@@ -22,6 +22,9 @@ namespace {
 constexpr uint32_t SU_Q = 128, SU_P = 64, SU_THREADS = 28 * 32, SU_BLOCK = SU_Q * 128;      // tokens of a chunk, rows of the state, bytes of 64 columns of a chunk
 constexpr uint32_t SU_STAGE = 5 * SU_BLOCK, SU_WX = 2 * SU_STAGE, SU_S = SU_WX + 2 * SU_BLOCK;
 constexpr size_t SU_SMEM = SU_S + SU_BLOCK + 1024;
+// registers of a thread: of the scores' warps, the states' and outputs', the others'; together those of the launch (896 threads with 72)
+constexpr uint32_t SU_SCORES_REGS = 56, SU_WORK_REGS = 88, SU_OTHER_REGS = 40;
+static_assert(256 * SU_SCORES_REGS + 512 * SU_WORK_REGS + 128 * SU_OTHER_REGS <= SU_THREADS * 72, "a split above the launch's registers waits forever");
 // tensor memory
 constexpr uint32_t SU_G = 0, SU_SCORES = 128, SU_YI = 192, SU_YX = 256, SU_U = 320, SU_COLUMNS = 512;
 
@@ -61,8 +64,8 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
     auto d_empty = [&](uint32_t c) { return bar0 + 8u * (12 + (c & 3u)); };
     auto o_full = [&](uint32_t c) { return bar0 + 8u * (16 + (c & 3u)); };             // odd_rows
     auto out_full = [&](uint32_t c, uint32_t block) { return bar0 + 8u * (20 + (c & 1u) * 4 + block); };      // both halves of 32 rows of output
-    const uint32_t g_full = bar0 + 8u * 28, g_empty = bar0 + 8u * 29, p_full = bar0 + 8u * 30, w_full = bar0 + 8u * 31, s_full = bar0 + 8u * 32, y_full = bar0 + 8u * 33, y_empty = bar0 + 8u * 34,
-                   u_full = bar0 + 8u * 35, last_products = bar0 + 8u * 36;
+    const uint32_t g_full = bar0 + 8u * 28, p_full = bar0 + 8u * 30, w_full = bar0 + 8u * 31, s_full = bar0 + 8u * 32, y_full = bar0 + 8u * 33, y_empty = bar0 + 8u * 34,
+                   u_full = bar0 + 8u * 35, last_products = bar0 + 8u * 36, s_free = bar0 + 8u * 29;
     auto two = [](uint32_t c) { return c >> 1 & 1u; };      // parities of rings of two and four
     auto four = [](uint32_t c) { return c >> 2 & 1u; };
 
@@ -81,7 +84,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                 for (uint32_t k = 0; k < 4; ++k) um_init(out_full(s, k), 2);
             }
             for (uint32_t s = 0; s < 4; ++s) { um_init(d_full(s), 1); um_init(d_empty(s), STATE ? 8 : 24); um_init(o_full(s), 8); }
-            um_init(g_full, 1); um_init(g_empty, 8); um_init(p_full, 8); um_init(w_full, 8); um_init(s_full, 8); um_init(y_full, 1); um_init(y_empty, 8); um_init(u_full, 1);
+            um_init(g_full, 1); um_init(s_free, 1); um_init(p_full, 8); um_init(w_full, 8); um_init(s_full, 8); um_init(y_full, 1); um_init(y_empty, 8); um_init(u_full, 1);
             um_init(last_products, 1);
             gave_up = 0;
             um_fence_init();
@@ -99,6 +102,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
     bool ok = true;
 
     if (warp < 8) {
+        um_fewer_registers<SU_SCORES_REGS>();
         // ================================ scores ================================
         if (!STATE) {
             // Blocks of 32 tokens up to the row block's own, the diagonal one: one warp has that and, of four, the one before it; the other one the rest.
@@ -110,17 +114,18 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             }
             for (uint32_t c = 0; c < chunks; ++c) {
                 const float *st = steps[c & 3u], *fr = front[c & 3u];
-                ok = um_wait(d_full(c), four(c), &gave_up, p.error, 0x701u);
+                ok = um_wait(d_full(c), four(c), &gave_up, 0x701u);
                 if (!ok) break;
                 const float mine = um_ldf(&fr[t]), ref = w ? um_ldf(&fr[32 * w - 1]) : 0.0f;
                 for (uint32_t jb = jb0; jb < jb1; ++jb) column[w][jb * 32 + lane] = um_ldf(&st[jb * 32 + lane]) * ss_exp2(ref - um_ldf(&fr[jb * 32 + lane]));
                 __syncwarp();
                 const float r = ss_exp2(mine - ref);
                 const float2 r2 = make_float2(r, r);
-                ok = um_wait(g_full, c & 1u, &gave_up, p.error, 0x702u);
-                if (ok && c) ok = um_wait(y_full, (c - 1) & 1u, &gave_up, p.error, 0x703u);      // the scores before are read
+                ok = um_wait(g_full, c & 1u, &gave_up, 0x702u);
+                if (ok && c) ok = um_wait(y_full, (c - 1) & 1u, &gave_up, 0x703u);      // the scores before are read
                 if (!ok) break;
                 um_fence_after();
+#pragma unroll 1
                 for (uint32_t k = 2 * jb0; k < 2 * jb1; ++k) {
                     uint32_t v[16], o[8];
                     um_ld16(tmem + lanes + SU_G + k * 16, v);
@@ -135,7 +140,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                     um_st8(tmem + lanes + SU_SCORES + k * 8, o);
                 }
                 if (half) {
-#pragma unroll
+#pragma unroll 1
                     for (uint32_t k = 0; k < 2; ++k) {
                         uint32_t v[16], o[8];
                         um_ld16(tmem + lanes + SU_G + w * 32 + k * 16, v);
@@ -154,12 +159,12 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                 }
                 um_wait_st();
                 um_fence_before();
-                um_arrive(g_empty);
                 um_arrive(p_full);
                 um_arrive(d_empty(c));
             }
         }
     } else if (warp < 16) {
+        um_more_registers<SU_WORK_REGS>();
         // ================================ state: column n = t, rows [32 half, 32 half + 32) ================================
         const uint32_t n = t, heads = a.heads * slices;
         const size_t at = (((size_t)s_.slot() * a.heads + h) * a.head_dim + slice * SU_P + half * 32) * N + n;
@@ -212,9 +217,9 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
         float total = 0.0f;
         for (uint32_t c = 0; c < chunks; ++c) {
             const uint32_t x0 = base + (c & 1u) * SU_STAGE, b0 = x0 + SU_BLOCK, valid = min(SU_Q, rows - c * SU_Q);
-            ok = um_wait(d_full(c), four(c), &gave_up, p.error, 0x704u);
-            if (ok) ok = um_wait(x_full(c), two(c), &gave_up, p.error, 0x705u);
-            if (ok && valid < SU_Q) ok = um_wait(bc_full(c), two(c), &gave_up, p.error, 0x717u);      // (b's rows are there)
+            ok = um_wait(d_full(c), four(c), &gave_up, 0x704u);
+            if (ok) ok = um_wait(x_full(c), two(c), &gave_up, 0x705u);
+            if (ok && valid < SU_Q) ok = um_wait(bc_full(c), two(c), &gave_up, 0x717u);      // (b's rows are there)
             if (!ok) break;
             // (the products that read the parts of chunk c - 1 are done: u_full was waited for)
             const float weight = um_ldf(&steps[c & 3u][t]) * ss_exp2(um_ldf(&back[c & 3u][t])), end = um_ldf(&front[c & 3u][SU_Q - 1]);
@@ -223,12 +228,11 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             bool odd = false;
             float2 check = make_float2(0.0f, 0.0f);      // stays 0 while all are finite
             if (t < valid) {
-                uint4 in[4];
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) in[i] = um_lds(x0 + chunk_of(t, i));
-#pragma unroll
+                uint4 next = um_lds(x0 + chunk_of(t, 0));
+#pragma unroll 1
                 for (uint32_t i = 0; i < 4; ++i) {
-                    const uint32_t v[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
+                    const uint32_t v[4] = {next.x, next.y, next.z, next.w}, o = chunk_of(t, i);
+                    next = um_lds(x0 + chunk_of(t, i < 3 ? i + 1 : i));
                     uint32_t hi[4], lo[4];
 #pragma unroll
                     for (uint32_t k = 0; k < 4; ++k) {
@@ -238,14 +242,15 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                         const float2 rest = ss_fma2(make_float2(um_lo(hi[k]), um_hi(hi[k])), make_float2(-1.0f, -1.0f), y);
                         lo[k] = um_pack(rest.x, rest.y);
                     }
-                    su_sts(base + SU_WX + chunk_of(t, i), hi[0], hi[1], hi[2], hi[3]);
-                    su_sts(base + SU_WX + SU_BLOCK + chunk_of(t, i), lo[0], lo[1], lo[2], lo[3]);
+                    su_sts(base + SU_WX + o, hi[0], hi[1], hi[2], hi[3]);
+                    su_sts(base + SU_WX + SU_BLOCK + o, lo[0], lo[1], lo[2], lo[3]);
                 }
                 odd = !(check.x + check.y == 0.0f);
                 if (odd) {      // not finite: not in the product with the scores
-#pragma unroll
+#pragma unroll 1
                     for (uint32_t i = 0; i < 4; ++i) {
-                        uint32_t v[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
+                        const uint4 in = um_lds(x0 + chunk_of(t, i));
+                        uint32_t v[4] = {in.x, in.y, in.z, in.w};
 #pragma unroll
                         for (uint32_t k = 0; k < 4; ++k) {
                             if ((v[k] & 0x7f80u) == 0x7f80u) v[k] &= 0xffff0000u;
@@ -255,6 +260,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                     }
                 }
             } else {            // behind the sequence
+#pragma unroll 1
                 for (uint32_t i = 0; i < 4; ++i) {
                     su_sts(x0 + chunk_of(t, i), 0, 0, 0, 0);
                     su_sts(b0 + chunk_of(t, i), 0, 0, 0, 0);
@@ -272,7 +278,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
 
             const float f = ss_exp2(end);
             const float2 f2 = make_float2(f, f);
-            ok = um_wait(u_full, c & 1u, &gave_up, p.error, 0x706u);
+            ok = um_wait(u_full, c & 1u, &gave_up, 0x706u);
             if (!ok) break;
             um_fence_after();
 #pragma unroll
@@ -288,7 +294,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             }
             um_fence_before();
             if (c + 1 < chunks) {
-                if (!STATE) ok = um_wait(y_full, c & 1u, &gave_up, p.error, 0x707u);      // the operand before is read
+                if (!STATE) ok = um_wait(s_free, c & 1u, &gave_up, 0x707u);      // the operand before is read
                 if (!ok) break;
                 store();
             }
@@ -302,26 +308,29 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             if (STATE && n == 0 && half == 0) p.logs[(size_t)tile * heads + blockIdx.x] = total;
         }
     } else if (warp < 24) {
+        um_more_registers<SU_WORK_REGS>();
         // ================================ output: row t, columns [32 half, 32 half + 32) ================================
         if (!STATE) {
             const float skip = a.d ? reinterpret_cast<const float*>(a.d)[h] : 0.0f;
             const bool gated = a.z != 0;
             const __nv_bfloat16* z = reinterpret_cast<const __nv_bfloat16*>(a.z) + (size_t)row0 * a.z_stride + col0 + half * 32;
             __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)row0 * a.out_stride + col0 + half * 32;
+            auto gate_of = [&](uint32_t c, uint32_t i) {      // eight of z, asked for a step ahead
+                const uint32_t r = c * SU_Q + t;
+                return gated && r < rows ? *reinterpret_cast<const uint4*>(z + (size_t)r * a.z_stride + 8 * i) : make_uint4(0, 0, 0, 0);
+            };
+            uint4 next = gate_of(0, 0);
             for (uint32_t c = 0; c < chunks; ++c) {
                 const uint32_t x0 = base + (c & 1u) * SU_STAGE, valid = min(SU_Q, rows - c * SU_Q), r = c * SU_Q + t;
                 const bool whole = w * 32 + 32 <= valid;      // all rows of the block are the sequence's
-                uint4 zv[4];
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) zv[i] = gated && t < valid ? *reinterpret_cast<const uint4*>(z + (size_t)r * a.z_stride + 8 * i) : make_uint4(0, 0, 0, 0);
                 if (c && half == 0) {      // the rows stored from x's place a chunk ago are read: x may come there
                     um_store_read();
                     um_arrive(x_empty(c - 1));
                 }
-                ok = um_wait(x_full(c), two(c), &gave_up, p.error, 0x708u);
-                if (ok) ok = um_wait(d_full(c), four(c), &gave_up, p.error, 0x709u);
-                if (ok) ok = um_wait(o_full(c), four(c), &gave_up, p.error, 0x70au);
-                if (ok) ok = um_wait(y_full, c & 1u, &gave_up, p.error, 0x70bu);
+                ok = um_wait(x_full(c), two(c), &gave_up, 0x708u);
+                if (ok) ok = um_wait(d_full(c), four(c), &gave_up, 0x709u);
+                if (ok) ok = um_wait(o_full(c), four(c), &gave_up, 0x70au);
+                if (ok) ok = um_wait(y_full, c & 1u, &gave_up, 0x70bu);
                 if (!ok) break;
                 um_fence_after();
                 const float f = ss_exp2(um_ldf(&front[c & 3u][t]));
@@ -329,16 +338,13 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                 uint32_t odd = 0;
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) odd |= odd_rows[c & 3u][half * 4 + i];
-#pragma unroll
+#pragma unroll 1
                 for (uint32_t i = 0; i < 4; ++i) {
                     uint32_t vi[8], vx[8];
                     um_ld8x2(tmem + lanes + SU_YI + half * 32 + i * 8, tmem + lanes + SU_YX + half * 32 + i * 8, vi, vx);
-                    if (i == 3) {
-                        um_fence_before();
-                        um_arrive(y_empty);
-                    }
                     const uint32_t chunk = x0 + t * 128 + (((half * 4 + i) ^ (t & 7u)) << 4);
-                    const uint4 xx = um_lds(chunk), zz = zv[i];
+                    const uint4 xx = um_lds(chunk), zz = next;
+                    next = gate_of(i < 3 ? c : c + 1, i < 3 ? i + 1 : 0);
                     const uint32_t xs[4] = {xx.x, xx.y, xx.z, xx.w}, zs[4] = {zz.x, zz.y, zz.z, zz.w};
                     float2 y[4];
 #pragma unroll
@@ -352,6 +358,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                     }
                     if (odd) {      // columns whose x was not finite at this token or before it in the chunk
                         const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x) + (size_t)(row0 + c * SU_Q) * a.x_stride + col0 + half * 32 + i * 8;
+#pragma unroll 1
                         for (uint32_t j = 0; j <= t; ++j)
                             if (odd_rows[c & 3u][half * 4 + (j >> 5)] >> (j & 31u) & 1u) {
 #pragma unroll
@@ -363,11 +370,13 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                     if (whole) su_sts(chunk, o.x, o.y, o.z, o.w);      // over x, which nobody needs any more
                     else if (t < valid) *reinterpret_cast<uint4*>(out + (size_t)r * a.out_stride + i * 8) = o;
                 }
+                um_fence_before();
+                um_arrive(y_empty);
                 if (whole) um_fence_proxy();
                 um_arrive(out_full(c, w));
                 um_arrive(d_empty(c));
                 if (half == 0) {
-                    ok = um_wait(out_full(c, w), two(c), &gave_up, p.error, 0x70cu);
+                    ok = um_wait(out_full(c, w), two(c), &gave_up, 0x70cu);
                     if (!ok) break;
                     if (whole && lane == 0) um_tma_store(&map_out, x0 + w * 4096, col0, row0 + c * SU_Q + w * 32);
                     __syncwarp();
@@ -375,134 +384,145 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             }
             um_store_done();
         }
-    } else if (warp == 24 || warp == 27) {
-        // ================================ b and c by TMA, x by another warp (its place is free later) ================================
-        const bool is_x = warp == 27;
-        auto full = [&](uint32_t c) { return is_x ? x_full(c) : bc_full(c); };
-        uint32_t asked = 0;
-        for (uint32_t c = 0; c < chunks; ++c) {
-            const uint32_t x0 = base + (c & 1u) * SU_STAGE, row = row0 + c * SU_Q;
-            ok = um_wait(is_x ? x_empty(c) : bc_empty(c), two(c) ^ 1u, &gave_up, p.error, is_x ? 0x70eu : 0x70du);
-            if (!ok) break;
-            if (um_elect()) {
-                if (is_x) {
-                    um_expect(x_full(c), SU_BLOCK);
-                    um_tma(x0, &map_x, col0, row, x_full(c));
-                    if (!STATE && a.z) um_tma_prefetch(&map_z, col0, row);      // (read by the threads themselves, a chunk and more later)
-                } else {
-                    um_expect(bc_full(c), SU_BLOCK * (STATE ? 1 : 2) * (N / 64));
-                    for (uint32_t i = 0; i < N / 64; ++i) {
-                        um_tma(x0 + SU_BLOCK * (1 + i), &map_b, group * N + i * 64, row, bc_full(c));
-                        if (!STATE) um_tma(x0 + SU_BLOCK * (3 + i), &map_c, group * N + i * 64, row, bc_full(c));
+    } else {
+        um_fewer_registers<SU_OTHER_REGS>();
+        if (warp == 24 || warp == 27) {
+            // ================================ b and c by TMA, x by another warp (its place is free later) ================================
+            const bool is_x = warp == 27;
+            auto full = [&](uint32_t c) { return is_x ? x_full(c) : bc_full(c); };
+            uint32_t asked = 0;
+            for (uint32_t c = 0; c < chunks; ++c) {
+                const uint32_t x0 = base + (c & 1u) * SU_STAGE, row = row0 + c * SU_Q;
+                ok = um_wait(is_x ? x_empty(c) : bc_empty(c), two(c) ^ 1u, &gave_up, is_x ? 0x70eu : 0x70du);
+                if (!ok) break;
+                if (um_elect()) {
+                    if (is_x) {
+                        um_expect(x_full(c), SU_BLOCK);
+                        um_tma(x0, &map_x, col0, row, x_full(c));
+                        if (!STATE && a.z) um_tma_prefetch(&map_z, col0, row);      // (read by the threads themselves, a chunk and more later)
+                    } else {
+                        um_expect(bc_full(c), SU_BLOCK * (STATE ? 1 : 2) * (N / 64));
+                        for (uint32_t i = 0; i < N / 64; ++i) {
+                            um_tma(x0 + SU_BLOCK * (1 + i), &map_b, group * N + i * 64, row, bc_full(c));
+                            if (!STATE) um_tma(x0 + SU_BLOCK * (3 + i), &map_c, group * N + i * 64, row, bc_full(c));
+                        }
                     }
                 }
+                __syncwarp();
+                ++asked;
             }
-            __syncwarp();
-            ++asked;
-        }
-        if (!ok)      // copies that are on their way end before the CTA does
-            for (uint32_t n = 1; n <= 2 && n <= asked; ++n) um_settle(full(asked - n), two(asked - n));
-    } else if (warp == 25) {
-        // ================================ products ================================
-        // shared-memory descriptors: 128-byte swizzle, 1024 bytes between groups of 8 rows, SU_BLOCK between blocks of 64 columns
-        constexpr uint64_t desc = (uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32, k_major = desc | (1u << 16), wide = desc | ((uint64_t)(SU_BLOCK >> 4) << 16);
-        constexpr uint32_t common = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24), a_wide = 1u << 15, b_wide = 1u << 16;
-        constexpr uint32_t i_scores = common | ((128u >> 3) << 17), i_y = common | b_wide | ((64u >> 3) << 17), i_u = common | a_wide | b_wide | ((128u >> 3) << 17);
-        auto scores = [&](uint32_t c) {
-            const uint32_t b0 = base + (c & 1u) * SU_STAGE + SU_BLOCK, c0 = b0 + 2 * SU_BLOCK;
-            ok = um_wait(bc_full(c), two(c), &gave_up, p.error, 0x70fu);
-            if (ok && c) ok = um_wait(g_empty, (c - 1) & 1u, &gave_up, p.error, 0x710u);
-            if (!ok) return;
-            um_fence_after();
-            if (um_elect()) {
+            if (!ok)      // copies that are on their way end before the CTA does
+                for (uint32_t n = 1; n <= 2 && n <= asked; ++n) um_settle(full(asked - n), two(asked - n));
+        } else if (warp == 25) {
+            // ================================ products ================================
+            // shared-memory descriptors: 128-byte swizzle, 1024 bytes between groups of 8 rows, SU_BLOCK between blocks of 64 columns
+            constexpr uint64_t desc = (uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32, k_major = desc | (1u << 16), wide = desc | ((uint64_t)(SU_BLOCK >> 4) << 16);
+            constexpr uint32_t common = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24), a_wide = 1u << 15, b_wide = 1u << 16;
+            constexpr uint32_t i_scores = common | ((128u >> 3) << 17), i_y = common | b_wide | ((64u >> 3) << 17), i_u = common | a_wide | b_wide | ((128u >> 3) << 17);
+            auto scores = [&](uint32_t c) {
+                const uint32_t b0 = base + (c & 1u) * SU_STAGE + SU_BLOCK, c0 = b0 + 2 * SU_BLOCK;
+                ok = um_wait(bc_full(c), two(c), &gave_up, 0x70fu);
+                if (!ok) return;
+                um_fence_after();
+                if (um_elect()) {
 #pragma unroll
-                for (uint32_t kk = 0; kk < N / 16; ++kk) {
-                    const uint32_t o = (kk >> 2) * SU_BLOCK + (kk & 3u) * 32u;
-                    um_mma_ss(tmem + SU_G, k_major | ((c0 + o) >> 4), k_major | ((b0 + o) >> 4), i_scores, kk != 0);
+                    for (uint32_t kk = 0; kk < N / 16; ++kk) {
+                        const uint32_t o = (kk >> 2) * SU_BLOCK + (kk & 3u) * 32u;
+                        um_mma_ss(tmem + SU_G, k_major | ((c0 + o) >> 4), k_major | ((b0 + o) >> 4), i_scores, kk != 0);
+                    }
+                    um_commit(g_full);
                 }
-                um_commit(g_full);
-            }
-            __syncwarp();
-        };
-        if (!STATE && chunks) scores(0);
-        for (uint32_t c = 0; c < chunks && ok; ++c) {
-            const uint32_t x0 = base + (c & 1u) * SU_STAGE, b0 = x0 + SU_BLOCK, c0 = b0 + 2 * SU_BLOCK;
-            if (!STATE) {
-                if (c + 1 < chunks) scores(c + 1);
-                if (ok) ok = um_wait(p_full, c & 1u, &gave_up, p.error, 0x711u);
-                if (ok) ok = um_wait(s_full, c & 1u, &gave_up, p.error, 0x712u);
-                if (ok && c) ok = um_wait(y_empty, (c - 1) & 1u, &gave_up, p.error, 0x713u);
-            } else if (ok) ok = um_wait(bc_full(c), two(c), &gave_up, p.error, 0x714u);
-            if (ok) ok = um_wait(w_full, c & 1u, &gave_up, p.error, 0x715u);
-            if (!ok) break;
-            um_fence_after();
-            if (um_elect()) {
-                if (!STATE) {
+                __syncwarp();
+            };
+            if (!STATE && chunks) scores(0);
+            // What needs no scores runs while they are made, and gives b's and c's place away early: the next chunk but one is there when its turn comes.
+            for (uint32_t c = 0; c < chunks && ok; ++c) {
+                const uint32_t x0 = base + (c & 1u) * SU_STAGE, b0 = x0 + SU_BLOCK, c0 = b0 + 2 * SU_BLOCK;
+                if (STATE) ok = um_wait(bc_full(c), two(c), &gave_up, 0x714u);
+                if (ok) ok = um_wait(w_full, c & 1u, &gave_up, 0x715u);
+                if (!ok) break;
+                um_fence_after();
+                if (um_elect()) {
+                    // (64 columns: operand A's second block is whatever lies behind; the sums' lanes 64 .. 127 are not read)
 #pragma unroll
-                    for (uint32_t kk = 0; kk < SU_Q / 16; ++kk) um_mma_ts(tmem + SU_YI, tmem + SU_SCORES + kk * 8u, wide | ((x0 + kk * 2048u) >> 4), i_y, kk != 0);
+                    for (uint32_t kk = 0; kk < SU_Q / 16; ++kk) um_mma_ss(tmem + SU_U, wide | ((b0 + kk * 2048u) >> 4), wide | ((base + SU_WX + kk * 2048u) >> 4), i_u, kk != 0);
+                    um_commit(u_full);
+                    if (STATE) {
+                        um_commit(bc_empty(c));
+                        um_commit(x_empty(c));
+                    }
+                }
+                __syncwarp();
+                if (STATE) continue;
+                ok = um_wait(p_full, c & 1u, &gave_up, 0x711u);      // (the scores' sums are read, too)
+                if (ok && c + 1 < chunks) scores(c + 1);
+                if (ok) ok = um_wait(s_full, c & 1u, &gave_up, 0x712u);
+                if (ok && c) ok = um_wait(y_empty, (c - 1) & 1u, &gave_up, 0x713u);
+                if (!ok) break;
+                um_fence_after();
+                if (um_elect()) {
 #pragma unroll
                     for (uint32_t kk = 0; kk < N / 16; ++kk)
                         um_mma_ss(tmem + SU_YX, k_major | ((c0 + (kk >> 2) * SU_BLOCK + (kk & 3u) * 32u) >> 4), wide | ((base + SU_S + kk * 2048u) >> 4), i_y, kk != 0);
+                    um_commit(s_free);
+                    um_commit(bc_empty(c));
+#pragma unroll
+                    for (uint32_t kk = 0; kk < SU_Q / 16; ++kk) um_mma_ts(tmem + SU_YI, tmem + SU_SCORES + kk * 8u, wide | ((x0 + kk * 2048u) >> 4), i_y, kk != 0);
                     um_commit(y_full);
                 }
-                // (64 columns: operand A's second block is whatever lies behind; the sums' lanes 64 .. 127 are not read)
-#pragma unroll
-                for (uint32_t kk = 0; kk < SU_Q / 16; ++kk) um_mma_ss(tmem + SU_U, wide | ((b0 + kk * 2048u) >> 4), wide | ((base + SU_WX + kk * 2048u) >> 4), i_u, kk != 0);
-                um_commit(u_full);
-                um_commit(bc_empty(c));
-                if (STATE) um_commit(x_empty(c));
+                __syncwarp();
             }
-            __syncwarp();
-        }
-        if (!ok) {
-            if (um_elect()) um_commit(last_products);
-            __syncwarp();
-            um_settle(last_products, 0);                                 // none in flight when tensor memory is given back
-        }
-    } else {
-        // ================================ steps: four tokens a lane ================================
-        const float rate = reinterpret_cast<const float*>(a.a)[h] * 1.4426950408889634f, bias = a.dt_bias ? reinterpret_cast<const float*>(a.dt_bias)[h] : 0.0f;
-        const __nv_bfloat16* dt = reinterpret_cast<const __nv_bfloat16*>(a.dt) + (size_t)row0 * a.dt_stride + h;
-        __nv_bfloat16 next[4];
-        auto fetch = [&](uint32_t c) {
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                const uint32_t r = c * SU_Q + 4 * lane + i;
-                next[i] = r < rows ? dt[(size_t)r * a.dt_stride] : __float2bfloat16_rn(0.0f);
+            if (!ok) {
+                if (um_elect()) um_commit(last_products);
+                __syncwarp();
+                um_settle(last_products, 0);                                 // none in flight when tensor memory is given back
             }
-        };
-        if (chunks) fetch(0);
-        for (uint32_t c = 0; c < chunks; ++c) {
-            float step[4], l[4];
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                const bool there = c * SU_Q + 4 * lane + i < rows;
-                step[i] = there ? ss_step(__bfloat162float(next[i]), bias, a.dt_softplus, a.dt_min, a.dt_max) : 0.0f;
-                l[i] = there ? step[i] * rate : 0.0f;
-                l[i] = l[i] < -256.0f ? -256.0f : l[i];      // (nothing is left of a state then; sums stay fine)
+        } else {
+            // ================================ steps: four tokens a lane ================================
+            const float rate = reinterpret_cast<const float*>(a.a)[h] * 1.4426950408889634f, bias = a.dt_bias ? reinterpret_cast<const float*>(a.dt_bias)[h] : 0.0f;
+            const __nv_bfloat16* dt = reinterpret_cast<const __nv_bfloat16*>(a.dt) + (size_t)row0 * a.dt_stride + h;
+            __nv_bfloat16 next[4];
+            auto fetch = [&](uint32_t c) {
+    #pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint32_t r = c * SU_Q + 4 * lane + i;
+                    next[i] = r < rows ? dt[(size_t)r * a.dt_stride] : __float2bfloat16_rn(0.0f);
+                }
+            };
+            if (chunks) fetch(0);
+            for (uint32_t c = 0; c < chunks; ++c) {
+                float step[4], l[4];
+    #pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const bool there = c * SU_Q + 4 * lane + i < rows;
+                    step[i] = there ? ss_step(__bfloat162float(next[i]), bias, a.dt_softplus, a.dt_min, a.dt_max) : 0.0f;
+                    l[i] = there ? step[i] * rate : 0.0f;
+                    l[i] = l[i] < -256.0f ? -256.0f : l[i];      // (nothing is left of a state then; sums stay fine)
+                }
+                if (c + 1 < chunks) fetch(c + 1);
+                const float f0 = l[0], f1 = f0 + l[1], f2 = f1 + l[2], f3 = f2 + l[3], b2 = l[3], b1 = b2 + l[2], b0 = b1 + l[1];
+                float up = f3, down = b0 + l[0];
+    #pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const float u = __shfl_up_sync(0xffffffffu, up, o), d = __shfl_down_sync(0xffffffffu, down, o);
+                    if (lane >= o) up += u;
+                    if (lane + o < 32) down += d;
+                }
+                float before = __shfl_up_sync(0xffffffffu, up, 1), behind = __shfl_down_sync(0xffffffffu, down, 1);
+                if (lane == 0) before = 0.0f;
+                if (lane == 31) behind = 0.0f;
+                ok = um_wait(d_empty(c), four(c) ^ 1u, &gave_up, 0x716u);
+                if (!ok) break;
+                *reinterpret_cast<float4*>(&steps[c & 3u][4 * lane]) = make_float4(step[0], step[1], step[2], step[3]);
+                *reinterpret_cast<float4*>(&front[c & 3u][4 * lane]) = make_float4(before + f0, before + f1, before + f2, before + f3);
+                *reinterpret_cast<float4*>(&back[c & 3u][4 * lane]) = make_float4(behind + b0, behind + b1, behind + b2, behind);
+                um_arrive(d_full(c));
             }
-            if (c + 1 < chunks) fetch(c + 1);
-            const float f0 = l[0], f1 = f0 + l[1], f2 = f1 + l[2], f3 = f2 + l[3], b2 = l[3], b1 = b2 + l[2], b0 = b1 + l[1];
-            float up = f3, down = b0 + l[0];
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const float u = __shfl_up_sync(0xffffffffu, up, o), d = __shfl_down_sync(0xffffffffu, down, o);
-                if (lane >= o) up += u;
-                if (lane + o < 32) down += d;
-            }
-            float before = __shfl_up_sync(0xffffffffu, up, 1), behind = __shfl_down_sync(0xffffffffu, down, 1);
-            if (lane == 0) before = 0.0f;
-            if (lane == 31) behind = 0.0f;
-            ok = um_wait(d_empty(c), four(c) ^ 1u, &gave_up, p.error, 0x716u);
-            if (!ok) break;
-            *reinterpret_cast<float4*>(&steps[c & 3u][4 * lane]) = make_float4(step[0], step[1], step[2], step[3]);
-            *reinterpret_cast<float4*>(&front[c & 3u][4 * lane]) = make_float4(before + f0, before + f1, before + f2, before + f3);
-            *reinterpret_cast<float4*>(&back[c & 3u][4 * lane]) = make_float4(behind + b0, behind + b1, behind + b2, behind);
-            um_arrive(d_full(c));
         }
     }
 
     __syncthreads();
+    if (tid == 0) um_report(&gave_up, p.error);
     um_fence_before();
     __syncthreads();
     if (warp == 0) {

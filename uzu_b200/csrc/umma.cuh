@@ -49,23 +49,19 @@ __device__ __forceinline__ uint64_t um_now() {
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     return t;
 }
-// false: the phase did not complete within about a second, or another role of the CTA has given up
-__device__ __noinline__ inline bool um_wait_long(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up, unsigned int* error, uint32_t code) {
-    const uint64_t t0 = um_now();
-    for (uint32_t tries = 1;; ++tries) {
-        if (um_try(bar, parity)) return true;
-        if (tries & 15u) continue;
-        if (*gave_up) return false;
-        if (um_now() - t0 > 1000000000ull) {
-            *gave_up = 1;
-            report_wait_error(error, code);
-            return false;
-        }
-    }
-}
-__device__ __forceinline__ bool um_wait(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up, unsigned int* error, uint32_t code) {      // by whole warps
+// By whole warps. false: the phase did not complete within about a second, or another role of the CTA has given up; gave_up then holds the code, which the CTA reports at its
+// end (um_report). Inline and short: a call would hold its caller's registers down, and many roles share the instruction caches.
+__device__ __forceinline__ bool um_wait(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up, uint32_t code) {
     if (__all_sync(0xffffffffu, um_try(bar, parity))) return true;
-    return __all_sync(0xffffffffu, um_wait_long(bar, parity, gave_up, error, code));
+    const uint64_t until = um_now() + 1000000000ull;
+    while (!__all_sync(0xffffffffu, um_try(bar, parity))) {
+        if (__any_sync(0xffffffffu, um_now() > until)) *gave_up = code;
+        if (__any_sync(0xffffffffu, *gave_up != 0)) return false;
+    }
+    return true;
+}
+__device__ __forceinline__ void um_report(volatile uint32_t* gave_up, unsigned int* error) {
+    if (*gave_up) report_wait_error(error, *gave_up);
 }
 __device__ __forceinline__ bool um_elect() {
     uint32_t p = 0;
@@ -130,6 +126,11 @@ __device__ __forceinline__ void um_st8(uint32_t taddr, const uint32_t (&v)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 __device__ __forceinline__ void um_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// a warpgroup's registers (of every thread; the warpgroups' shares together are what the block was launched with)
+template <uint32_t R>
+__device__ __forceinline__ void um_fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
+template <uint32_t R>
+__device__ __forceinline__ void um_more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
 __device__ __forceinline__ uint32_t um_pack(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
