@@ -213,16 +213,17 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                 um_arrive(s_full);
             }
         };
-        if (chunks) store();
-        float total = 0.0f;
-        for (uint32_t c = 0; c < chunks; ++c) {
+        float total = 0.0f, end = 0.0f;      // log2 of all decays, of the chunk's whose parts were made last
+        // x of chunk c times its weights, as two bf16 parts (the products that read the parts before are done)
+        auto parts_of = [&](uint32_t c) {
             const uint32_t x0 = base + (c & 1u) * SU_STAGE, b0 = x0 + SU_BLOCK, valid = min(SU_Q, rows - c * SU_Q);
             ok = um_wait(d_full(c), four(c), &gave_up, 0x704u);
             if (ok) ok = um_wait(x_full(c), two(c), &gave_up, 0x705u);
             if (ok && valid < SU_Q) ok = um_wait(bc_full(c), two(c), &gave_up, 0x717u);      // (b's rows are there)
-            if (!ok) break;
+            if (!ok) return;
             // (the products that read the parts of chunk c - 1 are done: u_full was waited for)
-            const float weight = um_ldf(&steps[c & 3u][t]) * ss_exp2(um_ldf(&back[c & 3u][t])), end = um_ldf(&front[c & 3u][SU_Q - 1]);
+            const float weight = um_ldf(&steps[c & 3u][t]) * ss_exp2(um_ldf(&back[c & 3u][t]));
+            end = um_ldf(&front[c & 3u][SU_Q - 1]);
             const float2 w2 = make_float2(weight, weight);
             total += end;
             bool odd = false;
@@ -275,7 +276,12 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             um_arrive(w_full);
             um_arrive(o_full(c));
             um_arrive(d_empty(c));
-
+        };
+        if (chunks) {
+            store();
+            parts_of(0);
+        }
+        for (uint32_t c = 0; c < chunks && ok; ++c) {
             const float f = ss_exp2(end);
             const float2 f2 = make_float2(f, f);
             ok = um_wait(u_full, c & 1u, &gave_up, 0x706u);
@@ -288,13 +294,15 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
 #pragma unroll
                 for (uint32_t j = 0; j < 16; j += 2) {
                     const float2 old = ss_fma2(f2, make_float2(S[k * 16 + j], S[k * 16 + j + 1]), make_float2(__uint_as_float(hi[j]), __uint_as_float(hi[j + 1])));
-                    S[k * 16 + j] = old.x + __uint_as_float(lo[j]);
-                    S[k * 16 + j + 1] = old.y + __uint_as_float(lo[j + 1]);
+                    const float2 now = ss_add2(old, make_float2(__uint_as_float(lo[j]), __uint_as_float(lo[j + 1])));
+                    S[k * 16 + j] = now.x;
+                    S[k * 16 + j + 1] = now.y;
                 }
             }
             um_fence_before();
             if (c + 1 < chunks) {
-                if (!STATE) ok = um_wait(s_free, c & 1u, &gave_up, 0x707u);      // the operand before is read
+                parts_of(c + 1);      // (first: the next sum waits for them)
+                if (!STATE && ok) ok = um_wait(s_free, c & 1u, &gave_up, 0x707u);      // the operand before is read
                 if (!ok) break;
                 store();
             }
