@@ -20,7 +20,8 @@ namespace uzu {
 namespace {
 
 constexpr uint32_t SU_Q = 128, SU_P = 64, SU_THREADS = 28 * 32, SU_BLOCK = SU_Q * 128;      // tokens of a chunk, rows of the state, bytes of 64 columns of a chunk
-constexpr uint32_t SU_STAGE = 5 * SU_BLOCK, SU_WX = 2 * SU_STAGE, SU_S = SU_WX + 2 * SU_BLOCK;
+// shared memory: x of three chunks (its place takes the chunk's results when nobody needs it any more), b of two, c, z, the parts, the state's operand
+constexpr uint32_t SU_B = 3 * SU_BLOCK, SU_C = SU_B + 4 * SU_BLOCK, SU_Z = SU_C + 2 * SU_BLOCK, SU_WX = SU_Z + SU_BLOCK, SU_S = SU_WX + 2 * SU_BLOCK;
 constexpr size_t SU_SMEM = SU_S + SU_BLOCK + 1024;
 // registers of a thread: of the scores' warps, the states' and outputs', the others'; together those of the launch (896 threads with 72)
 constexpr uint32_t SU_SCORES_REGS = 56, SU_WORK_REGS = 88, SU_OTHER_REGS = 40;
@@ -47,7 +48,7 @@ template <int N, bool STATE>
 __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c,
                                                                   const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_z, const __grid_constant__ ScanUmmaParams p) {
     extern __shared__ uint8_t su_raw[];
-    __shared__ __align__(8) uint64_t bars[41];
+    __shared__ __align__(8) uint64_t bars[47];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t gave_up;
     __shared__ __align__(16) float steps[4][SU_Q], front[4][SU_Q], back[4][SU_Q];      // [chunk & 3][token]: step, log2 of the decays up to it, behind it
@@ -56,18 +57,22 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
     const uzu_state_space_scan_args& a = p.a;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const uint32_t base = (um_smem(su_raw) + 1023u) & ~1023u, bar0 = um_smem(bars);
-    auto x_full = [&](uint32_t c) { return bar0 + 8u * (c & 1u); };
-    auto x_empty = [&](uint32_t c) { return bar0 + 8u * (2 + (c & 1u)); };
-    auto bc_full = [&](uint32_t c) { return bar0 + 8u * (4 + (c & 1u)); };
-    auto bc_empty = [&](uint32_t c) { return bar0 + 8u * (6 + (c & 1u)); };
-    auto d_full = [&](uint32_t c) { return bar0 + 8u * (8 + (c & 3u)); };
-    auto d_empty = [&](uint32_t c) { return bar0 + 8u * (12 + (c & 3u)); };
-    auto o_full = [&](uint32_t c) { return bar0 + 8u * (16 + (c & 3u)); };             // odd_rows
-    auto out_full = [&](uint32_t c, uint32_t block) { return bar0 + 8u * (20 + (c & 1u) * 4 + block); };      // both halves of 32 rows of output
-    const uint32_t g_full = bar0 + 8u * 28, p_full = bar0 + 8u * 30, w_full = bar0 + 8u * 31, s_full = bar0 + 8u * 32, y_full = bar0 + 8u * 33, y_empty = bar0 + 8u * 34,
-                   u_full = bar0 + 8u * 35, last_products = bar0 + 8u * 36, s_free = bar0 + 8u * 29;
-    auto two = [](uint32_t c) { return c >> 1 & 1u; };      // parities of rings of two and four
+    // rings of three (x), two (b), one and four (steps, odd_rows): a chunk's barrier, the parity of its use
+    auto x_full = [&](uint32_t c) { return bar0 + 8u * (c % 3u); };
+    auto x_empty = [&](uint32_t c) { return bar0 + 8u * (3 + c % 3u); };
+    auto b_full = [&](uint32_t c) { return bar0 + 8u * (6 + (c & 1u)); };
+    auto b_empty = [&](uint32_t c) { return bar0 + 8u * (8 + (c & 1u)); };
+    auto d_full = [&](uint32_t c) { return bar0 + 8u * (10 + (c & 3u)); };
+    auto d_empty = [&](uint32_t c) { return bar0 + 8u * (14 + (c & 3u)); };
+    auto o_full = [&](uint32_t c) { return bar0 + 8u * (18 + (c & 3u)); };             // odd_rows
+    auto out_full = [&](uint32_t c, uint32_t block) { return bar0 + 8u * (22 + (c % 3u) * 4 + block); };      // both halves of 32 rows of output
+    const uint32_t c_full = bar0 + 8u * 34, c_empty = bar0 + 8u * 35, z_full = bar0 + 8u * 36, z_empty = bar0 + 8u * 37, g_full = bar0 + 8u * 38, p_full = bar0 + 8u * 39, w_full = bar0 + 8u * 40,
+                   s_full = bar0 + 8u * 41, s_free = bar0 + 8u * 42, y_full = bar0 + 8u * 43, y_empty = bar0 + 8u * 44, u_full = bar0 + 8u * 45, last_products = bar0 + 8u * 46;
+    auto two = [](uint32_t c) { return c >> 1 & 1u; };
+    auto three = [](uint32_t c) { return c / 3u & 1u; };
     auto four = [](uint32_t c) { return c >> 2 & 1u; };
+    auto x_at = [&](uint32_t c) { return base + (c % 3u) * SU_BLOCK; };
+    auto b_at = [&](uint32_t c) { return base + SU_B + (c & 1u) * 2 * SU_BLOCK; };
 
     const uint32_t slices = a.head_dim / SU_P, h = blockIdx.x / slices, slice = blockIdx.x % slices, group = h / (a.heads / a.groups);
     const uint32_t tile = blockIdx.y, q = ss_find(p.table, tile);
@@ -79,12 +84,14 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
 
     if (warp == 0) {
         if (lane == 0) {
-            for (uint32_t s = 0; s < 2; ++s) {
-                um_init(x_full(s), 1); um_init(x_empty(s), STATE ? 1 : 4); um_init(bc_full(s), 1); um_init(bc_empty(s), 1);
+            for (uint32_t s = 0; s < 3; ++s) {
+                um_init(x_full(s), 1); um_init(x_empty(s), STATE ? 1 : 4);
                 for (uint32_t k = 0; k < 4; ++k) um_init(out_full(s, k), 2);
             }
+            for (uint32_t s = 0; s < 2; ++s) { um_init(b_full(s), 1); um_init(b_empty(s), 1); }
             for (uint32_t s = 0; s < 4; ++s) { um_init(d_full(s), 1); um_init(d_empty(s), STATE ? 8 : 24); um_init(o_full(s), 8); }
-            um_init(g_full, 1); um_init(s_free, 1); um_init(p_full, 8); um_init(w_full, 8); um_init(s_full, 8); um_init(y_full, 1); um_init(y_empty, 8); um_init(u_full, 1);
+            um_init(c_full, 1); um_init(c_empty, 1); um_init(z_full, 1); um_init(z_empty, 8); um_init(g_full, 1); um_init(p_full, 8); um_init(w_full, 8); um_init(s_full, 8); um_init(s_free, 1);
+            um_init(y_full, 1); um_init(y_empty, 8); um_init(u_full, 1);
             um_init(last_products, 1);
             gave_up = 0;
             um_fence_init();
@@ -216,10 +223,10 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
         float total = 0.0f, end = 0.0f;      // log2 of all decays, of the chunk's whose parts were made last
         // x of chunk c times its weights, as two bf16 parts (the products that read the parts before are done)
         auto parts_of = [&](uint32_t c) {
-            const uint32_t x0 = base + (c & 1u) * SU_STAGE, b0 = x0 + SU_BLOCK, valid = min(SU_Q, rows - c * SU_Q);
+            const uint32_t x0 = x_at(c), b0 = b_at(c), valid = min(SU_Q, rows - c * SU_Q);
             ok = um_wait(d_full(c), four(c), &gave_up, 0x704u);
-            if (ok) ok = um_wait(x_full(c), two(c), &gave_up, 0x705u);
-            if (ok && valid < SU_Q) ok = um_wait(bc_full(c), two(c), &gave_up, 0x717u);      // (b's rows are there)
+            if (ok) ok = um_wait(x_full(c), three(c), &gave_up, 0x705u);
+            if (ok && valid < SU_Q) ok = um_wait(b_full(c), two(c), &gave_up, 0x717u);      // (b's rows are there)
             if (!ok) return;
             // (the products that read the parts of chunk c - 1 are done: u_full was waited for)
             const float weight = um_ldf(&steps[c & 3u][t]) * ss_exp2(um_ldf(&back[c & 3u][t]));
@@ -321,21 +328,16 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
         if (!STATE) {
             const float skip = a.d ? reinterpret_cast<const float*>(a.d)[h] : 0.0f;
             const bool gated = a.z != 0;
-            const __nv_bfloat16* z = reinterpret_cast<const __nv_bfloat16*>(a.z) + (size_t)row0 * a.z_stride + col0 + half * 32;
             __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)row0 * a.out_stride + col0 + half * 32;
-            auto gate_of = [&](uint32_t c, uint32_t i) {      // eight of z, asked for a step ahead
-                const uint32_t r = c * SU_Q + t;
-                return gated && r < rows ? *reinterpret_cast<const uint4*>(z + (size_t)r * a.z_stride + 8 * i) : make_uint4(0, 0, 0, 0);
-            };
-            uint4 next = gate_of(0, 0);
             for (uint32_t c = 0; c < chunks; ++c) {
-                const uint32_t x0 = base + (c & 1u) * SU_STAGE, valid = min(SU_Q, rows - c * SU_Q), r = c * SU_Q + t;
+                const uint32_t x0 = x_at(c), valid = min(SU_Q, rows - c * SU_Q), r = c * SU_Q + t;
                 const bool whole = w * 32 + 32 <= valid;      // all rows of the block are the sequence's
                 if (c && half == 0) {      // the rows stored from x's place a chunk ago are read: x may come there
                     um_store_read();
                     um_arrive(x_empty(c - 1));
                 }
-                ok = um_wait(x_full(c), two(c), &gave_up, 0x708u);
+                ok = um_wait(x_full(c), three(c), &gave_up, 0x708u);
+                if (ok && gated) ok = um_wait(z_full, c & 1u, &gave_up, 0x718u);
                 if (ok) ok = um_wait(d_full(c), four(c), &gave_up, 0x709u);
                 if (ok) ok = um_wait(o_full(c), four(c), &gave_up, 0x70au);
                 if (ok) ok = um_wait(y_full, c & 1u, &gave_up, 0x70bu);
@@ -351,8 +353,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                     uint32_t vi[8], vx[8];
                     um_ld8x2(tmem + lanes + SU_YI + half * 32 + i * 8, tmem + lanes + SU_YX + half * 32 + i * 8, vi, vx);
                     const uint32_t chunk = x0 + t * 128 + (((half * 4 + i) ^ (t & 7u)) << 4);
-                    const uint4 xx = um_lds(chunk), zz = next;
-                    next = gate_of(i < 3 ? c : c + 1, i < 3 ? i + 1 : 0);
+                    const uint4 xx = um_lds(chunk), zz = um_lds(chunk - x0 + base + SU_Z);
                     const uint32_t xs[4] = {xx.x, xx.y, xx.z, xx.w}, zs[4] = {zz.x, zz.y, zz.z, zz.w};
                     float2 y[4];
 #pragma unroll
@@ -380,11 +381,12 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                 }
                 um_fence_before();
                 um_arrive(y_empty);
+                um_arrive(z_empty);      // (its values went into the results)
                 if (whole) um_fence_proxy();
                 um_arrive(out_full(c, w));
                 um_arrive(d_empty(c));
                 if (half == 0) {
-                    ok = um_wait(out_full(c, w), two(c), &gave_up, 0x70cu);
+                    ok = um_wait(out_full(c, w), three(c), &gave_up, 0x70cu);
                     if (!ok) break;
                     if (whole && lane == 0) um_tma_store(&map_out, x0 + w * 4096, col0, row0 + c * SU_Q + w * 32);
                     __syncwarp();
@@ -394,33 +396,66 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
         }
     } else {
         um_fewer_registers<SU_OTHER_REGS>();
-        if (warp == 24 || warp == 27) {
-            // ================================ b and c by TMA, x by another warp (its place is free later) ================================
-            const bool is_x = warp == 27;
-            auto full = [&](uint32_t c) { return is_x ? x_full(c) : bc_full(c); };
-            uint32_t asked = 0;
+        if (warp == 24) {
+            // ================================ b and c by TMA ================================
+            uint32_t asked = 0, asked_c = 0;
             for (uint32_t c = 0; c < chunks; ++c) {
-                const uint32_t x0 = base + (c & 1u) * SU_STAGE, row = row0 + c * SU_Q;
-                ok = um_wait(is_x ? x_empty(c) : bc_empty(c), two(c) ^ 1u, &gave_up, is_x ? 0x70eu : 0x70du);
+                const uint32_t row = row0 + c * SU_Q;
+                ok = um_wait(b_empty(c), two(c) ^ 1u, &gave_up, 0x70du);
                 if (!ok) break;
                 if (um_elect()) {
-                    if (is_x) {
-                        um_expect(x_full(c), SU_BLOCK);
-                        um_tma(x0, &map_x, col0, row, x_full(c));
-                        if (!STATE && a.z) um_tma_prefetch(&map_z, col0, row);      // (read by the threads themselves, a chunk and more later)
-                    } else {
-                        um_expect(bc_full(c), SU_BLOCK * (STATE ? 1 : 2) * (N / 64));
-                        for (uint32_t i = 0; i < N / 64; ++i) {
-                            um_tma(x0 + SU_BLOCK * (1 + i), &map_b, group * N + i * 64, row, bc_full(c));
-                            if (!STATE) um_tma(x0 + SU_BLOCK * (3 + i), &map_c, group * N + i * 64, row, bc_full(c));
-                        }
-                    }
+                    um_expect(b_full(c), SU_BLOCK * (N / 64));
+                    for (uint32_t i = 0; i < N / 64; ++i) um_tma(b_at(c) + SU_BLOCK * i, &map_b, group * N + i * 64, row, b_full(c));
                 }
                 __syncwarp();
                 ++asked;
+                if (STATE) continue;
+                ok = um_wait(c_empty, (c & 1u) ^ 1u, &gave_up, 0x719u);
+                if (!ok) break;
+                if (um_elect()) {
+                    um_expect(c_full, SU_BLOCK * (N / 64));
+                    for (uint32_t i = 0; i < N / 64; ++i) um_tma(base + SU_C + SU_BLOCK * i, &map_c, group * N + i * 64, row, c_full);
+                }
+                __syncwarp();
+                ++asked_c;
             }
-            if (!ok)      // copies that are on their way end before the CTA does
-                for (uint32_t n = 1; n <= 2 && n <= asked; ++n) um_settle(full(asked - n), two(asked - n));
+            if (!ok) {      // copies that are on their way end before the CTA does
+                for (uint32_t n = 1; n <= 2 && n <= asked; ++n) um_settle(b_full(asked - n), two(asked - n));
+                if (asked_c) um_settle(c_full, (asked_c - 1) & 1u);
+            }
+        } else if (warp == 27) {
+            // ================================ z and x by TMA: places that results leave ================================
+            uint32_t asked_x = 0, asked_z = 0;
+            auto x_of = [&](uint32_t c) {
+                if (c >= chunks || !ok) return;
+                ok = um_wait(x_empty(c), three(c) ^ 1u, &gave_up, 0x70eu);
+                if (!ok) return;
+                if (um_elect()) {
+                    um_expect(x_full(c), SU_BLOCK);
+                    um_tma(x_at(c), &map_x, col0, row0 + c * SU_Q, x_full(c));
+                }
+                __syncwarp();
+                ++asked_x;
+            };
+            x_of(0);
+            x_of(1);
+            for (uint32_t c = 0; c < chunks && ok; ++c) {
+                if (!STATE && a.z) {
+                    ok = um_wait(z_empty, (c & 1u) ^ 1u, &gave_up, 0x71au);
+                    if (!ok) break;
+                    if (um_elect()) {
+                        um_expect(z_full, SU_BLOCK);
+                        um_tma(base + SU_Z, &map_z, col0, row0 + c * SU_Q, z_full);
+                    }
+                    __syncwarp();
+                    ++asked_z;
+                }
+                x_of(c + 2);
+            }
+            if (!ok) {
+                for (uint32_t n = 1; n <= 3 && n <= asked_x; ++n) um_settle(x_full(asked_x - n), three(asked_x - n));
+                if (asked_z) um_settle(z_full, (asked_z - 1) & 1u);
+            }
         } else if (warp == 25) {
             // ================================ products ================================
             // shared-memory descriptors: 128-byte swizzle, 1024 bytes between groups of 8 rows, SU_BLOCK between blocks of 64 columns
@@ -428,8 +463,9 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             constexpr uint32_t common = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24), a_wide = 1u << 15, b_wide = 1u << 16;
             constexpr uint32_t i_scores = common | ((128u >> 3) << 17), i_y = common | b_wide | ((64u >> 3) << 17), i_u = common | a_wide | b_wide | ((128u >> 3) << 17);
             auto scores = [&](uint32_t c) {
-                const uint32_t b0 = base + (c & 1u) * SU_STAGE + SU_BLOCK, c0 = b0 + 2 * SU_BLOCK;
-                ok = um_wait(bc_full(c), two(c), &gave_up, 0x70fu);
+                const uint32_t b0 = b_at(c), c0 = base + SU_C;
+                ok = um_wait(b_full(c), two(c), &gave_up, 0x70fu);
+                if (ok) ok = um_wait(c_full, c & 1u, &gave_up, 0x71bu);
                 if (!ok) return;
                 um_fence_after();
                 if (um_elect()) {
@@ -445,8 +481,8 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             if (!STATE && chunks) scores(0);
             // What needs no scores runs while they are made, and gives b's and c's place away early: the next chunk but one is there when its turn comes.
             for (uint32_t c = 0; c < chunks && ok; ++c) {
-                const uint32_t x0 = base + (c & 1u) * SU_STAGE, b0 = x0 + SU_BLOCK, c0 = b0 + 2 * SU_BLOCK;
-                if (STATE) ok = um_wait(bc_full(c), two(c), &gave_up, 0x714u);
+                const uint32_t x0 = x_at(c), b0 = b_at(c), c0 = base + SU_C;
+                if (STATE) ok = um_wait(b_full(c), two(c), &gave_up, 0x714u);
                 if (ok) ok = um_wait(w_full, c & 1u, &gave_up, 0x715u);
                 if (!ok) break;
                 um_fence_after();
@@ -455,16 +491,12 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
 #pragma unroll
                     for (uint32_t kk = 0; kk < SU_Q / 16; ++kk) um_mma_ss(tmem + SU_U, wide | ((b0 + kk * 2048u) >> 4), wide | ((base + SU_WX + kk * 2048u) >> 4), i_u, kk != 0);
                     um_commit(u_full);
-                    if (STATE) {
-                        um_commit(bc_empty(c));
-                        um_commit(x_empty(c));
-                    }
+                    um_commit(b_empty(c));
+                    if (STATE) um_commit(x_empty(c));
                 }
                 __syncwarp();
                 if (STATE) continue;
-                ok = um_wait(p_full, c & 1u, &gave_up, 0x711u);      // (the scores' sums are read, too)
-                if (ok && c + 1 < chunks) scores(c + 1);
-                if (ok) ok = um_wait(s_full, c & 1u, &gave_up, 0x712u);
+                ok = um_wait(s_full, c & 1u, &gave_up, 0x712u);
                 if (ok && c) ok = um_wait(y_empty, (c - 1) & 1u, &gave_up, 0x713u);
                 if (!ok) break;
                 um_fence_after();
@@ -473,12 +505,19 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                     for (uint32_t kk = 0; kk < N / 16; ++kk)
                         um_mma_ss(tmem + SU_YX, k_major | ((c0 + (kk >> 2) * SU_BLOCK + (kk & 3u) * 32u) >> 4), wide | ((base + SU_S + kk * 2048u) >> 4), i_y, kk != 0);
                     um_commit(s_free);
-                    um_commit(bc_empty(c));
+                    um_commit(c_empty);
+                }
+                __syncwarp();
+                ok = um_wait(p_full, c & 1u, &gave_up, 0x711u);      // (the scores' sums are read, too)
+                if (!ok) break;
+                um_fence_after();
+                if (um_elect()) {
 #pragma unroll
                     for (uint32_t kk = 0; kk < SU_Q / 16; ++kk) um_mma_ts(tmem + SU_YI, tmem + SU_SCORES + kk * 8u, wide | ((x0 + kk * 2048u) >> 4), i_y, kk != 0);
                     um_commit(y_full);
                 }
                 __syncwarp();
+                if (c + 1 < chunks) scores(c + 1);
             }
             if (!ok) {
                 if (um_elect()) um_commit(last_products);
