@@ -20,8 +20,8 @@ namespace uzu {
 namespace {
 
 constexpr uint32_t SU_Q = 128, SU_P = 64, SU_THREADS = 28 * 32, SU_BLOCK = SU_Q * 128;      // tokens of a chunk, rows of the state, bytes of 64 columns of a chunk
-// shared memory: x of three chunks (its place takes the chunk's results when nobody needs it any more), b of two, c, z, the parts, the state's operand
-constexpr uint32_t SU_B = 3 * SU_BLOCK, SU_C = SU_B + 4 * SU_BLOCK, SU_Z = SU_C + 2 * SU_BLOCK, SU_WX = SU_Z + SU_BLOCK, SU_S = SU_WX + 2 * SU_BLOCK;
+// shared memory: x, z (whose place takes the chunk's results) and b of two chunks, c, the parts, the state's operand
+constexpr uint32_t SU_Z = 2 * SU_BLOCK, SU_B = SU_Z + 2 * SU_BLOCK, SU_C = SU_B + 4 * SU_BLOCK, SU_WX = SU_C + 2 * SU_BLOCK, SU_S = SU_WX + 2 * SU_BLOCK;
 constexpr size_t SU_SMEM = SU_S + SU_BLOCK + 1024;
 // registers of a thread: of the scores' warps, the states' and outputs', the others'; together those of the launch (896 threads with 72)
 constexpr uint32_t SU_SCORES_REGS = 56, SU_WORK_REGS = 88, SU_OTHER_REGS = 40;
@@ -48,7 +48,7 @@ template <int N, bool STATE>
 __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c,
                                                                   const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_z, const __grid_constant__ ScanUmmaParams p) {
     extern __shared__ uint8_t su_raw[];
-    __shared__ __align__(8) uint64_t bars[47];
+    __shared__ __align__(8) uint64_t bars[43];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t gave_up;
     __shared__ __align__(16) float steps[4][SU_Q], front[4][SU_Q], back[4][SU_Q];      // [chunk & 3][token]: step, log2 of the decays up to it, behind it
@@ -57,21 +57,23 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
     const uzu_state_space_scan_args& a = p.a;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const uint32_t base = (um_smem(su_raw) + 1023u) & ~1023u, bar0 = um_smem(bars);
-    // rings of three (x), two (b), one and four (steps, odd_rows): a chunk's barrier, the parity of its use
-    auto x_full = [&](uint32_t c) { return bar0 + 8u * (c % 3u); };
-    auto x_empty = [&](uint32_t c) { return bar0 + 8u * (3 + c % 3u); };
-    auto b_full = [&](uint32_t c) { return bar0 + 8u * (6 + (c & 1u)); };
-    auto b_empty = [&](uint32_t c) { return bar0 + 8u * (8 + (c & 1u)); };
-    auto d_full = [&](uint32_t c) { return bar0 + 8u * (10 + (c & 3u)); };
-    auto d_empty = [&](uint32_t c) { return bar0 + 8u * (14 + (c & 3u)); };
-    auto o_full = [&](uint32_t c) { return bar0 + 8u * (18 + (c & 3u)); };             // odd_rows
-    auto out_full = [&](uint32_t c, uint32_t block) { return bar0 + 8u * (22 + (c % 3u) * 4 + block); };      // both halves of 32 rows of output
-    const uint32_t c_full = bar0 + 8u * 34, c_empty = bar0 + 8u * 35, z_full = bar0 + 8u * 36, z_empty = bar0 + 8u * 37, g_full = bar0 + 8u * 38, p_full = bar0 + 8u * 39, w_full = bar0 + 8u * 40,
-                   s_full = bar0 + 8u * 41, s_free = bar0 + 8u * 42, y_full = bar0 + 8u * 43, y_empty = bar0 + 8u * 44, u_full = bar0 + 8u * 45, last_products = bar0 + 8u * 46;
+    // rings of two (x, z, b), one, and four (steps, odd_rows): a chunk's barrier, the parity of its use
+    auto x_full = [&](uint32_t c) { return bar0 + 8u * (c & 1u); };
+    auto x_empty = [&](uint32_t c) { return bar0 + 8u * (2 + (c & 1u)); };
+    auto b_full = [&](uint32_t c) { return bar0 + 8u * (4 + (c & 1u)); };
+    auto b_empty = [&](uint32_t c) { return bar0 + 8u * (6 + (c & 1u)); };
+    auto z_full = [&](uint32_t c) { return bar0 + 8u * (8 + (c & 1u)); };
+    auto z_empty = [&](uint32_t c) { return bar0 + 8u * (10 + (c & 1u)); };
+    auto d_full = [&](uint32_t c) { return bar0 + 8u * (12 + (c & 3u)); };
+    auto d_empty = [&](uint32_t c) { return bar0 + 8u * (16 + (c & 3u)); };
+    auto o_full = [&](uint32_t c) { return bar0 + 8u * (20 + (c & 3u)); };             // odd_rows; x and the steps have been seen by who arrives
+    auto out_full = [&](uint32_t c, uint32_t block) { return bar0 + 8u * (24 + (c & 1u) * 4 + block); };      // both halves of 32 rows of output
+    const uint32_t c_full = bar0 + 8u * 32, c_empty = bar0 + 8u * 33, g_full = bar0 + 8u * 34, p_full = bar0 + 8u * 35, w_full = bar0 + 8u * 36, s_full = bar0 + 8u * 37, s_free = bar0 + 8u * 38,
+                   y_full = bar0 + 8u * 39, y_empty = bar0 + 8u * 40, u_full = bar0 + 8u * 41, last_products = bar0 + 8u * 42;
     auto two = [](uint32_t c) { return c >> 1 & 1u; };
-    auto three = [](uint32_t c) { return c / 3u & 1u; };
     auto four = [](uint32_t c) { return c >> 2 & 1u; };
-    auto x_at = [&](uint32_t c) { return base + (c % 3u) * SU_BLOCK; };
+    auto x_at = [&](uint32_t c) { return base + (c & 1u) * SU_BLOCK; };
+    auto z_at = [&](uint32_t c) { return base + SU_Z + (c & 1u) * SU_BLOCK; };
     auto b_at = [&](uint32_t c) { return base + SU_B + (c & 1u) * 2 * SU_BLOCK; };
 
     const uint32_t slices = a.head_dim / SU_P, h = blockIdx.x / slices, slice = blockIdx.x % slices, group = h / (a.heads / a.groups);
@@ -84,13 +86,12 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
 
     if (warp == 0) {
         if (lane == 0) {
-            for (uint32_t s = 0; s < 3; ++s) {
-                um_init(x_full(s), 1); um_init(x_empty(s), STATE ? 1 : 4);
+            for (uint32_t s = 0; s < 2; ++s) {
+                um_init(x_full(s), 1); um_init(x_empty(s), STATE ? 1 : 8); um_init(b_full(s), 1); um_init(b_empty(s), 1); um_init(z_full(s), 1); um_init(z_empty(s), 4);
                 for (uint32_t k = 0; k < 4; ++k) um_init(out_full(s, k), 2);
             }
-            for (uint32_t s = 0; s < 2; ++s) { um_init(b_full(s), 1); um_init(b_empty(s), 1); }
             for (uint32_t s = 0; s < 4; ++s) { um_init(d_full(s), 1); um_init(d_empty(s), STATE ? 8 : 24); um_init(o_full(s), 8); }
-            um_init(c_full, 1); um_init(c_empty, 1); um_init(z_full, 1); um_init(z_empty, 8); um_init(g_full, 1); um_init(p_full, 8); um_init(w_full, 8); um_init(s_full, 8); um_init(s_free, 1);
+            um_init(c_full, 1); um_init(c_empty, 1); um_init(g_full, 1); um_init(p_full, 8); um_init(w_full, 8); um_init(s_full, 8); um_init(s_free, 1);
             um_init(y_full, 1); um_init(y_empty, 8); um_init(u_full, 1);
             um_init(last_products, 1);
             gave_up = 0;
@@ -104,6 +105,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
     __syncthreads();
     um_fence_after();
     const uint32_t tmem = tmem_slot, w = warp & 3u, half = warp >> 2 & 1u, t = w * 32 + lane, lanes = w << 21;      // of the first 24 warps: block of 32 rows, which of its two warps
+    auto chunk_of = [&](uint32_t row, uint32_t i) { return row * 128 + (((half * 4 + i) ^ (row & 7u)) << 4); };      // 16 bytes of a swizzled row, of this warp's half
     pdl_launch_dependents();
     pdl_wait();
     bool ok = true;
@@ -208,7 +210,6 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                 }
             }
         }
-        auto chunk_of = [&](uint32_t row, uint32_t i) { return row * 128 + (((half * 4 + i) ^ (row & 7u)) << 4); };      // 16 bytes of a swizzled row, of this warp's half
         auto store = [&]() {      // row n of the operand: its rows of the state
             if (!STATE) {
                 if (n < N) {
@@ -225,7 +226,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
         auto parts_of = [&](uint32_t c) {
             const uint32_t x0 = x_at(c), b0 = b_at(c), valid = min(SU_Q, rows - c * SU_Q);
             ok = um_wait(d_full(c), four(c), &gave_up, 0x704u);
-            if (ok) ok = um_wait(x_full(c), three(c), &gave_up, 0x705u);
+            if (ok) ok = um_wait(x_full(c), two(c), &gave_up, 0x705u);
             if (ok && valid < SU_Q) ok = um_wait(b_full(c), two(c), &gave_up, 0x717u);      // (b's rows are there)
             if (!ok) return;
             // (the products that read the parts of chunk c - 1 are done: u_full was waited for)
@@ -329,66 +330,79 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             const float skip = a.d ? reinterpret_cast<const float*>(a.d)[h] : 0.0f;
             const bool gated = a.z != 0;
             __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)row0 * a.out_stride + col0 + half * 32;
+            const float2 skip2 = make_float2(skip, skip);
             for (uint32_t c = 0; c < chunks; ++c) {
-                const uint32_t x0 = x_at(c), valid = min(SU_Q, rows - c * SU_Q), r = c * SU_Q + t;
+                const uint32_t valid = min(SU_Q, rows - c * SU_Q), r = c * SU_Q + t;
                 const bool whole = w * 32 + 32 <= valid;      // all rows of the block are the sequence's
-                if (c && half == 0) {      // the rows stored from x's place a chunk ago are read: x may come there
+                if (c && half == 0) {      // the results stored a chunk ago are read: z may come there
                     um_store_read();
-                    um_arrive(x_empty(c - 1));
+                    um_arrive(z_empty(c - 1));
                 }
-                ok = um_wait(x_full(c), three(c), &gave_up, 0x708u);
-                if (ok && gated) ok = um_wait(z_full, c & 1u, &gave_up, 0x718u);
-                if (ok) ok = um_wait(d_full(c), four(c), &gave_up, 0x709u);
-                if (ok) ok = um_wait(o_full(c), four(c), &gave_up, 0x70au);
+                ok = um_wait(o_full(c), four(c), &gave_up, 0x70au);
                 if (ok) ok = um_wait(y_full, c & 1u, &gave_up, 0x70bu);
                 if (!ok) break;
                 um_fence_after();
                 const float f = ss_exp2(um_ldf(&front[c & 3u][t]));
-                const float2 f2 = make_float2(f, f), skip2 = make_float2(skip, skip);
-                uint32_t odd = 0;
+                const float2 f2 = make_float2(f, f);
+                float2 ys[16];
+                uint32_t seen = 0;
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) odd |= odd_rows[c & 3u][half * 4 + i];
-#pragma unroll 1
                 for (uint32_t i = 0; i < 4; ++i) {
                     uint32_t vi[8], vx[8];
+                    const uint4 xx = um_lds(x_at(c) + chunk_of(t, i));
                     um_ld8x2(tmem + lanes + SU_YI + half * 32 + i * 8, tmem + lanes + SU_YX + half * 32 + i * 8, vi, vx);
-                    const uint32_t chunk = x0 + t * 128 + (((half * 4 + i) ^ (t & 7u)) << 4);
-                    const uint4 xx = um_lds(chunk), zz = um_lds(chunk - x0 + base + SU_Z);
-                    const uint32_t xs[4] = {xx.x, xx.y, xx.z, xx.w}, zs[4] = {zz.x, zz.y, zz.z, zz.w};
-                    float2 y[4];
+                    const uint32_t xs[4] = {xx.x, xx.y, xx.z, xx.w};
+                    seen ^= xx.x;
 #pragma unroll
                     for (uint32_t e = 0; e < 4; ++e) {
-                        y[e] = ss_fma2(f2, make_float2(__uint_as_float(vx[2 * e]), __uint_as_float(vx[2 * e + 1])), make_float2(__uint_as_float(vi[2 * e]), __uint_as_float(vi[2 * e + 1])));
-                        y[e] = ss_fma2(skip2, make_float2(um_lo(xs[e]), um_hi(xs[e])), y[e]);
+                        const float2 y = ss_fma2(f2, make_float2(__uint_as_float(vx[2 * e]), __uint_as_float(vx[2 * e + 1])), make_float2(__uint_as_float(vi[2 * e]), __uint_as_float(vi[2 * e + 1])));
+                        ys[4 * i + e] = ss_fma2(skip2, make_float2(um_lo(xs[e]), um_hi(xs[e])), y);
                     }
-                    if (gated) {
-#pragma unroll
-                        for (uint32_t e = 0; e < 4; ++e) y[e] = ss_mul2(y[e], ss_silu2(make_float2(um_lo(zs[e]), um_hi(zs[e]))));
-                    }
-                    if (odd) {      // columns whose x was not finite at this token or before it in the chunk
-                        const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x) + (size_t)(row0 + c * SU_Q) * a.x_stride + col0 + half * 32 + i * 8;
-#pragma unroll 1
-                        for (uint32_t j = 0; j <= t; ++j)
-                            if (odd_rows[c & 3u][half * 4 + (j >> 5)] >> (j & 31u) & 1u) {
-#pragma unroll
-                                for (uint32_t e = 0; e < 8; ++e)
-                                    if (!(fabsf(__bfloat162float(x[(size_t)j * a.x_stride + e])) < INFINITY)) (e & 1u ? y[e / 2].y : y[e / 2].x) = __int_as_float(0x7fc00000);
-                            }
-                    }
-                    const uint4 o = make_uint4(um_pack(y[0].x, y[0].y), um_pack(y[1].x, y[1].y), um_pack(y[2].x, y[2].y), um_pack(y[3].x, y[3].y));
-                    if (whole) su_sts(chunk, o.x, o.y, o.z, o.w);      // over x, which nobody needs any more
-                    else if (t < valid) *reinterpret_cast<uint4*>(out + (size_t)r * a.out_stride + i * 8) = o;
                 }
                 um_fence_before();
                 um_arrive(y_empty);
-                um_arrive(z_empty);      // (its values went into the results)
+                um_arrive_after(x_empty(c), seen, a.reserved0);
+                uint32_t odd = 0, bad = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) odd |= odd_rows[c & 3u][half * 4 + i];
+                if (odd) {      // columns whose x was not finite at this token or before it in the chunk
+                    const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x) + (size_t)(row0 + c * SU_Q) * a.x_stride + col0 + half * 32;
+#pragma unroll 1
+                    for (uint32_t j = 0; j <= t; ++j)
+                        if (odd_rows[c & 3u][half * 4 + (j >> 5)] >> (j & 31u) & 1u) {
+#pragma unroll 1
+                            for (uint32_t e = 0; e < 32; ++e)
+                                if (!(fabsf(__bfloat162float(x[(size_t)j * a.x_stride + e])) < INFINITY)) bad |= 1u << e;
+                        }
+                }
+                um_arrive(d_empty(c));
+                ok = um_wait(z_full(c), two(c), &gave_up, 0x718u);
+                if (!ok) break;
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint32_t chunk = z_at(c) + chunk_of(t, i);
+                    float2* y = ys + 4 * i;
+                    if (gated) {
+                        const uint4 zz = um_lds(chunk);
+                        const uint32_t zs[4] = {zz.x, zz.y, zz.z, zz.w};
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e) y[e] = ss_mul2(y[e], ss_silu2(make_float2(um_lo(zs[e]), um_hi(zs[e]))));
+                    }
+                    if (odd) {
+#pragma unroll
+                        for (uint32_t e = 0; e < 8; ++e)
+                            if (bad >> (8 * i + e) & 1u) (e & 1u ? y[e / 2].y : y[e / 2].x) = __int_as_float(0x7fc00000);
+                    }
+                    const uint4 o = make_uint4(um_pack(y[0].x, y[0].y), um_pack(y[1].x, y[1].y), um_pack(y[2].x, y[2].y), um_pack(y[3].x, y[3].y));
+                    if (whole) su_sts(chunk, o.x, o.y, o.z, o.w);      // over z
+                    else if (t < valid) *reinterpret_cast<uint4*>(out + (size_t)r * a.out_stride + i * 8) = o;
+                }
                 if (whole) um_fence_proxy();
                 um_arrive(out_full(c, w));
-                um_arrive(d_empty(c));
                 if (half == 0) {
-                    ok = um_wait(out_full(c, w), three(c), &gave_up, 0x70cu);
+                    ok = um_wait(out_full(c, w), two(c), &gave_up, 0x70cu);
                     if (!ok) break;
-                    if (whole && lane == 0) um_tma_store(&map_out, x0 + w * 4096, col0, row0 + c * SU_Q + w * 32);
+                    if (whole && lane == 0) um_tma_store(&map_out, z_at(c) + w * 4096, col0, row0 + c * SU_Q + w * 32);
                     __syncwarp();
                 }
             }
@@ -424,38 +438,34 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                 if (asked_c) um_settle(c_full, (asked_c - 1) & 1u);
             }
         } else if (warp == 27) {
-            // ================================ z and x by TMA: places that results leave ================================
+            // ================================ x and z by TMA ================================
             uint32_t asked_x = 0, asked_z = 0;
-            auto x_of = [&](uint32_t c) {
-                if (c >= chunks || !ok) return;
-                ok = um_wait(x_empty(c), three(c) ^ 1u, &gave_up, 0x70eu);
-                if (!ok) return;
+            for (uint32_t c = 0; c < chunks; ++c) {
+                ok = um_wait(x_empty(c), two(c) ^ 1u, &gave_up, 0x70eu);
+                if (!ok) break;
                 if (um_elect()) {
                     um_expect(x_full(c), SU_BLOCK);
                     um_tma(x_at(c), &map_x, col0, row0 + c * SU_Q, x_full(c));
                 }
                 __syncwarp();
                 ++asked_x;
-            };
-            x_of(0);
-            x_of(1);
-            for (uint32_t c = 0; c < chunks && ok; ++c) {
-                if (!STATE && a.z) {
-                    ok = um_wait(z_empty, (c & 1u) ^ 1u, &gave_up, 0x71au);
-                    if (!ok) break;
+                if (STATE) continue;
+                ok = um_wait(z_empty(c), two(c) ^ 1u, &gave_up, 0x71au);
+                if (!ok) break;
+                if (a.z) {
                     if (um_elect()) {
-                        um_expect(z_full, SU_BLOCK);
-                        um_tma(base + SU_Z, &map_z, col0, row0 + c * SU_Q, z_full);
+                        um_expect(z_full(c), SU_BLOCK);
+                        um_tma(z_at(c), &map_z, col0, row0 + c * SU_Q, z_full(c));
                     }
                     __syncwarp();
                     ++asked_z;
+                } else um_arrive(z_full(c));      // the place is free
+            }
+            if (!ok)
+                for (uint32_t n = 1; n <= 2; ++n) {
+                    if (n <= asked_x) um_settle(x_full(asked_x - n), two(asked_x - n));
+                    if (n <= asked_z) um_settle(z_full(asked_z - n), two(asked_z - n));
                 }
-                x_of(c + 2);
-            }
-            if (!ok) {
-                for (uint32_t n = 1; n <= 3 && n <= asked_x; ++n) um_settle(x_full(asked_x - n), three(asked_x - n));
-                if (asked_z) um_settle(z_full, (asked_z - 1) & 1u);
-            }
         } else if (warp == 25) {
             // ================================ products ================================
             // shared-memory descriptors: 128-byte swizzle, 1024 bytes between groups of 8 rows, SU_BLOCK between blocks of 64 columns
@@ -636,6 +646,7 @@ bool encode_scan_umma(uzu_command_buffer* cmd, const uzu_state_space_scan_args& 
     ScanUmmaParams p{};
     p.a = a;
     p.error = cmd->ctx->wait_errors.device_word;
+    p.a.reserved0 = 0;      // (um_arrive_after)
     for (uint32_t begin = 0; begin < a.sequence_count;) {
         begin = fill_sequences(p.table, order.data(), a.sequence_count, begin, [&](uint32_t rows) { return cut ? su_parts((uint32_t)(((uint64_t)rows + SU_Q - 1) / SU_Q), su_ctas(a), sms) : 1u; });
         // (one launch behind the other: the next may use the same scratch)
