@@ -285,35 +285,32 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             um_arrive(o_full(c));
             um_arrive(d_empty(c));
         };
-        if (chunks) {
-            store();
-            parts_of(0);
-        }
-        for (uint32_t c = 0; c < chunks && ok; ++c) {
-            const float f = ss_exp2(end);
-            const float2 f2 = make_float2(f, f);
-            ok = um_wait(u_full, c & 1u, &gave_up, 0x706u);
-            if (!ok) break;
-            um_fence_after();
-#pragma unroll
-            for (uint32_t k = 0; k < 2; ++k) {
-                uint32_t hi[16], lo[16];
-                um_ld16x2(tmem + lanes + SU_U + half * 32 + k * 16, tmem + lanes + SU_U + 64 + half * 32 + k * 16, hi, lo);
-#pragma unroll
-                for (uint32_t j = 0; j < 16; j += 2) {
-                    const float2 old = ss_fma2(f2, make_float2(S[k * 16 + j], S[k * 16 + j + 1]), make_float2(__uint_as_float(hi[j]), __uint_as_float(hi[j + 1])));
-                    const float2 now = ss_add2(old, make_float2(__uint_as_float(lo[j]), __uint_as_float(lo[j + 1])));
-                    S[k * 16 + j] = now.x;
-                    S[k * 16 + j + 1] = now.y;
-                }
-            }
-            um_fence_before();
-            if (c + 1 < chunks) {
-                parts_of(c + 1);      // (first: the next sum waits for them)
-                if (!STATE && ok) ok = um_wait(s_free, c & 1u, &gave_up, 0x707u);      // the operand before is read
+        for (uint32_t c = 0;; ++c) {
+            if (c) {      // the sum over chunk c - 1
+                const float f = ss_exp2(end);
+                const float2 f2 = make_float2(f, f);
+                ok = um_wait(u_full, (c - 1) & 1u, &gave_up, 0x706u);
                 if (!ok) break;
-                store();
+                um_fence_after();
+#pragma unroll
+                for (uint32_t k = 0; k < 2; ++k) {
+                    uint32_t hi[16], lo[16];
+                    um_ld16x2(tmem + lanes + SU_U + half * 32 + k * 16, tmem + lanes + SU_U + 64 + half * 32 + k * 16, hi, lo);
+#pragma unroll
+                    for (uint32_t j = 0; j < 16; j += 2) {
+                        const float2 old = ss_fma2(f2, make_float2(S[k * 16 + j], S[k * 16 + j + 1]), make_float2(__uint_as_float(hi[j]), __uint_as_float(hi[j + 1])));
+                        const float2 now = ss_add2(old, make_float2(__uint_as_float(lo[j]), __uint_as_float(lo[j + 1])));
+                        S[k * 16 + j] = now.x;
+                        S[k * 16 + j + 1] = now.y;
+                    }
+                }
+                um_fence_before();
             }
+            if (c == chunks) break;
+            parts_of(c);      // (first: the next sum waits for them)
+            if (!STATE && ok && c) ok = um_wait(s_free, (c - 1) & 1u, &gave_up, 0x707u);      // the operand before is read
+            if (!ok) break;
+            store();
         }
         if (ok && n < N) {
             float* to = STATE ? end_of(part) : slot;
@@ -472,62 +469,62 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             constexpr uint64_t desc = (uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32, k_major = desc | (1u << 16), wide = desc | ((uint64_t)(SU_BLOCK >> 4) << 16);
             constexpr uint32_t common = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24), a_wide = 1u << 15, b_wide = 1u << 16;
             constexpr uint32_t i_scores = common | ((128u >> 3) << 17), i_y = common | b_wide | ((64u >> 3) << 17), i_u = common | a_wide | b_wide | ((128u >> 3) << 17);
-            auto scores = [&](uint32_t c) {
-                const uint32_t b0 = b_at(c), c0 = base + SU_C;
-                ok = um_wait(b_full(c), two(c), &gave_up, 0x70fu);
-                if (ok) ok = um_wait(c_full, c & 1u, &gave_up, 0x71bu);
-                if (!ok) return;
-                um_fence_after();
-                if (um_elect()) {
-#pragma unroll
-                    for (uint32_t kk = 0; kk < N / 16; ++kk) {
-                        const uint32_t o = (kk >> 2) * SU_BLOCK + (kk & 3u) * 32u;
-                        um_mma_ss(tmem + SU_G, k_major | ((c0 + o) >> 4), k_major | ((b0 + o) >> 4), i_scores, kk != 0);
+            // What needs no scores runs while they are made.
+            for (uint32_t k = 0; k <= chunks; ++k) {
+                if (k) {
+                    const uint32_t c = k - 1, x0 = x_at(c), b0 = b_at(c), c0 = base + SU_C;
+                    if (STATE) ok = um_wait(b_full(c), two(c), &gave_up, 0x714u);
+                    if (ok) ok = um_wait(w_full, c & 1u, &gave_up, 0x715u);
+                    if (!ok) break;
+                    um_fence_after();
+                    if (um_elect()) {
+                        // (64 columns: operand A's second block is whatever lies behind; the sums' lanes 64 .. 127 are not read)
+#pragma unroll 1
+                        for (uint32_t kk = 0; kk < SU_Q / 16; ++kk) um_mma_ss(tmem + SU_U, wide | ((b0 + kk * 2048u) >> 4), wide | ((base + SU_WX + kk * 2048u) >> 4), i_u, kk != 0);
+                        um_commit(u_full);
+                        um_commit(b_empty(c));
+                        if (STATE) um_commit(x_empty(c));
                     }
-                    um_commit(g_full);
+                    __syncwarp();
+                    if (STATE) continue;
+                    ok = um_wait(s_full, c & 1u, &gave_up, 0x712u);
+                    if (ok && c) ok = um_wait(y_empty, (c - 1) & 1u, &gave_up, 0x713u);
+                    if (!ok) break;
+                    um_fence_after();
+                    if (um_elect()) {
+#pragma unroll 1
+                        for (uint32_t kk = 0; kk < N / 16; ++kk)
+                            um_mma_ss(tmem + SU_YX, k_major | ((c0 + (kk >> 2) * SU_BLOCK + (kk & 3u) * 32u) >> 4), wide | ((base + SU_S + kk * 2048u) >> 4), i_y, kk != 0);
+                        um_commit(s_free);
+                        um_commit(c_empty);
+                    }
+                    __syncwarp();
+                    ok = um_wait(p_full, c & 1u, &gave_up, 0x711u);      // (the scores' sums are read, too)
+                    if (!ok) break;
+                    um_fence_after();
+                    if (um_elect()) {
+#pragma unroll 1
+                        for (uint32_t kk = 0; kk < SU_Q / 16; ++kk) um_mma_ts(tmem + SU_YI, tmem + SU_SCORES + kk * 8u, wide | ((x0 + kk * 2048u) >> 4), i_y, kk != 0);
+                        um_commit(y_full);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
-            };
-            if (!STATE && chunks) scores(0);
-            // What needs no scores runs while they are made, and gives b's and c's place away early: the next chunk but one is there when its turn comes.
-            for (uint32_t c = 0; c < chunks && ok; ++c) {
-                const uint32_t x0 = x_at(c), b0 = b_at(c), c0 = base + SU_C;
-                if (STATE) ok = um_wait(b_full(c), two(c), &gave_up, 0x714u);
-                if (ok) ok = um_wait(w_full, c & 1u, &gave_up, 0x715u);
-                if (!ok) break;
-                um_fence_after();
-                if (um_elect()) {
-                    // (64 columns: operand A's second block is whatever lies behind; the sums' lanes 64 .. 127 are not read)
-#pragma unroll
-                    for (uint32_t kk = 0; kk < SU_Q / 16; ++kk) um_mma_ss(tmem + SU_U, wide | ((b0 + kk * 2048u) >> 4), wide | ((base + SU_WX + kk * 2048u) >> 4), i_u, kk != 0);
-                    um_commit(u_full);
-                    um_commit(b_empty(c));
-                    if (STATE) um_commit(x_empty(c));
+                if (k < chunks && !STATE) {
+                    const uint32_t b0 = b_at(k), c0 = base + SU_C;
+                    ok = um_wait(b_full(k), two(k), &gave_up, 0x70fu);
+                    if (ok) ok = um_wait(c_full, k & 1u, &gave_up, 0x71bu);
+                    if (!ok) break;
+                    um_fence_after();
+                    if (um_elect()) {
+#pragma unroll 1
+                        for (uint32_t kk = 0; kk < N / 16; ++kk) {
+                            const uint32_t o = (kk >> 2) * SU_BLOCK + (kk & 3u) * 32u;
+                            um_mma_ss(tmem + SU_G, k_major | ((c0 + o) >> 4), k_major | ((b0 + o) >> 4), i_scores, kk != 0);
+                        }
+                        um_commit(g_full);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
-                if (STATE) continue;
-                ok = um_wait(s_full, c & 1u, &gave_up, 0x712u);
-                if (ok && c) ok = um_wait(y_empty, (c - 1) & 1u, &gave_up, 0x713u);
-                if (!ok) break;
-                um_fence_after();
-                if (um_elect()) {
-#pragma unroll
-                    for (uint32_t kk = 0; kk < N / 16; ++kk)
-                        um_mma_ss(tmem + SU_YX, k_major | ((c0 + (kk >> 2) * SU_BLOCK + (kk & 3u) * 32u) >> 4), wide | ((base + SU_S + kk * 2048u) >> 4), i_y, kk != 0);
-                    um_commit(s_free);
-                    um_commit(c_empty);
-                }
-                __syncwarp();
-                ok = um_wait(p_full, c & 1u, &gave_up, 0x711u);      // (the scores' sums are read, too)
-                if (!ok) break;
-                um_fence_after();
-                if (um_elect()) {
-#pragma unroll
-                    for (uint32_t kk = 0; kk < SU_Q / 16; ++kk) um_mma_ts(tmem + SU_YI, tmem + SU_SCORES + kk * 8u, wide | ((x0 + kk * 2048u) >> 4), i_y, kk != 0);
-                    um_commit(y_full);
-                }
-                __syncwarp();
-                if (c + 1 < chunks) scores(c + 1);
             }
             if (!ok) {
                 if (um_elect()) um_commit(last_products);

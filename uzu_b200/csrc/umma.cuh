@@ -49,16 +49,28 @@ __device__ __forceinline__ uint64_t um_now() {
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     return t;
 }
-// By whole warps. false: the phase did not complete within about a second, or another role of the CTA has given up; gave_up then holds the code, which the CTA reports at its
-// end (um_report). Inline and short: a call would hold its caller's registers down, and many roles share the instruction caches.
+// By whole warps. false: the phase did not complete within about a second; gave_up then holds the code, which the CTA reports at its end (um_report), and the roles that wait for
+// this one run out the same way. As few instructions as it takes: a call would hold its caller's registers down, and what many roles run has to fit the instruction caches.
 __device__ __forceinline__ bool um_wait(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up, uint32_t code) {
-    if (__all_sync(0xffffffffu, um_try(bar, parity))) return true;
-    const uint64_t until = um_now() + 1000000000ull;
-    while (!__all_sync(0xffffffffu, um_try(bar, parity))) {
-        if (__any_sync(0xffffffffu, um_now() > until)) *gave_up = code;
-        if (__any_sync(0xffffffffu, *gave_up != 0)) return false;
-    }
-    return true;
+    uint32_t ok;
+    asm volatile(
+        "{ .reg .pred p, q; .reg .u64 t, e;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n"
+        "@p bra DONE_%=;\n"
+        "mov.u64 e, %%globaltimer;\n"
+        "add.u64 e, e, 1000000000;\n"
+        "WAIT_%=: mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n"
+        "@p bra DONE_%=;\n"
+        "mov.u64 t, %%globaltimer;\n"
+        "setp.lt.u64 q, t, e;\n"
+        "@q bra WAIT_%=;\n"
+        "DONE_%=: selp.u32 %0, 1, 0, p; }"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (__all_sync(0xffffffffu, ok)) return true;
+    *gave_up = code;
+    return false;
 }
 __device__ __forceinline__ void um_report(volatile uint32_t* gave_up, unsigned int* error) {
     if (*gave_up) report_wait_error(error, *gave_up);
