@@ -13,7 +13,7 @@ constexpr uint32_t CC_THREADS = 128;
 
 struct ConvParams {
     uzu_causal_conv_args a;
-    uint32_t strip;      // rows
+    uint32_t strip, groups;      // rows of a strip, blocks beside one another: those of a row run together
     SequenceTable table;
 };
 
@@ -29,23 +29,25 @@ __global__ void __launch_bounds__(CC_THREADS) causal_conv_kernel(const __grid_co
     pdl_launch_dependents();
     pdl_wait();
     const uzu_causal_conv_args& a = p.a;
-    const uint32_t c = (blockIdx.y * CC_THREADS + threadIdx.x) * VEC;
+    const uint32_t c = (blockIdx.x % p.groups * CC_THREADS + threadIdx.x) * VEC;
     if (c >= a.channels) return;
-    const uint32_t tile = blockIdx.x, q = ss_find(p.table, tile);
+    const uint32_t tile = blockIdx.x / p.groups, q = ss_find(p.table, tile);
     const PackedSequence s = p.table.s[q];
     const uint32_t t0 = (tile - s.tile0) * p.strip, t1 = min(t0 + p.strip, s.rows), kept = a.taps - 1;
     const T* in = reinterpret_cast<const T*>(a.input) + (size_t)s.first * a.input_stride + c;
     T* out = reinterpret_cast<T*>(a.output) + (size_t)s.first * a.output_stride + c;
     T* state = reinterpret_cast<T*>(a.state) + (size_t)s.slot() * kept * a.channels + c;
 
-    float w[TAPS][VEC], bias[VEC];
+    constexpr int PAIRS = (VEC + 1) / 2;      // (one channel: a pair's second half is nobody's)
+    float2 w[TAPS][PAIRS], bias[PAIRS];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-        bias[i] = a.bias ? reinterpret_cast<const float*>(a.bias)[c + i] : 0.0f;
+    for (int i = 0; i < 2 * PAIRS; ++i) {
+        const bool there = i < VEC;
+        (i & 1 ? bias[i / 2].y : bias[i / 2].x) = there && a.bias ? reinterpret_cast<const float*>(a.bias)[c + i] : 0.0f;
 #pragma unroll
         for (int j = 0; j < TAPS; ++j) {      // fewer taps than the kernel has: the oldest ones are zero
             const int k = j - (TAPS - (int)a.taps);
-            w[j][i] = k >= 0 ? reinterpret_cast<const float*>(a.weights)[(size_t)(c + i) * a.taps + k] : 0.0f;
+            (i & 1 ? w[j][i / 2].y : w[j][i / 2].x) = there && k >= 0 ? reinterpret_cast<const float*>(a.weights)[(size_t)(c + i) * a.taps + k] : 0.0f;
         }
     }
     // the inputs before the strip, oldest first
@@ -74,34 +76,46 @@ __global__ void __launch_bounds__(CC_THREADS) causal_conv_kernel(const __grid_co
             *reinterpret_cast<V*>(state + (size_t)k * a.channels) = v;
         }
     }
-    float u[TAPS][VEC];      // u[TAPS - 1]: the row at hand
+    float2 u[TAPS][PAIRS];      // u[TAPS - 1]: the row at hand
+    auto pairs = [](const V& v, float2 (&to)[PAIRS]) {
 #pragma unroll
-    for (int j = 0; j < TAPS - 1; ++j)
+        for (int i = 0; i < PAIRS; ++i) to[i] = make_float2(ss_f(v.v[2 * i]), VEC > 1 ? ss_f(v.v[VEC > 1 ? 2 * i + 1 : 0]) : 0.0f);
+    };
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) u[j][i] = ss_f(past[j].v[i]);
+    for (int j = 0; j < TAPS - 1; ++j) pairs(past[j], u[j]);
 
-    for (uint32_t t = t0; t < t1; t += BATCH) {
+    auto step = [&](const V& row) {
+        V o;
+        pairs(row, u[TAPS - 1]);
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+            float2 y = bias[i];
+#pragma unroll
+            for (int j = 0; j < TAPS; ++j) y = ss_fma2(w[j][i], u[j][i], y);
+            if (a.activation == UZU_ACT_SILU) y = ss_silu_pair(y);
+            o.v[2 * i] = ss_t<T>(y.x);
+            if (VEC > 1) o.v[VEC > 1 ? 2 * i + 1 : 0] = ss_t<T>(y.y);
+#pragma unroll
+            for (int j = 0; j < TAPS - 1; ++j) u[j][i] = u[j + 1][i];
+        }
+        return o;
+    };
+    const T* from = in + (size_t)t0 * a.input_stride;
+    T* to = out + (size_t)t0 * a.output_stride;
+    uint32_t left = t1 - t0;
+    for (; left >= BATCH; left -= BATCH) {
         V rows[BATCH];
 #pragma unroll
-        for (int b = 0; b < BATCH; ++b)
-            if (t + b < t1) rows[b] = *reinterpret_cast<const V*>(in + (size_t)(t + b) * a.input_stride);
+        for (int b = 0; b < BATCH; ++b) rows[b] = *reinterpret_cast<const V*>(from + (size_t)b * a.input_stride);
 #pragma unroll
-        for (int b = 0; b < BATCH; ++b) {
-            if (t + b >= t1) break;
-            V o;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                u[TAPS - 1][i] = ss_f(rows[b].v[i]);
-                float y = bias[i];
-#pragma unroll
-                for (int j = 0; j < TAPS; ++j) y = fmaf(w[j][i], u[j][i], y);
-                if (a.activation == UZU_ACT_SILU) y = ss_silu(y);
-                o.v[i] = ss_t<T>(y);
-#pragma unroll
-                for (int j = 0; j < TAPS - 1; ++j) u[j][i] = u[j + 1][i];
-            }
-            *reinterpret_cast<V*>(out + (size_t)(t + b) * a.output_stride) = o;
-        }
+        for (int b = 0; b < BATCH; ++b) *reinterpret_cast<V*>(to + (size_t)b * a.output_stride) = step(rows[b]);
+        from += (size_t)BATCH * a.input_stride;
+        to += (size_t)BATCH * a.output_stride;
+    }
+    for (; left; --left) {
+        *reinterpret_cast<V*>(to) = step(*reinterpret_cast<const V*>(from));
+        from += a.input_stride;
+        to += a.output_stride;
     }
 }
 
@@ -126,8 +140,9 @@ const char* conv_check(const uzu_causal_conv_args* a) {
 }
 
 template <typename T, int VEC>
-void conv_launch(uzu_command_buffer* cmd, const ConvParams& p) {
-    const dim3 grid(p.table.tiles, (p.a.channels + CC_THREADS * VEC - 1) / (CC_THREADS * VEC));
+void conv_launch(uzu_command_buffer* cmd, ConvParams& p) {
+    p.groups = (p.a.channels + CC_THREADS * VEC - 1) / (CC_THREADS * VEC);
+    const dim3 grid(p.table.tiles * p.groups);
     auto go = [&](auto kernel) { launch(cmd, "causal_conv_kernel", kernel, grid, dim3(CC_THREADS), 0, p); };
     if (p.a.taps <= 2) go(causal_conv_kernel<T, VEC, 2>);
     else if (p.a.taps == 3) go(causal_conv_kernel<T, VEC, 3>);
@@ -135,8 +150,8 @@ void conv_launch(uzu_command_buffer* cmd, const ConvParams& p) {
     else go(causal_conv_kernel<T, VEC, 8>);
 }
 template <typename T>
-void conv_by_alignment(uzu_command_buffer* cmd, const ConvParams& p) {
-    constexpr int VEC = 16 / sizeof(T);
+void conv_by_alignment(uzu_command_buffer* cmd, ConvParams& p) {
+    constexpr int VEC = 8 / sizeof(T);
     const uzu_causal_conv_args& a = p.a;
     const bool wide = a.channels % VEC == 0 && a.input_stride % VEC == 0 && a.output_stride % VEC == 0 && ((a.input | a.output | a.state) & 15u) == 0;
     if (wide) conv_launch<T, VEC>(cmd, p);

@@ -63,6 +63,13 @@ __device__ __forceinline__ float2 ss_silu2(float2 x) {
     const float2 d = ss_add2(make_float2(ss_exp2(e.x), ss_exp2(e.y)), make_float2(1.0f, 1.0f));
     return ss_mul2(x, make_float2(ss_rcp(d.x), ss_rcp(d.y)));
 }
+// two of them with one reciprocal, of the product (below -41 the sigmoid stays 2^-60): where special functions are what a loop waits for
+__device__ __forceinline__ float2 ss_silu_pair(float2 x) {
+    const float2 e = ss_mul2(x, make_float2(-1.4426950408889634f, -1.4426950408889634f));
+    const float2 d = ss_add2(make_float2(ss_exp2(fminf(e.x, 60.0f)), ss_exp2(fminf(e.y, 60.0f))), make_float2(1.0f, 1.0f));
+    const float r = ss_rcp(d.x * d.y);
+    return ss_mul2(ss_mul2(x, make_float2(r, r)), make_float2(d.y, d.x));
+}
 // a token's step (log1p: steps of 1e-3 keep their digits); not a number stays so
 __device__ __forceinline__ float ss_step(float dt, float bias, uint32_t softplus, float lo, float hi) {
     float s = dt + bias;
