@@ -190,6 +190,12 @@ def test_scan_forms(ctx, over):
     _scan(ctx, P.F32, 4, 1, 32, 32, RAGGED, 223, 9, **over)
 
 
+@pytest.mark.parametrize("dt", [P.BF16, P.F32])
+@pytest.mark.parametrize("rows,seqs", [(700, [(0, 700, 1, 0)]), (601, [(0, 300, 0, 1), (300, 301, 1, 0)]), (150, [(3, 140, 0, 0)])])
+def test_scan_token_by_token_in_parts(ctx, rows, seqs, dt):
+    _scan(ctx, dt, 2, 1, 40, 24, seqs, rows, 2)
+
+
 def test_scan_many_sequences(ctx):
     _scan(ctx, P.F32, 2, 1, 8, 8, [(3 * i, 1 + i % 3, i, i % 2) for i in range(300)], 900, 300)
 

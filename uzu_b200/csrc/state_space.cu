@@ -17,20 +17,29 @@ constexpr uint32_t SS_THREADS = 128, SS_BATCH = 16, SS_ROWS = 32;
 
 struct ScanParams {
     uzu_state_space_scan_args a;
+    float* ends;       // of the parts: [tile][heads, head_dim, state_size]; the last part's place holds a copy of the start
+    float* logs;       // [tile][heads]: the logarithm of all decays of a part
     SequenceTable table;
 };
 
-// GROUPS: of four columns a thread; columns past state_size are zeros
-template <typename T, int GROUPS>
+// GROUPS: of four columns a thread; columns past state_size are zeros. STATE: only the state at the end of every part but the last
+template <typename T, int GROUPS, bool STATE>
 __global__ void __launch_bounds__(SS_THREADS) state_space_scan_kernel(const __grid_constant__ ScanParams p) {
     constexpr uint32_t COLS = 16 * GROUPS, PER = SS_BATCH * COLS / SS_THREADS, XPER = SS_BATCH * SS_ROWS / SS_THREADS;
     __shared__ __align__(16) float bs[SS_BATCH][COLS], cs[SS_BATCH][COLS];
-    __shared__ float xs[SS_BATCH][SS_ROWS], ys[SS_BATCH][SS_ROWS], decay[SS_BATCH], step[SS_BATCH];
+    __shared__ float xs[SS_BATCH][SS_ROWS], ys[SS_BATCH][SS_ROWS], zs[SS_BATCH][SS_ROWS], decay[SS_BATCH], step[SS_BATCH];
     pdl_launch_dependents();
     pdl_wait();
     const uzu_state_space_scan_args& a = p.a;
     const uint32_t tid = threadIdx.x, h = blockIdx.y, p0 = blockIdx.x * SS_ROWS, part = tid & 3u, pl = tid >> 2, N = a.state_size, P = a.head_dim;
-    const PackedSequence s = p.table.s[blockIdx.z];
+    const uint32_t q = ss_find(p.table, blockIdx.z);
+    PackedSequence s = p.table.s[q];
+    const uint32_t parts = (q + 1 < p.table.count ? p.table.s[q + 1].tile0 : p.table.tiles) - s.tile0, part_of = blockIdx.z - s.tile0;
+    if (STATE && part_of + 1 == parts) return;
+    const uint32_t per = (s.rows + parts - 1) / parts, begin = min(s.rows, part_of * per);
+    const bool nothing = s.rows == 0;
+    s.first += begin;
+    s.rows = min(s.rows - begin, per);
     const bool mine = p0 + pl < P;
     const T* x = reinterpret_cast<const T*>(a.x) + (size_t)s.first * a.x_stride + (size_t)h * P + p0;
     const T* z = reinterpret_cast<const T*>(a.z) + (size_t)s.first * a.z_stride + (size_t)h * P + p0;
@@ -39,23 +48,37 @@ __global__ void __launch_bounds__(SS_THREADS) state_space_scan_kernel(const __gr
     const T* b = reinterpret_cast<const T*>(a.b) + (size_t)s.first * a.b_stride + group;
     const T* c = reinterpret_cast<const T*>(a.c) + (size_t)s.first * a.c_stride + group;
     T* out = reinterpret_cast<T*>(a.out) + (size_t)s.first * a.out_stride + (size_t)h * P + p0;
-    float* state = reinterpret_cast<float*>(a.state) + (((size_t)s.slot() * a.heads + h) * P + p0 + pl) * N;
+    const size_t in_state = ((size_t)h * P + p0 + pl) * N, whole_state = (size_t)a.heads * P * N;
+    float* state = reinterpret_cast<float*>(a.state) + s.slot() * whole_state + in_state;
+    auto end_of = [&](uint32_t k) { return p.ends + (s.tile0 + k) * whole_state + in_state; };
     const float rate = reinterpret_cast<const float*>(a.a)[h], skip = a.d ? reinterpret_cast<const float*>(a.d)[h] : 0.0f;
     const float dt_bias = a.dt_bias ? reinterpret_cast<const float*>(a.dt_bias)[h] : 0.0f;
 
     float2 S[2 * GROUPS];
+    auto each = [&](auto f) {      // of this thread's columns: index in S, column
 #pragma unroll
-    for (int i = 0; i < GROUPS; ++i) {
-        float v[4];
+        for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t n = 16 * i + 4 * part + j;
-            v[j] = mine && n < N && !s.fresh() ? state[n] : 0.0f;
+            for (int j = 0; j < 4; ++j) {
+                float& v = j & 1 ? S[2 * i + j / 2].y : S[2 * i + j / 2].x;
+                const uint32_t n = 16 * i + 4 * part + j;
+                if (mine && n < N) f(v, n);
+            }
+    };
+#pragma unroll
+    for (int i = 0; i < 2 * GROUPS; ++i) S[i] = make_float2(0.0f, 0.0f);
+    if (parts == 1 || (STATE && part_of == 0)) {
+        if (!s.fresh()) each([&](float& v, uint32_t n) { v = state[n]; });
+        if (STATE) each([&](float& v, uint32_t n) { end_of(parts - 1)[n] = v; });
+    } else if (!STATE) {
+        if (part_of == 0) each([&](float& v, uint32_t n) { v = end_of(parts - 1)[n]; });
+        for (uint32_t k = 0; k < part_of; ++k) {      // the parts before, in order
+            const float f = k ? expf(p.logs[(size_t)(s.tile0 + k) * a.heads + h]) : 0.0f;
+            each([&](float& v, uint32_t n) { v = k ? fmaf(f, v, end_of(k)[n]) : end_of(k)[n]; });
         }
-        S[2 * i] = make_float2(v[0], v[1]);
-        S[2 * i + 1] = make_float2(v[2], v[3]);
     }
-    T nb[PER], nc[PER], nx[XPER];
+    float log_sum = 0.0f;      // (thread 0 alone)
+    T nb[PER], nc[PER], nx[XPER], nz[XPER];
     float nd = 0.0f;
     auto fetch = [&](uint32_t t) {
 #pragma unroll
@@ -63,12 +86,14 @@ __global__ void __launch_bounds__(SS_THREADS) state_space_scan_kernel(const __gr
             const uint32_t e = tid + i * SS_THREADS, r = e / COLS, n = e % COLS;
             const bool there = t + r < s.rows && n < N;
             nb[i] = there ? b[(size_t)(t + r) * a.b_stride + n] : ss_t<T>(0.0f);
-            nc[i] = there ? c[(size_t)(t + r) * a.c_stride + n] : ss_t<T>(0.0f);
+            if (!STATE) nc[i] = there ? c[(size_t)(t + r) * a.c_stride + n] : ss_t<T>(0.0f);
         }
 #pragma unroll
         for (uint32_t i = 0; i < XPER; ++i) {
             const uint32_t e = tid + i * SS_THREADS, r = e / SS_ROWS, q = e % SS_ROWS;
-            nx[i] = t + r < s.rows && p0 + q < P ? x[(size_t)(t + r) * a.x_stride + q] : ss_t<T>(0.0f);
+            const bool there = t + r < s.rows && p0 + q < P;
+            nx[i] = there ? x[(size_t)(t + r) * a.x_stride + q] : ss_t<T>(0.0f);
+            if (!STATE) nz[i] = there && a.z ? z[(size_t)(t + r) * a.z_stride + q] : ss_t<T>(0.0f);
         }
         if (tid < SS_BATCH && t + tid < s.rows) nd = ss_f(dt[(size_t)(t + tid) * a.dt_stride]);
     };
@@ -79,70 +104,100 @@ __global__ void __launch_bounds__(SS_THREADS) state_space_scan_kernel(const __gr
         for (uint32_t i = 0; i < PER; ++i) {
             const uint32_t e = tid + i * SS_THREADS;
             bs[e / COLS][e % COLS] = ss_f(nb[i]);
-            cs[e / COLS][e % COLS] = ss_f(nc[i]);
+            if (!STATE) cs[e / COLS][e % COLS] = ss_f(nc[i]);
         }
 #pragma unroll
         for (uint32_t i = 0; i < XPER; ++i) {
             const uint32_t e = tid + i * SS_THREADS;
             xs[e / SS_ROWS][e % SS_ROWS] = ss_f(nx[i]);
+            if (!STATE) zs[e / SS_ROWS][e % SS_ROWS] = a.z ? ss_silu(ss_f(nz[i])) : 1.0f;
         }
-        if (tid < count) {
-            const float v = ss_step(nd, dt_bias, a.dt_softplus, a.dt_min, a.dt_max);
+        if (tid < SS_BATCH) {
+            const float v = tid < count ? ss_step(nd, dt_bias, a.dt_softplus, a.dt_min, a.dt_max) : 0.0f;
             step[tid] = v;
-            decay[tid] = expf(v * rate);
+            decay[tid] = tid < count ? expf(v * rate) : 1.0f;
+            if (STATE) log_sum += v * rate;
         }
         __syncthreads();
         if (t + SS_BATCH < s.rows) fetch(t + SS_BATCH);
+        // four tokens at a time: only a multiplication and an addition of the state depend on the token before, everything else of the four runs side by side (tokens behind the
+        // last have a decay of 1 and a step of 0)
 #pragma unroll 1
-        for (uint32_t r = 0; r < count; ++r) {
-            const float xv = xs[r][pl], sx = step[r] * xv, f = decay[r];
-            const float2 sx2 = make_float2(sx, sx), f2 = make_float2(f, f);
-            float2 y0 = make_float2(0.0f, 0.0f), y1 = y0;
+        for (uint32_t r0 = 0; r0 < count; r0 += 4) {
+            float y[4];
 #pragma unroll
-            for (int i = 0; i < GROUPS; ++i) {
-                const float4 bv = *reinterpret_cast<const float4*>(&bs[r][16 * i + 4 * part]), cv = *reinterpret_cast<const float4*>(&cs[r][16 * i + 4 * part]);
-                S[2 * i] = ss_fma2(f2, S[2 * i], ss_mul2(sx2, make_float2(bv.x, bv.y)));
-                S[2 * i + 1] = ss_fma2(f2, S[2 * i + 1], ss_mul2(sx2, make_float2(bv.z, bv.w)));
-                y0 = ss_fma2(S[2 * i], make_float2(cv.x, cv.y), y0);
-                y1 = ss_fma2(S[2 * i + 1], make_float2(cv.z, cv.w), y1);
+            for (uint32_t k = 0; k < 4; ++k) {
+                const uint32_t r = r0 + k;
+                const float sx = step[r] * xs[r][pl], f = decay[r];
+                const float2 sx2 = make_float2(sx, sx), f2 = make_float2(f, f);
+                float2 y0 = make_float2(0.0f, 0.0f), y1 = y0;
+#pragma unroll
+                for (int i = 0; i < GROUPS; ++i) {
+                    const float4 bv = *reinterpret_cast<const float4*>(&bs[r][16 * i + 4 * part]);
+                    S[2 * i] = ss_fma2(f2, S[2 * i], ss_mul2(sx2, make_float2(bv.x, bv.y)));
+                    S[2 * i + 1] = ss_fma2(f2, S[2 * i + 1], ss_mul2(sx2, make_float2(bv.z, bv.w)));
+                    if (STATE) continue;
+                    const float4 cv = *reinterpret_cast<const float4*>(&cs[r][16 * i + 4 * part]);
+                    y0 = ss_fma2(S[2 * i], make_float2(cv.x, cv.y), y0);
+                    y1 = ss_fma2(S[2 * i + 1], make_float2(cv.z, cv.w), y1);
+                }
+                y[k] = (y0.x + y0.y) + (y1.x + y1.y);
             }
-            float y = (y0.x + y0.y) + (y1.x + y1.y);
-            y += __shfl_xor_sync(0xffffffffu, y, 1);
-            y += __shfl_xor_sync(0xffffffffu, y, 2);
-            if (part == 0) ys[r][pl] = fmaf(skip, xv, y);
+            if (STATE) continue;
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) y[k] += __shfl_xor_sync(0xffffffffu, y[k], 1);
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) y[k] += __shfl_xor_sync(0xffffffffu, y[k], 2);
+            // thread `part` of a row writes its token
+            const float mine_y = part == 0 ? y[0] : part == 1 ? y[1] : part == 2 ? y[2] : y[3];
+            ys[r0 + part][pl] = fmaf(skip, xs[r0 + part][pl], mine_y);
         }
         __syncthreads();
 #pragma unroll
         for (uint32_t i = 0; i < XPER; ++i) {
             const uint32_t e = tid + i * SS_THREADS, r = e / SS_ROWS, q = e % SS_ROWS;
-            if (r < count && p0 + q < P) {
-                float y = ys[r][q];
-                if (a.z) y *= ss_silu(ss_f(z[(size_t)(t + r) * a.z_stride + q]));
-                out[(size_t)(t + r) * a.out_stride + q] = ss_t<T>(y);
-            }
+            if (!STATE && r < count && p0 + q < P) out[(size_t)(t + r) * a.out_stride + q] = ss_t<T>(ys[r][q] * zs[r][q]);
         }
     }
-    if (!mine) return;
+    if (STATE) {
+        each([&](float& v, uint32_t n) { end_of(part_of)[n] = v; });
+        if (tid < SS_BATCH) {
 #pragma unroll
-    for (int i = 0; i < GROUPS; ++i) {
-        const float v[4] = {S[2 * i].x, S[2 * i].y, S[2 * i + 1].x, S[2 * i + 1].y};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t n = 16 * i + 4 * part + j;
-            if (n < N) state[n] = v[j];
+            for (int o = 8; o > 0; o >>= 1) log_sum += __shfl_xor_sync(0xffffu, log_sum, o);
+            if (tid == 0 && p0 == 0) p.logs[(size_t)blockIdx.z * a.heads + h] = log_sum;
         }
-    }
+    } else if (part_of + 1 == parts && (!nothing || s.fresh())) each([&](float& v, uint32_t n) { state[n] = v; });
+}
+
+// how many parts a sequence is cut into where `ctas` CTAs would run without cutting (four an SM run beside one another): the pass over the parts' states costs less than the one
+// over the rows, so three parts pay
+uint32_t scan_parts(uint32_t rows, uint64_t ctas, uint32_t sms) {
+    const uint64_t room = 4ull * sms / std::max<uint64_t>(1, ctas);
+    if (room < 3 || rows < 8 * SS_BATCH) return 1;
+    const uint32_t want = (uint32_t)std::min<uint64_t>(room, rows / (2 * SS_BATCH)), per = (rows + want - 1) / want;
+    return (rows + per - 1) / per;
+}
+uint64_t scan_ctas(const uzu_state_space_scan_args& a) { return (uint64_t)a.sequence_count * a.heads * ((a.head_dim + SS_ROWS - 1) / SS_ROWS); }
+size_t scan_scratch_bytes(const uzu_state_space_scan_args& a, uint32_t sms) {
+    uint64_t tiles = 0;
+    for (uint32_t i = 0; i < a.sequence_count; ++i) tiles += scan_parts(a.sequences[i].rows, scan_ctas(a), sms);
+    return tiles == a.sequence_count ? 0 : tiles * a.heads * ((uint64_t)a.head_dim * a.state_size + 1) * 4;
 }
 
 template <typename T>
 void scan_launch(uzu_command_buffer* cmd, const ScanParams& p) {
-    const dim3 grid((p.a.head_dim + SS_ROWS - 1) / SS_ROWS, p.a.heads, p.table.count);
-    auto go = [&](auto kernel) { launch(cmd, "state_space_scan_kernel", kernel, grid, dim3(SS_THREADS), 0, p); };
-    const uint32_t n = p.a.state_size;
-    if (n <= 16) go(state_space_scan_kernel<T, 1>);
-    else if (n <= 64) go(state_space_scan_kernel<T, 4>);
-    else if (n <= 128) go(state_space_scan_kernel<T, 8>);
-    else go(state_space_scan_kernel<T, 16>);
+    const dim3 grid((p.a.head_dim + SS_ROWS - 1) / SS_ROWS, p.a.heads, p.table.tiles);
+    auto go = [&](auto state_only) {
+        constexpr bool ST = decltype(state_only)::value;
+        auto run = [&](auto kernel) { launch(cmd, "state_space_scan_kernel", kernel, grid, dim3(SS_THREADS), 0, p); };
+        const uint32_t n = p.a.state_size;
+        if (n <= 16) run(state_space_scan_kernel<T, 1, ST>);
+        else if (n <= 64) run(state_space_scan_kernel<T, 4, ST>);
+        else if (n <= 128) run(state_space_scan_kernel<T, 8, ST>);
+        else run(state_space_scan_kernel<T, 16, ST>);
+    };
+    if (p.table.tiles > p.table.count) go(std::true_type{});
+    go(std::false_type{});
 }
 
 const char* shape_check(uint32_t heads, uint32_t groups, uint32_t head_dim, uint32_t state_size, float dt_min, float dt_max, uint32_t data_type) {
@@ -375,7 +430,9 @@ uzu_status uzu_state_space_scan_validate(const uzu_state_space_scan_args* a) {
 }
 
 size_t uzu_state_space_scan_scratch_bytes(uzu_context* ctx, const uzu_state_space_scan_args* a) {
-    return ctx && a && a->sequences && ss_data_type(a->data_type) && a->heads && a->groups && scan_umma_applicable(*a) ? scan_umma_scratch_bytes(ctx, *a) : 0;
+    // (what the call's checks would refuse needs none)
+    if (!ctx || !a || (a->sequence_count && !a->sequences) || shape_check(a->heads, a->groups, a->head_dim, a->state_size, a->dt_min, a->dt_max, a->data_type)) return 0;
+    return scan_umma_applicable(*a) ? scan_umma_scratch_bytes(ctx, *a) : scan_scratch_bytes(*a, ctx->sm_count);
 }
 
 void uzu_state_space_scan_encode(uzu_command_buffer* cmd, const uzu_state_space_scan_args* a) {
@@ -388,8 +445,13 @@ void uzu_state_space_scan_encode(uzu_command_buffer* cmd, const uzu_state_space_
     if (scan_umma_applicable(*a) && encode_scan_umma(cmd, *a)) return;
     ScanParams p{};
     p.a = *a;
+    const uint32_t sms = cmd->ctx->sm_count;
+    const size_t need = scan_scratch_bytes(*a, sms);
+    const bool cut = need && a->scratch && a->scratch_bytes >= need;
     for (uint32_t begin = 0; begin < a->sequence_count;) {
-        begin = fill_sequences(p.table, a->sequences, a->sequence_count, begin, [](uint32_t) { return 1u; });
+        begin = fill_sequences(p.table, a->sequences, a->sequence_count, begin, [&](uint32_t rows) { return cut ? scan_parts(rows, scan_ctas(*a), sms) : 1u; });
+        p.ends = reinterpret_cast<float*>(a->scratch);      // (one launch behind the other: the next may use the same)
+        p.logs = p.ends + (uint64_t)p.table.tiles * a->heads * a->head_dim * a->state_size;
         if (a->data_type == UZU_DT_F32) scan_launch<float>(cmd, p);
         else if (a->data_type == UZU_DT_F16) scan_launch<__half>(cmd, p);
         else scan_launch<__nv_bfloat16>(cmd, p);
