@@ -47,7 +47,8 @@ struct XlParams {
 
 template <int NT, int PLANES>
 struct XlShape {
-    static constexpr uint32_t RED = XL_WARPS * 32 * NT * 8 * 4, STAGES = NT <= 2 ? 6 : NT == 4 ? 5 : 4;
+    static constexpr uint32_t TOK = NT * 8 + 1, RED = XL_WARPS * 32 * TOK * 4,      // tokens of a row of sums, and one place to keep rows off one another's banks
+                              STAGES = NT <= 2 ? 6 : NT == 4 ? 5 : 4;
     static constexpr size_t SMEM = STAGES * XL_STAGE + RED + 1024;
 };
 
@@ -79,19 +80,36 @@ __device__ __noinline__ bool xl_all(unsigned int* counter, volatile uint32_t* ga
     }
 }
 
+// eight values of a row
+__device__ __forceinline__ void xl_x8(const uzu_expert_layer_args& a, uint32_t t, uint32_t c, bool wide, float (&v)[8]) {
+    if (!wide) {
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) v[j] = xl_x(a, t, c + j);
+    } else if (a.data_type == UZU_DT_F32) {
+        const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.x) + (size_t)t * a.x_stride + c);
+        const float4 x = p[0], y = p[1];
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+    } else {
+        const uint4 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.x) + (size_t)t * a.x_stride + c);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) { v[2 * j] = um_lo(w[j]); v[2 * j + 1] = um_hi(w[j]); }
+    }
+}
+
 struct XlLists {
     uint32_t mask[XL_MAX_EXPERTS][2];      // tokens of an expert
     uint16_t expert[XL_MAX_EXPERTS];       // the chosen ones, ascending
     uint16_t base[XL_MAX_EXPERTS + 1];     // their pairs, in that order
-    uint8_t token[XL_MAX_PAIRS];
+    uint16_t token[XL_MAX_PAIRS];          // a pair's token, and behind it (64 times) which of the token's choices the expert is (31: shared)
     uint16_t id[XL_MAX_TOKENS][XL_MAX_TOP];
     float weight[XL_MAX_TOKENS][XL_MAX_TOP];
     uint32_t chosen;
 };
 
-// the choice for one token by a warp
+// the choice for one token by a warp, PER scores a lane
+template <int PER>
 __device__ void xl_choose(const uzu_expert_layer_args& a, const float* logits, uint32_t t, XlLists& l, bool write) {
-    constexpr int PER = 16;
     const uint32_t lane = threadIdx.x & 31u;
     float v[PER];
 #pragma unroll
@@ -159,7 +177,7 @@ __device__ void xl_choose(const uzu_expert_layer_args& a, const float* logits, u
 template <int NT, int PLANES>
 __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __grid_constant__ CUtensorMap map_up, const __grid_constant__ CUtensorMap map_down, const __grid_constant__ XlParams p) {
     using S = XlShape<NT, PLANES>;
-    constexpr uint32_t TOK = NT * 8;
+    constexpr uint32_t TOK = S::TOK;
     extern __shared__ uint8_t xl_raw[];
     __shared__ __align__(8) uint64_t bars[2 * S::STAGES];
     __shared__ volatile uint32_t gave_up;
@@ -203,6 +221,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
     {
         const uint32_t quads = (T + 3) / 4, pairs = E * quads;
         const bool split = pairs <= ctas;      // the CTA's warps share the columns
+        const bool wide = (a.x & 15u) == 0 && a.x_stride % 8 == 0;
         const __nv_bfloat16* router = reinterpret_cast<const __nv_bfloat16*>(a.router);
         for (uint32_t i = split ? cta : cta * XL_WARPS + warp; i < pairs && (split || warp < XL_WARPS); i += split ? ctas : ctas * XL_WARPS) {
             const uint32_t e = i / quads, tk = i % quads * 4;
@@ -214,8 +233,10 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
 #pragma unroll
                     for (uint32_t k = 0; k < 4; ++k)
                         if (tk + k < T) {
+float v[8];
+                            xl_x8(a, tk + k, c, wide, v);
 #pragma unroll
-                            for (uint32_t j = 0; j < 4; ++j) sum[k] = fmaf(um_hi(ws[j]), xl_x(a, tk + k, c + 2 * j + 1), fmaf(um_lo(ws[j]), xl_x(a, tk + k, c + 2 * j), sum[k]));
+                            for (uint32_t j = 0; j < 4; ++j) sum[k] = fmaf(um_hi(ws[j]), v[2 * j + 1], fmaf(um_lo(ws[j]), v[2 * j], sum[k]));
                         }
                 }
 #pragma unroll
@@ -241,7 +262,10 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
 
     // ---- 2: the choice ----
     if (ok) {
-        for (uint32_t t = warp; t < T; t += XL_THREADS / 32) xl_choose(a, logits, t, l, cta == 0);
+        for (uint32_t t = warp; t < T; t += XL_THREADS / 32) {
+            if (E <= 128) xl_choose<4>(a, logits, t, l, cta == 0);
+            else xl_choose<16>(a, logits, t, l, cta == 0);
+        }
         __syncthreads();
         if (warp == 0) {
             uint32_t count = 0, pairs = 0;
@@ -259,7 +283,13 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
                     l.expert[at] = (uint16_t)e;
                     l.base[at] = (uint16_t)pair;
                     for (uint32_t half = 0; half < 2; ++half)
-                        for (uint32_t m = l.mask[e][half]; m; m &= m - 1) l.token[pair++] = (uint8_t)(half * 32 + __ffs(m) - 1);
+                        for (uint32_t m = l.mask[e][half]; m; m &= m - 1) {
+                            const uint32_t t = half * 32 + __ffs(m) - 1;
+                            uint32_t j = 31;
+                            if (e < E)
+                                for (j = 0; j + 1 < a.top && l.id[t][j] != e; ++j) {}
+                            l.token[pair++] = (uint16_t)(j * 64 + t);
+                        }
                 }
                 count += __popc(there);
                 pairs += __shfl_sync(0xffffffffu, before, 31);
@@ -314,30 +344,29 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
 #pragma unroll
                     for (int j = 0; j < 4; ++j) acc[m][n][j] = 0.0f;
         };
-        // This warp's columns of a stage: operand B of tile n, a token's row from `src(n)` (null: no token), a plane `plane` elements behind the one before.
-        auto multiply = [&](uint32_t col, uint32_t width, size_t plane, uint32_t live, auto src) {
-            const uint32_t s = it % S::STAGES, c0 = col + warp * 64;
-            const bool there = c0 < width;
-            constexpr bool AHEAD = NT * PLANES <= 4;      // registers for B before the weights are there
-            uint4 b[AHEAD ? NT : 1][PLANES][2];
-            auto fetch = [&](int n, uint4 (&v)[PLANES][2]) {
-                const __nv_bfloat16* at = src(n);
+        // Operand B: eight tokens' columns of this warp, PLANES bf16 planes `plane` elements behind one another (no row: zeros)
+        auto ask = [&](const __nv_bfloat16* at, uint32_t col, uint32_t width, size_t plane, uint4 (&to)[PLANES][2]) {
 #pragma unroll
-                for (int pl = 0; pl < PLANES; ++pl)
+            for (int pl = 0; pl < PLANES; ++pl)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t c = c0 + (2 * t4 + i) * 8;
-                        v[pl][i] = at && c < width ? __ldcg(reinterpret_cast<const uint4*>(at + pl * plane + c)) : make_uint4(0, 0, 0, 0);
-                    }
-            };
-            if (AHEAD && there) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    if (live >> n & 1u) fetch(n, b[n]);
-            }
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t c = col + warp * 64 + (2 * t4 + i) * 8;
+                    to[pl][i] = at && c < width ? __ldcg(reinterpret_cast<const uint4*>(at + pl * plane + c)) : make_uint4(0, 0, 0, 0);
+                }
+        };
+        // A stage, for `count` tokens whose rows `src(k)` gives, eight at a time. The first eight of it were asked for a stage ago, into `first`; those of the next stage are asked for
+        // (`next`) before this one's products, since they come from L2 no faster than a stage.
+        uint4 first[PLANES][2];
+        auto multiply = [&](uint32_t col, uint32_t width, size_t plane, uint32_t count, auto src, auto next) {
+            const uint32_t s = it % S::STAGES;
+            const bool there = col + warp * 64 < width;
             if (ok) ok = um_wait(full(s), it / S::STAGES & 1u, &gave_up, 0x603u);
             if (!ok) return;
             uint32_t seen = 0;
+            uint4 b[PLANES][2];
+#pragma unroll
+            for (int pl = 0; pl < PLANES; ++pl) { b[pl][0] = first[pl][0]; b[pl][1] = first[pl][1]; }
+            next();
             if (there) {
                 const uint32_t box = ring + s * XL_STAGE + warp * XL_BOX + g * 128;
                 uint4 w[2][4];
@@ -350,20 +379,20 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
                     }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    if (!(live >> n & 1u)) continue;
-                    uint4 here[PLANES][2];
-                    if (!AHEAD) fetch(n, here);
+                    if (n * 8 >= count) break;
+                    uint4 v[PLANES][2];
+#pragma unroll
+                    for (int pl = 0; pl < PLANES; ++pl) { v[pl][0] = b[pl][0]; v[pl][1] = b[pl][1]; }
+                    if (n + 1 < NT && (n + 1) * 8 < count) ask((n + 1) * 8 + g < count ? src((n + 1) * 8 + g) : nullptr, col, width, plane, b);
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
-                        for (int pl = PLANES - 1; pl >= 0; --pl) {
-                            const uint4 v = AHEAD ? b[AHEAD ? n : 0][pl][i] : here[pl][i];
+                        for (int pl = PLANES - 1; pl >= 0; --pl)
 #pragma unroll
                             for (int m = 0; m < 2; ++m) {
-                                xl_mma(acc[m][n], w[i][2 * m].x, w[i][2 * m + 1].x, w[i][2 * m].y, w[i][2 * m + 1].y, v.x, v.y);
-                                xl_mma(acc[m][n], w[i][2 * m].z, w[i][2 * m + 1].z, w[i][2 * m].w, w[i][2 * m + 1].w, v.z, v.w);
+                                xl_mma(acc[m][n], w[i][2 * m].x, w[i][2 * m + 1].x, w[i][2 * m].y, w[i][2 * m + 1].y, v[pl][i].x, v[pl][i].y);
+                                xl_mma(acc[m][n], w[i][2 * m].z, w[i][2 * m + 1].z, w[i][2 * m].w, w[i][2 * m + 1].w, v[pl][i].z, v[pl][i].w);
                             }
-                        }
                 }
             }
             um_arrive_after(empty(s), seen, a.reserved0);
@@ -380,8 +409,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
-                        *reinterpret_cast<float2*>(&red[(warp * 32 + m * 16 + j * 8 + g) * TOK + n * 8 + 2 * t4]) = make_float2(acc[m][n][2 * j], acc[m][n][2 * j + 1]);
+                    for (int j = 0; j < 4; ++j) red[(warp * 32 + m * 16 + j / 2 * 8 + g) * TOK + n * 8 + 2 * t4 + j % 2] = acc[m][n][j];
             meet();
         };
         auto total = [&](uint32_t row, uint32_t tok) {
@@ -392,20 +420,26 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
         };
 
         // ---- 3: up ----
-        for (uint32_t u = cta; u < units; u += ctas) {
-            const uint32_t at = u / f_tiles, f0 = u % f_tiles * 16, base = l.base[at], count = l.base[at + 1] - base, e = l.expert[at];
-            const uint32_t live = (1u << ((count + 7) / 8)) - 1u;
+        auto ask_up = [&](uint32_t at, uint32_t s) {
+            if (at >= chosen) return;
+            const uint32_t base = l.base[at], count = l.base[at + 1] - base;
+            ask(g < count ? rows + (size_t)(l.token[base + g] & 63u) * D : nullptr, s * XL_COLS, D, row_plane, first);
+        };
+        const uint32_t ahead = ctas / f_tiles, over = ctas % f_tiles;      // a CTA's next unit: experts and tiles on
+        uint32_t at = cta / f_tiles, tile = cta % f_tiles;
+        ask_up(at, 0);
+        for (; at < chosen;) {
+            const uint32_t next_tile = tile + over < f_tiles ? tile + over : tile + over - f_tiles, next_at = at + ahead + (tile + over < f_tiles ? 0 : 1);
+            const uint32_t f0 = tile * 16, base = l.base[at], count = l.base[at + 1] - base;
             clear();
             for (uint32_t s = 0; s < up_stages && ok; ++s)
-                multiply(s * XL_COLS, D, row_plane, live, [&](int n) { return n * 8 + g < count ? rows + (size_t)l.token[base + n * 8 + g] * D : nullptr; });
+                multiply(s * XL_COLS, D, row_plane, count, [&](uint32_t k) { return rows + (size_t)(l.token[base + k] & 63u) * D; },
+                         [&]() { s + 1 < up_stages ? ask_up(at, s + 1) : ask_up(next_at, 0); });
             share();      // (also where a wait ran out: nobody is left waiting)
             for (uint32_t i = tid; i < count * 16; i += 256) {
-                const uint32_t f = i & 15u, k = i >> 4, tok = l.token[base + k];
+                const uint32_t f = i & 15u, k = i >> 4, pair = l.token[base + k], choice = pair >> 6;
                 if (f0 + f >= F) continue;
-                float w = 1.0f;
-                if (e < E)
-                    for (uint32_t j = 0; j < a.top; ++j)
-                        if (l.id[tok][j] == e) w = l.weight[tok][j];
+                const float w = choice < XL_MAX_TOP ? l.weight[pair & 63u][choice] : 1.0f;
                 const float v = act_f32(a.activation, total(16 + f, k)) * total(f, k) * w;
                 const __nv_bfloat16 hi = __float2bfloat16_rn(v);
                 __nv_bfloat16* to = hidden + (size_t)(base + k) * F + f0 + f;
@@ -413,6 +447,8 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
                 if (PLANES == 2) to[hidden_plane] = __float2bfloat16_rn(fabsf(v) < INFINITY ? v - __bfloat162float(hi) : 0.0f);
             }
             meet();
+            at = next_at;
+            tile = next_tile;
         }
         if (tid == 0) xl_all(counters + 1, &gave_up, 0x604u);
         meet();
@@ -424,25 +460,52 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
             if (a.data_type == UZU_DT_F32) reinterpret_cast<float*>(a.out)[(size_t)tok * a.out_stride + d] = v;
             else reinterpret_cast<__nv_bfloat16*>(a.out)[(size_t)tok * a.out_stride + d] = __float2bfloat16_rn(v);
         };
+        auto ask_down = [&](uint32_t expert, uint32_t s) {
+            const uint32_t base = l.base[expert], count = l.base[expert + 1] - base;
+            ask(g < count ? hidden + (size_t)(base + g) * F : nullptr, s * XL_COLS, F, hidden_plane, first);
+        };
+        uint32_t expert = 0, stage_of = 0;      // of the stage at hand
+        if (ok && begin < end) {
+            expert = (uint32_t)(begin % tile_stages) / f_stages;
+            stage_of = (uint32_t)(begin % tile_stages) % f_stages;
+            ask_down(expert, stage_of);
+        }
         for (uint64_t w = begin; w < end;) {
             const uint32_t tile = (uint32_t)(w / tile_stages);
             const uint64_t tile0 = (uint64_t)tile * tile_stages, tile1 = tile0 + tile_stages, stop = min(tile1, end);
             const bool whole = w == tile0 && stop == tile1;
             const uint32_t slot = begin > tile0 ? 0u : 1u;      // of this CTA's two tiles in parts
+            // an expert's sums belong to its own tokens: they are added to the warp's sums of all tokens when its stages end
+            for (uint32_t i = lane; i < 32 * TOK; i += 32) red[warp * 32 * TOK + i] = 0.0f;
+            __syncwarp();
             clear();
             for (; w < stop && ok; ++w) {
-                const uint32_t at = (uint32_t)(w - tile0) / f_stages, s = (uint32_t)(w - tile0) % f_stages, base = l.base[at], e = l.expert[at];
-                const uint64_t mask = (uint64_t)l.mask[e][1] << 32 | l.mask[e][0];
-                uint32_t live = 0;
+                const uint32_t s = stage_of, base = l.base[expert], count = l.base[expert + 1] - base, after = expert + 1 < chosen ? expert + 1 : 0;
+                const bool ends = s + 1 == f_stages;
+                multiply(s * XL_COLS, F, hidden_plane, count, [&](uint32_t k) { return hidden + (size_t)(base + k) * F; },
+                         [&]() { if (w + 1 < end) ask_down(ends ? after : expert, ends ? 0 : s + 1); });
+                stage_of = ends ? 0 : s + 1;
+                if (ends) expert = after;
+                if (!ends && w + 1 < stop) continue;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) live |= (mask >> (8 * n) & 0xffu) ? 1u << n : 0u;
-                multiply(s * XL_COLS, F, hidden_plane, live, [&](int n) {
-                    const uint32_t tok = n * 8 + g;
-                    return mask >> tok & 1u ? hidden + (size_t)(base + __popcll(mask & ((1ull << tok) - 1u))) * F : nullptr;
-                });
+                for (int n = 0; n < NT; ++n) {
+                    if (n * 8 >= count) break;
+#pragma unroll
+                    for (uint32_t j = 0; j < 2; ++j) {
+                        const uint32_t k = n * 8 + 2 * t4 + j;
+                        if (k >= count) continue;
+                        float* to = &red[(warp * 32 + g) * TOK + (l.token[base + k] & 63u)];
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            to[(m * 16) * TOK] += acc[m][n][j];
+                            to[(m * 16 + 8) * TOK] += acc[m][n][2 + j];
+                        }
+                    }
+                }
+                clear();
             }
             w = stop;
-            share();
+            meet();
             if (whole) {
                 if (ok)
                     for (uint32_t i = tid; i < 32 * T; i += 256)
