@@ -57,6 +57,9 @@ __device__ __forceinline__ void xl_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void xl_tma3(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint32_t z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
 __device__ __forceinline__ float xl_x(const uzu_expert_layer_args& a, uint32_t t, uint32_t c) {
     return a.data_type == UZU_DT_F32 ? reinterpret_cast<const float*>(a.x)[(size_t)t * a.x_stride + c] : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.x)[(size_t)t * a.x_stride + c]);
 }
@@ -308,7 +311,7 @@ float v[8];
 
     if (warp == XL_WARPS) {
         // ---- weights by TMA ----
-        auto stage = [&](const CUtensorMap* map, uint32_t col, uint32_t width, uint32_t row_a, uint32_t row_b) {
+        auto stage = [&](bool up, uint32_t col, uint32_t width, uint32_t row, uint32_t which) {
             const uint32_t s = it % S::STAGES;
             if (ok) ok = um_wait(empty(s), (it / S::STAGES & 1u) ^ 1u, &gave_up, 0x602u);
             if (!ok) return;
@@ -316,20 +319,27 @@ float v[8];
                 const uint32_t boxes = min(XL_WARPS, (width - col + 63) / 64);
                 um_expect(full(s), boxes * XL_BOX);
                 for (uint32_t b = 0; b < boxes; ++b) {
-                    um_tma(ring + s * XL_STAGE + b * XL_BOX, map, col + b * 64, row_a, full(s));
-                    um_tma(ring + s * XL_STAGE + b * XL_BOX + XL_BOX / 2, map, col + b * 64, row_b, full(s));
+                    if (up) xl_tma3(ring + s * XL_STAGE + b * XL_BOX, &map_up, col + b * 64, row, which, full(s));      // 16 up rows, 16 gate rows
+                    else um_tma(ring + s * XL_STAGE + b * XL_BOX, &map_down, col + b * 64, row, full(s));
                 }
             }
             __syncwarp();
             ++it;
         };
         for (uint32_t u = cta; u < units && ok; u += ctas) {
-            const uint32_t row = l.expert[u / f_tiles] * 2 * F + u % f_tiles * 16;
-            for (uint32_t s = 0; s < up_stages && ok; ++s) stage(&map_up, s * XL_COLS, D, row, row + F);
+            const uint32_t row = u % f_tiles * 16, which = 2 * l.expert[u / f_tiles];
+            for (uint32_t s = 0; s < up_stages && ok; ++s) stage(true, s * XL_COLS, D, row, which);
         }
-        for (uint64_t w = begin; w < end && ok; ++w) {
-            const uint32_t tile = (uint32_t)(w / tile_stages), at = (uint32_t)(w % tile_stages), row = l.expert[at / f_stages] * D + tile * 32;
-            stage(&map_down, at % f_stages * XL_COLS, F, row, row + 16);
+        if (begin < end) {
+            uint32_t tile = (uint32_t)(begin / tile_stages), at = (uint32_t)(begin % tile_stages) / f_stages, s = (uint32_t)(begin % tile_stages) % f_stages;
+            for (uint64_t w = begin; w < end && ok; ++w) {
+                stage(false, s * XL_COLS, F, l.expert[at] * D + tile * 32, 0);
+                if (++s < f_stages) continue;
+                s = 0;
+                if (++at < chosen) continue;
+                at = 0;
+                ++tile;
+            }
         }
         if (!ok)      // copies on their way end before the CTA does
             for (uint32_t n = 1; n <= S::STAGES && n <= it; ++n) um_settle(full((it - n) % S::STAGES), (it - n) / S::STAGES & 1u);
@@ -403,13 +413,15 @@ float v[8];
             asm volatile("bar.sync 1, 256;" ::: "memory");
         };
         // the warps' sums side by side: red[warp][row][token]
-        auto share = [&]() {
+        auto share = [&](uint32_t count) {
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+            for (int n = 0; n < NT; ++n) {
+                if (n * 8 >= count) break;
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int m = 0; m < 2; ++m)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) red[(warp * 32 + m * 16 + j / 2 * 8 + g) * TOK + n * 8 + 2 * t4 + j % 2] = acc[m][n][j];
+            }
             meet();
         };
         auto total = [&](uint32_t row, uint32_t tok) {
@@ -435,7 +447,7 @@ float v[8];
             for (uint32_t s = 0; s < up_stages && ok; ++s)
                 multiply(s * XL_COLS, D, row_plane, count, [&](uint32_t k) { return rows + (size_t)(l.token[base + k] & 63u) * D; },
                          [&]() { s + 1 < up_stages ? ask_up(at, s + 1) : ask_up(next_at, 0); });
-            share();      // (also where a wait ran out: nobody is left waiting)
+            share(count);      // (also where a wait ran out: nobody is left waiting)
             for (uint32_t i = tid; i < count * 16; i += 256) {
                 const uint32_t f = i & 15u, k = i >> 4, pair = l.token[base + k], choice = pair >> 6;
                 if (f0 + f >= F) continue;
@@ -613,7 +625,12 @@ void uzu_expert_layer_encode(uzu_command_buffer* cmd, const uzu_expert_layer_arg
     p.error = cmd->ctx->wait_errors.device_word;
     CUtensorMap up, down;
     const uint64_t all = a->experts + a->shared;
-    if (!um_map(&up, a->up_gate, a->width, all * 2 * a->ff, a->width, 16) || !um_map(&down, a->down, a->ff, all * a->width, a->ff, 16)) {
+    // up and gate rows of all experts in turn, in boxes of 16 of each
+    const cuuint64_t dims[3] = {a->width, a->ff, 2 * all}, strides[2] = {(cuuint64_t)a->width * 2, (cuuint64_t)a->ff * a->width * 2};
+    const cuuint32_t box[3] = {64, 16, 2}, steps[3] = {1, 1, 1};
+    if (!um_encoder() || um_encoder()(&up, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, (void*)a->up_gate, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS ||
+        !um_map(&down, a->down, a->ff, all * a->width, a->ff, 32)) {
         cmd->record_error(UZU_ERROR_CUDA, "expert_layer: cuTensorMapEncodeTiled failed");
         return;
     }
