@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(SS_THREADS) state_space_step_kernel(const __gr
             S[i][v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (p0 + pl >= P || n >= N) continue;
             const float* at = state + (size_t)pl * N + n;
-            if (vector) S[i][v] = *reinterpret_cast<const float4*>(at);
+            if (vector) S[i][v] = __ldcs(reinterpret_cast<const float4*>(at));      // (read once: not to push out what others share)
             else {
                 S[i][v].x = at[0];
                 if (n + 1 < N) S[i][v].y = at[1];
@@ -290,10 +290,15 @@ __global__ void __launch_bounds__(SS_THREADS) state_space_step_kernel(const __gr
             if (j < kept) u[j] = past[(size_t)j * channels + c];
         const T last_input = now[c];
         float y = bias ? bias[c] : 0.0f;
+        if (kept == 3 && (a.conv_weights & 15u) == 0) {
+            const float4 w4 = *reinterpret_cast<const float4*>(w + (size_t)c * 4);
+            y = fmaf(w4.w, ss_f(last_input), fmaf(w4.z, ss_f(u[2]), fmaf(w4.y, ss_f(u[1]), fmaf(w4.x, ss_f(u[0]), y))));
+        } else {
 #pragma unroll
-        for (uint32_t j = 0; j < 7; ++j)
-            if (j < kept) y = fmaf(w[(size_t)c * a.taps + j], ss_f(u[j]), y);
-        y = fmaf(w[(size_t)c * a.taps + kept], ss_f(last_input), y);
+            for (uint32_t j = 0; j < 7; ++j)
+                if (j < kept) y = fmaf(w[(size_t)c * a.taps + j], ss_f(u[j]), y);
+            y = fmaf(w[(size_t)c * a.taps + kept], ss_f(last_input), y);
+        }
         if (a.activation == UZU_ACT_SILU) y = ss_silu(y);
         if (i < xrows) {      // nobody else reads or writes these
             xs[i] = y;
@@ -309,12 +314,9 @@ __global__ void __launch_bounds__(SS_THREADS) state_space_step_kernel(const __gr
     __syncthreads();      // (and every thread of the CTA has read b's and c's inputs)
     if (kept && tid == 0) {
         unsigned int* ticket = reinterpret_cast<unsigned int*>(a.tickets) + (size_t)row * a.groups + g;
-        __threadfence();
+        // (no fence: what was read is in registers, which no later write changes)
         last = atomicAdd(ticket, 1u) == per_group * slices - 1;
-        if (last) {
-            __threadfence();
-            *ticket = 0;
-        }
+        if (last) *ticket = 0;
     }
 
     float y[PASSES];
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(SS_THREADS) state_space_step_kernel(const __gr
             y[i] = fmaf(s.x, cv.x, fmaf(s.y, cv.y, fmaf(s.z, cv.z, fmaf(s.w, cv.w, y[i]))));
             if (p0 + pl >= P || n >= N) continue;
             float* at = state + (size_t)pl * N + n;
-            if (vector) *reinterpret_cast<float4*>(at) = s;
+            if (vector) __stcs(reinterpret_cast<float4*>(at), s);
             else {
                 at[0] = s.x;
                 if (n + 1 < N) at[1] = s.y;
