@@ -251,6 +251,27 @@ __global__ void __launch_bounds__(SS_THREADS) state_space_step_kernel(const __gr
     const uint32_t* slots = reinterpret_cast<const uint32_t*>(a.slots);
     const uint32_t slot = slots ? slots[row] : row;
     if (slot >= a.slot_count) return;
+    // Asked for first: what the convolution takes, so that it is computed while the state is on its way. This CTA's channels: its rows of x, then b and c of the group.
+    constexpr int PER = (ROWS + 2 * COLS + SS_THREADS - 1) / SS_THREADS;
+    const uint32_t inner = a.heads * P, channels = inner + 2 * a.groups * N, kept = a.taps - 1, xrows = min(ROWS, P - p0);
+    const T* now = reinterpret_cast<const T*>(a.xbc) + (size_t)row * a.xbc_stride;
+    T* past = reinterpret_cast<T*>(a.conv_state) + (size_t)slot * kept * channels;
+    const float *w = reinterpret_cast<const float*>(a.conv_weights), *bias = reinterpret_cast<const float*>(a.conv_bias);
+    const bool four = kept == 3 && (a.conv_weights & 15u) == 0;
+    auto channel = [&](uint32_t i) { return i < xrows ? h * P + p0 + i : i < xrows + N ? inner + g * N + (i - xrows) : inner + a.groups * N + g * N + (i - xrows - N); };
+    T u[PER][8];      // the slot's inputs, oldest first, and (7) the row's own
+    float4 w4[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const uint32_t i = tid + k * SS_THREADS;
+        if (i >= xrows + 2 * N) break;
+        const uint32_t c = channel(i);
+#pragma unroll
+        for (uint32_t j = 0; j < 7; ++j)
+            if (j < kept) u[k][j] = past[(size_t)j * channels + c];
+        u[k][7] = now[c];
+        if (four) w4[k] = *reinterpret_cast<const float4*>(w + (size_t)c * 4);
+    }
     float* state = reinterpret_cast<float*>(a.state) + (((size_t)slot * a.heads + h) * P + p0) * N;
     const bool vector = N % 4 == 0 && (a.state & 15u) == 0;
     float4 S[PASSES][NV];
@@ -276,35 +297,25 @@ __global__ void __launch_bounds__(SS_THREADS) state_space_step_kernel(const __gr
         for (uint32_t r = tid; r < row; r += SS_THREADS) taken |= slots[r] == slot;
     if (__syncthreads_or(taken)) return;
 
-    // the convolution of this CTA's channels: its rows of x, then b and c of the group
-    const uint32_t inner = a.heads * P, channels = inner + 2 * a.groups * N, kept = a.taps - 1, xrows = min(ROWS, P - p0);
-    const T* now = reinterpret_cast<const T*>(a.xbc) + (size_t)row * a.xbc_stride;
-    T* past = reinterpret_cast<T*>(a.conv_state) + (size_t)slot * kept * channels;
-    const float *w = reinterpret_cast<const float*>(a.conv_weights), *bias = reinterpret_cast<const float*>(a.conv_bias);
-    auto channel = [&](uint32_t i) { return i < xrows ? h * P + p0 + i : i < xrows + N ? inner + g * N + (i - xrows) : inner + a.groups * N + g * N + (i - xrows - N); };
-    for (uint32_t i = tid; i < xrows + 2 * N; i += SS_THREADS) {
-        const uint32_t c = channel(i);
-        T u[8];
 #pragma unroll
-        for (uint32_t j = 0; j < 7; ++j)
-            if (j < kept) u[j] = past[(size_t)j * channels + c];
-        const T last_input = now[c];
+    for (int k = 0; k < PER; ++k) {
+        const uint32_t i = tid + k * SS_THREADS;
+        if (i >= xrows + 2 * N) break;
+        const uint32_t c = channel(i);
         float y = bias ? bias[c] : 0.0f;
-        if (kept == 3 && (a.conv_weights & 15u) == 0) {
-            const float4 w4 = *reinterpret_cast<const float4*>(w + (size_t)c * 4);
-            y = fmaf(w4.w, ss_f(last_input), fmaf(w4.z, ss_f(u[2]), fmaf(w4.y, ss_f(u[1]), fmaf(w4.x, ss_f(u[0]), y))));
-        } else {
+        if (four) y = fmaf(w4[k].w, ss_f(u[k][7]), fmaf(w4[k].z, ss_f(u[k][2]), fmaf(w4[k].y, ss_f(u[k][1]), fmaf(w4[k].x, ss_f(u[k][0]), y))));
+        else {
 #pragma unroll
             for (uint32_t j = 0; j < 7; ++j)
-                if (j < kept) y = fmaf(w[(size_t)c * a.taps + j], ss_f(u[j]), y);
-            y = fmaf(w[(size_t)c * a.taps + kept], ss_f(last_input), y);
+                if (j < kept) y = fmaf(w[(size_t)c * a.taps + j], ss_f(u[k][j]), y);
+            y = fmaf(w[(size_t)c * a.taps + kept], ss_f(u[k][7]), y);
         }
         if (a.activation == UZU_ACT_SILU) y = ss_silu(y);
         if (i < xrows) {      // nobody else reads or writes these
             xs[i] = y;
 #pragma unroll
             for (uint32_t j = 0; j < 7; ++j)
-                if (j < kept) past[(size_t)j * channels + c] = j + 1 < kept ? u[j + 1] : last_input;
+                if (j < kept) past[(size_t)j * channels + c] = j + 1 < kept ? u[k][j < 6 ? j + 1 : 6] : u[k][7];
         } else if (i < xrows + N) bs[i - xrows] = y;
         else cs[i - xrows - N] = y;
     }
