@@ -346,3 +346,278 @@ def test_step_rows_left_out(ctx):
 
 def test_step_many_rows(ctx):
     _step_case(ctx, P.BF16, 2, 1, 8, 8, 4, list(np.random.default_rng(1).permutation(400)[:391]), 400)
+
+
+# ---- values that are not finite, calls together, captured calls ----------------------------------------------------------------------------------------
+def _torch_scan(ctx, rows, heads, groups, dim, n, seed=0, slots=1, seqs=None, dt=P.BF16):
+    """a scan over torch tensors: (run, tensors)"""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    kept = {P.BF16: torch.bfloat16, P.F32: torch.float32}[dt]
+    inner, ch = heads * dim, heads * dim + 2 * groups * n
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    t = dict(xbc=r(rows, ch).to(kept), z=r(rows, inner).to(kept), dt=r(rows, heads).to(kept), a=-1 - 15 * torch.rand(heads, device="cuda", generator=g), d=r(heads), bias=r(heads) - 3,
+             state=r(slots, heads, dim, n), out=torch.zeros(rows, inner, device="cuda", dtype=kept))
+    tab = _table(seqs or [(0, rows, 0, 0)])
+    e = t["xbc"].element_size()
+    args = B.StateSpaceScanArgs(x=t["xbc"].data_ptr(), b=t["xbc"].data_ptr() + e * inner, c=t["xbc"].data_ptr() + e * (inner + groups * n), z=t["z"].data_ptr(), dt=t["dt"].data_ptr(),
+                                a=t["a"].data_ptr(), d=t["d"].data_ptr(), dt_bias=t["bias"].data_ptr(), state=t["state"].data_ptr(), out=t["out"].data_ptr(), sequences=C.addressof(tab),
+                                sequence_count=len(seqs or [0]), rows=rows, slots=slots, heads=heads, groups=groups, head_dim=dim, state_size=n, x_stride=ch, b_stride=ch, c_stride=ch,
+                                dt_stride=heads, z_stride=inner, out_stride=inner, dt_min=0.0, dt_max=float("inf"), dt_softplus=1, data_type=dt)
+    args.scratch_bytes = ctx.lib.uzu_state_space_scan_scratch_bytes(ctx.h, C.byref(args))
+    t["scratch"] = torch.empty(max(16, args.scratch_bytes), dtype=torch.uint8, device="cuda")
+    args.scratch = t["scratch"].data_ptr()
+
+    def run():
+        torch.cuda.synchronize()
+        with ctx.command_buffer("scan") as cmd:
+            cmd.encode("uzu_state_space_scan_encode", C.byref(args))
+    return run, t, (args, tab)
+
+
+@pytest.mark.parametrize("dt,dim,n", [(P.BF16, 64, 128), (P.BF16, 128, 64), (P.F32, 20, 12)])
+def test_scan_values_that_are_not_finite(ctx, dt, dim, n):
+    """an x that is infinite or no number shows in its own column from its token on, a b in its head group's later tokens, a c and a z in their token: nothing else changes"""
+    import torch
+    rows, heads, groups = 300, 4, 2
+    inner = heads * dim
+    run, t, keep = _torch_scan(ctx, rows, heads, groups, dim, n, slots=1, dt=dt)
+    state0 = t["state"].clone()
+    run()
+    clean = t["out"].clone()
+    clean_state = t["state"].clone()
+    assert bool(torch.isfinite(clean).all())
+    for name, where, value in [("xbc", (140, dim + 5), float("inf")), ("xbc", (17, 3), float("nan")), ("xbc", (255, inner - 1), -float("inf")), ("xbc", (200, inner + 4), float("inf")),
+                               ("xbc", (90, inner + groups * n + n + 2), float("nan")), ("z", (60, 2 * dim + 1), float("nan"))]:
+        old = t[name][where].clone()
+        t[name][where] = value
+        t["state"].copy_(state0)
+        run()
+        t[name][where] = old
+        row, col = where
+        hit = torch.zeros(rows, inner, dtype=torch.bool, device="cuda")
+        hit_state = torch.zeros_like(t["state"], dtype=torch.bool)
+        must = hit.clone()
+        if name == "z":
+            hit[row, col] = must[row, col] = True
+        elif col < inner:
+            hit[row:, col] = must[row, col] = True
+            hit_state[0, col // dim, col % dim] = True
+        elif col < inner + groups * n:      # b of group 0, one column of the state
+            hit[row:, :inner // groups] = True
+            must[row, :inner // groups] = True
+            hit_state[0, :heads // groups, :, col - inner] = True
+        else:                               # c of group 1
+            hit[row, inner // groups:] = must[row, inner // groups:] = True
+        out, state = t["out"], t["state"]
+        assert torch.equal(out[~hit], clean[~hit]), (name, where)
+        assert not bool(torch.isfinite(out[must]).any()), (name, where)
+        assert torch.equal(state[~hit_state], clean_state[~hit_state])
+
+
+def _captured(ctx, encode):
+    """what `encode(cmd)` enqueues, captured once on the context's stream: a function that replays it"""
+    import torch
+    stream = torch.cuda.ExternalStream(ctx.stream)
+    graph = torch.cuda.CUDAGraph()
+    h = C.c_void_p()
+    B._check(ctx.lib.uzu_command_buffer_create(ctx.h, b"captured", C.byref(h)))
+    B._check(ctx.lib.uzu_command_buffer_start_encoding(h))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        graph.capture_begin(capture_error_mode="relaxed")
+        encode(h)
+        graph.capture_end()
+    B._check(ctx.lib.uzu_command_buffer_end_encoding(h))
+    B._check(ctx.lib.uzu_command_buffer_submit(h))
+    B._check(ctx.lib.uzu_command_buffer_wait_until_completed(h))
+    ctx.lib.uzu_command_buffer_destroy(h)
+
+    def replay():
+        with torch.cuda.stream(stream):
+            graph.replay()
+        torch.cuda.synchronize()
+    return replay
+
+
+class _Mixer:
+    """a layer's state space mixer and its experts over torch tensors, as a host program runs them: prompt rows through convolution and scan, then tokens through the step, the
+    mixer's output rows through the experts"""
+
+    def __init__(self, ctx, seed=0, heads=8, groups=2, dim=64, n=128, taps=4, slots=6):
+        import torch
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        r = lambda *s: torch.randn(*s, device="cuda", generator=g)
+        self.torch, self.ctx, self.g = torch, ctx, g
+        self.heads, self.groups, self.dim, self.n, self.taps, self.slots = heads, groups, dim, n, taps, slots
+        self.inner, self.ch = heads * dim, heads * dim + 2 * groups * n
+        self.w, self.bias = r(self.ch, taps) / 2, 0.1 * r(self.ch)
+        self.a, self.d, self.dtb = -1 - 15 * torch.rand(heads, device="cuda", generator=g), r(heads), r(heads) - 3
+        self.conv_state = torch.zeros(slots, taps - 1, self.ch, device="cuda", dtype=torch.bfloat16)
+        self.state = torch.zeros(slots, heads, dim, n, device="cuda")
+        self.tickets = torch.zeros(64 * groups, dtype=torch.int32, device="cuda")
+        self.width, self.ff, self.experts, self.top = self.inner, 64, 8, 2
+        self.router = (r(8, self.inner) / self.inner ** 0.5).to(torch.bfloat16)
+        self.up, self.down = (r(8, 128, self.inner) / self.inner ** 0.5).to(torch.bfloat16), (r(8, self.inner, 64) / 8).to(torch.bfloat16)
+        self.kept = []
+
+    def rows(self, count):
+        return self.torch.randn(count, self.inner + self.ch + self.heads, device="cuda", generator=self.g).to(self.torch.bfloat16)
+
+    def prompt(self, proj, seqs):
+        """(encode, out): proj rows [z | xbc | dt]"""
+        t, n = self.torch, proj.shape[0]
+        xbc, out, tab = t.empty(n, self.ch, device="cuda", dtype=t.bfloat16), t.zeros(n, self.inner, device="cuda", dtype=t.bfloat16), _table(seqs)
+        row, e = proj.shape[1], 2
+        conv = B.CausalConvArgs(input=proj.data_ptr() + e * self.inner, output=xbc.data_ptr(), weights=self.w.data_ptr(), bias=self.bias.data_ptr(), state=self.conv_state.data_ptr(),
+                                sequences=C.addressof(tab), sequence_count=len(seqs), rows=n, slots=self.slots, channels=self.ch, taps=self.taps, input_stride=row, output_stride=self.ch,
+                                activation=B.ACT_SILU, data_type=B.DT_BF16)
+        gn = self.groups * self.n
+        scan = B.StateSpaceScanArgs(x=xbc.data_ptr(), b=xbc.data_ptr() + e * self.inner, c=xbc.data_ptr() + e * (self.inner + gn), z=proj.data_ptr(), dt=proj.data_ptr() + e * (self.inner + self.ch),
+                                    a=self.a.data_ptr(), d=self.d.data_ptr(), dt_bias=self.dtb.data_ptr(), state=self.state.data_ptr(), out=out.data_ptr(), sequences=C.addressof(tab),
+                                    sequence_count=len(seqs), rows=n, slots=self.slots, heads=self.heads, groups=self.groups, head_dim=self.dim, state_size=self.n, x_stride=self.ch, b_stride=self.ch,
+                                    c_stride=self.ch, dt_stride=row, z_stride=row, out_stride=self.inner, dt_min=0.0, dt_max=float("inf"), dt_softplus=1, data_type=B.DT_BF16)
+        scan.scratch_bytes = self.ctx.lib.uzu_state_space_scan_scratch_bytes(self.ctx.h, C.byref(scan))
+        scratch = t.empty(max(16, scan.scratch_bytes), dtype=t.uint8, device="cuda")
+        scan.scratch = scratch.data_ptr()
+        self.kept += [proj, xbc, out, tab, conv, scan, scratch]
+
+        def encode(h):
+            self.ctx.lib.uzu_causal_conv_encode(h, C.byref(conv))
+            self.ctx.lib.uzu_state_space_scan_encode(h, C.byref(scan))
+        return encode, out
+
+    def token(self, proj, slots):
+        """(encode, mixer rows, experts' rows)"""
+        t, n, e = self.torch, proj.shape[0], 2
+        out, mixed = t.zeros(n, self.inner, device="cuda", dtype=t.bfloat16), t.zeros(n, self.inner, device="cuda", dtype=t.bfloat16)
+        row = proj.shape[1]
+        step = B.StateSpaceStepArgs(xbc=proj.data_ptr() + e * self.inner, dt=proj.data_ptr() + e * (self.inner + self.ch), z=proj.data_ptr(), conv_weights=self.w.data_ptr(), conv_bias=self.bias.data_ptr(),
+                                    conv_state=self.conv_state.data_ptr(), a=self.a.data_ptr(), d=self.d.data_ptr(), dt_bias=self.dtb.data_ptr(), state=self.state.data_ptr(), out=out.data_ptr(),
+                                    slots=slots.data_ptr(), tickets=self.tickets.data_ptr(), rows=n, slot_count=self.slots, heads=self.heads, groups=self.groups, head_dim=self.dim, state_size=self.n,
+                                    taps=self.taps, xbc_stride=row, dt_stride=row, z_stride=row, out_stride=self.inner, dt_min=0.0, dt_max=float("inf"), dt_softplus=1, activation=B.ACT_SILU,
+                                    data_type=B.DT_BF16)
+        lay = B.ExpertLayerArgs(x=out.data_ptr(), out=mixed.data_ptr(), router=self.router.data_ptr(), up_gate=self.up.data_ptr(), down=self.down.data_ptr(), rows=n, width=self.width, ff=self.ff,
+                                experts=self.experts, top=self.top, shared=0, x_stride=self.inner, out_stride=self.inner, score=0, renormalise=0, weight_scale=1.0, activation=B.ACT_SILU,
+                                data_type=B.DT_BF16)
+        lay.scratch_bytes = self.ctx.lib.uzu_expert_layer_scratch_bytes(C.byref(lay))
+        scratch = t.zeros(lay.scratch_bytes, dtype=t.uint8, device="cuda")
+        lay.scratch = scratch.data_ptr()
+        self.kept += [proj, out, mixed, step, lay, scratch, slots]
+
+        def encode(h):
+            self.ctx.lib.uzu_state_space_step_encode(h, C.byref(step))
+            self.ctx.lib.uzu_expert_layer_encode(h, C.byref(lay))
+        return encode, out, mixed
+
+    def run(self, *encodes):
+        self.torch.cuda.synchronize()
+        with self.ctx.command_buffer("mixer") as cmd:
+            for f in encodes:
+                f(cmd.h)
+
+
+def test_prompt_then_tokens(ctx):
+    """three prompts in one pass, then five tokens of each: as if the whole had been one prompt each; the experts read the mixer's rows in the same buffer"""
+    import torch
+    whole, parted = _Mixer(ctx, seed=3), _Mixer(ctx, seed=3)
+    lengths = [150, 1, 260]
+    tokens = 5
+    rows = [whole.rows(n + tokens) for n in lengths]
+    ends = np.cumsum([n + tokens for n in lengths])
+    enc, ref = whole.prompt(torch.cat(rows), [(int(e) - n - tokens, n + tokens, 2 * i, 1) for i, (n, e) in enumerate(zip(lengths, ends))])
+    whole.run(enc)
+    starts = np.cumsum([0] + lengths)
+    enc, out = parted.prompt(torch.cat([r[:n] for r, n in zip(rows, lengths)]), [(int(s), n, 2 * i, 1) for i, (n, s) in enumerate(zip(lengths, starts))])
+    steps = [parted.token(torch.stack([r[n + k] for r, n in zip(rows, lengths)]), torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda")) for k in range(tokens)]
+    parted.run(enc, *[s[0] for s in steps])
+    for i, (n, e) in enumerate(zip(lengths, ends)):
+        mine = ref[int(e) - n - tokens:int(e)].float()
+        assert torch.equal(out[int(starts[i]):int(starts[i]) + n].float(), mine[:n])
+        for k in range(tokens):
+            got = steps[k][1][i].float()
+            # the prompt's path rounds the convolution's rows, scores and the state that is read out to bf16, the step nothing: a few half steps of the row's size
+            assert float((got - mine[n + k]).norm() / mine[n + k].norm()) <= 4 * 2.0 ** -8
+    assert all(bool(torch.isfinite(s[2]).all()) and bool((s[2] != 0).any()) for s in steps)
+    assert torch.equal(whole.conv_state[[0, 2, 4]].view(torch.int16), parted.conv_state[[0, 2, 4]].view(torch.int16))
+
+
+def test_captured_calls_follow_the_device(ctx):
+    """the four calls captured once and replayed: the same bits as run one by one, and a replay follows the slots that the device's list names then"""
+    import torch
+    eager, replayed = _Mixer(ctx, seed=5), _Mixer(ctx, seed=5)
+    prompt, token = eager.rows(200), eager.rows(3)
+    seqs = [(0, 130, 1, 1), (130, 70, 3, 0)]
+    for m in (eager, replayed):
+        m.state.normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+        m.conv_state.normal_(generator=torch.Generator(device="cuda").manual_seed(2))
+    lists = [[1, 3, 0], [5, -1, 1], [2, 2, 4]]
+    outs = []
+    first = eager.prompt(prompt, seqs)
+    outs_e = []
+    for k, sl in enumerate(lists):
+        s = eager.token(token, torch.tensor(sl, dtype=torch.int32, device="cuda"))
+        eager.run(first[0], s[0])
+        outs_e.append((first[1].clone(), s[1].clone(), s[2].clone()))
+    slots = torch.tensor(lists[0], dtype=torch.int32, device="cuda")
+    warm = _Mixer(ctx, seed=6)
+    warm.run(warm.prompt(prompt, seqs)[0], warm.token(token, slots)[0])      # (a kernel's first launch sets its shared memory, which is not captured)
+    p, s = replayed.prompt(prompt, seqs), replayed.token(token, slots)
+
+    def both(h):
+        p[0](h)
+        s[0](h)
+    replay = _captured(ctx, both)
+    for k, sl in enumerate(lists):
+        slots.copy_(torch.tensor(sl, dtype=torch.int32))
+        s[1].zero_()
+        torch.cuda.synchronize()
+        replay()
+        outs.append((p[1].clone(), s[1].clone(), s[2].clone()))
+        for a, b in zip(outs_e[k], outs[k]):
+            assert torch.equal(a.view(torch.int16), b.view(torch.int16)), k
+    assert torch.equal(eager.state, replayed.state) and torch.equal(eager.conv_state.view(torch.int16), replayed.conv_state.view(torch.int16))
+
+
+def test_two_contexts_at_once(ctx):
+    """the same calls on the streams of two contexts at the same time, each with its own scratch and tickets"""
+    import torch
+    with B.Context(0) as other:
+        alone = _Mixer(ctx, seed=8)
+        prompt, token = alone.rows(700), alone.rows(4)
+        sl = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device="cuda")
+        p, s = alone.prompt(prompt, [(0, 700, 2, 1)]), alone.token(token, sl)
+        alone.run(p[0], s[0], s[0], s[0])
+        pairs = []
+        for c in (ctx, other):
+            m = _Mixer(c, seed=8)
+            pairs.append((m, m.prompt(prompt, [(0, 700, 2, 1)]), m.token(token, sl)))
+        torch.cuda.synchronize()
+        cmds = [m.ctx.command_buffer("both") for m, _, _ in pairs]
+        for cmd in cmds:
+            cmd.__enter__()
+        for _, p2, _ in pairs:
+            p2[0](cmds[pairs.index(next(x for x in pairs if x[1] is p2))].h)
+        for _ in range(3):
+            for cmd, (_, _, s2) in zip(cmds, pairs):
+                s2[0](cmd.h)
+        for cmd in cmds:
+            cmd.__exit__(None, None, None)
+        for m, p2, s2 in pairs:
+            assert torch.equal(p[1].view(torch.int16), p2[1].view(torch.int16)) and torch.equal(s[1].view(torch.int16), s2[1].view(torch.int16)) and torch.equal(s[2].view(torch.int16), s2[2].view(torch.int16))
+            assert torch.equal(alone.state, m.state)
+
+
+def test_refused_calls_leave_everything_alone(ctx):
+    """an invalid call records the error, surfaced at the wait, and launches nothing"""
+    run, t, (args, tab) = _torch_scan(ctx, 10, 2, 1, 64, 64)
+    before = t["state"].clone()
+    args.dt_min = -1.0
+    with pytest.raises(B.UzuError, match="dt_min"):
+        run()
+    args.dt_min = 0.0
+    args.heads = 3
+    with pytest.raises(B.UzuError):
+        run()
+    import torch
+    assert torch.equal(t["state"], before) and not bool(t["out"].any())
