@@ -983,7 +983,7 @@ UZU_API uzu_status uzu_state_space_step_validate(const uzu_state_space_step_args
  *   weights = s; 2: s = sigmoid(logits), the `top` largest s, weights = s.  renormalise: weights / their sum;  weights * weight_scale. The lower index wins
  *   a tie; a logit that is NaN comes last.
  *   out[t] = sum_k weights[t, k] E_(ids[t, k])(x_t) + sum over shared experts E(x_t),   E(x) = down (act(gate) * up),  [up | gate] = up_gate x
- * x and out are bf16 or f32 rows, the weights bf16. f32 rows and hidden values enter the products as two bf16 parts, of bf16 rows the hidden values as one;
+ * x and out are bf16 or f32 rows, the weights bf16. f32 rows and hidden values enter the products as three bf16 parts (24 bits), of bf16 rows the hidden values as one;
  * products and sums are f32, summed in an order that only the shapes and the choice set. width and ff are multiples of 8, weights 16-byte aligned.
  * scratch: of uzu_expert_layer_scratch_bytes() bytes, 256-byte aligned, its first 16 KB zero before the first use; every call leaves it ready for the next,
  * of any sizes. Calls that may run at the same time do not share it. */

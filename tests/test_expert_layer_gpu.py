@@ -54,9 +54,9 @@ class _Layer:
         assert gap > 1e-6, "the case has two scores that 32 bits do not tell apart"
         assert np.array_equal(ids, rid)
         assert np.abs(weights - rw).max() <= 2e-6 * np.abs(rw).max() + (self.width + 16) * 2.0 ** -24 * 4 * np.abs(rw).max()
-        # products of bf16 parts in 32 bits: a rounding for each of the operands' 8 (16 with the remainder) columns and the warps' sums; hidden values and rows of
-        # f32 as two bf16 parts keep 16 bits, hidden values of bf16 rows 8; the gate's exponential
-        part = 2.0 ** -16 * 3 if dt == P.F32 else 2.0 ** -8
+        # products of bf16 parts in 32 bits: a rounding for each of the operands' 8 columns (24 of three parts) and the warps' sums; hidden values and rows of
+        # f32 as three bf16 parts keep 24 bits, hidden values of bf16 rows 8; the gate's exponential
+        part = 2.0 ** -24 * 3 * (self.width + self.ff) / 8 if dt == P.F32 else 2.0 ** -8
         unit = part + 2.0 ** -24 * ((self.width + self.ff) / 8 + 32) + 2.0 ** -20
         _check(P.of_kept(got, dt), ref, unit * mag, dt)
 

@@ -4,7 +4,7 @@
 // room, over the units and over the phases, so that the wait of all CTAs for the hidden values is spent filling the ring with rows of `down`. Eight warps multiply:
 // warp w has columns [64 w, 64 w + 64) of a stage, weights as operand A of m16n8k16, up to eight tokens as operand B from L2; which column of a chunk a thread has does
 // not matter to a sum, so a thread reads 16-byte chunks (2 t + i of a row of eight: no two of a phase share banks). The warps' sums are added in order in shared memory.
-//   1  logits: an (expert, four tokens) pair a warp, or a CTA where there are fewer pairs than CTAs; rows are copied as bf16 planes (f32 rows: value and remainder).
+//   1  logits: an (expert, four tokens) pair a warp, or a CTA where there are fewer pairs than CTAs; rows are copied as bf16 planes (f32 rows: three, 24 bits; with two, the results were 4.5e-6 off, a plain product in f32 1.3e-6).
 //   2  every CTA makes the choice for itself from the logits (waiting for one to do it would cost more), lists the chosen experts and their tokens.
 //   3  up: a unit is 16 rows of an expert's up and the 16 of its gate; hidden values, times the routing weight, go to scratch as bf16 planes.
 //   4  down: all stages of all 32-row tiles over all chosen experts, cut evenly over the CTAs; a tile that several have is summed by the last of them, in their order.
@@ -18,7 +18,7 @@ namespace uzu {
 namespace {
 
 constexpr uint32_t XL_WARPS = 8, XL_THREADS = 32 * XL_WARPS + 32, XL_STAGE = 32 * 1024, XL_COLS = 512, XL_BOX = 4096;
-constexpr uint32_t XL_MAX_TOKENS = 64, XL_MAX_EXPERTS = 528, XL_MAX_TOP = 16, XL_MAX_PAIRS = 64 * 32, XL_CTAS = 148, XL_MAX_WIDTH = 65536;
+constexpr uint32_t XL_MAX_TOKENS = 64, XL_MAX_EXPERTS = 528, XL_MAX_LISTED = 592 /* every expert, and 64 of at most 2048 pairs with 32 more */, XL_MAX_TOP = 16, XL_MAX_PAIRS = 64 * 32, XL_CTAS = 148, XL_MAX_WIDTH = 65536;
 
 // where what lies in the scratch; the counters and tickets are zero between calls
 struct XlScratch {
@@ -27,7 +27,7 @@ struct XlScratch {
 };
 inline XlScratch xl_scratch(const uzu_expert_layer_args& a) {
     auto up = [](uint64_t v) { return (v + 255) & ~255ull; };
-    const uint64_t planes = a.data_type == UZU_DT_F32 ? 2 : 1;
+    const uint64_t planes = a.data_type == UZU_DT_F32 ? 3 : 1;
     XlScratch s;
     s.logits = up(XlScratch::FIXED);
     s.rows = up(s.logits + (uint64_t)a.rows * a.experts * 4);
@@ -45,10 +45,12 @@ struct XlParams {
     unsigned int* error;
 };
 
-template <int NT, int PLANES>
+// Token tiles of eight that one reading of an expert's weights serves, rows of the call at most, bf16 planes of a value. (An expert with more tokens than that is listed, and
+// read, twice: with eight tiles the sums would not leave the registers that the products need.)
+template <int NT, int ROWS, int PLANES>
 struct XlShape {
-    static constexpr uint32_t TOK = NT * 8 + 1, RED = XL_WARPS * 32 * TOK * 4,      // tokens of a row of sums, and one place to keep rows off one another's banks
-                              STAGES = NT <= 2 ? 6 : NT == 4 ? 5 : 4;
+    static constexpr uint32_t TOK = ROWS + 1, RED = XL_WARPS * 32 * TOK * 4;      // tokens of a row of sums, and one place to keep rows off one another's banks
+    static constexpr uint32_t STAGES = ROWS <= 16 ? 6 : ROWS == 32 ? 5 : 4;
     static constexpr size_t SMEM = STAGES * XL_STAGE + RED + 1024;
 };
 
@@ -59,6 +61,16 @@ __device__ __forceinline__ void xl_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
 }
 __device__ __forceinline__ void xl_tma3(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint32_t z, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+// a value as PLANES bf16 parts, each what the ones before leave (of what is no number or infinite: the first alone, the product shows it by that)
+template <int PLANES>
+__device__ __forceinline__ void xl_planes(float v, __nv_bfloat16* to, size_t plane) {
+#pragma unroll
+    for (int pl = 0; pl < PLANES; ++pl) {
+        const __nv_bfloat16 part = __float2bfloat16_rn(v);
+        to[pl * plane] = part;
+        v = fabsf(v) < INFINITY ? v - __bfloat162float(part) : 0.0f;
+    }
 }
 __device__ __forceinline__ float xl_x(const uzu_expert_layer_args& a, uint32_t t, uint32_t c) {
     return a.data_type == UZU_DT_F32 ? reinterpret_cast<const float*>(a.x)[(size_t)t * a.x_stride + c] : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.x)[(size_t)t * a.x_stride + c]);
@@ -102,8 +114,8 @@ __device__ __forceinline__ void xl_x8(const uzu_expert_layer_args& a, uint32_t t
 
 struct XlLists {
     uint32_t mask[XL_MAX_EXPERTS][2];      // tokens of an expert
-    uint16_t expert[XL_MAX_EXPERTS];       // the chosen ones, ascending
-    uint16_t base[XL_MAX_EXPERTS + 1];     // their pairs, in that order
+    uint16_t expert[XL_MAX_LISTED];        // the chosen ones, ascending; one with many tokens several times
+    uint16_t base[XL_MAX_LISTED + 1];      // their pairs, in that order
     uint16_t token[XL_MAX_PAIRS];          // a pair's token, and behind it (64 times) which of the token's choices the expert is (31: shared)
     uint16_t id[XL_MAX_TOKENS][XL_MAX_TOP];
     float weight[XL_MAX_TOKENS][XL_MAX_TOP];
@@ -177,9 +189,9 @@ __device__ void xl_choose(const uzu_expert_layer_args& a, const float* logits, u
 
 }  // namespace
 
-template <int NT, int PLANES>
+template <int NT, int ROWS, int PLANES>
 __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __grid_constant__ CUtensorMap map_up, const __grid_constant__ CUtensorMap map_down, const __grid_constant__ XlParams p) {
-    using S = XlShape<NT, PLANES>;
+    using S = XlShape<NT, ROWS, PLANES>;
     constexpr uint32_t TOK = S::TOK;
     extern __shared__ uint8_t xl_raw[];
     __shared__ __align__(8) uint64_t bars[2 * S::STAGES];
@@ -216,10 +228,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
     // ---- 1: rows as planes, logits ----
     for (uint32_t i = cta * XL_THREADS + tid; i < T * D; i += ctas * XL_THREADS) {
         const float v = xl_x(a, i / D, i % D);
-        const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-        rows[i] = hi;
-        // (not of what is no number or infinite: the product shows it by the first part alone)
-        if (PLANES == 2) rows[row_plane + i] = __float2bfloat16_rn(fabsf(v) < INFINITY ? v - __bfloat162float(hi) : 0.0f);
+        xl_planes<PLANES>(v, rows + i, row_plane);
     }
     {
         const uint32_t quads = (T + 3) / 4, pairs = E * quads;
@@ -273,18 +282,19 @@ float v[8];
         if (warp == 0) {
             uint32_t count = 0, pairs = 0;
             for (uint32_t e0 = 0; e0 < all; e0 += 32) {
-                const uint32_t e = e0 + lane, n = e < all ? __popc(l.mask[e][0]) + __popc(l.mask[e][1]) : 0u, there = __ballot_sync(0xffffffffu, n != 0);
-                uint32_t before = n;      // pairs of the experts below, this one's included
+                const uint32_t e = e0 + lane, n = e < all ? __popc(l.mask[e][0]) + __popc(l.mask[e][1]) : 0u, times = (n + 8 * NT - 1) / (8 * NT);
+                uint32_t before = n | times << 16;      // pairs and entries of the experts below, this one's included
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const uint32_t v = __shfl_up_sync(0xffffffffu, before, o);
                     if (lane >= o) before += v;
                 }
                 if (n) {
-                    const uint32_t at = count + __popc(there & ((1u << lane) - 1u));
-                    uint32_t pair = pairs + before - n;
-                    l.expert[at] = (uint16_t)e;
-                    l.base[at] = (uint16_t)pair;
+                    uint32_t pair = pairs + (before & 0xffffu) - n;
+                    for (uint32_t k = 0; k < times; ++k) {
+                        l.expert[count + (before >> 16) - times + k] = (uint16_t)e;
+                        l.base[count + (before >> 16) - times + k] = (uint16_t)(pair + k * 8 * NT);
+                    }
                     for (uint32_t half = 0; half < 2; ++half)
                         for (uint32_t m = l.mask[e][half]; m; m &= m - 1) {
                             const uint32_t t = half * 32 + __ffs(m) - 1;
@@ -294,8 +304,9 @@ float v[8];
                             l.token[pair++] = (uint16_t)(j * 64 + t);
                         }
                 }
-                count += __popc(there);
-                pairs += __shfl_sync(0xffffffffu, before, 31);
+                const uint32_t sums = __shfl_sync(0xffffffffu, before, 31);
+                count += sums >> 16;
+                pairs += sums & 0xffffu;
             }
             if (lane == 0) {
                 l.base[count] = (uint16_t)pairs;
@@ -453,10 +464,7 @@ float v[8];
                 if (f0 + f >= F) continue;
                 const float w = choice < XL_MAX_TOP ? l.weight[pair & 63u][choice] : 1.0f;
                 const float v = act_f32(a.activation, total(16 + f, k)) * total(f, k) * w;
-                const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-                __nv_bfloat16* to = hidden + (size_t)(base + k) * F + f0 + f;
-                to[0] = hi;
-                if (PLANES == 2) to[hidden_plane] = __float2bfloat16_rn(fabsf(v) < INFINITY ? v - __bfloat162float(hi) : 0.0f);
+                xl_planes<PLANES>(v, hidden + (size_t)(base + k) * F + f0 + f, hidden_plane);
             }
             meet();
             at = next_at;
@@ -575,21 +583,21 @@ const char* xl_check(const uzu_expert_layer_args* a, bool run) {
     return nullptr;
 }
 
-template <int NT, int PLANES>
+template <int NT, int ROWS, int PLANES>
 void xl_launch(uzu_command_buffer* cmd, const XlParams& p, const CUtensorMap& up, const CUtensorMap& down) {
     static std::atomic<uint64_t> opted{0};
-    opt_in_dynamic_smem(cmd, expert_layer_kernel<NT, PLANES>, (int)XlShape<NT, PLANES>::SMEM, opted);
+    opt_in_dynamic_smem(cmd, expert_layer_kernel<NT, ROWS, PLANES>, (int)XlShape<NT, ROWS, PLANES>::SMEM, opted);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(std::min<uint32_t>(cmd->ctx->sm_count, XL_CTAS));
     cfg.blockDim = dim3(XL_THREADS);
-    cfg.dynamicSmemBytes = XlShape<NT, PLANES>::SMEM;
+    cfg.dynamicSmemBytes = XlShape<NT, ROWS, PLANES>::SMEM;
     cfg.stream = cmd->ctx->stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeCooperative;      // all CTAs run together, or the launch fails
     attr[0].val.cooperative = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, expert_layer_kernel<NT, PLANES>, up, down, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, expert_layer_kernel<NT, ROWS, PLANES>, up, down, p);
     if (e != cudaSuccess) {
         cmd->record_error(UZU_ERROR_CUDA, std::string("expert_layer_kernel: ") + cudaGetErrorString(e));
         cudaGetLastError();
@@ -637,12 +645,12 @@ void uzu_expert_layer_encode(uzu_command_buffer* cmd, const uzu_expert_layer_arg
     // token tiles of eight: the smallest kernel that holds the rows (a larger one's ring is shorter)
     auto go = [&](auto planes) {
         constexpr int PL = decltype(planes)::value;
-        if (a->rows <= 8) xl_launch<1, PL>(cmd, p, up, down);
-        else if (a->rows <= 16) xl_launch<2, PL>(cmd, p, up, down);
-        else if (a->rows <= 32) xl_launch<4, PL>(cmd, p, up, down);
-        else xl_launch<8, PL>(cmd, p, up, down);
+        if (a->rows <= 8) xl_launch<1, 8, PL>(cmd, p, up, down);
+        else if (a->rows <= 16) xl_launch<2, 16, PL>(cmd, p, up, down);
+        else if (a->rows <= 32) xl_launch<4, 32, PL>(cmd, p, up, down);
+        else xl_launch<4, 64, PL>(cmd, p, up, down);
     };
-    if (a->data_type == UZU_DT_F32) go(std::integral_constant<int, 2>{});
+    if (a->data_type == UZU_DT_F32) go(std::integral_constant<int, 3>{});
     else go(std::integral_constant<int, 1>{});
 }
 
