@@ -1,8 +1,10 @@
 // Short causal convolution over packed sequences: y[t, c] = act(bias[c] + sum_j w[c, j] u[t - taps + 1 + j, c]).
 //
-// Bound by memory: a value is read and written once, 2 taps flops each. A thread has 16 bytes of channels (8 of 16 bits, 4 of 32) and walks a strip of a sequence's
-// rows with the last taps - 1 of them in registers, eight rows of loads under way at a time; a strip reads taps - 1 rows of the one before it again (from L2). The
-// strip that starts a sequence reads the slot's inputs and then writes the new ones: nobody else touches these channels of the slot, so the order is its own.
+// Bound by memory: a value is read and written once, 2 taps flops each; special functions (an exponential a value, a reciprocal for two) take half of that time beside it. A
+// thread has 8 bytes of channels (four of 16 bits, two of 32) and walks a strip of a sequence's rows with the last taps - 1 of them in registers, eight rows of loads under way
+// at a time; a strip reads taps - 1 rows of the one before it again (from L2). 16384 rows of 10240 bf16 channels, 4 taps, 16 sequences: 137 us, 4.9 TB/s of the 6.45 of a copy
+// (16 bytes a thread 178 us: fewer warps; 4 bytes 223; batches of four rows 146; limits on the registers 170 to 284).
+// The strip that starts a sequence reads the slot's inputs and then writes the new ones: nobody else touches these channels of the slot, so the order is its own.
 #include "state_space.cuh"
 
 namespace uzu {
