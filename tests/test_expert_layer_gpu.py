@@ -135,3 +135,26 @@ def test_values_that_are_not_finite_stay_in_their_row(ctx):
     _, got, *_ = lay.run(10, 2, P.BF16, x=bad)
     keep = [r for r in range(10) if r not in (3, 7)]
     assert np.array_equal(got[keep], clean[keep]) and not np.isfinite(P.of_kept(got[[3, 7]], P.BF16)).all()
+
+
+@pytest.mark.parametrize("score", [0, 1, 2])
+@pytest.mark.parametrize("experts,top", [(8, 2), (8, 8), (64, 6), (300, 16)])
+def test_choice_of_logits_that_are_not_finite(ctx, experts, top, score):
+    """choices of such tokens are distinct experts, NaN last; the other tokens keep theirs (their sums' order may differ: it follows the choice of all)"""
+    lay = _Layer(ctx, 128, 64, experts, 0, seed=11)
+    x = lay.rng.standard_normal((9, 128))
+    _, clean, ids0, w0, _ = lay.run(9, top, P.F32, score=score, x=x)
+    r, u, d = (P.of_kept(v, P.BF16) for v in lay.host)
+    _, _, _, mag, _ = P.experts(P.of_kept(P.to_kept(x, P.F32), P.F32), r, lay.bias.astype(np.float64), u, d, top, 0, score, 0, 1.0, P.silu)
+    bad = x.copy()
+    bad[2, 5], bad[4, :], bad[6, 1] = np.inf, np.nan, -np.inf
+    _, got, ids, w, _ = lay.run(9, top, P.F32, score=score, x=bad)
+    keep = [0, 1, 3, 5, 7, 8]
+    assert np.array_equal(ids[keep], ids0[keep]) and np.array_equal(w[keep], w0[keep])
+    # both sums are within the unit that `_Layer.check` derives, and their last rounding
+    unit = 2.0 ** -24 * 3 * (128 + 64) / 8 + 2.0 ** -24 * ((128 + 64) / 8 + 32) + 2.0 ** -20
+    assert (np.abs(got[keep] - clean[keep]) <= 2 * (unit * mag[keep] + P.HALF_STEP[P.F32] * np.abs(clean[keep]) + 1e-30)).all()
+    assert ids.max() < experts and all(len(set(r)) == top for r in ids.tolist())
+    assert np.array_equal(ids[4], np.arange(top)) and (score == 2 or np.isnan(w[4]).all())
+    if score == 1:
+        assert np.array_equal(ids[2], np.arange(top)) and np.isnan(w[2]).all()

@@ -152,7 +152,10 @@ __device__ void xl_choose(const uzu_expert_layer_args& a, const float* logits, u
         }
         sum = warp_sum(sum);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) v[i] /= sum;
+        for (int i = 0; i < PER; ++i) {
+            v[i] /= sum;
+            if (v[i] != v[i]) v[i] = -INFINITY;      // (an infinite logit, or none that is a number: the lanes have to agree on an order)
+        }
     }
     uint32_t taken = 0;
     float mine = 0.0f, first = 0.0f;      // lane k: the score of choice k
@@ -175,6 +178,7 @@ __device__ void xl_choose(const uzu_expert_layer_args& a, const float* logits, u
         if (k == 0) first = best;
         if (lane == k) { mine = best; mine_id = at; }
     }
+    if (a.score == UZU_EXPERT_SCORE_ALL && mine == -INFINITY) mine = __int_as_float(0x7fc00000);
     float w = lane < a.top ? mine : 0.0f;
     if (a.score == UZU_EXPERT_SCORE_CHOSEN) {
         w = lane < a.top ? expf(mine - first) : 0.0f;
@@ -249,7 +253,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
 #pragma unroll
                     for (uint32_t k = 0; k < 4; ++k)
                         if (tk + k < T) {
-float v[8];
+                            float v[8];
                             xl_x8(a, tk + k, c, wide, v);
 #pragma unroll
                             for (uint32_t j = 0; j < 4; ++j) sum[k] = fmaf(um_hi(ws[j]), v[2 * j + 1], fmaf(um_lo(ws[j]), v[2 * j], sum[k]));
