@@ -4,14 +4,15 @@
 // room, over the units and over the phases, so that the wait of all CTAs for the hidden values is spent filling the ring with rows of `down`. Eight warps multiply:
 // warp w has columns [64 w, 64 w + 64) of a stage, weights as operand A of m16n8k16, up to eight tokens as operand B from L2; which column of a chunk a thread has does
 // not matter to a sum, so a thread reads 16-byte chunks (2 t + i of a row of eight: no two of a phase share banks). The warps' sums are added in order in shared memory.
-//   1  logits: an (expert, four tokens) pair a warp, or a CTA where there are fewer pairs than CTAs; rows are copied as bf16 planes (f32 rows: three, 24 bits; with two, the results were 4.5e-6 off, a plain product in f32 1.3e-6).
+//   1  logits: an (expert, four tokens) pair a warp, or a CTA where there are fewer pairs than CTAs; rows are copied as bf16 planes (f32 rows: three, 24 bits, and a stage's products summed by themselves: the results are 2.8e-7 off, in one
+//      running sum of matrix instructions 1.8e-6, with two planes 4.5e-6; a plain product in f32 1.3e-6).
 //   2  every CTA makes the choice for itself from the logits (waiting for one to do it would cost more), lists the chosen experts and their tokens.
 //   3  up: a unit is 16 rows of an expert's up and the 16 of its gate; hidden values, times the routing weight, go to scratch as bf16 planes.
 //   4  down: all stages of all 32-row tiles over all chosen experts, cut evenly over the CTAs; a tile that several have is summed by the last of them, in their order.
 // In both products an expert's tokens stand side by side, eight a tile; the rows of the next stage are asked for a stage ahead.
 // Two waits for all CTAs, behind phases 1 and 3. They and the ring's barriers are bounded (wait_errors.h).
 // One token of 8 experts of 4096 x 14336, two chosen: 125 us, 5.6 TB/s of the 6.45 of a copy (router, choice and the two waits take 12). 16 tokens of 64 experts of 2048 x 1408, six
-// chosen and two shared: 185 us of 142. 48 f32 tokens of 128 experts of 2048 x 768: 356 us of 179, bound by the warps' way through a stage (three planes, 1400 cycles where the
+// chosen and two shared: 185 us of 142. 48 f32 tokens of 128 experts of 2048 x 768: 370 us of 179, bound by the warps' way through a stage (three planes, 1400 cycles where the
 // bytes take 1400) and the 39 units' ends of 1500 cycles each.
 #include <algorithm>
 
@@ -383,6 +384,11 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
                     to[pl][i] = at && c < width ? __ldcg(reinterpret_cast<const uint4*>(at + pl * plane + c)) : make_uint4(0, 0, 0, 0);
                 }
         };
+        // 16 rows times 32 columns of eight tokens
+        auto pair = [&](float (&c)[4], const uint4& lo, const uint4& hi, const uint4& b) {
+            xl_mma(c, lo.x, hi.x, lo.y, hi.y, b.x, b.y);
+            xl_mma(c, lo.z, hi.z, lo.w, hi.w, b.z, b.w);
+        };
         // A stage, for `count` tokens whose rows `src(k)` gives, eight at a time. The first eight of it were asked for a stage ago, into `first`; those of the next stage are asked for
         // (`next`) before this one's products, since they come from L2 no faster than a stage.
         uint4 first[PLANES][2];
@@ -413,15 +419,24 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
 #pragma unroll
                     for (int pl = 0; pl < PLANES; ++pl) { v[pl][0] = b[pl][0]; v[pl][1] = b[pl][1]; }
                     if (n + 1 < NT && (n + 1) * 8 < count) ask((n + 1) * 8 + g < count ? src((n + 1) * 8 + g) : nullptr, col, width, plane, b);
+                    if (PLANES == 1) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                        for (int i = 0; i < 2; ++i)
 #pragma unroll
-                        for (int pl = PLANES - 1; pl >= 0; --pl)
+                            for (int m = 0; m < 2; ++m) pair(acc[m][n], w[i][2 * m], w[i][2 * m + 1], v[0][i]);
+                    } else {
+                        // A matrix instruction cuts its sum off where an addition rounds it: a stage's products, smallest planes first, have sums of their own
 #pragma unroll
-                            for (int m = 0; m < 2; ++m) {
-                                xl_mma(acc[m][n], w[i][2 * m].x, w[i][2 * m + 1].x, w[i][2 * m].y, w[i][2 * m + 1].y, v[pl][i].x, v[pl][i].y);
-                                xl_mma(acc[m][n], w[i][2 * m].z, w[i][2 * m + 1].z, w[i][2 * m].w, w[i][2 * m + 1].w, v[pl][i].z, v[pl][i].w);
-                            }
+                        for (int m = 0; m < 2; ++m) {
+                            float stage[4] = {};
+#pragma unroll
+                            for (int pl = PLANES - 1; pl >= 0; --pl)
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) pair(stage, w[i][2 * m], w[i][2 * m + 1], v[pl][i]);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) acc[m][n][j] += stage[j];
+                        }
+                    }
                 }
             }
             um_arrive_after(empty(s), seen, a.reserved0);
