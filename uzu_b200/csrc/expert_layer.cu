@@ -12,7 +12,7 @@
 // In both products an expert's tokens stand side by side, eight a tile; the rows of the next stage are asked for a stage ahead.
 // Two waits for all CTAs, behind phases 1 and 3. They and the ring's barriers are bounded (wait_errors.h).
 // One token of 8 experts of 4096 x 14336, two chosen: 125 us, 5.6 TB/s of the 6.45 of a copy (router, choice and the two waits take 12). 16 tokens of 64 experts of 2048 x 1408, six
-// chosen and two shared: 185 us of 142. 48 f32 tokens of 128 experts of 2048 x 768: 370 us of 179, bound by the warps' way through a stage (three planes, 1400 cycles where the
+// chosen and two shared: 185 us of 142. 48 f32 tokens of 128 experts of 2048 x 768: 351 us of 179, bound by the warps' way through a stage (three planes, 1400 cycles where the
 // bytes take 1400) and the 39 units' ends of 1500 cycles each.
 #include <algorithm>
 
@@ -23,7 +23,7 @@ namespace uzu {
 namespace {
 
 constexpr uint32_t XL_WARPS = 8, XL_THREADS = 32 * XL_WARPS + 32, XL_STAGE = 32 * 1024, XL_COLS = 512, XL_BOX = 4096;
-constexpr uint32_t XL_MAX_TOKENS = 64, XL_MAX_EXPERTS = 528, XL_MAX_LISTED = 592 /* every expert, and 64 of at most 2048 pairs with 32 more */, XL_MAX_TOP = 16, XL_MAX_PAIRS = 64 * 32, XL_CTAS = 148, XL_MAX_WIDTH = 65536;
+constexpr uint32_t XL_MAX_TOKENS = 64, XL_MAX_EXPERTS = 528, XL_MAX_LISTED = 656 /* every expert, and 128 of at most 2048 pairs with 16 more */, XL_MAX_TOP = 16, XL_MAX_PAIRS = 64 * 32, XL_CTAS = 148, XL_MAX_WIDTH = 65536;
 
 // where what lies in the scratch; the counters and tickets are zero between calls
 struct XlScratch {
@@ -51,7 +51,8 @@ struct XlParams {
 };
 
 // Token tiles of eight that one reading of an expert's weights serves, rows of the call at most, bf16 planes of a value. (An expert with more tokens than that is listed, and
-// read, twice: with eight tiles the sums would not leave the registers that the products need.)
+// read, twice: with eight tiles the sums would not leave the registers that the products need. Of three planes two tiles: with four some registers are spilled, and 24, 40 and 64
+// rows of four layers took 2 to 7 percent longer, also where most experts have more than 16 tokens: 1024 x 512, 8 of 32 experts, 64 rows 147 us, 145 with two.)
 template <int NT, int ROWS, int PLANES>
 struct XlShape {
     static constexpr uint32_t TOK = ROWS + 1, RED = XL_WARPS * 32 * TOK * 4;      // tokens of a row of sums, and one place to keep rows off one another's banks
@@ -667,11 +668,11 @@ void uzu_expert_layer_encode(uzu_command_buffer* cmd, const uzu_expert_layer_arg
     }
     // token tiles of eight: the smallest kernel that holds the rows (a larger one's ring is shorter)
     auto go = [&](auto planes) {
-        constexpr int PL = decltype(planes)::value;
+        constexpr int PL = decltype(planes)::value, most = PL == 1 ? 4 : 2;
         if (a->rows <= 8) xl_launch<1, 8, PL>(cmd, p, up, down);
         else if (a->rows <= 16) xl_launch<2, 16, PL>(cmd, p, up, down);
-        else if (a->rows <= 32) xl_launch<4, 32, PL>(cmd, p, up, down);
-        else xl_launch<4, 64, PL>(cmd, p, up, down);
+        else if (a->rows <= 32) xl_launch<most, 32, PL>(cmd, p, up, down);
+        else xl_launch<most, 64, PL>(cmd, p, up, down);
     };
     if (a->data_type == UZU_DT_F32) go(std::integral_constant<int, 3>{});
     else go(std::integral_constant<int, 1>{});
