@@ -918,7 +918,7 @@ typedef struct uzu_row_sequence { uint32_t first_row, rows, slot, fresh; } uzu_r
 /* Short causal convolution per channel over packed sequences, for prompts and for single rows:
  *   output[t, c] = act(bias[c] + sum_j weights[c, j] * u[t - taps + 1 + j, c])
  * where u are the sequence's rows behind the taps - 1 inputs that its slot holds, oldest first; the slot takes the last taps - 1 inputs. One rounding, of
- * the output. Channels, strides and pointers of whole 16-byte groups take vector loads, others single ones. */
+ * the output. Channels and strides of whole 8-byte groups behind 16-byte aligned pointers take vector loads, others single ones. */
 typedef struct uzu_causal_conv_args {
     uint64_t input, output;        /* data_type [rows, channels] */
     uint64_t weights, bias;        /* f32 [channels, taps], optional f32 [channels] */

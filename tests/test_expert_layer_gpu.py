@@ -158,3 +158,22 @@ def test_choice_of_logits_that_are_not_finite(ctx, experts, top, score):
     assert np.array_equal(ids[4], np.arange(top)) and (score == 2 or np.isnan(w[4]).all())
     if score == 1:
         assert np.array_equal(ids[2], np.arange(top)) and np.isnan(w[2]).all()
+
+
+@pytest.mark.parametrize("dt", [P.BF16, P.F32])
+def test_slices_of_the_same_rows(ctx, dt):
+    """out beside x in the same wide rows: the same bits as apart, and x stays"""
+    lay, rows, w = _Layer(ctx, 128, 64, 8, 1, seed=12), 21, 128
+    x, apart, *_ = lay.run(rows, 2, dt)
+    wide = np.zeros((rows, 2 * w), P.to_kept(x, dt).dtype)
+    wide[:, :w] = P.to_kept(x, dt)
+    buf = ctx.upload(wide)
+    a = B.ExpertLayerArgs(x=buf.ptr, out=buf.ptr + w * wide.itemsize, router=lay.bufs[0].ptr, router_bias=lay.bufs[3].ptr, up_gate=lay.bufs[1].ptr, down=lay.bufs[2].ptr, rows=rows, width=w, ff=64,
+                          experts=8, top=2, shared=1, x_stride=2 * w, out_stride=2 * w, weight_scale=1.0, activation=B.ACT_SILU, data_type=dt)
+    a.scratch_bytes = ctx.lib.uzu_expert_layer_scratch_bytes(C.byref(a))
+    scratch = ctx.upload(np.zeros(a.scratch_bytes, np.uint8))
+    a.scratch = scratch.ptr
+    with ctx.command_buffer("experts") as cmd:
+        cmd.encode("uzu_expert_layer_encode", C.byref(a))
+    got = buf.numpy(wide.dtype, wide.shape)
+    assert np.array_equal(got[:, :w], wide[:, :w]) and np.array_equal(got[:, w:], apart)

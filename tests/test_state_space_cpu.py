@@ -138,3 +138,13 @@ def test_experts_refused(lib, over, part):
 def test_experts_taken(lib):
     assert lib.uzu_expert_layer_validate(C.byref(_experts(lib))) == 0 and lib.uzu_expert_layer_validate(C.byref(_experts(lib, rows=0, x=0))) == 0
     assert lib.uzu_expert_layer_scratch_bytes(C.byref(_experts(lib, width=60))) == 0
+
+
+def test_experts_side_by_side(lib):
+    """x and out as slices of the same wide rows: side by side they share nothing, a column less apart they do"""
+    base = 1 << 20
+    beside = dict(x=base, out=base + 64 * 2, x_stride=128, out_stride=128)
+    assert lib.uzu_expert_layer_validate(C.byref(_experts(lib, **beside))) == 0
+    assert lib.uzu_expert_layer_validate(C.byref(_experts(lib, **{**beside, "x": base + 64 * 2, "out": base}))) == 0
+    _refused(lib, "uzu_expert_layer_validate", _experts(lib, **{**beside, "out": base + 63 * 2}), "overlap")
+    _refused(lib, "uzu_expert_layer_validate", _experts(lib, **{**beside, "out_stride": 129}), "overlap")

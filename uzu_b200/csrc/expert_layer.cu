@@ -16,6 +16,7 @@
 // bytes take 1400) and the 39 units' ends of 1500 cycles each.
 #include <algorithm>
 
+#include "row_sequences.h"
 #include "umma.cuh"
 
 namespace uzu {
@@ -602,8 +603,7 @@ const char* xl_check(const uzu_expert_layer_args* a, bool run) {
     const uint64_t size = a->data_type == UZU_DT_F32 ? 4 : 2;
     if ((a->x | a->out) % size || (a->router | a->up_gate | a->down) % 16 || (a->router_bias | a->ids | a->weights) % 4) return "an operand is not aligned";
     if (a->scratch % 256 || a->scratch_bytes < xl_scratch(*a).total) return "the scratch is too small or not 256-byte aligned";
-    const uint64_t x_bytes = ((uint64_t)(a->rows - 1) * a->x_stride + a->width) * size, out_bytes = ((uint64_t)(a->rows - 1) * a->out_stride + a->width) * size;
-    if (a->x < a->out + out_bytes && a->out < a->x + x_bytes) return "x and out overlap";
+    if (rows_overlap(a->x, a->x_stride, a->width, a->out, a->out_stride, a->width, a->rows, size)) return "x and out overlap";
     return nullptr;
 }
 
