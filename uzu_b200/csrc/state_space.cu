@@ -9,7 +9,7 @@
 // Step: bound by the state, read and written once. A CTA has up to 64 rows p of one head of one sequence. What the convolution takes is asked for first, then all of the state;
 // the CTA convolves its x channels and its group's b and c while that comes. The conv slots of b and c are read by all CTAs of the group: each counts itself when it has
 // them, the last one writes the new inputs and takes the count back to zero. 64 rows of 80 heads of 64 x 128: 72 us, 4.7 TB/s of the 6.45 of a copy; 256 rows of 128 heads 483 us
-// (four CTAs an SM do not cover all of a CTA's phases; 32 rows a CTA: 5 percent slower; one CTA an SM that streams the state through shared memory by bulk copies: slower too).
+// (three CTAs an SM, by registers, do not cover all of a CTA's phases; 32 rows a CTA: 5 percent slower; one CTA an SM that streams the state through shared memory by bulk copies: slower too).
 #include "state_space.cuh"
 
 namespace uzu {
