@@ -65,3 +65,23 @@ def test_conv_gate_of_large_sums(ctx, dt, channels, taps):
     small = (ref > -1e-15) & (ref < 0)
     part = (taps + 4) * 2.0 ** -23 * mag + 2.0 ** -20 + P.HALF_STEP[dt]
     assert (np.abs(got - ref) <= part * np.abs(ref) * 1.1 + P.TINY[dt] + np.minimum(mag, 1000) * 2.0 ** -149)[small].all()
+
+
+@pytest.mark.parametrize("dt", [P.BF16, P.F32])
+@pytest.mark.parametrize("taps", [1, 2, 3, 4, 5, 6, 7, 8])
+@pytest.mark.parametrize("act", [B.ACT_SILU, B.ACT_IDENTITY])
+def test_conv_infinite_inputs_reach_their_window_only(ctx, dt, taps, act):
+    """an input that is infinite or no number shows in the taps rows that read it, in its channel, and nowhere else"""
+    rng = np.random.default_rng(taps)
+    rows, channels, seqs = 60, 24, [(0, 45, 1, 0), (45, 15, 0, 1)]
+    u, w, st = rng.standard_normal((rows, channels)), rng.standard_normal((channels, taps)), rng.standard_normal((2, max(taps - 1, 1), channels))
+    clean, _ = _run_conv(ctx, u, w, seqs, dt, 2, act=act, state=st)
+    hit = np.zeros((rows, channels), bool)
+    for row, channel, value in [(3, 2, np.inf), (20, 9, np.nan), (31, 23, -np.inf), (44, 5, np.inf), (46, 0, np.nan)]:
+        u[row, channel] = value
+        hit[row:min(row + taps, 45 if row < 45 else rows), channel] = True
+    got, _ = _run_conv(ctx, u, w, seqs, dt, 2, act=act, state=st)
+    assert not np.isfinite(got[hit]).any()
+    beside = ~hit & hit.reshape(rows, channels // 2, 2)[:, :, ::-1].reshape(rows, channels)      # the gate takes one reciprocal for two channels: 2^-21 of the value each time, and its rounding
+    assert np.array_equal(got[~hit & ~beside], clean[~hit & ~beside])
+    assert (np.abs(got - clean)[beside] <= (2.0 ** -20 + 2 * P.HALF_STEP[dt]) * np.abs(clean[beside])).all()

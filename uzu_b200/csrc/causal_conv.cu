@@ -53,19 +53,20 @@ template <typename T, int VEC, int TAPS>
 __device__ __forceinline__ void conv_keep(const ConvParams& p, const PackedSequence& s) {
     using V = ConvVec<T, VEC>;
     const uzu_causal_conv_args& a = p.a;
-    const uint32_t c = (blockIdx.x % p.groups * CC_THREADS + threadIdx.x) * VEC, kept = a.taps - 1;
+    constexpr uint32_t kept = TAPS - 1;
+    const uint32_t c = (blockIdx.x % p.groups * CC_THREADS + threadIdx.x) * VEC;
     const T* in = reinterpret_cast<const T*>(a.input) + (size_t)s.first * a.input_stride + c;
     T* state = reinterpret_cast<T*>(a.state) + (size_t)s.slot() * kept * a.channels + c;
+    V v[TAPS > 1 ? TAPS - 1 : 1];      // (all read before one is written)
 #pragma unroll
-    for (uint32_t k = 0; k < TAPS - 1; ++k) {      // (ascending: a place that moves up is read before it is written)
-        if (k >= kept) break;
-        V v;
+    for (uint32_t k = 0; k < kept; ++k) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v.v[i] = ss_t<T>(0.0f);
-        if (s.rows + k >= kept) v = *reinterpret_cast<const V*>(in + (size_t)(s.rows + k - kept) * a.input_stride);
-        else if (!s.fresh()) v = *reinterpret_cast<const V*>(state + (size_t)(s.rows + k) * a.channels);
-        *reinterpret_cast<V*>(state + (size_t)k * a.channels) = v;
+        for (int i = 0; i < VEC; ++i) v[k].v[i] = ss_t<T>(0.0f);
+        if (s.rows + k >= kept) v[k] = *reinterpret_cast<const V*>(in + (size_t)(s.rows + k - kept) * a.input_stride);
+        else if (!s.fresh()) v[k] = *reinterpret_cast<const V*>(state + (size_t)(s.rows + k) * a.channels);
     }
+#pragma unroll
+    for (uint32_t k = 0; k < kept; ++k) *reinterpret_cast<V*>(state + (size_t)k * a.channels) = v[k];
 }
 
 template <typename T, int VEC, int TAPS>
@@ -79,7 +80,8 @@ __global__ void __launch_bounds__(CC_THREADS) causal_conv_kernel(const __grid_co
     if (c >= a.channels) return;
     const uint32_t tile = blockIdx.x / p.groups, q = ss_find(p.table, tile);
     const PackedSequence s = p.table.s[q];
-    const uint32_t t0 = (tile - s.tile0) * p.strip, t1 = min(t0 + p.strip, s.rows), kept = a.taps - 1;
+    const uint32_t t0 = (tile - s.tile0) * p.strip, t1 = min(t0 + p.strip, s.rows);
+    constexpr uint32_t kept = TAPS - 1;
     const T* in = reinterpret_cast<const T*>(a.input) + (size_t)s.first * a.input_stride + c;
     T* out = reinterpret_cast<T*>(a.output) + (size_t)s.first * a.output_stride + c;
     T* state = reinterpret_cast<T*>(a.state) + (size_t)s.slot() * kept * a.channels + c;
@@ -91,21 +93,16 @@ __global__ void __launch_bounds__(CC_THREADS) causal_conv_kernel(const __grid_co
         const bool there = i < VEC;
         (i & 1 ? bias[i / 2].y : bias[i / 2].x) = there && a.bias ? reinterpret_cast<const float*>(a.bias)[c + i] : 0.0f;
 #pragma unroll
-        for (int j = 0; j < TAPS; ++j) {      // fewer taps than the kernel has: the oldest ones are zero
-            const int k = j - (TAPS - (int)a.taps);
-            (i & 1 ? w[j][i / 2].y : w[j][i / 2].x) = there && k >= 0 ? reinterpret_cast<const float*>(a.weights)[(size_t)(c + i) * a.taps + k] : 0.0f;
-        }
+        for (int j = 0; j < TAPS; ++j) (i & 1 ? w[j][i / 2].y : w[j][i / 2].x) = there ? reinterpret_cast<const float*>(a.weights)[(size_t)(c + i) * TAPS + j] : 0.0f;
     }
     // the inputs before the strip, oldest first
     V past[TAPS > 1 ? TAPS - 1 : 1];
 #pragma unroll
     for (int j = 0; j < TAPS - 1; ++j) {
-        const int k = j - (TAPS - 1 - (int)kept);      // of the slot's inputs
 #pragma unroll
         for (int i = 0; i < VEC; ++i) past[j].v[i] = ss_t<T>(0.0f);
-        if (k < 0) continue;
-        if (t0) past[j] = *reinterpret_cast<const V*>(in + (size_t)(t0 - kept + k) * a.input_stride);
-        else if (!s.fresh()) past[j] = *reinterpret_cast<const V*>(state + (size_t)k * a.channels);
+        if (t0) past[j] = *reinterpret_cast<const V*>(in + (size_t)(t0 - kept + j) * a.input_stride);
+        else if (!s.fresh()) past[j] = *reinterpret_cast<const V*>(state + (size_t)j * a.channels);
     }
     float2 u[TAPS][PAIRS];      // u[TAPS - 1]: the row at hand
     auto pairs = [](const V& v, float2 (&to)[PAIRS]) {
@@ -178,10 +175,17 @@ void conv_launch(uzu_command_buffer* cmd, ConvParams& p) {
     p.groups = (p.a.channels + CC_THREADS * VEC - 1) / (CC_THREADS * VEC);
     const dim3 grid(p.table.tiles * p.groups);
     auto go = [&](auto kernel) { launch(cmd, "causal_conv_kernel", kernel, grid, dim3(CC_THREADS), 0, p); };
-    if (p.a.taps <= 2) go(causal_conv_kernel<T, VEC, 2>);
-    else if (p.a.taps == 3) go(causal_conv_kernel<T, VEC, 3>);
-    else if (p.a.taps == 4) go(causal_conv_kernel<T, VEC, 4>);
-    else go(causal_conv_kernel<T, VEC, 8>);
+    // (a kernel for each number of taps: one with more would multiply rows outside the window by zeros, which makes NaN of an infinity)
+    switch (p.a.taps) {
+        case 1: return go(causal_conv_kernel<T, VEC, 1>);
+        case 2: return go(causal_conv_kernel<T, VEC, 2>);
+        case 3: return go(causal_conv_kernel<T, VEC, 3>);
+        case 4: return go(causal_conv_kernel<T, VEC, 4>);
+        case 5: return go(causal_conv_kernel<T, VEC, 5>);
+        case 6: return go(causal_conv_kernel<T, VEC, 6>);
+        case 7: return go(causal_conv_kernel<T, VEC, 7>);
+        default: return go(causal_conv_kernel<T, VEC, 8>);
+    }
 }
 template <typename T>
 void conv_by_alignment(uzu_command_buffer* cmd, ConvParams& p) {
