@@ -103,6 +103,22 @@ __device__ __noinline__ bool xl_all(unsigned int* counter, volatile uint32_t* ga
     }
 }
 
+// A CTA is done; the last one makes the scratch ready for the next call. Where a wait ran out some CTAs had no share of `down`, and tiles in parts still hold the tickets of the others.
+__device__ __forceinline__ void xl_leave(const XlParams& p, uint32_t gave_up) {
+    unsigned int* counters = reinterpret_cast<unsigned int*>(p.a.scratch);
+    if (gave_up) {
+        atomicExch(counters + 3, 1u);
+        __threadfence();
+    }
+    if (atomicAdd(counters + 2, 1u) != gridDim.x - 1) return;      // (behind a fence of the thread's own since its last ticket)
+    if (atomicExch(counters + 3, 0u)) {
+        __threadfence();
+        for (uint32_t i = 0; i < (p.a.width + 31) / 32; ++i) counters[XlScratch::TICKETS / 4 + i] = 0;
+    }
+    counters[0] = counters[1] = counters[2] = 0;
+    __threadfence();
+}
+
 // eight values of a row
 __device__ __forceinline__ void xl_x8(const uzu_expert_layer_args& a, uint32_t t, uint32_t c, bool wide, float (&v)[8]) {
     if (!wide) {
@@ -581,10 +597,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
     }
     __syncthreads();
     if (tid == 0) um_report(&gave_up, p.error);
-    if (tid == 0 && atomicAdd(counters + 2, 1u) == ctas - 1) {      // the last one out: for the next call
-        counters[0] = counters[1] = counters[2] = 0;
-        __threadfence();
-    }
+    if (tid == 0) xl_leave(p, gave_up);
 }
 
 namespace {
