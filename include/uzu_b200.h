@@ -981,7 +981,8 @@ UZU_API uzu_status uzu_state_space_step_validate(const uzu_state_space_step_args
 /* A whole layer of routed experts for 1 .. 64 tokens in one launch: router, choice, the chosen experts' gated units, the shared experts, the weighted sum.
  *   logits = x router^T + router_bias.  score 0: the `top` largest logits, weights = softmax over them; 1: s = softmax over all logits, the `top` largest s,
  *   weights = s; 2: s = sigmoid(logits), the `top` largest s, weights = s.  renormalise: weights / their sum;  weights * weight_scale. The lower index wins
- *   a tie; a logit that is NaN comes last. Where no softmax of a token is a number, it takes the lowest indices, with weights that are NaN.
+ *   a tie; a logit that is NaN comes last (for score 0 it counts as -infinity), with a weight of 0. Where no softmax is a number (no logit above -infinity, or one of +infinity) the weights are NaN, and score 1
+ *   takes the lowest indices.
  *   out[t] = sum_k weights[t, k] E_(ids[t, k])(x_t) + sum over shared experts E(x_t),   E(x) = down (act(gate) * up),  [up | gate] = up_gate x
  * x and out are bf16 or f32 rows, the weights bf16. f32 rows and hidden values enter the products as three bf16 parts (24 bits), of bf16 rows the hidden values as one;
  * products and sums are f32, summed in an order that only the shapes and the choice set. width and ff are multiples of 8, weights 16-byte aligned.

@@ -25,3 +25,22 @@ def test_scratch_after_a_wait_that_ran_out(ctx):
         assert not spoilt.numpy(np.uint8, (16 << 20,))[:16384].any()
         for _ in range(3):
             assert np.array_equal(lay.run(11, 4, P.F32, x=x, scratch=spoilt)[1], clean)
+
+
+@pytest.mark.parametrize("score", [0, 1, 2])
+@pytest.mark.parametrize("experts", [9, 100, 300])
+@pytest.mark.parametrize("low", [-200.0, -np.inf])
+def test_logits_that_are_no_number_come_last(ctx, experts, score, low):
+    """behind scores that come to 0, whatever their indices (for score 0 they count as -infinity); the chosen weights are numbers"""
+    bias = np.full(experts, low, np.float32)
+    bias[[0, 3, experts - 2]] = np.nan
+    bias[[5, experts - 1]] = 1.0, 2.0
+    lay = _Layer(ctx, 64, 32, experts, 0, seed=22)
+    lay.bufs[0], lay.bufs[3] = ctx.upload(np.zeros((experts, 64), np.uint16)), ctx.upload(bias)
+    if score == 0:
+        bias[np.isnan(bias) & (low == -np.inf)] = low
+    order = [experts - 1, 5] + [e for e in range(experts) if bias[e] == low] + ([] if (bias == low).sum() == experts - 2 else [0, 3, experts - 2])
+    top = min(9, experts)
+    _, got, ids, w, _ = lay.run(5, top, P.F32, score=score)
+    assert np.array_equal(ids, np.tile(order[:top], (5, 1))) and np.isfinite(w).all() and np.isfinite(got).all()
+    assert (w[:, 2:] == 0).all() and (w[:, :2] > 0).all()

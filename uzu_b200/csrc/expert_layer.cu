@@ -151,32 +151,33 @@ template <int PER>
 __device__ void xl_choose(const uzu_expert_layer_args& a, const float* logits, uint32_t t, XlLists& l, bool write) {
     const uint32_t lane = threadIdx.x & 31u;
     float v[PER];
+    bool scored = true;      // softmax over all: there is one
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const uint32_t e = lane + 32 * i;
         v[i] = e < a.experts ? __ldcg(logits + (size_t)t * a.experts + e) : -INFINITY;
-        if (v[i] != v[i]) v[i] = -INFINITY;
     }
     if (a.score == UZU_EXPERT_SCORE_SIGMOID) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) v[i] = lane + 32 * i < a.experts ? 1.0f / (1.0f + expf(-v[i])) : -INFINITY;
+        for (int i = 0; i < PER; ++i) v[i] = 1.0f / (1.0f + expf(-v[i]));
     } else if (a.score == UZU_EXPERT_SCORE_ALL) {
-        float most = v[0], sum = 0.0f;
+        float most = -INFINITY, sum = 0.0f;
 #pragma unroll
-        for (int i = 1; i < PER; ++i) most = fmaxf(most, v[i]);
+        for (int i = 0; i < PER; ++i) most = fmaxf(most, v[i]);      // (passes over what is no number)
         most = warp_max(most);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            v[i] = lane + 32 * i < a.experts ? expf(v[i] - most) : -INFINITY;
-            if (lane + 32 * i < a.experts) sum += v[i];
+            v[i] = expf(v[i] - most);      // (an infinite largest one: no number, as all others come to 0)
+            if (v[i] == v[i]) sum += v[i];
         }
         sum = warp_sum(sum);
+        scored = sum > 0.0f;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            v[i] /= sum;
-            if (v[i] != v[i]) v[i] = -INFINITY;      // (an infinite logit, or none that is a number: the lanes have to agree on an order)
-        }
+        for (int i = 0; i < PER; ++i) v[i] = scored ? v[i] / sum : -INFINITY;      // (the lanes have to agree on an order)
     }
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (v[i] != v[i]) v[i] = -INFINITY;      // behind scores that come to 0 too
     uint32_t taken = 0;
     float mine = 0.0f, first = 0.0f;      // lane k: the score of choice k
     uint32_t mine_id = 0;
@@ -198,7 +199,7 @@ __device__ void xl_choose(const uzu_expert_layer_args& a, const float* logits, u
         if (k == 0) first = best;
         if (lane == k) { mine = best; mine_id = at; }
     }
-    if (a.score == UZU_EXPERT_SCORE_ALL && mine == -INFINITY) mine = __int_as_float(0x7fc00000);
+    if (a.score != UZU_EXPERT_SCORE_CHOSEN && mine == -INFINITY) mine = scored ? 0.0f : __int_as_float(0x7fc00000);
     float w = lane < a.top ? mine : 0.0f;
     if (a.score == UZU_EXPERT_SCORE_CHOSEN) {
         w = lane < a.top ? expf(mine - first) : 0.0f;
