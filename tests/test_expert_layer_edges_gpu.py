@@ -44,3 +44,33 @@ def test_logits_that_are_no_number_come_last(ctx, experts, score, low):
     _, got, ids, w, _ = lay.run(5, top, P.F32, score=score)
     assert np.array_equal(ids, np.tile(order[:top], (5, 1))) and np.isfinite(w).all() and np.isfinite(got).all()
     assert (w[:, 2:] == 0).all() and (w[:, :2] > 0).all()
+
+
+def _bf16(v):
+    return P.to_kept(np.asarray(v), P.BF16)
+
+
+def test_f32_values_above_the_largest_of_bf16(ctx):
+    """rows and hidden values that are finite in f32 but not as one bf16 part"""
+    most = float(np.finfo(np.float32).max)
+    lay = _Layer(ctx, 64, 32, 6, 1, seed=23)
+    lay.host[0][:, 0] = 0
+    lay.host[1][:, :, 0] = _bf16(2.0 ** -126)
+    lay.bufs[0], lay.bufs[1] = ctx.upload(lay.host[0]), ctx.upload(lay.host[1])
+    x = lay.rng.standard_normal((9, 64))
+    x[:, 0] = [most, -most, 3.399e38, -3.3963e38, 3.3895e38, 1.0, 0.0, 3.0e38, most]
+    lay.check(9, 2, P.F32, x=x)
+
+
+def test_f32_hidden_values_above_the_largest_of_bf16(ctx):
+    lay = _Layer(ctx, 64, 32, 3, 0, seed=24)
+    lay.host[0][:] = 0
+    lay.host[1][:] = 0
+    lay.host[1][:, :, 0], lay.host[1][:, :, 1] = _bf16(2.0 ** 64 * (1 - 2.0 ** -8)), _bf16(2.0 ** 64 * 2.0 ** -8 * 0.75)
+    lay.host[2][:] = _bf16(2.0 ** -126 * np.sign(P.of_kept(lay.host[2], P.BF16)))
+    lay.bufs[:3] = [ctx.upload(v) for v in lay.host]
+    x = np.zeros((4, 64))
+    x[:, 0] = x[:, 1] = [1.0, 0.5, 0.999, 1.0]
+    hidden = (2.0 ** 64 * (1 - 2.0 ** -10)) ** 2
+    assert 2.0 ** 128 * (1 - 2.0 ** -9) < hidden < float(np.finfo(np.float32).max)      # (the least that rounds to an infinite bf16)
+    lay.check(4, 1, P.F32, act=B.ACT_IDENTITY, x=x)

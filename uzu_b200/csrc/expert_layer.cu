@@ -70,12 +70,13 @@ __device__ __forceinline__ void xl_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
 __device__ __forceinline__ void xl_tma3(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint32_t z, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
-// a value as PLANES bf16 parts, each what the ones before leave (of what is no number or infinite: the first alone, the product shows it by that)
+// A value as PLANES bf16 parts, each what the ones before leave (of what is no number or infinite: the first alone, the product shows it by that). Several parts are cut off, not
+// rounded: three keep the 24 bits all the same, and a value above the largest bf16 number is not infinite.
 template <int PLANES>
 __device__ __forceinline__ void xl_planes(float v, __nv_bfloat16* to, size_t plane) {
 #pragma unroll
     for (int pl = 0; pl < PLANES; ++pl) {
-        const __nv_bfloat16 part = __float2bfloat16_rn(v);
+        const __nv_bfloat16 part = PLANES > 1 ? __float2bfloat16_rz(v) : __float2bfloat16_rn(v);
         to[pl * plane] = part;
         v = fabsf(v) < INFINITY ? v - __bfloat162float(part) : 0.0f;
     }
