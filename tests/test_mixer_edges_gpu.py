@@ -85,3 +85,103 @@ def test_conv_infinite_inputs_reach_their_window_only(ctx, dt, taps, act):
     beside = ~hit & hit.reshape(rows, channels // 2, 2)[:, :, ::-1].reshape(rows, channels)      # the gate takes one reciprocal for two channels: 2^-21 of the value each time, and its rounding
     assert np.array_equal(got[~hit & ~beside], clean[~hit & ~beside])
     assert (np.abs(got - clean)[beside] <= (2.0 ** -20 + 2 * P.HALF_STEP[dt]) * np.abs(clean[beside])).all()
+
+
+def _run_scan(ctx, v, heads, groups, dim, n, seqs, slots, dt=P.BF16, state=None, scratch=True):
+    """v: x, z, b, c, dt rows, a, d, dt_bias. (out, state) in float64"""
+    rows = v["x"].shape[0]
+    X, Z, Bm, Cm, D = (_Rows(ctx, v[k], dt) for k in ("x", "z", "b", "c", "dt"))
+    out = _Rows(ctx, np.zeros((rows, heads * dim)), dt)
+    st = np.zeros((slots, heads, dim, n), np.float32) if state is None else state
+    f32 = [ctx.upload(np.asarray(w, np.float32)) for w in (v["a"], v["d"], v["dt_bias"], st)]
+    t = _table(seqs)
+    a = B.StateSpaceScanArgs(x=X.ptr, dt=D.ptr, b=Bm.ptr, c=Cm.ptr, z=Z.ptr, a=f32[0].ptr, d=f32[1].ptr, dt_bias=f32[2].ptr, state=f32[3].ptr, out=out.ptr, sequences=C.addressof(t),
+                             sequence_count=len(seqs), rows=rows, slots=slots, heads=heads, groups=groups, head_dim=dim, state_size=n, x_stride=X.stride, dt_stride=D.stride, b_stride=Bm.stride,
+                             c_stride=Cm.stride, z_stride=Z.stride, out_stride=out.stride, dt_min=0.0, dt_max=float("inf"), dt_softplus=1, data_type=dt)
+    if scratch:
+        a.scratch_bytes = ctx.lib.uzu_state_space_scan_scratch_bytes(ctx.h, C.byref(a))
+        sc = ctx.buffer(max(16, a.scratch_bytes), B.BUFFER_DEVICE)
+        a.scratch = sc.ptr
+    with ctx.command_buffer("scan") as cmd:
+        cmd.encode("uzu_state_space_scan_encode", C.byref(a))
+    return out.get()[0], f32[3].numpy(np.float32, st.shape).astype(np.float64), a.scratch_bytes
+
+
+def _scan_rows(rng, rows, heads, groups, dim, n):
+    v = {k: rng.standard_normal((rows, w)) for k, w in (("x", heads * dim), ("z", heads * dim), ("b", groups * n), ("c", groups * n), ("dt", heads))}
+    v["a"], v["d"], v["dt_bias"] = -(1 + 15 * rng.random(heads)), rng.standard_normal(heads), np.zeros(heads)
+    return v
+
+
+@pytest.mark.parametrize("dim,n", [(64, 128), (128, 64)])
+@pytest.mark.parametrize("loud", [32, 64, 96])
+def test_quiet_tokens_behind_loud_ones(ctx, dim, n, loud):
+    """Tokens of large steps and no input wipe the state out and add nothing: what follows in their chunk is as without them, to the bit (blocks of 32 tokens have sums of their own; a
+    difference of sums over the loud tokens too would lose the quiet ones' digits)."""
+    heads, groups = 32, 2
+    v = _scan_rows(np.random.default_rng(loud), 128, heads, groups, dim, n)
+    v["dt"] -= 4.0                       # steps of about 0.02
+    v["dt"][:loud], v["x"][:loud] = 40.0, 0.0
+    behind = {k: w[loud:] if w.shape[0] == 128 else w for k, w in v.items()}
+    out, state, _ = _run_scan(ctx, v, heads, groups, dim, n, [(0, 128, 0, 1)], 1)
+    ref, after, _ = _run_scan(ctx, behind, heads, groups, dim, n, [(0, 128 - loud, 0, 1)], 1)
+    assert np.isfinite(out).all() and not out[:loud].any() and ref.any()
+    assert np.array_equal(out[loud:], ref) and np.array_equal(state, after)
+
+
+@pytest.mark.parametrize("dim,n", [(64, 128), (128, 64)])
+def test_loud_and_quiet_tokens(ctx, dim, n):
+    """steps of 1e-3 and of 40 side by side, against the recurrence in 64 bits, whose errors are carried along token by token"""
+    heads, groups, rows = 4, 2, 300
+    rng = np.random.default_rng(dim)
+    v = _scan_rows(rng, rows, heads, groups, dim, n)
+    v["dt"] = np.where(rng.random((rows, heads)) < 0.3, 40.0, rng.standard_normal((rows, heads)) - 5)
+    v["dt"][40:90] -= 45.0 * (v["dt"][40:90] > 20)       # a quiet stretch
+    st = rng.standard_normal((1, heads, dim, n)).astype(np.float32)
+    out, state, _ = _run_scan(ctx, v, heads, groups, dim, n, [(0, rows, 0, 0)], 1, state=st)
+    k = lambda w, *s: P.of_kept(P.to_kept(w, P.BF16), P.BF16).reshape(rows, *s)
+    x, z, b, c = k(v["x"], heads, dim), k(v["z"], heads, dim), k(v["b"], groups, n), k(v["c"], groups, n)
+    a, d = v["a"].astype(np.float32).astype(np.float64), v["d"].astype(np.float32).astype(np.float64)
+    step = P.steps(k(v["dt"], heads), 0.0)
+    ref, rstate, mag, smag = P.scan(x, step, b, c, z, a, d, st.astype(np.float64), [(0, rows, 0, 0)])
+    # Of a decay over several tokens: each token's own part |step a| of it with three roundings, and a block's sum (at most 32 of 150) with six where it is a difference of two.
+    # e, m: errors and magnitudes of the state in the recurrence over absolute values
+    bb = np.repeat(np.abs(b), heads // groups, 1)
+    m = np.abs(st[0]).astype(np.float64)
+    e = np.zeros_like(m)
+    bound = np.zeros_like(ref)
+    cc = np.repeat(np.abs(c), heads // groups, 1)
+    for t in range(rows):
+        l = np.minimum(np.abs(step[t] * a), 104.0)
+        f = np.exp(-np.abs(step[t] * a))[:, None, None]
+        add = (step[t][:, None] * np.abs(x[t]))[:, :, None] * bb[t][:, None, :]
+        e = f * (e + 2.0 ** -24 * (4 + 8 * l)[:, None, None] * m) + 2.0 ** -24 * 6 * add
+        m = f * m + add
+        bound[t] = (e * cc[t][:, None, :]).sum(-1)
+    # the state's sum: inputs as two bf16 parts
+    assert (np.abs(state[0] - rstate[0]) <= e + 2.0 ** -16 * m + 2.0 ** -24 * np.abs(rstate[0]) + 2.0 ** -140).all()
+    gate = np.abs(P.silu(z))
+    bound = bound + (2.0 ** -8 + np.log(2) * 6 * 2.0 ** -24 * 32 * 150 + 2.0 ** -24 * (n + 8)) * mag
+    bound = bound * gate + (2.0 ** -21 + 2.0 ** -22 * np.abs(z)) * np.abs(ref)
+    got = out.reshape(rows, heads, dim)
+    assert np.isfinite(got).all()
+    assert (np.abs(got - ref) <= P.HALF_STEP[P.BF16] * (np.abs(ref) + bound) + P.TINY[P.BF16] + bound).all()
+
+
+@pytest.mark.parametrize("dt,dim,n", [(P.BF16, 64, 128), (P.BF16, 128, 64), (P.F32, 20, 12)])
+def test_a_step_that_is_no_number(ctx, dt, dim, n):
+    """makes its head's outputs from its token on and its head's state no number; nothing before it, no other head"""
+    heads, groups, rows = 4, 2, 300
+    v = _scan_rows(np.random.default_rng(7), rows, heads, groups, dim, n)
+    v["dt"] -= 3.0
+    clean, cstate, _ = _run_scan(ctx, v, heads, groups, dim, n, [(0, rows, 0, 1)], 1, dt=dt)
+    for row in (0, 45, 127, 128, 201, 299):
+        w = dict(v, dt=v["dt"].copy())
+        w["dt"][row, 1] = np.nan
+        out, state, _ = _run_scan(ctx, w, heads, groups, dim, n, [(0, rows, 0, 1)], 1, dt=dt)
+        hit = np.zeros((rows, heads, dim), bool)
+        hit[row:, 1] = True
+        out, ref = out.reshape(hit.shape), clean.reshape(hit.shape)
+        assert np.isnan(out[hit]).all() and np.array_equal(out[~hit], ref[~hit])
+        others = [0, 2, 3]
+        assert np.isnan(state[0, 1]).all() and np.array_equal(state[0, others], cstate[0, others])

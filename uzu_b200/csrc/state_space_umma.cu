@@ -2,9 +2,10 @@
 //   y_i = sum_(j <= i) 2^(L_i - L_j) step_j (c_i . b_j) x_j  +  2^(L_i) S c_i  +  d x_i,      S' = 2^(L_end) S + sum_j 2^(L_end - L_j) step_j x_j b_j^T
 // A CTA walks one sequence (or a part of it) for 64 rows of one head:
 //   copy     x, b and c of a chunk by TMA, two stages
-//   steps    one warp: step sizes, sums of logarithms from the front and from the end (each accurate where its weights are not small)
+//   steps    one warp: step sizes, sums of logarithms of each block of 32 tokens from its front and from its end (accurate where their weights are not small)
 //   scores   c b^T out of tensor memory, times 2^(L_i - L_j) step_j, back as bf16 operand A. Below the diagonal's 32 x 32 blocks the factor is a product of a row's and
-//            a column's, both relative to the row block's start, so that neither overflows (decays are at most 1) and no exponential is taken per element.
+//            a column's, both relative to the row block's start, so that neither overflows (decays are at most 1) and no exponential is taken per element. In the
+//            diagonal's blocks the exponent is a difference of sums of at most 32 tokens of at most 150 each: off by 2^-11 at most, where a score's rounding is 2^-8.
 //   state    x times its weight as two bf16 parts (16 bits: the state keeps what f32 sums need) for the state's sum, the state in registers, f32, its bf16 copy as operand
 //   output   the two sums, d x and the gate
 //   issue    scores c b^T (128 x 128), their product with x (64), c S (64), b^T [x hi | x lo] (128 columns, both parts at one reading of b)
@@ -55,7 +56,8 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
     __shared__ __align__(8) uint64_t bars[43];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t gave_up;
-    __shared__ __align__(16) float steps[4][SU_Q], front[4][SU_Q], back[4][SU_Q];      // [chunk & 3][token]: step, log2 of the decays up to it, behind it
+    __shared__ __align__(16) float steps[4][SU_Q], front[4][SU_Q], back[4][SU_Q];      // [chunk & 3][token]: step, log2 of the decays of its block of 32 up to it, behind it
+    __shared__ __align__(16) float4 blocks[4][4];                                      // [chunk & 3][block]: log2 of all decays of the block, of those before it, behind it, of the chunk
     __shared__ __align__(16) float column[4][96];                                      // of a row block of scores: step_j 2^(L_ref - L_j)
     __shared__ volatile uint32_t odd_rows[4][8];                                       // [chunk & 3][half, row block]: rows with an x that is not finite
     const uzu_state_space_scan_args& a = p.a;
@@ -126,13 +128,18 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                 um_wait_st();
             }
             for (uint32_t c = 0; c < chunks; ++c) {
-                const float *st = steps[c & 3u], *fr = front[c & 3u];
+                const float *st = steps[c & 3u], *fr = front[c & 3u], *bk = back[c & 3u];
                 ok = um_wait(d_full(c), four(c), &gave_up, 0x701u);
                 if (!ok) break;
-                const float mine = um_ldf(&fr[t]), ref = w ? um_ldf(&fr[32 * w - 1]) : 0.0f;
-                for (uint32_t jb = jb0; jb < jb1; ++jb) column[w][jb * 32 + lane] = um_ldf(&st[jb * 32 + lane]) * ss_exp2(ref - um_ldf(&fr[jb * 32 + lane]));
+                const float mine = um_ldf(&fr[t]);
+                float between = 0.0f;      // the blocks between a column's and the row's
+#pragma unroll 1
+                for (uint32_t jb = w; jb-- > jb0;) {
+                    if (jb < jb1) column[w][jb * 32 + lane] = um_ldf(&st[jb * 32 + lane]) * ss_exp2(um_ldf(&bk[jb * 32 + lane]) + between);
+                    between += um_ldf(&blocks[c & 3u][jb].x);
+                }
                 __syncwarp();
-                const float r = ss_exp2(mine - ref);
+                const float r = ss_exp2(mine);
                 const float2 r2 = make_float2(r, r);
                 ok = um_wait(g_full, c & 1u, &gave_up, 0x702u);
                 if (ok && c) ok = um_wait(y_full, (c - 1) & 1u, &gave_up, 0x703u);      // the scores before are read
@@ -234,8 +241,8 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
             if (ok && valid < SU_Q) ok = um_wait(b_full(c), two(c), &gave_up, 0x717u);      // (b's rows are there)
             if (!ok) return;
             // (the products that read the parts of chunk c - 1 are done: u_full was waited for)
-            const float weight = um_ldf(&steps[c & 3u][t]) * ss_exp2(um_ldf(&back[c & 3u][t]));
-            end = um_ldf(&front[c & 3u][SU_Q - 1]);
+            const float weight = um_ldf(&steps[c & 3u][t]) * ss_exp2(um_ldf(&back[c & 3u][t]) + um_ldf(&blocks[c & 3u][w].z));
+            end = um_ldf(&blocks[c & 3u][w].w);
             const float2 w2 = make_float2(weight, weight);
             total += end;
             bool odd = false;
@@ -343,7 +350,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                 if (ok) ok = um_wait(y_full, c & 1u, &gave_up, 0x70bu);
                 if (!ok) break;
                 um_fence_after();
-                const float f = ss_exp2(um_ldf(&front[c & 3u][t]));
+                const float f = ss_exp2(um_ldf(&front[c & 3u][t]) + um_ldf(&blocks[c & 3u][w].y));
                 const float2 f2 = make_float2(f, f);
                 float2 ys[16];
                 uint32_t seen = 0;
@@ -555,25 +562,34 @@ __global__ void __launch_bounds__(SU_THREADS, 1) scan_umma_kernel(const __grid_c
                     const bool there = c * SU_Q + 4 * lane + i < rows;
                     step[i] = there ? ss_step(__bfloat162float(next[i]), bias, a.dt_softplus, a.dt_min, a.dt_max) : 0.0f;
                     l[i] = there ? step[i] * rate : 0.0f;
-                    l[i] = l[i] < -256.0f ? -256.0f : l[i];      // (nothing is left of a state then; sums stay fine)
+                    l[i] = l[i] < -150.0f ? -150.0f : l[i];      // (nothing is left of a state then; sums stay fine)
                 }
                 if (c + 1 < chunks) fetch(c + 1);
                 const float f0 = l[0], f1 = f0 + l[1], f2 = f1 + l[2], f3 = f2 + l[3], b2 = l[3], b1 = b2 + l[2], b0 = b1 + l[1];
+                // Sums of blocks of 32 tokens: a difference of sums from the chunk's start on would lose the digits of quiet tokens behind loud ones.
+                const int of = lane & 7u;
                 float up = f3, down = b0 + l[0];
     #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const float u = __shfl_up_sync(0xffffffffu, up, o), d = __shfl_down_sync(0xffffffffu, down, o);
-                    if (lane >= o) up += u;
-                    if (lane + o < 32) down += d;
+                for (int o = 1; o < 8; o <<= 1) {
+                    const float u = __shfl_up_sync(0xffffffffu, up, o, 8), d = __shfl_down_sync(0xffffffffu, down, o, 8);
+                    if (of >= o) up += u;
+                    if (of + o < 8) down += d;
                 }
-                float before = __shfl_up_sync(0xffffffffu, up, 1), behind = __shfl_down_sync(0xffffffffu, down, 1);
-                if (lane == 0) before = 0.0f;
-                if (lane == 31) behind = 0.0f;
+                float before = __shfl_up_sync(0xffffffffu, up, 1, 8), behind = __shfl_down_sync(0xffffffffu, down, 1, 8);
+                if (of == 0) before = 0.0f;
+                if (of == 7) behind = 0.0f;
+                float sum[4];
+    #pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] = __shfl_sync(0xffffffffu, up, 8 * i + 7);
+                const uint32_t block = lane >> 3;
+                const float front_of = (block > 0 ? sum[0] : 0.0f) + (block > 1 ? sum[1] : 0.0f) + (block > 2 ? sum[2] : 0.0f);
+                const float back_of = (block < 1 ? sum[1] : 0.0f) + (block < 2 ? sum[2] : 0.0f) + (block < 3 ? sum[3] : 0.0f);
                 ok = um_wait(d_empty(c), four(c) ^ 1u, &gave_up, 0x716u);
                 if (!ok) break;
                 *reinterpret_cast<float4*>(&steps[c & 3u][4 * lane]) = make_float4(step[0], step[1], step[2], step[3]);
                 *reinterpret_cast<float4*>(&front[c & 3u][4 * lane]) = make_float4(before + f0, before + f1, before + f2, before + f3);
                 *reinterpret_cast<float4*>(&back[c & 3u][4 * lane]) = make_float4(behind + b0, behind + b1, behind + b2, behind);
+                if (of == 7) blocks[c & 3u][block] = make_float4(up, front_of, back_of, sum[0] + sum[1] + sum[2] + sum[3]);
                 um_arrive(d_full(c));
             }
         }
