@@ -20,7 +20,7 @@ def test_scratch_after_a_wait_that_ran_out(ctx):
     for _ in range(2):
         held[:4] = np.array([2 ** 32 - 74], np.uint32).view(np.uint8)
         spoilt = ctx.upload(held)
-        with pytest.raises(B.UzuError):
+        with pytest.raises(B.UzuError, match="code 0x80[1-4]"):
             lay.run(11, 4, P.F32, x=x, scratch=spoilt)
         assert not spoilt.numpy(np.uint8, (16 << 20,))[:16384].any()
         for _ in range(3):

@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
         }
     }
     __syncthreads();
-    if (tid == 0) xl_all(counters, &gave_up, 0x601u);
+    if (tid == 0) xl_all(counters, &gave_up, 0x801u);
     __syncthreads();
     bool ok = !gave_up;
 
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
         // ---- weights by TMA ----
         auto stage = [&](bool up, uint32_t col, uint32_t width, uint32_t row, uint32_t which) {
             const uint32_t s = it % S::STAGES;
-            if (ok) ok = um_wait(empty(s), (it / S::STAGES & 1u) ^ 1u, &gave_up, 0x602u);
+            if (ok) ok = um_wait(empty(s), (it / S::STAGES & 1u) ^ 1u, &gave_up, 0x802u);
             if (!ok) return;
             if (um_elect()) {
                 const uint32_t boxes = min(XL_WARPS, (width - col + 63) / 64);
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
         auto multiply = [&](uint32_t col, uint32_t width, size_t plane, uint32_t count, auto src, auto next) {
             const uint32_t s = it % S::STAGES;
             const bool there = col + warp * 64 < width;
-            if (ok) ok = um_wait(full(s), it / S::STAGES & 1u, &gave_up, 0x603u);
+            if (ok) ok = um_wait(full(s), it / S::STAGES & 1u, &gave_up, 0x803u);
             if (!ok) return;
             uint32_t seen = 0;
             uint4 b[PLANES][2];
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
             at = next_at;
             tile = next_tile;
         }
-        if (tid == 0) xl_all(counters + 1, &gave_up, 0x604u);
+        if (tid == 0) xl_all(counters + 1, &gave_up, 0x804u);
         meet();
         ok = ok && !gave_up;
 

@@ -86,10 +86,6 @@ __device__ __forceinline__ void um_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void um_tma(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
-// asked into L2
-__device__ __forceinline__ void um_tma_prefetch(const CUtensorMap* map, uint32_t x, uint32_t y) {
-    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
-}
 // rows of shared memory to global memory; the group of them is read when um_store_read returns
 __device__ __forceinline__ void um_tma_store(const CUtensorMap* map, uint32_t src, uint32_t x, uint32_t y) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n\tcp.async.bulk.commit_group;" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");

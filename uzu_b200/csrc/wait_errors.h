@@ -1,6 +1,8 @@
 // Barrier waits that ran out inside a kernel. Such a kernel stores a code to its context's word in mapped host memory, skips what it can no longer compute
 // and returns; whoever next waits for the context's work on the host finds the code here and reports an error instead of results. Plain C++: a test on
 // the host uses the same class.
+// A code says which kernel it was: 1 .. 3 dense_umma.cu, 0x1xx qmm_scaled.cu, 0x4xx decode_linear.cu, 0x5xx attention_umma.cu, 0x6xx qmm_wide.cu, 0x7xx state_space_umma.cu,
+// 0x8xx expert_layer.cu.
 #pragma once
 #include <atomic>
 #include <cstdint>
