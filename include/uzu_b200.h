@@ -984,7 +984,7 @@ UZU_API uzu_status uzu_state_space_step_validate(const uzu_state_space_step_args
  *   a tie; a logit that is NaN comes last (for score 0 it counts as -infinity), with a weight of 0. Where no softmax is a number (no logit above -infinity, or one of +infinity) the weights are NaN, and score 1
  *   takes the lowest indices.
  *   out[t] = sum_k weights[t, k] E_(ids[t, k])(x_t) + sum over shared experts E(x_t),   E(x) = down (act(gate) * up),  [up | gate] = up_gate x
- * x and out are bf16 or f32 rows, the weights bf16. f32 rows and hidden values enter the products as three bf16 parts (24 bits), of bf16 rows the hidden values as one;
+ * x and out are bf16 or f32 rows, the weights bf16. f32 rows and hidden values enter the products as three bf16 parts (24 bits), of bf16 rows the hidden values as two;
  * products and sums are f32, summed in an order that only the shapes and the choice set. width and ff are multiples of 8, weights 16-byte aligned.
  * scratch: of uzu_expert_layer_scratch_bytes() bytes, 256-byte aligned, its first 16 KB zero before the first use; every call leaves it ready for the next,
  * of any sizes. Calls that may run at the same time do not share it. */

@@ -74,3 +74,24 @@ def test_f32_hidden_values_above_the_largest_of_bf16(ctx):
     hidden = (2.0 ** 64 * (1 - 2.0 ** -10)) ** 2
     assert 2.0 ** 128 * (1 - 2.0 ** -9) < hidden < float(np.finfo(np.float32).max)      # (the least that rounds to an infinite bf16)
     lay.check(4, 1, P.F32, act=B.ACT_IDENTITY, x=x)
+
+
+@pytest.mark.parametrize("rows", [1, 7, 16, 30, 64])
+def test_bf16_rows_keep_products_of_16_bits(ctx, rows):
+    """hidden values that are products of two 8-bit numbers reach `down` whole: differences of them, exact in 32 bits, are the results to the bit"""
+    width, ff = 64, 32
+    lay = _Layer(ctx, width, ff, 8, 0, seed=25)
+    lay.host[0][:] = 0
+    lay.host[1][:] = _bf16(1 + lay.rng.integers(0, 128, lay.host[1].shape) / 128)
+    down = np.zeros((8, width, ff))
+    d = np.arange(width)
+    down[:, d, d % ff], down[:, d, (d + 1 + d // ff) % ff] = 1.0, -1.0
+    lay.host[2][:] = _bf16(down)
+    lay.bufs[:3] = [ctx.upload(v) for v in lay.host]
+    x = np.eye(64)[:rows]
+    _, got, ids, w, _ = lay.run(rows, 1, P.BF16, act=B.ACT_IDENTITY, x=x)
+    assert (w == 1).all()
+    y = np.stack([P.of_kept(lay.host[1][ids[r, 0]], P.BF16)[:, r] for r in range(rows)])
+    hidden = y[:, :ff] * y[:, ff:]
+    ref = hidden[:, d % ff] - hidden[:, (d + 1 + d // ff) % ff]
+    assert np.array_equal(got, P.to_kept(ref, P.BF16))

@@ -7,8 +7,8 @@
 //   1  logits: an (expert, four tokens) pair a warp, or a CTA where there are fewer pairs than CTAs; rows are copied as bf16 planes (f32 rows: three, 24 bits, and a stage's products summed by themselves: the results are 2.8e-7 off, in one
 //      running sum of matrix instructions 1.8e-6, with two planes 4.5e-6; a plain product in f32 1.3e-6).
 //   2  every CTA makes the choice for itself from the logits (waiting for one to do it would cost more), lists the chosen experts and their tokens.
-//   3  up: a unit is 16 rows of an expert's up and the 16 of its gate; hidden values, times the routing weight, go to scratch as bf16 planes (of bf16 rows one: the rounding
-//      that a bf16 model's layers have there anyway; the results are 0.0024 off, 0.0017 of it their own rounding).
+//   3  up: a unit is 16 rows of an expert's up and the 16 of its gate; hidden values, times the routing weight, go to scratch as bf16 planes (of bf16 rows two, 16 bits: with one the
+//      results were 0.0024 off where their own rounding is 0.0017, and took 2 percent less time).
 //   4  down: all stages of all 32-row tiles over all chosen experts, cut evenly over the CTAs; a tile that several have is summed by the last of them, in their order.
 // In both products an expert's tokens stand side by side, eight a tile; the rows of the next stage are asked for a stage ahead.
 // Two waits for all CTAs, behind phases 1 and 3. They and the ring's barriers are bounded (wait_errors.h).
@@ -27,6 +27,9 @@ namespace {
 constexpr uint32_t XL_WARPS = 8, XL_THREADS = 32 * XL_WARPS + 32, XL_STAGE = 32 * 1024, XL_COLS = 512, XL_BOX = 4096;
 constexpr uint32_t XL_MAX_TOKENS = 64, XL_MAX_EXPERTS = 528, XL_MAX_LISTED = 656 /* every expert, and 128 of at most 2048 pairs with 16 more */, XL_MAX_TOP = 16, XL_MAX_PAIRS = 64 * 32, XL_CTAS = 148, XL_MAX_WIDTH = 65536;
 
+// bf16 planes of hidden values, where rows have `planes`
+constexpr uint32_t xl_hidden_planes(uint32_t planes) { return planes == 1 ? 2 : planes; }
+
 // where what lies in the scratch; the counters and tickets are zero between calls
 struct XlScratch {
     uint64_t logits, rows, hidden, partials, total;
@@ -39,7 +42,7 @@ inline XlScratch xl_scratch(const uzu_expert_layer_args& a) {
     s.logits = up(XlScratch::FIXED);
     s.rows = up(s.logits + (uint64_t)a.rows * a.experts * 4);
     s.hidden = up(s.rows + planes * a.rows * a.width * 2);
-    s.partials = up(s.hidden + planes * a.rows * (a.top + a.shared) * a.ff * 2);
+    s.partials = up(s.hidden + xl_hidden_planes(planes) * a.rows * (a.top + a.shared) * a.ff * 2);
     s.total = up(s.partials + (uint64_t)XL_CTAS * 2 * 32 * a.rows * 4);
     return s;
 }
@@ -118,6 +121,18 @@ __device__ __forceinline__ void xl_leave(const XlParams& p, uint32_t gave_up) {
     }
     counters[0] = counters[1] = counters[2] = 0;
     __threadfence();
+}
+
+// Operand B: eight tokens' columns from `col` on, 16 of a thread, P bf16 planes `plane` elements behind one another (no row: zeros)
+template <int P, int N>
+__device__ __forceinline__ void xl_ask(const __nv_bfloat16* at, uint32_t col, uint32_t width, size_t plane, uint4 (&to)[N][2]) {
+#pragma unroll
+    for (int pl = 0; pl < P; ++pl)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t c = col + (2 * (threadIdx.x & 3u) + i) * 8;
+            to[pl][i] = at && c < width ? __ldcg(reinterpret_cast<const uint4*>(at + pl * plane + c)) : make_uint4(0, 0, 0, 0);
+        }
 }
 
 // eight values of a row
@@ -223,6 +238,7 @@ template <int NT, int ROWS, int PLANES>
 __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __grid_constant__ CUtensorMap map_up, const __grid_constant__ CUtensorMap map_down, const __grid_constant__ XlParams p) {
     using S = XlShape<NT, ROWS, PLANES>;
     constexpr uint32_t TOK = S::TOK;
+    constexpr int HIDDEN = xl_hidden_planes(PLANES);
     extern __shared__ uint8_t xl_raw[];
     __shared__ __align__(8) uint64_t bars[2 * S::STAGES];
     __shared__ volatile uint32_t gave_up;
@@ -395,16 +411,6 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
 #pragma unroll
                     for (int j = 0; j < 4; ++j) acc[m][n][j] = 0.0f;
         };
-        // Operand B: eight tokens' columns of this warp, PLANES bf16 planes `plane` elements behind one another (no row: zeros)
-        auto ask = [&](const __nv_bfloat16* at, uint32_t col, uint32_t width, size_t plane, uint4 (&to)[PLANES][2]) {
-#pragma unroll
-            for (int pl = 0; pl < PLANES; ++pl)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t c = col + warp * 64 + (2 * t4 + i) * 8;
-                    to[pl][i] = at && c < width ? __ldcg(reinterpret_cast<const uint4*>(at + pl * plane + c)) : make_uint4(0, 0, 0, 0);
-                }
-        };
         // 16 rows times 32 columns of eight tokens
         auto pair = [&](float (&c)[4], const uint4& lo, const uint4& hi, const uint4& b) {
             xl_mma(c, lo.x, hi.x, lo.y, hi.y, b.x, b.y);
@@ -412,16 +418,17 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
         };
         // A stage, for `count` tokens whose rows `src(k)` gives, eight at a time. The first eight of it were asked for a stage ago, into `first`; those of the next stage are asked for
         // (`next`) before this one's products, since they come from L2 no faster than a stage.
-        uint4 first[PLANES][2];
-        auto multiply = [&](uint32_t col, uint32_t width, size_t plane, uint32_t count, auto src, auto next) {
+        uint4 first[HIDDEN][2];
+        auto multiply = [&](auto planes, uint32_t col, uint32_t width, size_t plane, uint32_t count, auto src, auto next) {
             const uint32_t s = it % S::STAGES;
             const bool there = col + warp * 64 < width;
             if (ok) ok = um_wait(full(s), it / S::STAGES & 1u, &gave_up, 0x803u);
             if (!ok) return;
             uint32_t seen = 0;
-            uint4 b[PLANES][2];
+            constexpr int P = decltype(planes)::value;
+            uint4 b[HIDDEN][2];
 #pragma unroll
-            for (int pl = 0; pl < PLANES; ++pl) { b[pl][0] = first[pl][0]; b[pl][1] = first[pl][1]; }
+            for (int pl = 0; pl < P; ++pl) { b[pl][0] = first[pl][0]; b[pl][1] = first[pl][1]; }
             next();
             if (there) {
                 const uint32_t box = ring + s * XL_STAGE + warp * XL_BOX + g * 128;
@@ -436,22 +443,24 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     if (n * 8 >= count) break;
-                    uint4 v[PLANES][2];
+                    uint4 v[HIDDEN][2];
 #pragma unroll
-                    for (int pl = 0; pl < PLANES; ++pl) { v[pl][0] = b[pl][0]; v[pl][1] = b[pl][1]; }
-                    if (n + 1 < NT && (n + 1) * 8 < count) ask((n + 1) * 8 + g < count ? src((n + 1) * 8 + g) : nullptr, col, width, plane, b);
+                    for (int pl = 0; pl < P; ++pl) { v[pl][0] = b[pl][0]; v[pl][1] = b[pl][1]; }
+                    if (n + 1 < NT && (n + 1) * 8 < count) xl_ask<P>((n + 1) * 8 + g < count ? src((n + 1) * 8 + g) : nullptr, col + warp * 64, width, plane, b);
                     if (PLANES == 1) {
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
+                        for (int pl = P - 1; pl >= 0; --pl)
 #pragma unroll
-                            for (int m = 0; m < 2; ++m) pair(acc[m][n], w[i][2 * m], w[i][2 * m + 1], v[0][i]);
+                            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                for (int m = 0; m < 2; ++m) pair(acc[m][n], w[i][2 * m], w[i][2 * m + 1], v[pl][i]);
                     } else {
                         // A matrix instruction cuts its sum off where an addition rounds it: a stage's products, smallest planes first, have sums of their own
 #pragma unroll
                         for (int m = 0; m < 2; ++m) {
                             float stage[4] = {};
 #pragma unroll
-                            for (int pl = PLANES - 1; pl >= 0; --pl)
+                            for (int pl = P - 1; pl >= 0; --pl)
 #pragma unroll
                                 for (int i = 0; i < 2; ++i) pair(stage, w[i][2 * m], w[i][2 * m + 1], v[pl][i]);
 #pragma unroll
@@ -490,7 +499,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
         auto ask_up = [&](uint32_t at, uint32_t s) {
             if (at >= chosen) return;
             const uint32_t base = l.base[at], count = l.base[at + 1] - base;
-            ask(g < count ? rows + (size_t)(l.token[base + g] & 63u) * D : nullptr, s * XL_COLS, D, row_plane, first);
+            xl_ask<PLANES>(g < count ? rows + (size_t)(l.token[base + g] & 63u) * D : nullptr, s * XL_COLS + warp * 64, D, row_plane, first);
         };
         const uint32_t ahead = ctas / f_tiles, over = ctas % f_tiles;      // a CTA's next unit: experts and tiles on
         uint32_t at = cta / f_tiles, tile = cta % f_tiles;
@@ -500,7 +509,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
             const uint32_t f0 = tile * 16, base = l.base[at], count = l.base[at + 1] - base;
             clear();
             for (uint32_t s = 0; s < up_stages && ok; ++s)
-                multiply(s * XL_COLS, D, row_plane, count, [&](uint32_t k) { return rows + (size_t)(l.token[base + k] & 63u) * D; },
+                multiply(std::integral_constant<int, PLANES>{}, s * XL_COLS, D, row_plane, count, [&](uint32_t k) { return rows + (size_t)(l.token[base + k] & 63u) * D; },
                          [&]() { s + 1 < up_stages ? ask_up(at, s + 1) : ask_up(next_at, 0); });
             share(count);      // (also where a wait ran out: nobody is left waiting)
             for (uint32_t i = tid; i < count * 16; i += 256) {
@@ -508,7 +517,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
                 if (f0 + f >= F) continue;
                 const float w = choice < XL_MAX_TOP ? l.weight[pair & 63u][choice] : 1.0f;
                 const float v = act_f32(a.activation, total(16 + f, k)) * total(f, k) * w;
-                xl_planes<PLANES>(v, hidden + (size_t)(base + k) * F + f0 + f, hidden_plane);
+                xl_planes<HIDDEN>(v, hidden + (size_t)(base + k) * F + f0 + f, hidden_plane);
             }
             meet();
             at = next_at;
@@ -526,7 +535,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
         };
         auto ask_down = [&](uint32_t expert, uint32_t s) {
             const uint32_t base = l.base[expert], count = l.base[expert + 1] - base;
-            ask(g < count ? hidden + (size_t)(base + g) * F : nullptr, s * XL_COLS, F, hidden_plane, first);
+            xl_ask<HIDDEN>(g < count ? hidden + (size_t)(base + g) * F : nullptr, s * XL_COLS + warp * 64, F, hidden_plane, first);
         };
         uint32_t expert = 0, stage_of = 0;      // of the stage at hand
         if (ok && begin < end) {
@@ -546,7 +555,7 @@ __global__ void __launch_bounds__(XL_THREADS, 1) expert_layer_kernel(const __gri
             for (; w < stop && ok; ++w) {
                 const uint32_t s = stage_of, base = l.base[expert], count = l.base[expert + 1] - base, after = expert + 1 < chosen ? expert + 1 : 0;
                 const bool ends = s + 1 == f_stages;
-                multiply(s * XL_COLS, F, hidden_plane, count, [&](uint32_t k) { return hidden + (size_t)(base + k) * F; },
+                multiply(std::integral_constant<int, HIDDEN>{}, s * XL_COLS, F, hidden_plane, count, [&](uint32_t k) { return hidden + (size_t)(base + k) * F; },
                          [&]() { if (w + 1 < end) ask_down(ends ? after : expert, ends ? 0 : s + 1); });
                 stage_of = ends ? 0 : s + 1;
                 if (ends) expert = after;
