@@ -95,3 +95,24 @@ def test_bf16_rows_keep_products_of_16_bits(ctx, rows):
     hidden = y[:, :ff] * y[:, ff:]
     ref = hidden[:, d % ff] - hidden[:, (d + 1 + d // ff) % ff]
     assert np.array_equal(got, P.to_kept(ref, P.BF16))
+
+
+@pytest.mark.parametrize("dt", [P.F32, P.BF16])
+@pytest.mark.parametrize("experts,spread", [(512, True), (512, False), (16, False)])
+def test_the_longest_lists(ctx, dt, experts, spread):
+    """64 rows, 16 chosen and 16 shared: every expert by some rows and the shared ones by all, or the same few experts by all rows"""
+    lay = _Layer(ctx, 64, 24, experts, 16, seed=26)
+    if spread:      # row r reads its choices from its column
+        router = np.full((experts, 64), -8.0)
+        r, j = np.arange(64)[:, None], np.arange(16)[None, :]
+        router[(8 * r + 5 * j) % experts, np.broadcast_to(r, (64, 16))] = 8 - j / 4
+        lay.host[0][:], x = _bf16(router), np.eye(64)
+        lay.bias[:] = 0
+    else:
+        x = 0.01 * lay.rng.standard_normal((64, 64))
+        lay.bias[:] = 0
+        lay.bias[np.arange(16) * (experts // 16)] = 10 + np.arange(16)
+    lay.bufs[0], lay.bufs[3] = ctx.upload(lay.host[0]), ctx.upload(lay.bias)
+    lay.check(64, 16, dt, x=x)
+    ids = lay.run(64, 16, dt, x=x)[2]
+    assert len(np.unique(ids)) == (experts if spread else 16)

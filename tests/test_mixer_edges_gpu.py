@@ -185,3 +185,64 @@ def test_a_step_that_is_no_number(ctx, dt, dim, n):
         assert np.isnan(out[hit]).all() and np.array_equal(out[~hit], ref[~hit])
         others = [0, 2, 3]
         assert np.isnan(state[0, 1]).all() and np.array_equal(state[0, others], cstate[0, others])
+
+
+@pytest.mark.parametrize("shift", [-4.0, -8.0])
+@pytest.mark.parametrize("cut", [(2, 1, 64, 128, [(0, 2500, 1, 0)]), (4, 4, 64, 64, [(0, 1500, 0, 0), (1500, 40, 1, 1)]), (2, 2, 128, 64, [(3, 1290, 0, 1)])])
+def test_parts_and_whole_agree(ctx, cut, shift):
+    """the same rows in parts (with a scratch), whole, and whole again: the whole ones to the bit, the parts within both sides' roundings of the recurrence"""
+    heads, groups, dim, n, seqs = cut
+    rows = max(f + m for f, m, _, _ in seqs)
+    rng = np.random.default_rng(rows)
+    v = _scan_rows(rng, rows, heads, groups, dim, n)
+    v["dt"] += shift
+    st = rng.standard_normal((2, heads, dim, n)).astype(np.float32)
+    parts, pstate, scratch = _run_scan(ctx, v, heads, groups, dim, n, seqs, 2, state=st)
+    whole, wstate, _ = _run_scan(ctx, v, heads, groups, dim, n, seqs, 2, state=st, scratch=False)
+    again, astate, _ = _run_scan(ctx, v, heads, groups, dim, n, seqs, 2, state=st, scratch=False)
+    assert scratch > 0 and np.array_equal(whole, again) and np.array_equal(wstate, astate)
+    k = lambda w, *s: P.of_kept(P.to_kept(w, P.BF16), P.BF16).reshape(rows, *s)
+    a = v["a"].astype(np.float32).astype(np.float64)
+    step = P.steps(k(v["dt"], heads), 0.0)
+    z = k(v["z"], heads, dim)
+    ref, state, mag, smag = P.scan(k(v["x"], heads, dim), step, k(v["b"], groups, n), k(v["c"], groups, n), z, a, v["d"].astype(np.float32).astype(np.float64), st.astype(np.float64), seqs)
+    # a token's decay is off by three roundings and |step a| of four, its state by two; over the longest sequence, for the head of the largest sum
+    unit = 2.0 ** -24 * (max(5 * m + 4 * float(np.abs(step * a)[f:f + m].sum(0).max()) for f, m, _, _ in seqs) + n + 8)
+    assert (np.abs(pstate - wstate) <= 2 * ((unit + 2.0 ** -16) * smag + 2.0 ** -24 * np.abs(state))).all()
+    cov = np.zeros(rows, bool)
+    for f, m, _, _ in seqs:
+        cov[f:f + m] = True
+    bound = ((unit + 2.0 ** -8) * mag * np.abs(P.silu(z)) + (2.0 ** -21 + 2.0 ** -22 * np.abs(z) + P.HALF_STEP[P.BF16]) * np.abs(ref))[cov]
+    assert (np.abs(parts - whole).reshape(ref.shape)[cov] <= 2 * 1.01 * bound + P.TINY[P.BF16]).all()
+
+
+@pytest.mark.parametrize("dt", [P.BF16, P.F32, P.F16])
+@pytest.mark.parametrize("heads,groups,dim,n", [(4, 2, 64, 128), (6, 3, 33, 20)])
+def test_step_without_a_list_of_slots(ctx, dt, heads, groups, dim, n):
+    """row r is slot r: three calls as with the list 0, 1, ..., to the bit, and the slots behind the rows stay"""
+    rng = np.random.default_rng(heads)
+    rows, slots, taps, inner = 3, 5, 4, heads * dim
+    ch = inner + 2 * groups * n
+    w, cbias = rng.standard_normal((ch, taps)).astype(np.float32), rng.standard_normal(ch).astype(np.float32)
+    conv0, st0 = P.to_kept(rng.standard_normal((slots, taps - 1, ch)), dt), rng.standard_normal((slots, heads, dim, n)).astype(np.float32)
+    f32 = [ctx.upload(u) for u in (w, cbias, -(1 + 15 * rng.random(heads)).astype(np.float32), rng.standard_normal(heads).astype(np.float32), (rng.standard_normal(heads) - 3).astype(np.float32))]
+    listed = ctx.upload(np.arange(rows, dtype=np.uint32))
+    tokens = [[_Rows(ctx, rng.standard_normal((rows, u)), dt) for u in (ch, inner, heads)] for _ in range(3)]
+    results = []
+    for names in (listed.ptr, 0):
+        conv_b, st_b, tick = ctx.upload(conv0), ctx.upload(st0), ctx.upload(np.zeros(rows * groups, np.uint32))
+        outs = []
+        for X, Z, D in tokens:
+            out = _Rows(ctx, np.zeros((rows, inner)), dt)
+            a = B.StateSpaceStepArgs(xbc=X.ptr, dt=D.ptr, z=Z.ptr, conv_weights=f32[0].ptr, conv_bias=f32[1].ptr, conv_state=conv_b.ptr, a=f32[2].ptr, d=f32[3].ptr, dt_bias=f32[4].ptr,
+                                     state=st_b.ptr, out=out.ptr, slots=names, tickets=tick.ptr, rows=rows, slot_count=slots, heads=heads, groups=groups, head_dim=dim, state_size=n, taps=taps,
+                                     xbc_stride=X.stride, dt_stride=D.stride, z_stride=Z.stride, out_stride=out.stride, dt_min=0.0, dt_max=float("inf"), dt_softplus=1, activation=B.ACT_SILU,
+                                     data_type=dt)
+            with ctx.command_buffer("step") as cmd:
+                cmd.encode("uzu_state_space_step_encode", C.byref(a))
+            outs.append(out.get()[0])
+            assert not tick.numpy(np.uint32, (rows * groups,)).any()
+        results.append((np.stack(outs), conv_b.numpy(_np(dt), conv0.shape), st_b.numpy(np.float32, st0.shape)))
+    for with_list, without in zip(*results):
+        assert np.array_equal(with_list, without)
+    assert np.array_equal(results[1][1][rows:], conv0[rows:]) and np.array_equal(results[1][2][rows:], st0[rows:]) and not np.array_equal(results[1][2][:rows], st0[:rows])
