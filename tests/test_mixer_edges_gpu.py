@@ -41,8 +41,9 @@ def test_conv_gate_far_from_zero(ctx, dt, shift):
     finite = np.isfinite(ref)
     assert finite.any() and np.array_equal(np.isnan(got), np.isnan(ref)) and np.array_equal(got[np.isinf(ref)], ref[np.isinf(ref)])
     x, ref, got = x[finite], ref[finite], got[finite]
-    # an exponential of x log2 e (its own error, the exponent's rounding), at most six more roundings; below 2^-126 the exponential's last place is 2^-149
-    bound = (2.0 ** -21 + 2.0 ** -22 * np.minimum(np.abs(x), 200.0)) * np.abs(ref) + np.minimum(np.abs(x), 2.0 ** 100) * 2.0 ** -149
+    # an exponential of x log2 e (its own error, the exponent's rounding), at most six more roundings. Below -87.3 the reciprocal of 1 + e^-x is no normal number any more and taken as 0:
+    # off by the value, which is less than 88 * 2^-126 there, and 0 where e^-x is infinite in 32 bits
+    bound = (2.0 ** -21 + 2.0 ** -22 * np.minimum(np.abs(x), 200.0)) * np.abs(ref) + np.where(x < -87.3, np.abs(ref), 0.0)
     assert (np.abs(got - ref) <= P.HALF_STEP[dt] * (np.abs(ref) + bound) + P.TINY[dt] + bound).all(), [(a, b, c) for a, b, c, m in zip(x, got, ref, np.abs(got - ref) > bound + P.HALF_STEP[dt] * np.abs(ref) + P.TINY[dt]) if m][:8]
 
 
@@ -64,7 +65,8 @@ def test_conv_gate_of_large_sums(ctx, dt, channels, taps):
     # the sums' own errors move such a value by a part of itself only
     small = (ref > -1e-15) & (ref < 0)
     part = (taps + 4) * 2.0 ** -23 * mag + 2.0 ** -20 + P.HALF_STEP[dt]
-    assert (np.abs(got - ref) <= part * np.abs(ref) * 1.1 + P.TINY[dt] + np.minimum(mag, 1000) * 2.0 ** -149)[small].all()
+    none = np.where(np.abs(ref) < 2.0 ** -119, np.abs(ref), 0.0)      # (0 below -87.3)
+    assert (np.abs(got - ref) <= part * np.abs(ref) * 1.1 + P.TINY[dt] + none)[small].all()
 
 
 @pytest.mark.parametrize("dt", [P.BF16, P.F32])
@@ -82,9 +84,7 @@ def test_conv_infinite_inputs_reach_their_window_only(ctx, dt, taps, act):
         hit[row:min(row + taps, 45 if row < 45 else rows), channel] = True
     got, _ = _run_conv(ctx, u, w, seqs, dt, 2, act=act, state=st)
     assert not np.isfinite(got[hit]).any()
-    beside = ~hit & hit.reshape(rows, channels // 2, 2)[:, :, ::-1].reshape(rows, channels)      # the gate takes one reciprocal for two channels: 2^-21 of the value each time, and its rounding
-    assert np.array_equal(got[~hit & ~beside], clean[~hit & ~beside])
-    assert (np.abs(got - clean)[beside] <= (2.0 ** -20 + 2 * P.HALF_STEP[dt]) * np.abs(clean[beside])).all()
+    assert np.array_equal(got[~hit], clean[~hit])
 
 
 def _run_scan(ctx, v, heads, groups, dim, n, seqs, slots, dt=P.BF16, state=None, scratch=True):

@@ -1,9 +1,10 @@
 // Short causal convolution over packed sequences: y[t, c] = act(bias[c] + sum_j w[c, j] u[t - taps + 1 + j, c]).
 //
-// Bound by memory: a value is read and written once, 2 taps flops each; special functions (an exponential a value, a reciprocal for two) take half of that time beside it. A
-// thread has 8 bytes of channels (four of 16 bits, two of 32) and walks a strip of a sequence's rows with the last taps - 1 of them in registers, eight rows of loads under way
-// at a time; a strip reads taps - 1 rows of the one before it again (from L2). 16384 rows of 10240 bf16 channels, 4 taps, 16 sequences: 137 us, 4.9 TB/s of the 6.45 of a copy
-// (16 bytes a thread 178 us: fewer warps; 4 bytes 223; batches of four rows 146; limits on the registers 170 to 284).
+// Bound by memory: a value is read and written once, 2 taps flops each, an exponential and a reciprocal. A thread has 8 bytes of channels (four of 16 bits, two of 32) and walks a strip
+// of a sequence's rows with the last taps - 1 of them in registers, eight rows of loads under way at a time; a strip reads taps - 1 rows of the one before it again (from L2). 16384 rows
+// of 10240 bf16 channels, 4 taps, 16 sequences: 125 us, 5.4 TB/s of the 6.45 of a copy (one reciprocal for two gates, whose denominators had to be cut for it, 131; and with that 16
+// bytes a thread 178: fewer warps; 4 bytes 223; batches of four rows 146; limits on the registers 170 to 284). Rows off whole groups of 8 bytes take
+// one channel a thread: 153 us (f32: 233 against 213).
 // The strip that starts a sequence reads the slot's inputs and, behind its rows, writes the new ones: nobody else touches these channels of the slot, so the order is its own.
 #include "state_space.cuh"
 
@@ -23,30 +24,6 @@ template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) ConvVec {
     T v[VEC];
 };
-
-// Sums far below zero, where the walk's gate is not the function: they are formed again (in the same order) and their results written over. Values so far off are rare: this is not made
-// to be fast, and the walk only looks once a strip whether there was one (16384 x 10240 bf16: 136 us, with a look for every pair 143, for every row 152).
-template <typename T, int VEC>
-__device__ __noinline__ void conv_far(const ConvParams& p) {
-    const uzu_causal_conv_args& a = p.a;
-    const uint32_t tile = blockIdx.x / p.groups, c0 = (blockIdx.x % p.groups * CC_THREADS + threadIdx.x) * VEC;
-    const PackedSequence s = p.table.s[ss_find(p.table, tile)];
-    const uint32_t t0 = (tile - s.tile0) * p.strip, t1 = min(t0 + p.strip, s.rows), kept = a.taps - 1;
-#pragma unroll 1
-    for (uint32_t t = t0; t < t1; ++t)
-#pragma unroll 1
-        for (uint32_t c = c0; c < c0 + VEC; ++c) {
-            float y = a.bias ? reinterpret_cast<const float*>(a.bias)[c] : 0.0f;
-#pragma unroll 1
-            for (uint32_t j = 0; j < a.taps; ++j) {      // t + j - kept: of the sequence's rows, behind the slot's inputs
-                float u = 0.0f;
-                if (t + j >= kept) u = ss_f(reinterpret_cast<const T*>(a.input)[(size_t)(s.first + (t + j - kept)) * a.input_stride + c]);
-                else if (!s.fresh()) u = ss_f(reinterpret_cast<const T*>(a.state)[((size_t)s.slot() * kept + t + j) * a.channels + c]);
-                y = fmaf(reinterpret_cast<const float*>(a.weights)[(size_t)c * a.taps + j], u, y);
-            }
-            if (-1.4426950408889634f * y > 60.0f) reinterpret_cast<T*>(a.output)[(size_t)(s.first + t) * a.output_stride + c] = ss_t<T>(ss_silu_far(y));
-        }
-}
 
 // the last `kept` inputs of (slot, rows), by the strip that starts the sequence: nobody else touches these channels of the slot
 template <typename T, int VEC, int TAPS>
@@ -112,7 +89,6 @@ __global__ void __launch_bounds__(CC_THREADS) causal_conv_kernel(const __grid_co
 #pragma unroll
     for (int j = 0; j < TAPS - 1; ++j) pairs(past[j], u[j]);
 
-    float most = 0.0f;
     auto step = [&](const V& row) {
         V o;
         pairs(row, u[TAPS - 1]);
@@ -121,7 +97,7 @@ __global__ void __launch_bounds__(CC_THREADS) causal_conv_kernel(const __grid_co
             float2 y = bias[i];
 #pragma unroll
             for (int j = 0; j < TAPS; ++j) y = ss_fma2(w[j][i], u[j][i], y);
-            if (a.activation == UZU_ACT_SILU) y = ss_silu_pair(y, most);
+            if (a.activation == UZU_ACT_SILU) y = ss_silu2(y);
             o.v[2 * i] = ss_t<T>(y.x);
             if (VEC > 1) o.v[VEC > 1 ? 2 * i + 1 : 0] = ss_t<T>(y.y);
 #pragma unroll
@@ -146,7 +122,6 @@ __global__ void __launch_bounds__(CC_THREADS) causal_conv_kernel(const __grid_co
         from += a.input_stride;
         to += a.output_stride;
     }
-    if (most >= 0x1p60f) conv_far<T, VEC>(p);
     if (t0 == 0) conv_keep<T, VEC, TAPS>(p, s);
 }
 

@@ -35,11 +35,6 @@ __device__ __forceinline__ float ss_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float ss_exp2_small(float x) {      // numbers below 2^-126 too
-    float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float ss_rcp(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -68,17 +63,6 @@ __device__ __forceinline__ float2 ss_silu2(float2 x) {
     const float2 d = ss_add2(make_float2(ss_exp2(e.x), ss_exp2(e.y)), make_float2(1.0f, 1.0f));
     return ss_mul2(x, make_float2(ss_rcp(d.x), ss_rcp(d.y)));
 }
-// two of them with one reciprocal, of the product of both denominators (each cut at 2^60: their product stays a normal number): where special functions are what a loop waits for.
-// Where -x log2 e is above 60 a denominator is cut and the value not that of the function; `most` is at least 2^60 after such a one, and the caller takes ss_silu_far.
-__device__ __forceinline__ float2 ss_silu_pair(float2 x, float& most) {
-    const float2 e = ss_mul2(x, make_float2(-1.4426950408889634f, -1.4426950408889634f));
-    const float2 d = ss_add2(make_float2(ss_exp2(fminf(e.x, 60.0f)), ss_exp2(fminf(e.y, 60.0f))), make_float2(1.0f, 1.0f));
-    const float both = d.x * d.y, r = ss_rcp(both);
-    most = fmaxf(most, both);
-    return ss_mul2(x, ss_mul2(make_float2(r, r), make_float2(d.y, d.x)));      // (r d first: x r may be too small to keep its digits)
-}
-// -x log2 e > 60: the denominator's 1 is nothing beside the exponential. Down to the smallest numbers; -infinity gives NaN (as infinity times 0)
-__device__ __forceinline__ float ss_silu_far(float x) { return x * ss_exp2_small(1.4426950408889634f * x); }
 // a token's step (log1p: steps of 1e-3 keep their digits); not a number stays so
 __device__ __forceinline__ float ss_step(float dt, float bias, uint32_t softplus, float lo, float hi) {
     float s = dt + bias;
