@@ -935,7 +935,7 @@ UZU_API uzu_status uzu_causal_conv_validate(const uzu_causal_conv_args* args);
 /* Selective state space scan over packed sequences: one decay per head and token, head h reads group h / (heads / groups) of b and c. With
  *   step = dt + dt_bias[h];  dt_softplus: step <- softplus(step);  step <- min(max(step, dt_min), dt_max)
  *   S_t = exp(step a[h]) S_(t-1) + step x_t b_t^T   (per head [head_dim, state_size]);   y_t = S_t c_t + d[h] x_t;   out = y * silu(z)  (z optional)
- * The state f32 [slots, heads, head_dim, state_size] is read and written back per sequence. a is negative in a model (decays below 1); nothing checks it.
+ * The state f32 [slots, heads, head_dim, state_size] is read and written back per sequence. a is at most 0 (decays up to 1; nothing checks it, and growing states may overflow on the way where the recurrence does not).
  * dt_min >= 0. bf16 rows with head_dim a multiple of 64, state_size 64 or 128 and pointers and strides of whole 16-byte groups run in chunks of 128 tokens on
  * the tensor cores (csrc/state_space_umma.cu): states, decays and sums are f32 there too, decayed inputs enter the state as two bf16 parts (16 bits), scores
  * and the state that is read out are rounded to bf16. An input that is not finite leaves NaN or infinity in what depends on it and in nothing else; which of the

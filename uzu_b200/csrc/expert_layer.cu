@@ -12,9 +12,9 @@
 //   4  down: all stages of all 32-row tiles over all chosen experts, cut evenly over the CTAs; a tile that several have is summed by the last of them, in their order.
 // In both products an expert's tokens stand side by side, eight a tile; the rows of the next stage are asked for a stage ahead.
 // Two waits for all CTAs, behind phases 1 and 3. They and the ring's barriers are bounded (wait_errors.h).
-// One token of 8 experts of 4096 x 14336, two chosen: 125 us, 5.6 TB/s of the 6.45 of a copy (router, choice and the two waits take 12). 16 tokens of 64 experts of 2048 x 1408, six
-// chosen and two shared: 185 us of 142. 48 f32 tokens of 128 experts of 2048 x 768: 351 us of 179, bound by the warps' way through a stage (three planes, 1400 cycles where the
-// bytes take 1400) and the 39 units' ends of 1500 cycles each.
+// One token of 8 experts of 4096 x 14336, two chosen: 125 us, 5.6 TB/s of the 6.45 of a copy (router, choice and the two waits take 12). Of 64 experts of 2048 x 1408, six chosen and
+// two shared: 16 bf16 tokens 182 to 191 us of 142, 32 273, 64 336; f32 250, 311, 407. 48 f32 tokens of 128 experts of 2048 x 768: 349 us of 179, bound by the warps' way through a stage
+// (three planes, 1400 cycles where the bytes take 1400) and the 39 units' ends of 1500 cycles each.
 #include <algorithm>
 
 #include "row_sequences.h"

@@ -4,11 +4,12 @@
 // Scan: a CTA has 32 rows p of a head's state, four threads a row with every fourth group of four columns in registers. Rows of 16 tokens are converted into shared
 // memory while the batch before them is walked, four tokens side by side. Bound by the way through a batch (3 us of 16 tokens with one CTA an SM: its loads, two barriers,
 // the walk): long sequences of few heads are cut into parts whose states are summed first, so that several CTAs share an SM. Two sequences of 1001 f32 tokens, 24 heads of 64 x 64:
-// 67 us (whole 125 us); 1400 bf16 tokens of 80 heads of 64 x 40 some 300 us.
+// 70 us (whole 125 us); 1400 bf16 tokens of 80 heads of 64 x 40 280 us; 8192 tokens of 64 heads of 64 x 128 1370 us in f16 and 1210 in f32 (bf16 on the tensor cores 112). Up to a state
+// size of 128 the kernels spill 4 to 36 bytes of a thread's registers.
 //
 // Step: bound by the state, read and written once. A CTA has up to 64 rows p of one head of one sequence. What the convolution takes is asked for first, then all of the state;
 // the CTA convolves its x channels and its group's b and c while that comes. The conv slots of b and c are read by all CTAs of the group: each counts itself when it has
-// them, the last one writes the new inputs and takes the count back to zero. 64 rows of 80 heads of 64 x 128: 72 us, 4.7 TB/s of the 6.45 of a copy; 256 rows of 128 heads 483 us
+// them, the last one writes the new inputs and takes the count back to zero. 64 rows of 80 heads of 64 x 128: 74 us, 4.6 TB/s (as many bytes multiplied in place: 53 us); 256 rows of 128 heads 486 us
 // (three CTAs an SM, by registers, do not cover all of a CTA's phases; 32 rows a CTA: 5 percent slower; one CTA an SM that streams the state through shared memory by bulk copies: slower too).
 #include "state_space.cuh"
 

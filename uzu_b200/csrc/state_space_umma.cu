@@ -15,7 +15,10 @@
 // Two warps share a block of 32 rows in each role; the roles' loops are short and stand once, since seven of them share the instruction caches (with unrolled loops and waits of forty
 // instructions a chunk took 40 percent longer).
 // What bounds it: the roles' way through a chunk and the handshakes between them, 5700 cycles where the products take 1500 and the bytes 2000 (16384 tokens of 128 heads of 64 x
-// 128: 385 us against a floor of 137; nine sequences of 8192 tokens in all, 64 heads: 114 against 38; token by token 9.1 ms and 1.8 ms).
+// 128: 380 us against a floor of 137; nine sequences of 8192 tokens in all, 64 heads: 112 against 38, with 64 x 64 110; token by token, as f16 rows go, 1.4 ms). With state_size 64 some 400
+// bytes of a thread's registers are spilled.
+// Scores and the state that is read out are one bf16 part each: outputs are 0.0017 to 0.0025 off (norms, against 64 bits) where their own rounding is 0.0017. With two parts of both they
+// are off by that alone, in 15 to 17 percent more time (129 and 450 us: longer ways of two roles, not the products).
 // Every barrier wait is bounded (wait_errors.h).
 #include "state_space.cuh"
 #include "umma.cuh"
