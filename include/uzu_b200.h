@@ -935,7 +935,8 @@ UZU_API uzu_status uzu_causal_conv_validate(const uzu_causal_conv_args* args);
 /* Selective state space scan over packed sequences: one decay per head and token, head h reads group h / (heads / groups) of b and c. With
  *   step = dt + dt_bias[h];  dt_softplus: step <- softplus(step);  step <- min(max(step, dt_min), dt_max)
  *   S_t = exp(step a[h]) S_(t-1) + step x_t b_t^T   (per head [head_dim, state_size]);   y_t = S_t c_t + d[h] x_t;   out = y * silu(z)  (z optional)
- * The state f32 [slots, heads, head_dim, state_size] is read and written back per sequence. a is at most 0 (decays up to 1; nothing checks it, and growing states may overflow on the way where the recurrence does not).
+ * The state f32 [slots, heads, head_dim, state_size] is read and written back per sequence. a is at most 0 (decays up to 1; nothing checks it, and
+ * with growing states parts of a sum may overflow where the recurrence does not).
  * dt_min >= 0. bf16 rows with head_dim a multiple of 64, state_size 64 or 128 and pointers and strides of whole 16-byte groups run in chunks of 128 tokens on
  * the tensor cores (csrc/state_space_umma.cu): states, decays and sums are f32 there too, decayed inputs enter the state as two bf16 parts (16 bits), scores
  * and the state that is read out are rounded to bf16. An input that is not finite leaves NaN or infinity in what depends on it and in nothing else; which of the
@@ -981,8 +982,8 @@ UZU_API uzu_status uzu_state_space_step_validate(const uzu_state_space_step_args
 /* A whole layer of routed experts for 1 .. 64 tokens in one launch: router, choice, the chosen experts' gated units, the shared experts, the weighted sum.
  *   logits = x router^T + router_bias.  score 0: the `top` largest logits, weights = softmax over them; 1: s = softmax over all logits, the `top` largest s,
  *   weights = s; 2: s = sigmoid(logits), the `top` largest s, weights = s.  renormalise: weights / their sum;  weights * weight_scale. The lower index wins
- *   a tie; a logit that is NaN comes last (for score 0 it counts as -infinity), with a weight of 0. Where no softmax is a number (no logit above -infinity, or one of +infinity) the weights are NaN, and score 1
- *   takes the lowest indices.
+ *   a tie; a logit that is NaN comes last (for score 0 it counts as -infinity), with a weight of 0. Where no softmax is a number (no logit above -infinity, or
+ *   one of +infinity) the weights are NaN, and score 1 takes the lowest indices.
  *   out[t] = sum_k weights[t, k] E_(ids[t, k])(x_t) + sum over shared experts E(x_t),   E(x) = down (act(gate) * up),  [up | gate] = up_gate x
  * x and out are bf16 or f32 rows, the weights bf16. f32 rows and hidden values enter the products as three bf16 parts (24 bits), of bf16 rows the hidden values as two;
  * products and sums are f32, summed in an order that only the shapes and the choice set. width and ff are multiples of 8, weights 16-byte aligned.

@@ -5,7 +5,7 @@
 //   steps    one warp: step sizes, sums of logarithms of each block of 32 tokens from its front and from its end (accurate where their weights are not small)
 //   scores   c b^T out of tensor memory, times 2^(L_i - L_j) step_j, back as bf16 operand A. Below the diagonal's 32 x 32 blocks the factor is a product of a row's and
 //            a column's, both relative to the row block's start, so that neither overflows (decays are at most 1) and no exponential is taken per element. In the
-//            diagonal's blocks the exponent is a difference of sums of at most 32 tokens of at most 150 each: off by 2^-11 at most, where a score's rounding is 2^-8.
+//            diagonal's blocks the exponent is a difference of sums of at most 32 tokens of at most 150 each: off by a few 2^-12, where a score's rounding is 2^-8.
 //   state    x times its weight as two bf16 parts (16 bits: the state keeps what f32 sums need) for the state's sum, the state in registers, f32, its bf16 copy as operand
 //   output   the two sums, d x and the gate
 //   issue    scores c b^T (128 x 128), their product with x (64), c S (64), b^T [x hi | x lo] (128 columns, both parts at one reading of b)
@@ -18,7 +18,7 @@
 // 128: 380 us against a floor of 137; nine sequences of 8192 tokens in all, 64 heads: 112 against 38, with 64 x 64 110; token by token, as f16 rows go, 1.4 ms). With state_size 64 some 400
 // bytes of a thread's registers are spilled.
 // Scores and the state that is read out are one bf16 part each: outputs are 0.0017 to 0.0025 off (norms, against 64 bits) where their own rounding is 0.0017. With two parts of both they
-// are off by that alone, in 15 to 17 percent more time (129 and 450 us: longer ways of two roles, not the products).
+// are off by that alone, in 15 to 17 percent more time (129 and 450 us: longer ways of two roles, not the products); with two parts of the state alone 0.0017, in 9 to 12 percent more.
 // Every barrier wait is bounded (wait_errors.h).
 #include "state_space.cuh"
 #include "umma.cuh"
