@@ -1007,6 +1007,131 @@ UZU_API void uzu_expert_layer_encode(uzu_command_buffer* cmd, const uzu_expert_l
 UZU_API uzu_status uzu_expert_layer_validate(const uzu_expert_layer_args* args);
 UZU_API size_t uzu_expert_layer_scratch_bytes(const uzu_expert_layer_args* args);
 
+/* ---- A cache of 8 bits, attention over it, eviction, and the verification of drafted tokens (extensions) ------------------------------------------
+ * Keys and values of served sequences in a pool of blocks of `block_tokens` tokens, a byte a number and one scale for each block and head; a number is
+ * code * scale. Scales are powers of two, so that each such number is a bf16 number and a code does not depend on how a scale was computed: the smallest
+ * 2^e, e >= -100, with which the block's largest magnitude is at most 127 (i8) or 448 (e4m3) scales; 0 where all are zeros. Codes are rounded to nearest,
+ * ties to even. A number that is not finite, or of 2^120 and more, makes the scale of its block and head NaN, and with it every score or sum that reads
+ * them, until the block is begun again. Codes that do not come from these entries are finite ones (no e4m3 code 0x7f or 0xff in a token that a sequence has).
+ * Which sequences a pass has is read on the device, so a captured call follows it: their block numbers, how many tokens they have, where their rows are.
+ * Token j of sequence i is at tables[i, j / block_tokens]. A block number that is not below `blocks` is no block: its tokens are seen by nobody and rows
+ * for it are dropped. Rows that belong to no sequence, and tokens behind a sequence's last, keep what they hold. max_length and max_rows bound what the
+ * device may find (they size launches and scratch); tokens and rows behind them are left out. Blocks that a call writes belong to one of its sequences
+ * only; read-only ones may be shared. Buffers of one call do not overlap; arrays are aligned to their elements, codes to 16 bytes. The _validate calls
+ * make the checks of the _encode ones (UZU_ERROR_INVALID_ARGUMENT) and need no device. */
+typedef enum uzu_cache_code { UZU_CACHE_CODE_I8 = 0, UZU_CACHE_CODE_E4M3 = 1 } uzu_cache_code;
+typedef struct uzu_quantized_cache {
+    uint64_t key_codes, value_codes;     /* u8 [blocks, kv_heads, block_tokens, head_dim] */
+    uint64_t key_scales, value_scales;   /* f32 [blocks, kv_heads] */
+    uint64_t key_weights;                /* optional f32 [blocks, kv_heads, block_tokens]: the attention weight that a token has had, summed up */
+    uint32_t blocks, kv_heads, block_tokens /* 16 | 32 | 64 */, head_dim /* a multiple of 16 up to 256 */;
+    uint32_t code_type;                  /* uzu_cache_code */
+    uint32_t reserved0;
+} uzu_quantized_cache;
+typedef struct uzu_cache_sequences {
+    uint64_t tables;               /* u32 [count, table_stride] (DEVICE, as the two below) */
+    uint64_t lengths;              /* u32 [count]: tokens of a sequence in the cache before this pass */
+    uint64_t row_offsets;          /* u32 [count + 1]: rows [row_offsets[i], row_offsets[i + 1]) are sequence i's, its tokens from lengths[i] on */
+    uint32_t count, table_stride, rows, max_rows, max_length /* the pass's rows included; below 2^31, as rows */;
+    uint32_t reserved0;
+} uzu_cache_sequences;
+
+/* New tokens into the cache: key and value rows (data_type [rows, kv_heads * head_dim], rotated and normed already) become codes. A token that joins a begun
+ * block keeps the block's scale or makes it larger: the codes before it are then rounded to the new scale. key_weights of new tokens start at 0.
+ * new_lengths (optional, u32 [count], not the same array as lengths): lengths + rows, for the pass after the layers that share them. */
+typedef struct uzu_quantized_cache_append_args {
+    uzu_quantized_cache cache;
+    uzu_cache_sequences sequences;
+    uint64_t keys, values, new_lengths;
+    uint32_t key_stride, value_stride;   /* elements between rows */
+    uint32_t data_type;            /* UZU_DT_BF16 | UZU_DT_F32 | UZU_DT_F16 */
+    uint32_t reserved0;
+} uzu_quantized_cache_append_args;
+UZU_API void uzu_quantized_cache_append_encode(uzu_command_buffer* cmd, const uzu_quantized_cache_append_args* args);
+UZU_API uzu_status uzu_quantized_cache_append_validate(const uzu_quantized_cache_append_args* args);
+
+/* The numbers back: tokens from lengths[i] on, as many as sequence i has rows (lengths here: the first token that is read), to rows of data_type (bf16 and
+ * f32 hold them exactly, f16 rounds). keys or values may be 0. Rows of tokens that are not there keep what they hold. */
+typedef struct uzu_quantized_cache_read_args {
+    uzu_quantized_cache cache;
+    uzu_cache_sequences sequences;
+    uint64_t keys, values;
+    uint32_t key_stride, value_stride;
+    uint32_t data_type;
+    uint32_t reserved0;
+} uzu_quantized_cache_read_args;
+UZU_API void uzu_quantized_cache_read_encode(uzu_command_buffer* cmd, const uzu_quantized_cache_read_args* args);
+UZU_API uzu_status uzu_quantized_cache_read_validate(const uzu_quantized_cache_read_args* args);
+
+/* Causal softmax attention of the pass's rows over the cache, the rows' own tokens included (append them first): for single tokens, drafted tokens and
+ * prompts. Row t of sequence i is token p = lengths[i] + t and sees the tokens j <= p with p - j < window (window 0: all) or j < keep_first; head h reads key / value
+ * head h / (heads / kv_heads).
+ *   s = scale * query . key;  softcap > 0: s <- softcap * tanh(s / softcap);  w = softmax over the seen tokens (with sinks: exp(sinks[h]) joins the sum)
+ *   out[t, h, :] = sum_j w_j value_j      (zeros for a row that sees nothing)
+ *   weight_rows > 0: key_weights[j, g] += sum of w_j over the last weight_rows rows of a sequence and the heads of group g (0xffffffff: all its rows)
+ * A query that is not finite makes its row NaN. Scores, weights and sums are f32. bf16 and f16 queries enter the products as they are, f32 ones as two f16
+ * parts (22 bits, relative to the row's largest); weights as two f16 parts (22 bits), or of bf16 prompts on tcgen05 (csrc/quantized_cache_umma.cu) two bf16 parts.
+ * Sums run in an order that the shapes, the lengths and max_length set.
+ * scratch: of uzu_quantized_cache_attention_scratch_bytes() bytes, 256-byte aligned, its first 64 KB zero before the first use; every call leaves it ready for the next,
+ * of any sizes. Calls that may run at the same time do not share it. */
+typedef struct uzu_quantized_cache_attention_args {
+    uzu_quantized_cache cache;
+    uzu_cache_sequences sequences;
+    uint64_t query;                /* data_type, row t and head h at t * query_row_stride + h * query_head_stride elements */
+    uint64_t out;                  /* data_type [rows, heads * head_dim], rows out_stride apart */
+    uint64_t sinks;                /* optional f32 [heads] */
+    uint64_t scratch, scratch_bytes;
+    uint32_t heads, query_row_stride, query_head_stride, out_stride, window, keep_first, weight_rows;
+    float scale, softcap;
+    uint32_t data_type;            /* UZU_DT_BF16 | UZU_DT_F32 | UZU_DT_F16 */
+} uzu_quantized_cache_attention_args;
+UZU_API void uzu_quantized_cache_attention_encode(uzu_command_buffer* cmd, const uzu_quantized_cache_attention_args* args);
+UZU_API uzu_status uzu_quantized_cache_attention_validate(const uzu_quantized_cache_attention_args* args);
+UZU_API size_t uzu_quantized_cache_attention_scratch_bytes(uzu_context* ctx, const uzu_quantized_cache_attention_args* args);
+
+/* Sequences of more than `budget` tokens cut down to `budget`, each key head by itself: the first keep_first tokens, the last keep_last, and of those between
+ * the ones with the largest key_weights (the lower index wins a tie, NaN comes last). They move up in their order to tokens 0 .. budget - 1 of the same
+ * table, blocks are coded anew as if their tokens had been appended to begun-anew blocks in one pass, and key_weights move along. Sequences of at most `budget` tokens
+ * are left as they are. Tables stay; the blocks behind budget are the caller's to use again. sequences.row_offsets, rows and max_rows are not used.
+ * new_lengths u32 [count]: min(length, budget), not the same array as lengths. indices (optional, u32 [count, kv_heads, budget]): the token that each kept
+ * one was, 0xffffffff behind the last.
+ * scratch: of uzu_quantized_cache_evict_scratch_bytes() bytes, 256-byte aligned, content free before and after. Calls that may run at the same time do not
+ * share it. */
+typedef struct uzu_quantized_cache_evict_args {
+    uzu_quantized_cache cache;     /* with key_weights */
+    uzu_cache_sequences sequences;
+    uint64_t new_lengths, indices;
+    uint64_t scratch, scratch_bytes;
+    uint32_t budget, keep_first, keep_last /* together at most budget */;
+    uint32_t reserved0;
+} uzu_quantized_cache_evict_args;
+UZU_API void uzu_quantized_cache_evict_encode(uzu_command_buffer* cmd, const uzu_quantized_cache_evict_args* args);
+UZU_API uzu_status uzu_quantized_cache_evict_validate(const uzu_quantized_cache_evict_args* args);
+UZU_API size_t uzu_quantized_cache_evict_scratch_bytes(uzu_context* ctx, const uzu_quantized_cache_evict_args* args);
+
+/* Verification of drafted tokens: which of a sequence's drafts the target model keeps, and the token behind them, so that the result is distributed as the
+ * target's own samples are. With p_k = softmax(target_logits[i, k] / temperature), q_k = softmax(draft_logits[i, k] / draft_temperature):
+ *   draft k = 0, 1, .. is kept while uniforms[i, k] * q_k(draft) < p_k(draft); behind the first that is not kept, the token is drawn from max(p_k - q_k, 0),
+ *   behind the last draft from p (and from p where that difference is zero everywhere): the smallest token whose cumulative weight is more than
+ *   uniforms[i, drafts] times the sum of all.
+ * Without draft_logits the drafts are certain (q = 1 at the draft). temperature 0: a draft is kept if it is the largest target logit (the lowest index of several),
+ * and the token behind is that logit's; uniforms and draft_logits are not read then. draft_counts (optional, u32 [sequences], DEVICE): drafts of a sequence, at most `drafts`.
+ * accepted u32 [sequences]; tokens u32 [sequences, drafts + 1]: the kept drafts, the token behind them, UZU_NO_TOKEN in the rest. Logits of -infinity have no
+ * weight; rows without a distribution (a NaN or +infinity among the logits, or nothing above -infinity) keep no draft and give UZU_NO_TOKEN as the token behind;
+ * a drafted token that is not below vocab is not kept. Sums that decide a token are f64. uniforms are in [0, 1); temperatures other than 0 at least 2^-60. */
+#define UZU_NO_TOKEN 0xFFFFFFFFu
+typedef struct uzu_draft_verify_args {
+    uint64_t target_logits;        /* data_type [sequences * (drafts + 1), vocab], rows target_stride apart */
+    uint64_t draft_logits;         /* optional data_type [sequences * drafts, vocab], rows draft_stride apart */
+    uint64_t drafted, draft_counts, uniforms;    /* u32 [sequences, drafts], optional u32 [sequences], f32 [sequences, drafts + 1] */
+    uint64_t tokens, accepted;
+    uint32_t sequences, drafts /* 0 .. 16 */, vocab, target_stride, draft_stride;
+    float temperature, draft_temperature;
+    uint32_t data_type;            /* UZU_DT_BF16 | UZU_DT_F32 | UZU_DT_F16 */
+} uzu_draft_verify_args;
+UZU_API void uzu_draft_verify_encode(uzu_command_buffer* cmd, const uzu_draft_verify_args* args);
+UZU_API uzu_status uzu_draft_verify_validate(const uzu_draft_verify_args* args);
+
 /* ---- Host engine (C++ mirror of the reference's backend-agnostic Rust host code) ---------- *
  * No Rust toolchain exists in the build image, so the layer above the kernels -- Engine /
  * LanguageModel / LanguageModelStream / Decoder / Transformer / TransformerLayer (engine/mod.rs:15-43,

@@ -51,6 +51,8 @@ pub const UZU_ACTIVATION_TRANSFORM_QUANTIZE_WITH_GROUP_SUMS: u32 = 3;
 pub const UZU_EXPERT_SCORE_CHOSEN: u32 = 0;
 pub const UZU_EXPERT_SCORE_ALL: u32 = 1;
 pub const UZU_EXPERT_SCORE_SIGMOID: u32 = 2;
+pub const UZU_CACHE_CODE_I8: u32 = 0;
+pub const UZU_CACHE_CODE_E4M3: u32 = 1;
 pub const UZU_SAMPLING_GREEDY: u32 = 0;
 pub const UZU_SAMPLING_STOCHASTIC: u32 = 1;
 
@@ -1080,6 +1082,120 @@ pub struct uzu_expert_layer_args {
     pub reserved0: u32,
 }
 
+/// 64 bytes
+#[repr(C)] #[derive(Default, Clone, Copy)]
+pub struct uzu_quantized_cache {
+    pub key_codes: u64,
+    pub value_codes: u64,
+    pub key_scales: u64,
+    pub value_scales: u64,
+    pub key_weights: u64,
+    pub blocks: u32,
+    pub kv_heads: u32,
+    pub block_tokens: u32,
+    pub head_dim: u32,
+    pub code_type: u32,
+    pub reserved0: u32,
+}
+
+/// 48 bytes
+#[repr(C)] #[derive(Default, Clone, Copy)]
+pub struct uzu_cache_sequences {
+    pub tables: u64,
+    pub lengths: u64,
+    pub row_offsets: u64,
+    pub count: u32,
+    pub table_stride: u32,
+    pub rows: u32,
+    pub max_rows: u32,
+    pub max_length: u32,
+    pub reserved0: u32,
+}
+
+/// 152 bytes
+#[repr(C)] #[derive(Default, Clone, Copy)]
+pub struct uzu_quantized_cache_append_args {
+    pub cache: uzu_quantized_cache,
+    pub sequences: uzu_cache_sequences,
+    pub keys: u64,
+    pub values: u64,
+    pub new_lengths: u64,
+    pub key_stride: u32,
+    pub value_stride: u32,
+    pub data_type: u32,
+    pub reserved0: u32,
+}
+
+/// 144 bytes
+#[repr(C)] #[derive(Default, Clone, Copy)]
+pub struct uzu_quantized_cache_read_args {
+    pub cache: uzu_quantized_cache,
+    pub sequences: uzu_cache_sequences,
+    pub keys: u64,
+    pub values: u64,
+    pub key_stride: u32,
+    pub value_stride: u32,
+    pub data_type: u32,
+    pub reserved0: u32,
+}
+
+/// 192 bytes
+#[repr(C)] #[derive(Default, Clone, Copy)]
+pub struct uzu_quantized_cache_attention_args {
+    pub cache: uzu_quantized_cache,
+    pub sequences: uzu_cache_sequences,
+    pub query: u64,
+    pub out: u64,
+    pub sinks: u64,
+    pub scratch: u64,
+    pub scratch_bytes: u64,
+    pub heads: u32,
+    pub query_row_stride: u32,
+    pub query_head_stride: u32,
+    pub out_stride: u32,
+    pub window: u32,
+    pub keep_first: u32,
+    pub weight_rows: u32,
+    pub scale: f32,
+    pub softcap: f32,
+    pub data_type: u32,
+}
+
+/// 160 bytes
+#[repr(C)] #[derive(Default, Clone, Copy)]
+pub struct uzu_quantized_cache_evict_args {
+    pub cache: uzu_quantized_cache,
+    pub sequences: uzu_cache_sequences,
+    pub new_lengths: u64,
+    pub indices: u64,
+    pub scratch: u64,
+    pub scratch_bytes: u64,
+    pub budget: u32,
+    pub keep_first: u32,
+    pub keep_last: u32,
+    pub reserved0: u32,
+}
+
+/// 88 bytes
+#[repr(C)] #[derive(Default, Clone, Copy)]
+pub struct uzu_draft_verify_args {
+    pub target_logits: u64,
+    pub draft_logits: u64,
+    pub drafted: u64,
+    pub draft_counts: u64,
+    pub uniforms: u64,
+    pub tokens: u64,
+    pub accepted: u64,
+    pub sequences: u32,
+    pub drafts: u32,
+    pub vocab: u32,
+    pub target_stride: u32,
+    pub draft_stride: u32,
+    pub temperature: f32,
+    pub draft_temperature: f32,
+    pub data_type: u32,
+}
+
 /// 56 bytes
 #[repr(C)] #[derive(Default, Clone, Copy)]
 pub struct uzu_engine_options {
@@ -1178,6 +1294,13 @@ pub const STRUCT_SIZES: &[(&str, usize)] = &[
     ("uzu_state_space_scan_args", std::mem::size_of::<uzu_state_space_scan_args>()),
     ("uzu_state_space_step_args", std::mem::size_of::<uzu_state_space_step_args>()),
     ("uzu_expert_layer_args", std::mem::size_of::<uzu_expert_layer_args>()),
+    ("uzu_quantized_cache", std::mem::size_of::<uzu_quantized_cache>()),
+    ("uzu_cache_sequences", std::mem::size_of::<uzu_cache_sequences>()),
+    ("uzu_quantized_cache_append_args", std::mem::size_of::<uzu_quantized_cache_append_args>()),
+    ("uzu_quantized_cache_read_args", std::mem::size_of::<uzu_quantized_cache_read_args>()),
+    ("uzu_quantized_cache_attention_args", std::mem::size_of::<uzu_quantized_cache_attention_args>()),
+    ("uzu_quantized_cache_evict_args", std::mem::size_of::<uzu_quantized_cache_evict_args>()),
+    ("uzu_draft_verify_args", std::mem::size_of::<uzu_draft_verify_args>()),
     ("uzu_engine_options", std::mem::size_of::<uzu_engine_options>()),
     ("uzu_sampling_method", std::mem::size_of::<uzu_sampling_method>()),
     ("uzu_model_info", std::mem::size_of::<uzu_model_info>()),
@@ -1315,6 +1438,18 @@ extern "C" {
     pub fn uzu_expert_layer_encode(cmd: *mut uzu_command_buffer, args: *const uzu_expert_layer_args);
     pub fn uzu_expert_layer_validate(args: *const uzu_expert_layer_args) -> c_int;
     pub fn uzu_expert_layer_scratch_bytes(args: *const uzu_expert_layer_args) -> usize;
+    pub fn uzu_quantized_cache_append_encode(cmd: *mut uzu_command_buffer, args: *const uzu_quantized_cache_append_args);
+    pub fn uzu_quantized_cache_append_validate(args: *const uzu_quantized_cache_append_args) -> c_int;
+    pub fn uzu_quantized_cache_read_encode(cmd: *mut uzu_command_buffer, args: *const uzu_quantized_cache_read_args);
+    pub fn uzu_quantized_cache_read_validate(args: *const uzu_quantized_cache_read_args) -> c_int;
+    pub fn uzu_quantized_cache_attention_encode(cmd: *mut uzu_command_buffer, args: *const uzu_quantized_cache_attention_args);
+    pub fn uzu_quantized_cache_attention_validate(args: *const uzu_quantized_cache_attention_args) -> c_int;
+    pub fn uzu_quantized_cache_attention_scratch_bytes(ctx: *mut uzu_context, args: *const uzu_quantized_cache_attention_args) -> usize;
+    pub fn uzu_quantized_cache_evict_encode(cmd: *mut uzu_command_buffer, args: *const uzu_quantized_cache_evict_args);
+    pub fn uzu_quantized_cache_evict_validate(args: *const uzu_quantized_cache_evict_args) -> c_int;
+    pub fn uzu_quantized_cache_evict_scratch_bytes(ctx: *mut uzu_context, args: *const uzu_quantized_cache_evict_args) -> usize;
+    pub fn uzu_draft_verify_encode(cmd: *mut uzu_command_buffer, args: *const uzu_draft_verify_args);
+    pub fn uzu_draft_verify_validate(args: *const uzu_draft_verify_args) -> c_int;
     pub fn uzu_engine_create(ctx: *mut uzu_context, model_dir: *const c_char, opts: *const uzu_engine_options, out: *mut *mut uzu_engine) -> c_int;
     pub fn uzu_engine_destroy(e: *mut uzu_engine);
     pub fn uzu_engine_info(e: *const uzu_engine, out: *mut uzu_model_info) -> c_int;

@@ -18,6 +18,8 @@ u32, u64, f32 = C.c_uint32, C.c_uint64, C.c_float
 
 # enums (include/uzu_b200.h)
 DT_BF16, DT_F32, DT_F16 = 0, 1, 2
+CACHE_CODE_I8, CACHE_CODE_E4M3 = 0, 1
+NO_TOKEN = 0xFFFFFFFF
 QMODE_U4, QMODE_I8, QMODE_U8 = 0, 1, 2
 QMETHOD_SCALE_BIAS, QMETHOD_SCALE_ZERO_POINT, QMETHOD_SCALE_SYMMETRIC = 0, 1, 2
 B_FULL_PRECISION, B_SCALE_BIAS, B_SCALE_ZERO_POINT, B_SCALE_SYMMETRIC = 0, 1, 2, 3
@@ -286,7 +288,29 @@ ExpertLayerArgs = _struct("uzu_expert_layer_args", [
 
 MAIN_SLOT = 0xFFFFFFFF
 
-ABI_STRUCTS = [RowSequence, CausalConvArgs, StateSpaceScanArgs, StateSpaceStepArgs, ExpertLayerArgs, SideStepArgs, SideAttentionArgs, EmbeddingF32Args, GluArgs, StreamMixArgs, DeltaPrepareArgs, GatedDeltaArgs, GatedDeltaStepArgs, ExpGatesArgs, NormAddArgs, TokenGateArgs, MinGruArgs, RetentionArgs, WindowAttentionPrepareArgs, WindowAttentionArgs, TopkRouteArgs, RoutedCombineArgs, SigmoidAttentionPrepareArgs, SigmoidAttentionArgs, DenseLinearArgs, GroupRmsNormArgs, TableRouteArgs, GeneralDeltaArgs, HeadNormGateArgs, LatentPrepareArgs, LatentAttentionArgs,
+# A cache of 8 bits and the verification of drafted tokens. tables, lengths and row_offsets are u32 arrays in device memory
+QuantizedCache = _struct("uzu_quantized_cache", [
+    ("key_codes", u64), ("value_codes", u64), ("key_scales", u64), ("value_scales", u64), ("key_weights", u64), ("blocks", u32), ("kv_heads", u32),
+    ("block_tokens", u32), ("head_dim", u32), ("code_type", u32), ("reserved0", u32)])
+CacheSequences = _struct("uzu_cache_sequences", [
+    ("tables", u64), ("lengths", u64), ("row_offsets", u64), ("count", u32), ("table_stride", u32), ("rows", u32), ("max_rows", u32), ("max_length", u32), ("reserved0", u32)])
+QuantizedCacheAppendArgs = _struct("uzu_quantized_cache_append_args", [
+    ("cache", QuantizedCache), ("sequences", CacheSequences), ("keys", u64), ("values", u64), ("new_lengths", u64), ("key_stride", u32), ("value_stride", u32),
+    ("data_type", u32), ("reserved0", u32)])
+QuantizedCacheReadArgs = _struct("uzu_quantized_cache_read_args", [
+    ("cache", QuantizedCache), ("sequences", CacheSequences), ("keys", u64), ("values", u64), ("key_stride", u32), ("value_stride", u32), ("data_type", u32), ("reserved0", u32)])
+QuantizedCacheAttentionArgs = _struct("uzu_quantized_cache_attention_args", [
+    ("cache", QuantizedCache), ("sequences", CacheSequences), ("query", u64), ("out", u64), ("sinks", u64), ("scratch", u64), ("scratch_bytes", u64), ("heads", u32),
+    ("query_row_stride", u32), ("query_head_stride", u32), ("out_stride", u32), ("window", u32), ("keep_first", u32), ("weight_rows", u32), ("scale", f32), ("softcap", f32),
+    ("data_type", u32)])
+QuantizedCacheEvictArgs = _struct("uzu_quantized_cache_evict_args", [
+    ("cache", QuantizedCache), ("sequences", CacheSequences), ("new_lengths", u64), ("indices", u64), ("scratch", u64), ("scratch_bytes", u64), ("budget", u32),
+    ("keep_first", u32), ("keep_last", u32), ("reserved0", u32)])
+DraftVerifyArgs = _struct("uzu_draft_verify_args", [
+    ("target_logits", u64), ("draft_logits", u64), ("drafted", u64), ("draft_counts", u64), ("uniforms", u64), ("tokens", u64), ("accepted", u64), ("sequences", u32),
+    ("drafts", u32), ("vocab", u32), ("target_stride", u32), ("draft_stride", u32), ("temperature", f32), ("draft_temperature", f32), ("data_type", u32)])
+
+ABI_STRUCTS = [RowSequence, QuantizedCache, CacheSequences, QuantizedCacheAppendArgs, QuantizedCacheReadArgs, QuantizedCacheAttentionArgs, QuantizedCacheEvictArgs, DraftVerifyArgs, CausalConvArgs, StateSpaceScanArgs, StateSpaceStepArgs, ExpertLayerArgs, SideStepArgs, SideAttentionArgs, EmbeddingF32Args, GluArgs, StreamMixArgs, DeltaPrepareArgs, GatedDeltaArgs, GatedDeltaStepArgs, ExpGatesArgs, NormAddArgs, TokenGateArgs, MinGruArgs, RetentionArgs, WindowAttentionPrepareArgs, WindowAttentionArgs, TopkRouteArgs, RoutedCombineArgs, SigmoidAttentionPrepareArgs, SigmoidAttentionArgs, DenseLinearArgs, GroupRmsNormArgs, TableRouteArgs, GeneralDeltaArgs, HeadNormGateArgs, LatentPrepareArgs, LatentAttentionArgs,
                DeltaNetFusedUpdateArgs, QkNormConfig, AttentionPrepareNormArgs, FusedLinearArgs, RingParams, TrieNode, KvCopy, MatmulArgs, NormalizationArgs, QkvNormArgs, AttentionPrepareArgs, AttentionArgs,
                AttentionTwoPass2Args, KvCacheUpdateArgs, GatedActMulArgs, QuantizedEmbeddingLookupArgs, UnifiedSamplingArgs,
                DeltaNetConvUpdateArgs, DeltaNetUpdateArgs, EngineOptions, SamplingMethod, ModelInfo, TpAllGatherArgs]
@@ -323,7 +347,10 @@ uzu_min_gru_encode uzu_retention_encode uzu_window_attention_prepare_encode uzu_
 uzu_exp_gates_encode uzu_norm_add_encode uzu_token_gate_encode uzu_embedding_f32_scaled_encode uzu_rows_to_bf16_encode
 uzu_side_step_encode uzu_side_attention_encode uzu_embedding_f32_position_encode uzu_glu_encode uzu_stream_mix_encode uzu_delta_prepare_encode uzu_gated_delta_encode uzu_gated_delta_step_encode
 uzu_causal_conv_encode uzu_causal_conv_validate uzu_state_space_scan_encode uzu_state_space_scan_validate uzu_state_space_scan_scratch_bytes
-uzu_state_space_step_encode uzu_state_space_step_validate uzu_expert_layer_encode uzu_expert_layer_validate uzu_expert_layer_scratch_bytes""".split()
+uzu_state_space_step_encode uzu_state_space_step_validate uzu_expert_layer_encode uzu_expert_layer_validate uzu_expert_layer_scratch_bytes
+uzu_quantized_cache_append_encode uzu_quantized_cache_append_validate uzu_quantized_cache_read_encode uzu_quantized_cache_read_validate
+uzu_quantized_cache_attention_encode uzu_quantized_cache_attention_validate uzu_quantized_cache_attention_scratch_bytes
+uzu_quantized_cache_evict_encode uzu_quantized_cache_evict_validate uzu_quantized_cache_evict_scratch_bytes uzu_draft_verify_encode uzu_draft_verify_validate""".split()
 
 _lib = None
 
@@ -499,6 +526,18 @@ def load() -> C.CDLL:
         "uzu_expert_layer_encode": (None, [vp, C.POINTER(ExpertLayerArgs)]),
         "uzu_expert_layer_validate": (C.c_int, [C.POINTER(ExpertLayerArgs)]),
         "uzu_expert_layer_scratch_bytes": (C.c_size_t, [C.POINTER(ExpertLayerArgs)]),
+        "uzu_quantized_cache_append_encode": (None, [vp, C.POINTER(QuantizedCacheAppendArgs)]),
+        "uzu_quantized_cache_append_validate": (C.c_int, [C.POINTER(QuantizedCacheAppendArgs)]),
+        "uzu_quantized_cache_read_encode": (None, [vp, C.POINTER(QuantizedCacheReadArgs)]),
+        "uzu_quantized_cache_read_validate": (C.c_int, [C.POINTER(QuantizedCacheReadArgs)]),
+        "uzu_quantized_cache_attention_encode": (None, [vp, C.POINTER(QuantizedCacheAttentionArgs)]),
+        "uzu_quantized_cache_attention_validate": (C.c_int, [C.POINTER(QuantizedCacheAttentionArgs)]),
+        "uzu_quantized_cache_attention_scratch_bytes": (C.c_size_t, [vp, C.POINTER(QuantizedCacheAttentionArgs)]),
+        "uzu_quantized_cache_evict_encode": (None, [vp, C.POINTER(QuantizedCacheEvictArgs)]),
+        "uzu_quantized_cache_evict_validate": (C.c_int, [C.POINTER(QuantizedCacheEvictArgs)]),
+        "uzu_quantized_cache_evict_scratch_bytes": (C.c_size_t, [vp, C.POINTER(QuantizedCacheEvictArgs)]),
+        "uzu_draft_verify_encode": (None, [vp, C.POINTER(DraftVerifyArgs)]),
+        "uzu_draft_verify_validate": (C.c_int, [C.POINTER(DraftVerifyArgs)]),
         "uzu_token_gate_encode": (None, [vp, C.POINTER(TokenGateArgs)]),
         "uzu_rows_to_bf16_encode": (None, [vp, u64, u32, u64, u32, u32]),
         "uzu_embedding_f32_scaled_encode": (None, [vp, u64, u64, u32, u64, u32, u32, u32, f32]),

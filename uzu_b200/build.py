@@ -58,6 +58,10 @@ SOURCES = {
     "state_space.cu": [],
     "state_space_umma.cu": [],
     "expert_layer.cu": [],
+    "quantized_cache.cu": [],
+    "quantized_cache_attention.cu": [],
+    "quantized_cache_evict.cu": [],
+    "draft_verify.cu": [],
     "engine.cu": [],
 }
 

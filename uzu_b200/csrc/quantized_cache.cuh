@@ -1,0 +1,135 @@
+// What the kernels of the 8-bit cache share: its sequences as the device finds them, codes and scales, and the host's checks of the cache and its sequences.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "row_sequences.h"
+
+namespace uzu {
+
+// A number that is not below this makes its block and head not a number: code * scale stays finite for all others, and is a bf16 number.
+constexpr uint32_t kCacheHugeBits = 0x7b800000u;      // 2^120
+constexpr int kCacheLeastExponent = -100;
+constexpr uint32_t kNoIndex = 0xffffffffu;
+
+// tokens that a sequence can have: what the host bounds and its table holds
+inline uint32_t cache_capacity(const uzu_cache_sequences& s, uint32_t block_tokens) {
+    const uint64_t table = (uint64_t)s.table_stride * block_tokens;
+    return (uint32_t)(table < s.max_length ? table : s.max_length);
+}
+
+// null, or what is wrong
+inline const char* check_cache(const uzu_quantized_cache& c) {
+    if (c.code_type > UZU_CACHE_CODE_E4M3) return "code_type must be i8 or e4m3";
+    if (c.block_tokens != 16 && c.block_tokens != 32 && c.block_tokens != 64) return "block_tokens must be 16, 32 or 64";
+    if (c.head_dim == 0 || c.head_dim > 256 || c.head_dim % 16) return "head_dim must be a multiple of 16 up to 256";
+    if (c.kv_heads == 0 || c.kv_heads > 65535) return "kv_heads must be in 1 .. 65535";
+    if (!c.blocks) return "a cache without blocks";
+    if (!c.key_codes || !c.value_codes || !c.key_scales || !c.value_scales) return "null cache";
+    if ((c.key_codes | c.value_codes) % 16 || (c.key_scales | c.value_scales | c.key_weights) % 4) return "the cache is not aligned";
+    return nullptr;
+}
+inline const char* check_cache_sequences(const uzu_cache_sequences& s, bool with_rows) {
+    if (s.count > 65535) return "at most 65535 sequences";
+    if (s.max_length >> 31 || s.rows >> 31) return "max_length and rows are below 2^31";
+    if (!s.count) return nullptr;
+    if (!s.tables || !s.lengths || (with_rows && !s.row_offsets)) return "null sequences";
+    if ((s.tables | s.lengths | (with_rows ? s.row_offsets : 0)) % 4) return "the sequences are not aligned";
+    if (!s.table_stride || !s.max_length) return "table_stride and max_length are at least 1";
+    if ((uint64_t)s.table_stride * s.count >> 40) return "tables are too large";
+    return nullptr;
+}
+struct CacheSpan {
+    uint64_t at, bytes;
+};
+// whether [at, at + bytes) meets an array of the cache
+inline bool meets_cache(const uzu_quantized_cache& c, uint64_t at, uint64_t bytes) {
+    const uint64_t pairs = (uint64_t)c.blocks * c.kv_heads, codes = pairs * c.block_tokens * c.head_dim;
+    const CacheSpan spans[5] = {{c.key_codes, codes}, {c.value_codes, codes}, {c.key_scales, pairs * 4}, {c.value_scales, pairs * 4}, {c.key_weights, pairs * c.block_tokens * 4}};
+    for (const CacheSpan& s : spans)
+        if (bytes_overlap(at, bytes, s.at, s.bytes)) return true;
+    return false;
+}
+inline bool cache_meets_itself(const uzu_quantized_cache& c) {
+    const uint64_t pairs = (uint64_t)c.blocks * c.kv_heads, codes = pairs * c.block_tokens * c.head_dim;
+    const CacheSpan spans[5] = {{c.key_codes, codes}, {c.value_codes, codes}, {c.key_scales, pairs * 4}, {c.value_scales, pairs * 4}, {c.key_weights, pairs * c.block_tokens * 4}};
+    for (int i = 0; i < 5; ++i)
+        for (int j = 0; j < i; ++j)
+            if (bytes_overlap(spans[i].at, spans[i].bytes, spans[j].at, spans[j].bytes)) return true;
+    return false;
+}
+// whether a written array meets what says which sequences there are
+inline bool meets_sequences(const uzu_cache_sequences& s, uint64_t at, uint64_t bytes) {
+    return bytes_overlap(at, bytes, s.tables, (uint64_t)s.count * s.table_stride * 4) || bytes_overlap(at, bytes, s.lengths, (uint64_t)s.count * 4) ||
+           bytes_overlap(at, bytes, s.row_offsets, ((uint64_t)s.count + 1) * 4);
+}
+
+// attention of a prompt's rows on tcgen05 (quantized_cache_umma.cu); maxima and sums (f32 [rows, heads, 2], optional) are of every row
+bool quantized_cache_umma_applicable(const uzu_quantized_cache_attention_args& a);
+void encode_quantized_cache_umma(uzu_command_buffer* cmd, const uzu_quantized_cache_attention_args& a, uint64_t row_stats);
+
+#ifdef __CUDACC__
+struct CacheSequence {
+    uint32_t row, rows, length;      // first row, rows of the pass, tokens before it: whatever the device holds, inside the arrays
+};
+__device__ __forceinline__ CacheSequence cache_sequence(const uzu_cache_sequences& s, uint32_t capacity, uint32_t i) {
+    CacheSequence q;
+    q.length = min(reinterpret_cast<const uint32_t*>(s.lengths)[i], capacity);
+    const uint32_t *offsets = reinterpret_cast<const uint32_t*>(s.row_offsets), begin = min(offsets[i], s.rows), end = min(offsets[i + 1], s.rows);
+    q.row = begin;
+    q.rows = end > begin ? min(end - begin, s.max_rows) : 0u;
+    return q;
+}
+__device__ __forceinline__ uint32_t cache_block(const uzu_cache_sequences& s, uint32_t sequence, uint32_t nth) {      // (nth is below table_stride)
+    return reinterpret_cast<const uint32_t*>(s.tables)[(size_t)sequence * s.table_stride + nth];
+}
+
+// the smallest scale that brings magnitudes of up to `most` into the codes' range; NaN for what has none
+template <int CODE>
+__device__ __forceinline__ float cache_scale(uint32_t most_bits) {
+    if (most_bits >= kCacheHugeBits) return __uint_as_float(0x7fc00000u);
+    if (most_bits == 0) return 0.0f;
+    // 127 = 2^6 * (1 + 0x7e0000 / 2^23), 448 = 2^8 * (1 + 0x600000 / 2^23)
+    constexpr uint32_t top = CODE == UZU_CACHE_CODE_I8 ? 0x7e0000u : 0x600000u;
+    constexpr int power = CODE == UZU_CACHE_CODE_I8 ? 6 : 8;
+    const int e = (int)(most_bits >> 23) - 127 - power + ((most_bits & 0x7fffffu) > top ? 1 : 0);
+    return __uint_as_float((uint32_t)(max(e, kCacheLeastExponent) + 127) << 23);
+}
+// 1 / scale, exact; 0 for scales without codes (0, NaN)
+__device__ __forceinline__ float cache_inverse(float scale) { return scale > 0.0f ? __uint_as_float((254u << 23) - __float_as_uint(scale)) : 0.0f; }
+
+__device__ __forceinline__ uint32_t cache_pack_i8(float a, float b, float c, float d) {      // (already within +-127)
+    return ((uint32_t)__float2int_rn(a) & 0xffu) | ((uint32_t)__float2int_rn(b) & 0xffu) << 8 | ((uint32_t)__float2int_rn(c) & 0xffu) << 16 | (uint32_t)__float2int_rn(d) << 24;
+}
+__device__ __forceinline__ uint32_t cache_pack_e4m3(float a, float b, float c, float d) {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+    return (uint32_t)lo | (uint32_t)hi << 16;
+}
+template <int CODE>
+__device__ __forceinline__ uint32_t cache_pack(float a, float b, float c, float d) {
+    return CODE == UZU_CACHE_CODE_I8 ? cache_pack_i8(a, b, c, d) : cache_pack_e4m3(a, b, c, d);
+}
+// two codes (bytes of the low half) as f16 numbers, exact
+__device__ __forceinline__ uint32_t cache_e4m3x2_f16x2(uint32_t w) {
+    uint32_t r;
+    asm("{ .reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.rn.f16x2.e4m3x2 %0, lo; }" : "=r"(r) : "r"(w));
+    return r;
+}
+// four codes to numbers
+template <int CODE>
+__device__ __forceinline__ void cache_unpack(uint32_t w, float (&x)[4]) {
+    if (CODE == UZU_CACHE_CODE_I8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(w >> (8 * i));
+    } else {
+        const uint32_t lo = cache_e4m3x2_f16x2(w), hi = cache_e4m3x2_f16x2(w >> 16);
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+    }
+}
+#endif
+
+}  // namespace uzu

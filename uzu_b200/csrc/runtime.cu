@@ -107,6 +107,8 @@ size_t uzu_abi_struct_size(const char* name) {
     UZU_SZ(uzu_sigmoid_attention_prepare_args) UZU_SZ(uzu_sigmoid_attention_args)
     UZU_SZ(uzu_side_step_args) UZU_SZ(uzu_side_attention_args) UZU_SZ(uzu_embedding_f32_args) UZU_SZ(uzu_glu_args) UZU_SZ(uzu_stream_mix_args) UZU_SZ(uzu_delta_prepare_args) UZU_SZ(uzu_gated_delta_args) UZU_SZ(uzu_gated_delta_step_args)
     UZU_SZ(uzu_row_sequence) UZU_SZ(uzu_causal_conv_args) UZU_SZ(uzu_state_space_scan_args) UZU_SZ(uzu_state_space_step_args) UZU_SZ(uzu_expert_layer_args)
+    UZU_SZ(uzu_quantized_cache) UZU_SZ(uzu_cache_sequences) UZU_SZ(uzu_quantized_cache_append_args) UZU_SZ(uzu_quantized_cache_read_args) UZU_SZ(uzu_quantized_cache_attention_args)
+    UZU_SZ(uzu_quantized_cache_evict_args) UZU_SZ(uzu_draft_verify_args)
     UZU_SZ(uzu_exp_gates_args) UZU_SZ(uzu_norm_add_args) UZU_SZ(uzu_token_gate_args)
     UZU_SZ(uzu_min_gru_args) UZU_SZ(uzu_retention_args) UZU_SZ(uzu_window_attention_prepare_args) UZU_SZ(uzu_window_attention_args)
 #undef UZU_SZ
