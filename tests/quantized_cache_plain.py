@@ -8,7 +8,7 @@ from tests.state_space_plain import BF16, F16, F32, of_kept, to_kept  # noqa: F4
 I8, E4M3 = 0, 1
 LARGEST = {I8: 127.0, E4M3: 448.0}
 NO_INDEX = 0xFFFFFFFF
-HUGE = 2.0 ** 120
+HUGE = 2.0 ** 96
 
 
 def _e4m3_table():
@@ -106,8 +106,8 @@ class Cache:
                     self.weights[b, :, lo - first:hi - first] = 0
         return min(length + len(rows[0]), capacity)
 
-    def attend(self, table, length, q, capacity, scale, window=0, first=0, cap=0.0, sinks=None, weight_rows=0, q_error=0.0):
-        """q [rows, query heads, dim]. (out, bound of its error before the last rounding), and the same of what the weights of each key grow by: [tokens, heads]"""
+    def attend(self, table, length, q, capacity, scale, window=0, first=0, cap=0.0, sinks=None, weight_rows=0, q_error=0.0, tensor=False):
+        """q [rows, query heads, dim]; tensor: on tcgen05. (out, bound of its error before the last rounding), and the same of what the weights of each key grow by: [tokens, heads]"""
         n, hq, d = q.shape
         per = hq // self.heads
         end = min(length + n, capacity)
@@ -132,6 +132,7 @@ class Cache:
                 err = mag * ((d / 16 + 3) * 2.0 ** -22 + q_error)
                 if cap:
                     s = cap * np.tanh(s / cap)
+                    err = err + (cap * 2.0 ** -21 if tensor else 0.0)      # 1 - 2 / (1 + e^2x): roundings of numbers of up to 2
                 err = err + (np.abs(s) + np.abs(s).max()) * 2.0 ** -22
                 with np.errstate(invalid="ignore"):
                     top = s.max() if sinks is None else max(s.max(), sinks[h])
@@ -143,6 +144,8 @@ class Cache:
                     out[t, h] = w @ vv
                     # A small weight's second f16 part ends at the subnormal spacing: off by 2^-25 of what is at most 2^15 for the row's largest weight, 2^-40 of that one
                     bound[t, h] = (w * (part + (len(js) / 16 + 60) * 2.0 ** -23) + 2.0 ** -40 * w.max(initial=0)) @ np.abs(vv)
+                    # On tcgen05 a weight is one f16 number: half a step of 11 bits, and below the normal ones half of 2^-24, lifted by 2^7 and lowered by 2^8 at most
+                    bound[t, h] += ((w * 2.0 ** -12 + 2.0 ** -24 * w.max(initial=0)) @ np.abs(vv)) if tensor else 0.0
                 if t >= n - min(weight_rows, n):
                     grow[js, g] += w
                     grow_bound[js, g] += w * (part + (per * n + 4) * 2.0 ** -23)

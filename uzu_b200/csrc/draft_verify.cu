@@ -1,8 +1,10 @@
 // Verification of drafted tokens against the target's probabilities, and the token behind the kept ones.
 //
-// A cluster of CTAs has a sequence; a warp has the same run of the vocabulary in every row. One reading of all rows gives each row's maximum and sum (f32, sums of exponentials by
-// lane, in f64 from there on); the CTAs exchange them and all come to the same first refusal. Only the row that a token is drawn from is read again (it lies in L2), in f64, as is the
-// draft's: where a sum of weights passes its aim must not depend on f32 roundings. The sum of each warp's run, then the warp where the aim lies looks for the token.
+// A cluster of CTAs has a sequence; a warp has the same run of the vocabulary in every row, and asks for the next row's numbers before it sums up one's. One reading of all rows
+// gives each row's maximum and sum (f32 in a warp, f64 from there on); the CTAs exchange them and all come to the same first refusal. Only the row that a token is drawn from is read
+// again (it lies in L2), in f64, as is the draft's: where a sum of weights passes its aim must not depend on f32 roundings. One pass gives all its sums: which tokens have p > q is
+// known from the f32 sums but for those where both are alike to 2^-22 or so, which have next to no weight either way; so the weights of the others are summed before their
+// divisors are known, numerators and denominators by themselves. Then the warp's run where the sum passes the aim is looked through by its whole CTA.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -13,7 +15,7 @@ namespace uzu {
 
 namespace {
 
-constexpr uint32_t DV_THREADS = 512, DV_WARPS = DV_THREADS / 32, DV_CLUSTER = 8, DV_TILE = 256, DV_DRAFTS = 16, DV_ROWS = 2 * DV_DRAFTS + 1;
+constexpr uint32_t DV_TILE = 256, DV_GROUP = 4, DV_DRAFTS = 16, DV_ROWS = 2 * DV_DRAFTS + 1;
 
 constexpr float DV_COLDEST = 0x1p-60f;      // (1 / temperature stays a number)
 
@@ -22,6 +24,9 @@ struct DvParams {
     uint32_t tiles;      // of 256 tokens, of a warp
 };
 
+template <typename T> __device__ __forceinline__ T dv_nothing();
+template <> __device__ __forceinline__ __nv_bfloat16 dv_nothing() { return __ushort_as_bfloat16(0xff80u); }
+template <> __device__ __forceinline__ __half dv_nothing() { return __ushort_as_half(0xfc00u); }
 template <typename T> __device__ __forceinline__ float dv_f(T v);
 template <> __device__ __forceinline__ float dv_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <> __device__ __forceinline__ float dv_f(__half v) { return __half2float(v); }
@@ -29,47 +34,91 @@ template <> __device__ __forceinline__ float dv_f(float v) { return v; }
 
 // a lane's eight tokens of a tile; -infinity behind the last
 template <typename T, bool WIDE>
-__device__ __forceinline__ void dv_load(const T* row, uint32_t at, uint32_t vocab, float (&x)[8]) {
+__device__ __forceinline__ void dv_load(const T* row, uint32_t at, uint32_t vocab, T (&v)[8]) {
     if (WIDE && at + 8 <= vocab) {
-        alignas(16) T v[8];
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(v)[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(row + at) + 16 * i);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = dv_f(v[i]);
+        for (int i = 0; i < (int)(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(row + at)[i];
     } else {
+        T none;
+        if constexpr (sizeof(T) == 4) none = -INFINITY;
+        else none = dv_nothing<T>();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = at + i < vocab ? dv_f(row[at + i]) : -INFINITY;
+        for (int i = 0; i < 8; ++i) v[i] = at + i < vocab ? row[at + i] : none;
     }
 }
+
+__device__ __forceinline__ float dv_exp2(float x) {      // 2 ulp; what is below 2^-126 is zero
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 2^y for -1000 <= y <= 0, within 2^-37 of itself: the series of the exponential around the nearest power of two
+__device__ __forceinline__ double dv_power(double y) {
+    constexpr double magic = 6755399441055744.0;      // 1.5 * 2^52: a sum with it has the rounded integer in its low word
+    const double t = y + magic, f = y - (t - magic);
+    constexpr double l = 0.69314718055994530942;      // ln 2
+    constexpr double c2 = l * l / 2, c3 = c2 * l / 3, c4 = c3 * l / 4, c5 = c4 * l / 5, c6 = c5 * l / 6, c7 = c6 * l / 7, c8 = c7 * l / 8, c9 = c8 * l / 9;
+    double v = fma(c9, f, c8);
+    v = fma(v, f, c7);
+    v = fma(v, f, c6);
+    v = fma(v, f, c5);
+    v = fma(v, f, c4);
+    v = fma(v, f, c3);
+    v = fma(v, f, c2);
+    v = fma(v, f, l);
+    v = fma(v, f, 1.0);
+    return __hiloint2double(__double2hiint(v) + (__double2loint(t) << 20), __double2loint(v));
+}
+// weights exp((x - most) / temperature) of a row whose largest number is `most`
+struct DvHeat {
+    double k, b;      // x k + b: the exponent of 2
+    __device__ __forceinline__ DvHeat(float most, float temperature) : k(1.4426950408889634074 / (double)temperature), b(-(double)most * k) {}
+    __device__ __forceinline__ double operator()(float x) const {
+        const double y = fma((double)x, k, b);
+        return y >= -1000.0 ? dv_power(y) : 0.0;
+    }
+};
 
 struct DvRow {
     float most;          // NaN: no distribution
     uint32_t index;      // of the largest, the lowest of several
     double sum;          // of exp((x - most) / temperature)
 };
-struct DvShared {
-    DvRow part[DV_ROWS], row[DV_ROWS];      // this CTA's run; the whole vocabulary
-    float warp_most[DV_WARPS];
-    double warp_sum[DV_WARPS], cta_sum;
-    double sums[2];
-    uint32_t warp_index[DV_WARPS], accepted, token;
-};
-
 __device__ __forceinline__ double dv_warp_sum(double v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
+// parts of a row, one a lane (most = -infinity: nothing), to a whole one in all lanes; per: log2 e / temperature
+__device__ __forceinline__ DvRow dv_merge(DvRow m, float per) {
+    const float top = warp_max(m.most);
+    DvRow all;
+    all.most = top;
+    all.index = __reduce_min_sync(0xffffffffu, m.most == top ? m.index : UZU_NO_TOKEN);
+    // (a part of nothing but -infinity and NaN has a sum that is NaN; NaN stays NaN)
+    all.sum = dv_warp_sum(m.most == -INFINITY ? m.sum : m.most == top ? (top < INFINITY ? m.sum : m.sum * __longlong_as_double(0x7ff8000000000000ll)) : m.sum * (double)exp2f((m.most - top) * per));
+    return all;
+}
 
-template <typename T, bool WIDE>
-__global__ void __cluster_dims__(DV_CLUSTER, 1, 1) __launch_bounds__(DV_THREADS) draft_verify_kernel(const __grid_constant__ DvParams p) {
+template <uint32_t WARPS>
+struct DvShared {
+    DvRow part[DV_ROWS], row[DV_ROWS];      // this CTA's run; the whole vocabulary
+    float row_most[DV_ROWS][WARPS], row_sum[DV_ROWS][WARPS];
+    uint32_t row_index[DV_ROWS][WARPS];
+    double sums[4][WARPS], cta[4];
+    uint32_t accepted, token;
+};
+
+template <typename T, bool WIDE, uint32_t WARPS, uint32_t CLUSTER>
+__global__ void __launch_bounds__(WARPS * 32) draft_verify_kernel(const __grid_constant__ DvParams p) {
     namespace cg = cooperative_groups;
-    __shared__ DvShared s;
+    static_assert(WARPS <= 32 && CLUSTER <= 32, "a lane for each");
+    __shared__ DvShared<WARPS> s;
     cg::cluster_group cluster = cg::this_cluster();
     pdl_launch_dependents();
     pdl_wait();
     const uzu_draft_verify_args& a = p.a;
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, rank = cluster.block_rank(), sequence = blockIdx.x / DV_CLUSTER, k1 = a.drafts + 1, vocab = a.vocab;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, rank = cluster.block_rank(), sequence = blockIdx.x / CLUSTER, k1 = a.drafts + 1, vocab = a.vocab;
     const bool greedy = a.temperature == 0.0f, with_draft = a.draft_logits && !greedy;
     const uint32_t count = a.draft_counts ? min(reinterpret_cast<const uint32_t*>(a.draft_counts)[sequence], a.drafts) : a.drafts;
     const uint32_t rows = count + 1 + (with_draft ? count : 0u);      // targets, then drafts
@@ -79,79 +128,89 @@ __global__ void __cluster_dims__(DV_CLUSTER, 1, 1) __launch_bounds__(DV_THREADS)
         return r <= count ? reinterpret_cast<const T*>(a.target_logits) + ((size_t)sequence * k1 + r) * a.target_stride
                           : reinterpret_cast<const T*>(a.draft_logits) + ((size_t)sequence * a.drafts + (r - count - 1)) * a.draft_stride;
     };
-    const uint32_t first = (rank * DV_WARPS + warp) * p.tiles * DV_TILE;      // this warp's run of tokens (behind the last one there is none)
+    const uint32_t first = (rank * WARPS + warp) * p.tiles * DV_TILE;      // this warp's run of tokens (behind the last one there is none)
     const float per_target = greedy ? 1.0f : 1.4426950408889634f / a.temperature, per_draft = with_draft ? 1.4426950408889634f / a.draft_temperature : 1.0f;
 
-    // ---- maxima and sums of all rows ----
-    for (uint32_t r = 0; r < rows; ++r) {
-        const T* row = row_of(r);
-        const float per = r <= count ? per_target : per_draft;
-        float most = -INFINITY, sum = 0.0f;
-        uint32_t index = UZU_NO_TOKEN;
-        for (uint32_t t = 0; t < p.tiles; ++t) {
-            const uint32_t at = first + t * DV_TILE + lane * 8;
-            if (at >= vocab) break;
-            float x[8], m = -INFINITY;
-            dv_load<T, WIDE>(row, at, vocab, x);
+    // ---- maxima and sums of all rows, some tiles of a row at a time ----
+    {
+        const uint32_t groups = (p.tiles + DV_GROUP - 1) / DV_GROUP, all = rows * groups;
+        alignas(16) T next[DV_GROUP][8];
+        auto ask = [&](uint32_t r, uint32_t group) {
+            const T* row = row_of(r);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, x[i]);
+            for (uint32_t t = 0; t < DV_GROUP; ++t) {
+                const uint32_t tile = group * DV_GROUP + t;
+                dv_load<T, WIDE>(row, tile < p.tiles ? first + tile * DV_TILE + lane * 8 : vocab, vocab, next[t]);
+            }
+        };
+        ask(0, 0);
+        float most = -INFINITY, sum = 0.0f;
+        uint32_t index = UZU_NO_TOKEN, r = 0, group = 0;
+        for (uint32_t n = 0; n < all; ++n) {
+            alignas(16) T x[DV_GROUP][8];
+#pragma unroll
+            for (uint32_t t = 0; t < DV_GROUP; ++t)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[t][i] = next[t][i];
+            const uint32_t now = r, at = first + group * (DV_GROUP * DV_TILE) + lane * 8;
+            const bool last = ++group == groups;
+            if (last) {
+                group = 0;
+                ++r;
+            }
+            if (n + 1 < all) ask(r, group);
+            const float per = now <= count ? per_target : per_draft;
+            float m = -INFINITY;
+#pragma unroll
+            for (uint32_t t = 0; t < DV_GROUP; ++t)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) m = fmaxf(m, dv_f(x[t][i]));
             if (m > most) {
                 if (greedy) {
 #pragma unroll
-                    for (int i = 7; i >= 0; --i)
-                        if (x[i] == m) index = at + i;
+                    for (int t = DV_GROUP - 1; t >= 0; --t)
+#pragma unroll
+                        for (int i = 7; i >= 0; --i)
+                            if (dv_f(x[t][i]) == m) index = at + t * DV_TILE + i;
                 }
                 sum *= exp2f((most - m) * per);
                 most = m;
             }
             const float base = most == -INFINITY ? 0.0f : most;
-            float add = 0.0f;
+            float add[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) add += exp2f((x[i] - base) * per);
-            sum += add;
-        }
-        float top = warp_max(most);
-        double whole = dv_warp_sum(most == -INFINITY ? (double)sum : (double)sum * exp2f((most - top) * per));      // (a NaN among nothing else stays one)
-        if (greedy) {
-            uint32_t best = most == top ? index : UZU_NO_TOKEN;
-            best = __reduce_min_sync(0xffffffffu, best);
-            index = best;
-        }
-        if (lane == 0) {
-            s.warp_most[warp] = top;
-            s.warp_sum[warp] = whole;
-            s.warp_index[warp] = index;
+            for (uint32_t t = 0; t < DV_GROUP; ++t)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) add[i & 1] += dv_exp2((dv_f(x[t][i]) - base) * per);
+            sum += add[0] + add[1];
+            if (!last) continue;
+            const float top = warp_max(most);
+            sum = warp_sum(most == -INFINITY || most == top ? sum : sum * dv_exp2((most - top) * per));      // (a NaN among nothing else stays one)
+            if (greedy) index = __reduce_min_sync(0xffffffffu, most == top ? index : UZU_NO_TOKEN);
+            if (lane == 0) {
+                s.row_most[now][warp] = top;
+                s.row_sum[now][warp] = sum;
+                s.row_index[now][warp] = index;
+            }
+            most = -INFINITY;
+            sum = 0.0f;
+            index = UZU_NO_TOKEN;
         }
         __syncthreads();
-        if (tid == 0) {
+        for (uint32_t q = warp; q < rows; q += WARPS) {
             DvRow m{-INFINITY, UZU_NO_TOKEN, 0.0};
-            for (uint32_t w = 0; w < DV_WARPS; ++w)
-                if (s.warp_most[w] > m.most) {
-                    m.most = s.warp_most[w];
-                    m.index = s.warp_index[w];
-                }
-            for (uint32_t w = 0; w < DV_WARPS; ++w) m.sum += s.warp_most[w] == -INFINITY ? s.warp_sum[w] : s.warp_sum[w] * exp2((double)(s.warp_most[w] - m.most) * per);
-            s.part[r] = m;
+            if (lane < WARPS) m = DvRow{s.row_most[q][lane], s.row_index[q][lane], (double)s.row_sum[q][lane]};
+            m = dv_merge(m, q <= count ? per_target : per_draft);
+            if (lane == 0) s.part[q] = m;
         }
-        __syncthreads();
     }
     cluster.sync();
-    if (tid < rows) {
-        const float per = tid <= count ? per_target : per_draft;
+    for (uint32_t q = warp; q < rows; q += WARPS) {
         DvRow m{-INFINITY, UZU_NO_TOKEN, 0.0};
-        for (uint32_t c = 0; c < DV_CLUSTER; ++c) {
-            const DvRow& o = *cluster.map_shared_rank(&s.part[tid], c);
-            if (o.most > m.most) {
-                m.most = o.most;
-                m.index = o.index;
-            }
-        }
-        for (uint32_t c = 0; c < DV_CLUSTER; ++c) {
-            const DvRow& o = *cluster.map_shared_rank(&s.part[tid], c);
-            m.sum += o.most == -INFINITY ? o.sum : o.sum * exp2((double)(o.most - m.most) * per);
-        }
+        if (lane < CLUSTER) m = *cluster.map_shared_rank(&s.part[q], lane);
+        m = dv_merge(m, q <= count ? per_target : per_draft);
         if (!(m.most > -INFINITY && m.most < INFINITY) || !(m.sum < INFINITY)) m.most = __uint_as_float(0x7fc00000u);
-        s.row[tid] = m;
+        if (lane == 0) s.row[q] = m;
     }
     __syncthreads();
 
@@ -160,15 +219,15 @@ __global__ void __cluster_dims__(DV_CLUSTER, 1, 1) __launch_bounds__(DV_THREADS)
         bool kept = false;
         if (lane < count) {
             const uint32_t token = drafted[lane];
-            const DvRow &t = s.row[lane];
+            const DvRow& t = s.row[lane];
             if (token < vocab && t.most == t.most) {
                 if (greedy) kept = token == t.index;
                 else {
-                    const double pt = exp(((double)dv_f(row_of(lane)[token]) - t.most) / a.temperature) / t.sum;
+                    const double pt = DvHeat(t.most, a.temperature)(dv_f(row_of(lane)[token])) / t.sum;
                     double qt = 1.0;
                     if (with_draft) {
                         const DvRow& d = s.row[count + 1 + lane];
-                        qt = d.most == d.most ? exp(((double)dv_f(row_of(count + 1 + lane)[token]) - d.most) / a.draft_temperature) / d.sum : INFINITY;
+                        qt = d.most == d.most ? DvHeat(d.most, a.draft_temperature)(dv_f(row_of(count + 1 + lane)[token])) / d.sum : INFINITY;
                     }
                     kept = (double)uniforms[lane] * qt < pt;
                 }
@@ -181,154 +240,116 @@ __global__ void __cluster_dims__(DV_CLUSTER, 1, 1) __launch_bounds__(DV_THREADS)
     const uint32_t at_row = s.accepted;
     const DvRow target = s.row[at_row];
     const bool residual = at_row < count, against = residual && with_draft;
-    bool valid = target.most == target.most;
-    if (against) valid = valid && s.row[count + 1 + at_row].most == s.row[count + 1 + at_row].most;
-    uint32_t token = valid && greedy ? target.index : UZU_NO_TOKEN;
-
-    if (valid && !greedy) {
-        // ---- one row in f64 ----
-        const T *row = row_of(at_row), *draft = against ? row_of(count + 1 + at_row) : row;
-        const double top = target.most, draft_top = against ? s.row[count + 1 + at_row].most : 0.0, per = 1.0 / (double)a.temperature, draft_per = against ? 1.0 / (double)a.draft_temperature : 0.0;
-        const uint32_t without = residual && !with_draft ? drafted[at_row] : UZU_NO_TOKEN;      // a certain draft has all of q
-        // sums over the cluster, in the order of the vocabulary
-        auto over_cluster = [&](double mine) {
-            mine = dv_warp_sum(mine);
-            __syncthreads();
-            if (lane == 0) s.warp_sum[warp] = mine;
-            __syncthreads();
-            if (tid == 0) {
-                double v = 0.0;
-                for (uint32_t w = 0; w < DV_WARPS; ++w) v += s.warp_sum[w];
-                s.cta_sum = v;
-            }
-            cluster.sync();
-            double all = 0.0;
-            for (uint32_t c = 0; c < DV_CLUSTER; ++c) all += *cluster.map_shared_rank(&s.cta_sum, c);
-            return all;
-        };
-        double z = 1.0, draft_z = 1.0;
-        if (against) {
-            double sum = 0.0, draft_sum = 0.0;
-            for (uint32_t t = 0; t < p.tiles; ++t) {
-                const uint32_t at = first + t * DV_TILE + lane * 8;
-                if (at >= vocab) break;
-                float x[8], y[8];
-                dv_load<T, WIDE>(row, at, vocab, x);
-                dv_load<T, WIDE>(draft, at, vocab, y);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    sum += exp(((double)x[i] - top) * per);
-                    draft_sum += exp(((double)y[i] - draft_top) * draft_per);
-                }
-            }
-            z = over_cluster(sum);
-            cluster.sync();
-            draft_z = over_cluster(draft_sum);
-            cluster.sync();
-        }
-        bool plain = !against;      // weights are the target's alone
-        auto weight = [&](float x, float y, uint32_t i) {
-            if (i == without) return 0.0;
-            const double w = exp(((double)x - top) * per);
-            return plain ? w : fmax(w / z - exp(((double)y - draft_top) * draft_per) / draft_z, 0.0);
-        };
-        auto run = [&]() {
-            double sum = 0.0;
-            for (uint32_t t = 0; t < p.tiles; ++t) {
-                const uint32_t at = first + t * DV_TILE + lane * 8;
-                if (at >= vocab) break;
-                float x[8], y[8];
-                dv_load<T, WIDE>(row, at, vocab, x);
-                if (!plain) dv_load<T, WIDE>(draft, at, vocab, y);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sum += weight(x[i], plain ? 0.0f : y[i], at + i);
-            }
-            return sum;
-        };
-        double all = over_cluster(run());
-        if (!(all > 0.0)) {      // nothing is left of the difference: the target's own weights
-            cluster.sync();
-            plain = true;
-            all = over_cluster(run());
-        }
-        // the CTA, then the warp, where the sum passes the aim (or the last one with any weight)
-        const double aim = (double)uniforms[a.drafts] * all;
-        double before = 0.0, mine_before = 0.0;
-        uint32_t owner = 0;
-        bool passed = false;
-        for (uint32_t c = 0; c < DV_CLUSTER && !passed; ++c) {
-            const double v = *cluster.map_shared_rank(&s.cta_sum, c);
-            if (v > 0.0) {
-                owner = c;
-                mine_before = before;
-                passed = before + v > aim;
-            }
-            before += v;
-        }
-        if (owner == rank) {
-            uint32_t owner_warp = 0;
-            double at_warp = mine_before, sum = mine_before;
-            passed = false;
-            for (uint32_t w = 0; w < DV_WARPS && !passed; ++w) {
-                const double v = s.warp_sum[w];
-                if (v > 0.0) {
-                    owner_warp = w;
-                    at_warp = sum;
-                    passed = sum + v > aim;
-                }
-                sum += v;
-            }
-            if (warp == owner_warp) {
-                uint32_t last = UZU_NO_TOKEN, hit = UZU_NO_TOKEN;      // the last token with any weight, the one that passes
-                double sum = at_warp;
-                for (uint32_t t = 0; t < p.tiles && hit == UZU_NO_TOKEN; ++t) {
-                    const uint32_t at = first + t * DV_TILE + lane * 8;
-                    double w[8], mine = 0.0;
-                    float x[8], y[8];
-                    if (at < vocab) {
-                        dv_load<T, WIDE>(row, at, vocab, x);
-                        if (!plain) dv_load<T, WIDE>(draft, at, vocab, y);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        w[i] = at < vocab ? weight(x[i], plain ? 0.0f : y[i], at + i) : 0.0;
-                        mine += w[i];
-                    }
-                    double upto = mine;
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const double v = __shfl_up_sync(0xffffffffu, upto, o);
-                        if (lane >= (uint32_t)o) upto += v;
-                    }
-                    double at_lane = sum + (upto - mine);
-                    uint32_t found = UZU_NO_TOKEN, mine_last = 0;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        at_lane += w[i];
-                        if (w[i] > 0.0) {
-                            mine_last = at + i + 1;
-                            if (found == UZU_NO_TOKEN && at_lane > aim) found = at + i;
-                        }
-                    }
-                    hit = __reduce_min_sync(0xffffffffu, found);
-                    mine_last = __reduce_max_sync(0xffffffffu, mine_last);
-                    if (mine_last) last = mine_last - 1;
-                    sum += __shfl_sync(0xffffffffu, upto, 31);
-                }
-                if (lane == 0) s.token = hit != UZU_NO_TOKEN ? hit : last;
-            }
-            __syncthreads();
-            token = s.token;
-            if (tid < k1) reinterpret_cast<uint32_t*>(a.tokens)[(size_t)sequence * k1 + tid] = tid < at_row ? drafted[tid] : tid == at_row ? token : UZU_NO_TOKEN;
-            if (tid == 0) reinterpret_cast<uint32_t*>(a.accepted)[sequence] = at_row;
-        }
-        cluster.sync();      // (nobody leaves while its sums are read)
-        return;
-    }
-    if (rank == 0) {
+    const DvRow other = against ? s.row[count + 1 + at_row] : target;
+    const bool valid = target.most == target.most && other.most == other.most;
+    auto answer = [&](uint32_t token) {
         if (tid < k1) reinterpret_cast<uint32_t*>(a.tokens)[(size_t)sequence * k1 + tid] = tid < at_row ? drafted[tid] : tid == at_row ? token : UZU_NO_TOKEN;
         if (tid == 0) reinterpret_cast<uint32_t*>(a.accepted)[sequence] = at_row;
+    };
+    if (!valid || greedy) {      // (alike in all CTAs)
+        if (rank == 0) answer(valid ? target.index : UZU_NO_TOKEN);
+        cluster.sync();      // (nobody leaves while its parts are read)
+        return;
     }
-    cluster.sync();
+    // ---- one row in f64: sums of p's and q's weights, and of both where p is above q ----
+    const T *row = row_of(at_row), *draft = against ? row_of(count + 1 + at_row) : row;
+    const DvHeat heat(target.most, a.temperature), draft_heat(other.most, against ? a.draft_temperature : a.temperature);
+    const uint32_t without = residual && !with_draft ? drafted[at_row] : UZU_NO_TOKEN;      // a certain draft has all of q
+    {
+        double sum[4] = {0.0, 0.0, 0.0, 0.0};
+        for (uint32_t t = 0; t < p.tiles; ++t) {
+            const uint32_t at = first + t * DV_TILE + lane * 8;
+            if (at >= vocab) break;
+            alignas(16) T x[8], y[8];
+            dv_load<T, WIDE>(row, at, vocab, x);
+            if (against) dv_load<T, WIDE>(draft, at, vocab, y);
+#pragma unroll 4
+            for (int i = 0; i < 8; ++i) {
+                const double w = at + i == without ? 0.0 : heat(dv_f(x[i]));
+                sum[0] += w;
+                if (!against) continue;
+                const double v = draft_heat(dv_f(y[i]));
+                sum[1] += v;
+                if (w * other.sum > v * target.sum) {
+                    sum[2] += w;
+                    sum[3] += v;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i && !against) break;
+            sum[i] = dv_warp_sum(sum[i]);
+            if (lane == 0) s.sums[i][warp] = sum[i];
+        }
+        __syncthreads();
+        if (warp < 4 && (warp == 0 || against)) {
+            const double v = dv_warp_sum(lane < WARPS ? s.sums[warp][lane] : 0.0);
+            if (lane == 0) s.cta[warp] = v;
+        }
+        cluster.sync();
+    }
+    double parts[4] = {0.0, 0.0, 0.0, 0.0}, all[4] = {0.0, 0.0, 0.0, 0.0};      // of CTA `lane`, of the whole vocabulary
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (i && !against) break;
+        if (lane < CLUSTER) parts[i] = *cluster.map_shared_rank(&s.cta[i], lane);
+        all[i] = dv_warp_sum(parts[i]);
+    }
+    cluster.sync();      // (from here on nobody reads another CTA's shared memory)
+    const double inv = against ? 1.0 / all[0] : 1.0, draft_inv = against ? 1.0 / all[1] : 0.0;
+    double whole = against ? all[2] * inv - all[3] * draft_inv : all[0];
+    const bool plain = !against || !(whole > 0x1p-44);      // (nothing is left of the difference but roundings: the target's own weights)
+    if (plain) whole = all[0];
+    auto left = [&](double w, double w_over, double v_over) { return plain ? w : fmax(w_over * inv - v_over * draft_inv, 0.0); };
+    // the first of the lanes' parts, in their order, where the sum from `before` on passes the aim, else the last with any weight; before: the sum up to it
+    const double aim = (double)uniforms[a.drafts] * whole;
+    bool hit = false;
+    auto find = [&](double mine, double& before) {
+        double upto = mine;
+        for (int o = 1; o < 32; o <<= 1) {
+            const double v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= (uint32_t)o) upto += v;
+        }
+        const uint32_t some = __ballot_sync(0xffffffffu, mine > 0.0), passed = __ballot_sync(0xffffffffu, mine > 0.0 && before + upto > aim);
+        const uint32_t at = passed ? __ffs(passed) - 1 : some ? 31 - __clz(some) : 0;
+        before += __shfl_sync(0xffffffffu, upto - mine, at);
+        hit = passed != 0;
+        return at;
+    };
+    double before = 0.0;
+    const uint32_t owner = find(left(parts[0], parts[2], parts[3]), before);
+    if (owner != rank) return;
+    const uint32_t owner_warp = find(lane < WARPS ? left(s.sums[0][lane], against ? s.sums[2][lane] : 0.0, against ? s.sums[3][lane] : 0.0) : 0.0, before);
+    // its run by the whole CTA, a token a thread
+    const uint32_t run = (rank * WARPS + owner_warp) * p.tiles * DV_TILE, end = min(run + p.tiles * DV_TILE, vocab);
+    uint32_t token = UZU_NO_TOKEN;
+    for (uint32_t at0 = run; at0 < end; at0 += WARPS * 32) {
+        const uint32_t at = at0 + tid;
+        double w = 0.0;
+        if (at < end && at != without) {
+            w = heat(dv_f(row[at]));
+            if (!plain) w = fmax(w * inv - draft_heat(dv_f(draft[at])) * draft_inv, 0.0);
+        }
+        const double mine = dv_warp_sum(w);
+        __syncthreads();      // (the sums before are read)
+        if (lane == 0) s.sums[0][warp] = mine;
+        __syncthreads();
+        const double sums = lane < WARPS ? s.sums[0][lane] : 0.0, chunk = dv_warp_sum(sums);
+        if (!(chunk > 0.0)) continue;
+        double from = before;
+        const uint32_t in_warp = find(sums, from);
+        const bool last = hit;
+        if (warp == in_warp) {
+            const uint32_t l = find(w, from);
+            if (lane == 0) s.token = at0 + in_warp * 32 + l;
+        }
+        __syncthreads();
+        token = s.token;
+        if (last) break;
+        before += chunk;
+    }
+    answer(token);
 }
 
 const char* verify_check(const uzu_draft_verify_args* a) {
@@ -356,6 +377,38 @@ const char* verify_check(const uzu_draft_verify_args* a) {
     return nullptr;
 }
 
+template <typename F>
+void by_type(uint32_t data_type, F f) {
+    if (data_type == UZU_DT_F32) f(float());
+    else if (data_type == UZU_DT_F16) f(__half());
+    else f(__nv_bfloat16());
+}
+
+template <typename T, bool WIDE, uint32_t WARPS, uint32_t CLUSTER>
+void dv_launch(uzu_command_buffer* cmd, const uzu_draft_verify_args& a) {
+    DvParams p{};
+    p.a = a;
+    p.tiles = (a.vocab + CLUSTER * WARPS * DV_TILE - 1) / (CLUSTER * WARPS * DV_TILE);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(a.sequences * CLUSTER);
+    cfg.blockDim = dim3(WARPS * 32);
+    cfg.stream = cmd->ctx->stream;
+    cudaLaunchAttribute attr[2];
+    cfg.attrs = attr;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CLUSTER;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+    if (cmd->dependent()) {
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs = 2;
+    }
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, draft_verify_kernel<T, WIDE, WARPS, CLUSTER>, p);
+    if (e != cudaSuccess) cmd->record_error(UZU_ERROR_CUDA, std::string("draft_verify_kernel: ") + cudaGetErrorString(e));
+    cmd->launches++;
+}
+
 }  // namespace
 }  // namespace uzu
 
@@ -375,16 +428,15 @@ void uzu_draft_verify_encode(uzu_command_buffer* cmd, const uzu_draft_verify_arg
         return;
     }
     if (!a->sequences) return;
-    DvParams p{};
-    p.a = *a;
-    p.tiles = (a->vocab + DV_CLUSTER * DV_WARPS * DV_TILE - 1) / (DV_CLUSTER * DV_WARPS * DV_TILE);
     const uint64_t size = a->data_type == UZU_DT_F32 ? 4 : 2;
     const bool wide = ((a->target_logits | a->draft_logits) & 15u) == 0 && a->target_stride * size % 16 == 0 && (!a->draft_logits || a->draft_stride * size % 16 == 0);
-    const dim3 grid(a->sequences * DV_CLUSTER);
-    auto go = [&](auto kernel) { launch(cmd, "draft_verify_kernel", kernel, grid, dim3(DV_THREADS), 0, p); };
-    if (a->data_type == UZU_DT_F32) wide ? go(draft_verify_kernel<float, true>) : go(draft_verify_kernel<float, false>);
-    else if (a->data_type == UZU_DT_F16) wide ? go(draft_verify_kernel<__half, true>) : go(draft_verify_kernel<__half, false>);
-    else wide ? go(draft_verify_kernel<__nv_bfloat16, true>) : go(draft_verify_kernel<__nv_bfloat16, false>);
+    // few sequences: as many SMs a sequence as a cluster may have
+    const bool few = (uint64_t)a->sequences * 16 <= (uint64_t)cmd->ctx->sm_count;
+    by_type(a->data_type, [&](auto t) {
+        using T = decltype(t);
+        if (few) wide ? dv_launch<T, true, 16, 8>(cmd, *a) : dv_launch<T, false, 16, 8>(cmd, *a);
+        else wide ? dv_launch<T, true, 8, 8>(cmd, *a) : dv_launch<T, false, 8, 8>(cmd, *a);
+    });
 }
 
 }  // extern "C"
