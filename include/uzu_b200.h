@@ -1011,7 +1011,7 @@ UZU_API size_t uzu_expert_layer_scratch_bytes(const uzu_expert_layer_args* args)
  * Keys and values of served sequences in a pool of blocks of `block_tokens` tokens, a byte a number and one scale for each block and head; a number is
  * code * scale. Scales are powers of two, so that each such number is a bf16 number and a code does not depend on how a scale was computed: the smallest
  * 2^e, e >= -100, with which the block's largest magnitude is at most 127 (i8) or 448 (e4m3) scales; 0 where all are zeros. Codes are rounded to nearest,
- * ties to even. A number that is not finite, or of 2^120 and more, makes the scale of its block and head NaN, and with it every score or sum that reads
+ * ties to even. A number that is not finite, or of 2^96 and more, makes the scale of its block and head NaN, and with it every score or sum that reads
  * them, until the block is begun again. Codes that do not come from these entries are finite ones (no e4m3 code 0x7f or 0xff in a token that a sequence has).
  * Which sequences a pass has is read on the device, so a captured call follows it: their block numbers, how many tokens they have, where their rows are.
  * Token j of sequence i is at tables[i, j / block_tokens]. A block number that is not below `blocks` is no block: its tokens are seen by nobody and rows
@@ -1070,7 +1070,9 @@ UZU_API uzu_status uzu_quantized_cache_read_validate(const uzu_quantized_cache_r
  *   out[t, h, :] = sum_j w_j value_j      (zeros for a row that sees nothing)
  *   weight_rows > 0: key_weights[j, g] += sum of w_j over the last weight_rows rows of a sequence and the heads of group g (0xffffffff: all its rows)
  * A query that is not finite makes its row NaN. Scores, weights and sums are f32. bf16 and f16 queries enter the products as they are, f32 ones as two f16
- * parts (22 bits, relative to the row's largest); weights as two f16 parts (22 bits), or of bf16 prompts on tcgen05 (csrc/quantized_cache_umma.cu) two bf16 parts.
+ * parts (22 bits, relative to the row's largest); weights as two f16 parts (22 bits, or within 2^-40 of the row's largest weight). A sequence's
+ * bf16 rows of up to 128 channels run on tcgen05 (csrc/quantized_cache_umma.cu) where they are more than 64 pairs of a row and a head of a key head's group, scale is above 0 and
+ * query and out are whole 16-byte groups: weights are one f16 number there (11 bits, or within 2^-24 of the row's largest).
  * Sums run in an order that the shapes, the lengths and max_length set.
  * scratch: of uzu_quantized_cache_attention_scratch_bytes() bytes, 256-byte aligned, its first 64 KB zero before the first use; every call leaves it ready for the next,
  * of any sizes. Calls that may run at the same time do not share it. */

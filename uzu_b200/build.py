@@ -60,6 +60,7 @@ SOURCES = {
     "expert_layer.cu": [],
     "quantized_cache.cu": [],
     "quantized_cache_attention.cu": [],
+    "quantized_cache_umma.cu": [],
     "quantized_cache_evict.cu": [],
     "draft_verify.cu": [],
     "engine.cu": [],

@@ -8,10 +8,11 @@
 
 namespace uzu {
 
-// A number that is not below this makes its block and head not a number: code * scale stays finite for all others, and is a bf16 number.
-constexpr uint32_t kCacheHugeBits = 0x7b800000u;      // 2^120
+// A number that is not below this makes its block and head not a number: code * scale stays finite for all others, and is a bf16 number, and so do sums over many tokens.
+constexpr uint32_t kCacheHugeBits = 0x6f800000u;      // 2^96
 constexpr int kCacheLeastExponent = -100;
 constexpr uint32_t kNoIndex = 0xffffffffu;
+constexpr uint32_t kCacheFewPairs = 64;      // (row, head) pairs of a sequence and a key head that the kernel for few rows takes where the tcgen05 kernel takes the others
 
 // tokens that a sequence can have: what the host bounds and its table holds
 inline uint32_t cache_capacity(const uzu_cache_sequences& s, uint32_t block_tokens) {

@@ -1,10 +1,12 @@
 // Attention of a few rows over the 8-bit cache, and the sums of attention weight for each of its tokens.
 //
-// A CTA has 16 (row, head) pairs of a key head and a part of the keys they see; its four warps take 16 keys at a time, in turns. Bytes go by cp.async into a ring that each lane
-// keeps for itself (it reads what it copied, so a step needs no barrier) and become f16 numbers in registers, exactly; products run on mma.sync m16n8k16 with the pairs as rows:
+// A CTA has 8 or more (row, head) pairs of a key head and a part of the keys they see; each of its four warps takes a run of them, 32 keys at a time. Bytes go by cp.async into a
+// ring that each lane keeps for itself (it reads what it copied, so a step needs no barrier) and become f16 numbers in registers, exactly. Products run on mma.sync m16n8k16 with the
+// keys as rows, then the channels, and the pairs as columns, eight a product, so that few pairs waste little:
 //   scores  a lane copies 16 codes in a row of a key, which are its four channels of four products; the order of channels within a sum is free as long as the query has the same;
-//   output  a lane copies a row of codes of four keys, the keys of its own weights, and pairs them by bytes: the column of a product is any channel.
-// So no code is exchanged and nothing is converted twice. A step's products start from zero and are added to the f32 sums times the block's scale; scales of keys multiply scores.
+//   output  a lane copies a row of codes of four keys, the keys of its own weights, and pairs them by bytes: the row of a product is any channel.
+// So no code is exchanged and nothing is converted twice; weights are turned by movmatrix. Products of bf16 and f16 rows are added up by the tensor cores in units of the block's value
+// scale, and rescaled where it changes; scales of keys multiply scores.
 // Queries are brought to 2^14 .. 2^15 by a power of two for each row, which is exact; f32 ones are two f16 parts. A weight, up to 2^15, is two f16 parts: with one, every
 // eighth bf16 result or so would be the neighbour of the right one.
 #include "quantized_cache.cuh"
@@ -13,22 +15,29 @@ namespace uzu {
 
 namespace {
 
-constexpr uint32_t QA_WARPS = 4, QA_THREADS = QA_WARPS * 32, QA_ROWS = 16, QA_STEP = 16;
+constexpr uint32_t QA_WARPS = 4, QA_THREADS = QA_WARPS * 32, QA_STEP = 32, QA_HALF = 16;      // keys of a step, which is two halves with blocks and scales of their own
+constexpr uint32_t QA_SUM = 256;
+constexpr uint64_t QA_SCORES = 256u << 20;      // bytes of scores that are kept at most
 constexpr uint32_t QA_TICKETS = 16384;      // words at the start of the scratch
 constexpr float QA_LIFT = 15.0f;            // weights are relative to 2^-15 of the largest so far: 22 bits down to 2^-29 of it, and off by 2^-40 of it at most below that
 
 struct QaParams {
     uzu_quantized_cache_attention_args a;
-    uint32_t capacity, group, tiles, splits;
+    uint32_t capacity, group, tiles, splits, shift, few;      // shift: log2 of a block's tokens; few: sequences with more pairs than that are another kernel's
     uint32_t* tickets;
     float *partials, *stats;      // stats: of every row and head, the largest score (in units of ln 2) and what a weight is multiplied by; null: not asked for
+    float* scores;                // of the sequences of few pairs: [sequence, key head, pair, score_stride]; null: not kept
+    uint32_t score_stride, score_pairs, tile_rows;
 };
 
-template <int DP>
+// DP: channels a head has at most; NT: eights of pairs
+template <int DP, int NT>
 struct QaShape {
-    static constexpr uint32_t STEP_BYTES = 32 * DP, STAGE = STEP_BYTES + 128, STAGES = DP == 256 ? 3 : 4, RING = QA_WARPS * STAGES * STAGE;
+    static constexpr uint32_t HALF_BYTES = 32 * DP, STEP_BYTES = 2 * HALF_BYTES, STAGE = STEP_BYTES + 128, STAGES = DP == 64 ? 3 : 2, RING = QA_WARPS * STAGES * STAGE;
     static constexpr uint32_t K_LOADS = DP / 32, V_UNIT = DP == 64 ? 8 : 16, V_UNITS = DP == 64 ? 1 : DP / 128;
-    static constexpr uint32_t QUERY = DP / 16 * 512;      // one part's fragments
+    static constexpr uint32_t ROWS = 8 * NT, QUERY = NT * DP / 16 * 256;      // one part's fragments
+    static constexpr uint32_t CTAS = DP == 256 ? 1 : 3;                       // of an SM
+    static constexpr bool KEPT = NT * DP <= 128;                              // the queries' fragments stay in registers (of one part)
 };
 
 __device__ __forceinline__ uint32_t qa_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -41,18 +50,11 @@ __device__ __forceinline__ void qa_copy8(uint32_t to, const void* from, bool the
 __device__ __forceinline__ void qa_copy4(uint32_t to, const void* from) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory"); }
 __device__ __forceinline__ void qa_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void qa_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ uint4 qa_lds16(uint32_t at) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint2 qa_lds8(uint32_t at) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
-    return v;
-}
+extern __shared__ __align__(128) uint8_t qa_raw[];
+__device__ __forceinline__ uint4 qa_lds16(uint32_t offset) { return *reinterpret_cast<const uint4*>(qa_raw + offset); }      // (of the dynamic shared memory)
+__device__ __forceinline__ uint2 qa_lds8(uint32_t offset) { return *reinterpret_cast<const uint2*>(qa_raw + offset); }
 __device__ __forceinline__ void qa_mma(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
@@ -60,6 +62,11 @@ __device__ __forceinline__ float qa_exp2(float x) {      // 2 ulp; weights below
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ uint32_t qa_turn(uint32_t v) {      // an 8 x 8 tile of f16 numbers
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
 }
 __device__ __forceinline__ uint32_t qa_pack(float a, float b) {
     const __half2 v = __floats2half2_rn(a, b);
@@ -85,9 +92,9 @@ __device__ __forceinline__ void qa_pairs(uint32_t w, uint32_t& lo, uint32_t& hi)
     }
 }
 
-// Steps of 16 keys that rows of tokens [first, last] of a sequence can see: the first kept ones, then the window's.
+// Steps of 32 keys that rows of tokens [first, last] of a sequence can see: the first kept ones, then the window's.
 struct QaSteps {
-    uint32_t kept, begin, steps, end;      // steps of first keys, the window's first key (a multiple of 16), all steps, one behind the last key
+    uint32_t kept, begin, steps, end;      // steps of first keys, the window's first key (a multiple of 32), all steps, one behind the last key
     __device__ __forceinline__ QaSteps(uint32_t first, uint32_t last, uint32_t window, uint32_t keep_first, uint32_t capacity) {
         end = min(last + 1u, capacity);
         begin = window && first >= window ? (first - window + 1u) & ~(QA_STEP - 1u) : 0u;
@@ -101,56 +108,75 @@ struct QaSteps {
     __device__ __forceinline__ uint32_t key(uint32_t step) const { return step < kept ? step * QA_STEP : begin + (step - kept) * QA_STEP; }
 };
 
-// The queries of a tile of 16 pairs as fragments of operand A, in shared memory: part, product, lane. Pair r is row r / group, head r % group of the key head.
-// factor[r]: what a sum of products is multiplied by (but for the block's scale) to become a score in units of ln 2, or a fraction of the cap.
-template <typename T, int DP>
-__device__ __forceinline__ void qa_query(const QaParams& p, const CacheSequence& q, uint32_t head0, uint32_t pair0, uint32_t pairs, uint32_t at, float* factor) {
+template <typename T>
+__device__ __forceinline__ float qa_number(T v, bool f16) {
+    if constexpr (sizeof(T) == 4) return v;
+    else return f16 ? __half2float(__ushort_as_half(v)) : __uint_as_float((uint32_t)v << 16);
+}
+// The queries of a tile of pairs as fragments of operand B, in shared memory: part, eight of pairs, product, lane. Pair r is row r / group, head r % group of the key head.
+// factor[r]: what a sum of products is multiplied by (but for the block's scale) to become a score in units of ln 2, or a fraction of the cap. By all threads, with barriers.
+template <typename T, int DP, int NT>
+__device__ __forceinline__ void qa_query(const QaParams& p, const CacheSequence& q, uint32_t head0, uint32_t pair0, uint32_t pairs, uint32_t at, float* factor, uint32_t* most_of) {
+    using S = QaShape<DP, NT>;
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
+    constexpr uint32_t UNITS = NT * DP / 64, EACH = (UNITS + QA_WARPS - 1) / QA_WARPS;      // of 8 pairs and 64 channels, a warp's
     const uzu_quantized_cache_attention_args& a = p.a;
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3u, dim = a.cache.head_dim;
-    if (warp >= 2) return;      // warp 0: rows 0 .. 7, warp 1: rows 8 .. 15
-    const uint32_t row = g + 8 * warp, r = pair0 + row;
-    const T* from = reinterpret_cast<const T*>(a.query);
-    const bool there = r < pairs;
-    if (there) from += (size_t)(q.row + r / p.group) * a.query_row_stride + (size_t)(head0 + r % p.group) * a.query_head_stride;
-    uint32_t most = 0;
-    for (uint32_t s = 0; s < DP / 64; ++s) {
-        const uint32_t d0 = s * 64 + c * 16;
-        if (there && d0 < dim)
-            for (uint32_t j = 0; j < 16; ++j) {
-                const float v = sizeof(T) == 4 ? *reinterpret_cast<const float*>(from + d0 + j) : sizeof(T) == 2 && a.data_type == UZU_DT_F16 ? __half2float(reinterpret_cast<const __half*>(from)[d0 + j]) : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(from)[d0 + j]);
-                most = max(most, __float_as_uint(v) & 0x7fffffffu);
-            }
+    const bool f16 = a.data_type == UZU_DT_F16, wide = ((a.query | (uint64_t)a.query_row_stride * sizeof(T) | (uint64_t)a.query_head_stride * sizeof(T)) & 15u) == 0;
+    if (threadIdx.x < S::ROWS) most_of[threadIdx.x] = 0;
+    __syncthreads();
+    alignas(16) T x[EACH][16];
+#pragma unroll
+    for (uint32_t e = 0; e < EACH; ++e) {
+        const uint32_t u = warp + e * QA_WARPS, r = pair0 + u % NT * 8 + g, d0 = u / NT * 64 + c * 16;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[e][j] = 0;
+        if (u >= UNITS || r >= pairs || d0 >= dim) continue;
+        const T* from = reinterpret_cast<const T*>(a.query) + (size_t)(q.row + r / p.group) * a.query_row_stride + (size_t)(head0 + r % p.group) * a.query_head_stride + d0;
+        if (wide) {
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(T); ++j) reinterpret_cast<uint4*>(x[e])[j] = reinterpret_cast<const uint4*>(from)[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[e][j] = from[j];
+        }
     }
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    const int e = most ? max(-100, min(100, 14 + 127 - (int)(most >> 23))) : 0;
-    const float up = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
-    if (c == 0) factor[row] = most >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : a.softcap > 0.0f ? a.scale / a.softcap * down : a.scale * 1.4426950408889634f * down;
-    for (uint32_t s = 0; s < DP / 64; ++s) {
-        const uint32_t d0 = s * 64 + c * 16;
-        for (uint32_t k = 0; k < 4; ++k) {
-            float x[4];
-            for (uint32_t j = 0; j < 4; ++j) {
-                x[j] = 0.0f;
-                if (there && d0 < dim) {
-                    const uint32_t i = d0 + 4 * k + j;
-                    x[j] = up * (sizeof(T) == 4 ? *reinterpret_cast<const float*>(from + i) : sizeof(T) == 2 && a.data_type == UZU_DT_F16 ? __half2float(reinterpret_cast<const __half*>(from)[i]) : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(from)[i]));
-                }
-            }
+#pragma unroll
+    for (uint32_t e = 0; e < EACH; ++e) {
+        const uint32_t u = warp + e * QA_WARPS;
+        uint32_t most = 0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) most = max(most, __float_as_uint(qa_number(x[e][j], f16)) & 0x7fffffffu);
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        if (u < UNITS && c == 0) atomicMax(&most_of[u % NT * 8 + g], most);
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t e = 0; e < EACH; ++e) {
+        const uint32_t u = warp + e * QA_WARPS, n = u % NT, s = u / NT;
+        if (u >= UNITS) continue;
+        const uint32_t most = most_of[n * 8 + g];
+        const int power = most ? max(-100, min(100, 14 + 127 - (int)(most >> 23))) : 0;
+        const float up = __uint_as_float((uint32_t)(power + 127) << 23), down = __uint_as_float((uint32_t)(127 - power) << 23);
+        if (s == 0 && c == 0) factor[n * 8 + g] = most >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : a.softcap > 0.0f ? a.scale / a.softcap * down : a.scale * 1.4426950408889634f * down;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = up * qa_number(x[e][4 * k + j], f16);
+#pragma unroll
             for (int part = 0; part < PARTS; ++part) {
-                const uint32_t lo = qa_pack(x[0], x[1]), hi = qa_pack(x[2], x[3]);
-                // fragment words: 0 row g first pair, 1 row g + 8 first pair, 2 row g second pair, 3 row g + 8 second pair
-                const uint32_t to = at + part * QaShape<DP>::QUERY + (s * 4 + k) * 512 + lane * 16 + warp * 4;
-                asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"(lo) : "memory");
-                asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + 8), "r"(hi) : "memory");
+                const uint32_t lo = qa_pack(y[0], y[1]), hi = qa_pack(y[2], y[3]);
+                *reinterpret_cast<uint2*>(qa_raw + at + part * S::QUERY + ((n * (DP / 16) + s * 4 + k) * 32 + lane) * 8) = make_uint2(lo, hi);
                 if (part + 1 < PARTS) {
                     const float2 l = qa_unpack(lo), h = qa_unpack(hi);
-                    x[0] -= l.x; x[1] -= l.y; x[2] -= h.x; x[3] -= h.y;
+                    y[0] -= l.x; y[1] -= l.y; y[2] -= h.x; y[3] -= h.y;
                 }
             }
         }
     }
+    __syncthreads();
 }
 
 // what a row of this lane sees
@@ -162,224 +188,336 @@ struct QaRow {
     }
 };
 
-// A score from a sum of products
-__device__ __forceinline__ float qa_score(float sum, float factor, float cap) {
-    const float x = sum * factor;
-    return cap > 0.0f ? cap * 1.4426950408889634f * tanhf(x) : x;
+// the queries' fragments, from shared memory or, once read, from registers
+template <int DP, int NT, int PARTS, bool KEPT>
+struct QaQuery {
+    using S = QaShape<DP, NT>;
+    uint2 kept[KEPT ? NT * DP / 16 : 1];
+    uint32_t at;
+    __device__ __forceinline__ QaQuery(uint32_t query, uint32_t lane) : at(query + lane * 8) {
+        if (KEPT) {
+#pragma unroll
+            for (int i = 0; i < NT * DP / 16; ++i) kept[i] = qa_lds8(at + i * 256);
+        }
+    }
+    __device__ __forceinline__ uint2 get(int part, int i) const { return KEPT && part == 0 ? kept[i] : qa_lds8(at + part * S::QUERY + i * 256); }
+};
+// Scores of 16 keys (rows g, g + 8) and pairs 2 quad, + 1 of each eight, in units of ln 2 (or, with a cap, behind it); word(n): the lane's codes, of both keys by turns
+template <int CODE, int DP, int NT, int PARTS, typename Query, typename Word>
+__device__ __forceinline__ void qa_scores(const Query& query, Word word, const float (&factor)[NT][2], float key_scale, float softcap, float (&s)[NT][4]) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
+#pragma unroll
+    for (int b = 0; b < DP / 64; ++b) {
+        const uint4 w[2] = {word(2 * b), word(2 * b + 1)};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            uint4 f;      // a key's channels: row g, row g + 8, then the second two channels of each
+            qa_pairs<CODE>(reinterpret_cast<const uint32_t*>(&w[0])[k], f.x, f.z);
+            qa_pairs<CODE>(reinterpret_cast<const uint32_t*>(&w[1])[k], f.y, f.w);
+#pragma unroll
+            for (int part = PARTS - 1; part >= 0; --part)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint2 x = query.get(part, n * (DP / 16) + b * 4 + k);
+                    qa_mma(s[n], f, x.x, x.y);
+                }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const float times[2] = {factor[n][0] * key_scale, factor[n][1] * key_scale};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] *= times[i & 1];
+    }
+    if (softcap > 0.0f) {
+        const float cap = softcap * 1.4426950408889634f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[n][i] = cap * tanhf(s[n][i]);
+    }
 }
 
-template <typename T, int CODE, int DP>
-__global__ void __launch_bounds__(QA_THREADS) quantized_cache_attention_kernel(const __grid_constant__ QaParams p) {
-    using S = QaShape<DP>;
+template <typename T, int CODE, int DP, int NT>
+__global__ void __launch_bounds__(QA_THREADS, QaShape<DP, NT>::CTAS) quantized_cache_attention_kernel(const __grid_constant__ QaParams p) {
+    using S = QaShape<DP, NT>;
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
-    extern __shared__ __align__(128) uint8_t qa_raw[];
-    __shared__ float factors[QA_ROWS], tops[QA_WARPS][QA_ROWS], sums[QA_WARPS][QA_ROWS];
-    __shared__ uint32_t last_of_all;
+    constexpr uint32_t ROWS = S::ROWS;
+    __shared__ float factors[ROWS], tops[QA_WARPS][ROWS], sums[QA_WARPS][ROWS];
+    __shared__ uint32_t mosts[ROWS], last_of_all;
     const uzu_quantized_cache_attention_args& a = p.a;
     const uzu_quantized_cache& c = a.cache;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, quad = lane & 3u;
-    const uint32_t ring = qa_smem(qa_raw) + warp * S::STAGES * S::STAGE, query = qa_smem(qa_raw) + S::RING;
+    const uint32_t ring = warp * S::STAGES * S::STAGE, query = S::RING, raw = qa_smem(qa_raw);
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t sequence = blockIdx.z, head = blockIdx.y, split = blockIdx.x % p.splits, tile = blockIdx.x / p.splits;
     const CacheSequence q = cache_sequence(a.sequences, p.capacity, sequence);
-    const uint32_t pairs = q.rows * p.group, pair0 = tile * QA_ROWS;
-    if (pair0 >= pairs) return;
+    const uint32_t pairs = q.rows * p.group, pair0 = tile * ROWS;
+    if (pair0 >= pairs || pairs > p.few) return;
     const uint32_t dim = c.head_dim, bt = c.block_tokens;
-    const uint32_t token0 = q.length + pair0 / p.group, token1 = q.length + min(pair0 + QA_ROWS - 1u, pairs - 1u) / p.group;
+    const uint32_t token0 = q.length + pair0 / p.group, token1 = q.length + min(pair0 + ROWS - 1u, pairs - 1u) / p.group;
     const QaSteps steps(token0, token1, a.window, a.keep_first, p.capacity);
-    const uint32_t from = (uint32_t)((uint64_t)steps.steps * split / p.splits), to = (uint32_t)((uint64_t)steps.steps * (split + 1) / p.splits);
+    // this warp's run of steps: neighbours share a block's scales
+    const uint32_t part = split * QA_WARPS + warp, parts = p.splits * QA_WARPS;
+    const uint32_t from = (uint32_t)((uint64_t)steps.steps * part / parts), to = (uint32_t)((uint64_t)steps.steps * (part + 1) / parts);
 
     const uint32_t* table = reinterpret_cast<const uint32_t*>(a.sequences.tables) + (size_t)sequence * a.sequences.table_stride;
+    // (the blocks of the next step to be copied are asked for a step ahead: of halves 0 and 1, the same one where blocks have 32 tokens)
+    uint32_t next_block[2];
+    auto ask = [&](uint32_t step) {
+        if (step >= to) return;
+        const uint32_t key = steps.key(step);
+        next_block[0] = table[key >> p.shift];
+        next_block[1] = p.shift > 4 ? next_block[0] : key + QA_HALF < steps.end ? table[(key + QA_HALF) >> p.shift] : 0xffffffffu;
+    };
+    ask(from);
+    const uint32_t k_lane = g * dim + quad * 16, v_lane = quad * 2 * dim + g * S::V_UNIT, k_to = lane * 16, v_to = 16 * DP + lane * S::V_UNIT;
+    const uint8_t *const all_keys = reinterpret_cast<const uint8_t*>(c.key_codes), *const all_values = reinterpret_cast<const uint8_t*>(c.value_codes);
+    const float* const all_scales = reinterpret_cast<const float*>(lane & 1u ? c.value_scales : c.key_scales);
     auto copy = [&](uint32_t step, uint32_t slot) {
         if (step < to) {
-            const uint32_t key0 = steps.key(step), block = table[key0 / bt], at = ring + slot * S::STAGE;
-            const bool there = block < c.blocks;
-            const size_t pair = (size_t)(there ? block : 0u) * c.kv_heads + head;
-            const uint32_t in_block = key0 % bt, left = steps.end - key0;      // keys of the step that are there
-            const uint8_t *keys = reinterpret_cast<const uint8_t*>(c.key_codes) + (pair * bt + in_block) * dim, *values = reinterpret_cast<const uint8_t*>(c.value_codes) + (pair * bt + in_block) * dim;
+            const uint32_t key0 = steps.key(step), blocks[2] = {next_block[0], next_block[1]};
+            ask(step + 1);
+            const uint32_t at = raw + ring + slot * S::STAGE, left = steps.end - key0;      // keys of the step that are there
+            if (blocks[0] < c.blocks && blocks[1] < c.blocks && left >= QA_STEP && dim == DP) {
 #pragma unroll
-            for (uint32_t n = 0; n < S::K_LOADS; ++n) {
-                const uint32_t key = (n & 1u) * 8 + g, d = (n >> 1) * 64 + quad * 16;
-                const bool ok = there && key < left && d < dim;
-                qa_copy16(at + n * 512 + lane * 16, keys + (ok ? key * dim + d : 0u), ok);
-            }
+                for (uint32_t h = 0; h < 2; ++h) {
+                    const size_t first = ((((size_t)blocks[h] * c.kv_heads + head) << p.shift) + ((key0 + h * QA_HALF) & (bt - 1u))) * DP;
+                    const uint8_t *keys = all_keys + first + k_lane, *values = all_values + first + v_lane;
 #pragma unroll
-            for (uint32_t n = 0; n < 4 * S::V_UNITS; ++n) {
-                const uint32_t k = n & 3u, key = (k >> 1) * 8 + quad * 2 + (k & 1u), d = (g + 8 * (n >> 2)) * S::V_UNIT;
-                const bool ok = there && key < left && d < dim;
-                const uint32_t to_v = at + 16 * DP + n * (32 * S::V_UNIT) + lane * S::V_UNIT;
-                if (S::V_UNIT == 16) qa_copy16(to_v, values + (ok ? key * dim + d : 0u), ok);
-                else qa_copy8(to_v, values + (ok ? key * dim + d : 0u), ok);
+                    for (uint32_t n = 0; n < S::K_LOADS; ++n) qa_copy16(at + h * S::HALF_BYTES + k_to + n * 512, keys + (n & 1u) * 8 * DP + (n >> 1) * 64, true);
+#pragma unroll
+                    for (uint32_t n = 0; n < 4 * S::V_UNITS; ++n) {
+                        const uint8_t* v = values + ((n >> 1 & 1u) * 8 + (n & 1u)) * DP + (n >> 2) * 8 * S::V_UNIT;
+                        if (S::V_UNIT == 16) qa_copy16(at + h * S::HALF_BYTES + v_to + n * (32 * S::V_UNIT), v, true);
+                        else qa_copy8(at + h * S::HALF_BYTES + v_to + n * (32 * S::V_UNIT), v, true);
+                    }
+                }
+            } else {      // a part of the step's keys, or of the channels: zeros for the rest
+#pragma unroll 1
+                for (uint32_t h = 0; h < 2; ++h) {
+                    const bool there = blocks[h] < c.blocks;
+                    const uint32_t mine = left > h * QA_HALF ? left - h * QA_HALF : 0u;
+                    const size_t first = ((((size_t)(there ? blocks[h] : 0u) * c.kv_heads + head) << p.shift) + ((key0 + h * QA_HALF) & (bt - 1u))) * dim;
+#pragma unroll 1
+                    for (uint32_t n = 0; n < S::K_LOADS; ++n) {
+                        const bool ok = there && (n & 1u) * 8 + g < mine && (n >> 1) * 64 + quad * 16 < dim;
+                        qa_copy16(at + h * S::HALF_BYTES + k_to + n * 512, all_keys + (ok ? first + k_lane + (n & 1u) * 8 * dim + (n >> 1) * 64 : 0u), ok);
+                    }
+#pragma unroll 1
+                    for (uint32_t n = 0; n < 4 * S::V_UNITS; ++n) {
+                        const uint32_t key = (n >> 1 & 1u) * 8 + (n & 1u);
+                        const bool ok = there && key + quad * 2 < mine && (g + 8 * (n >> 2)) * S::V_UNIT < dim;
+                        const uint8_t* v = all_values + (ok ? first + v_lane + key * dim + (n >> 2) * 8 * S::V_UNIT : 0u);
+                        if (S::V_UNIT == 16) qa_copy16(at + h * S::HALF_BYTES + v_to + n * (32 * S::V_UNIT), v, ok);
+                        else qa_copy8(at + h * S::HALF_BYTES + v_to + n * (32 * S::V_UNIT), v, ok);
+                    }
+                }
             }
-            if (lane < 2) qa_copy4(at + S::STEP_BYTES + lane * 4, reinterpret_cast<const float*>(lane ? c.value_scales : c.key_scales) + pair);
-            if (lane == 2) asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + S::STEP_BYTES + 8), "r"((uint32_t)there) : "memory");
+            // scales of keys and values of both halves, then which halves have a block
+            if (lane < 4) {
+                const uint32_t block = blocks[lane >> 1];
+                qa_copy4(at + S::STEP_BYTES + lane * 4, all_scales + ((size_t)(block < c.blocks ? block : 0u) * c.kv_heads + head));
+            }
+            if (lane == 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + S::STEP_BYTES + 16), "r"((blocks[0] < c.blocks ? 1u : 0u) | (blocks[1] < c.blocks ? 2u : 0u)) : "memory");
         }
         qa_commit();
     };
 #pragma unroll
-    for (uint32_t s = 0; s < S::STAGES - 1; ++s) copy(from + warp + s * QA_WARPS, s);
-    qa_query<T, DP>(p, q, head * p.group, pair0, pairs, query, factors);
-    __syncthreads();
+    for (uint32_t s = 0; s < S::STAGES - 1; ++s) copy(from + s, s);
+    qa_query<T, DP, NT>(p, q, head * p.group, pair0, pairs, query, factors, mosts);
 
-    QaRow row[2];
-    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f}, factor[2];
+    QaRow row[NT][2];
+    float top[NT][2], sum[NT][2], factor[NT][2], acc[NT][DP / 16][4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const uint32_t r = pair0 + g + 8 * h;
-        row[h].live = r < pairs;
-        row[h].index = q.length + (r < pairs ? r : pairs - 1u) / p.group;
-        factor[h] = factors[g + 8 * h];
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t r = pair0 + n * 8 + 2 * quad + h;
+            row[n][h].live = r < pairs;
+            row[n][h].index = q.length + (r < pairs ? r : pairs - 1u) / p.group;
+            factor[n][h] = factors[n * 8 + 2 * quad + h];
+            top[n][h] = -INFINITY;
+            sum[n][h] = 0.0f;
+        }
+#pragma unroll
+        for (int m = 0; m < DP / 16; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[n][m][i] = 0.0f;
     }
-    float acc[DP / 8][4];
-#pragma unroll
-    for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
 
+    const QaQuery<DP, NT, PARTS, S::KEPT> fragments(query, lane);
+    // what acc is counted in (0: nothing yet): a block's value scale, so that its products are added where they are made, or 1
+    float unit = 0.0f;
+    constexpr float LOWER = 1.0f / (1 << (int)QA_LIFT);
     uint32_t slot = 0;
-    for (uint32_t step = from + warp; step < to; step += QA_WARPS) {
-        copy(step + (S::STAGES - 1) * QA_WARPS, slot ? slot - 1 : S::STAGES - 1);
+    for (uint32_t step = from; step < to; ++step) {
+        copy(step + S::STAGES - 1, slot ? slot - 1 : S::STAGES - 1);
         qa_wait<S::STAGES - 1>();
         __syncwarp();
         const uint32_t at = ring + slot * S::STAGE, key0 = steps.key(step);
         slot = slot + 1 == S::STAGES ? 0 : slot + 1;
-        float key_scale, value_scale;
-        uint32_t there;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(key_scale) : "r"(at + S::STEP_BYTES) : "memory");
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(value_scale) : "r"(at + S::STEP_BYTES + 4) : "memory");
-        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(there) : "r"(at + S::STEP_BYTES + 8) : "memory");
-        if (!there) {
-            __syncwarp();
-            continue;
+        const float4 scales_at = *reinterpret_cast<const float4*>(qa_raw + at + S::STEP_BYTES);
+        const float scales[4] = {scales_at.x, scales_at.y, scales_at.z, scales_at.w};      // of keys and values, of both halves
+        const uint32_t there = *reinterpret_cast<const uint32_t*>(qa_raw + at + S::STEP_BYTES + 16);
+        float s[2][NT][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            qa_scores<CODE, DP, NT, PARTS>(fragments, [&](int n) { return qa_lds16(at + h * S::HALF_BYTES + k_to + n * 512); }, factor, scales[2 * h], a.softcap, s[h]);
+        // keys g, g + 8 of a half, pairs 2 quad, + 1 of each eight
+        const bool all = there == 3 && key0 + QA_STEP - 1 <= token0 && key0 + QA_STEP <= steps.end && (!a.window || token1 - key0 < a.window);
+        if (!all) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!(there >> h & 1u) || !row[n][i & 1].sees(key0 + h * QA_HALF + g + 8 * (i >> 1), steps.end, a.window, a.keep_first)) s[h][n][i] = -INFINITY;
         }
-
-        float s[2][4];
+        if (p.scores) {      // (for the weights' sums)
+            float* const mine = p.scores + (((size_t)sequence * c.kv_heads + head) * p.score_pairs + pair0) * p.score_stride + key0;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[t][i] = 0.0f;
+                for (int e = 0; e < 2; ++e)
+                    if (row[n][e].live) {
+                        float* at_row = mine + (size_t)(n * 8 + 2 * quad + e) * p.score_stride + g;
 #pragma unroll
-        for (int b = 0; b < DP / 64; ++b) {
-            const uint4 w[2] = {qa_lds16(at + (2 * b) * 512 + lane * 16), qa_lds16(at + (2 * b + 1) * 512 + lane * 16)};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-#pragma unroll
-                for (int part = PARTS - 1; part >= 0; --part) {
-                    const uint4 f = qa_lds16(query + part * S::QUERY + (b * 4 + k) * 512 + lane * 16);
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        uint32_t lo, hi;
-                        qa_pairs<CODE>(reinterpret_cast<const uint32_t*>(&w[t])[k], lo, hi);
-                        qa_mma(s[t], f, lo, hi);
+                        for (int h = 0; h < 2; ++h) {
+                            at_row[h * QA_HALF] = s[h][n][e];
+                            at_row[h * QA_HALF + 8] = s[h][n][2 + e];
+                        }
                     }
-                }
-            }
         }
-        // keys 8 t + 2 quad, + 1 of rows g, g + 8
-        const bool all = key0 + QA_STEP - 1 <= token0 && key0 + QA_STEP <= steps.end && (!a.window || token1 - key0 < a.window);
-        float most[2] = {-INFINITY, -INFINITY};
+        float keep[NT][2];
+        bool moved = false;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float x = qa_score(s[t][i], factor[i >> 1] * key_scale, a.softcap);
-                if (!all && !row[i >> 1].sees(key0 + 8 * t + 2 * quad + (i & 1), steps.end, a.window, a.keep_first)) x = -INFINITY;
-                s[t][i] = x;
-                most[i >> 1] = fmaxf(most[i >> 1], x);
+            for (int e = 0; e < 2; ++e) {
+                float most = fmaxf(fmaxf(s[0][n][e], s[0][n][2 + e]), fmaxf(s[1][n][e], s[1][n][2 + e]));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+                const float next = fmaxf(top[n][e], most);
+                keep[n][e] = next == top[n][e] ? 1.0f : qa_exp2(top[n][e] - next);
+                moved |= next != top[n][e];
+                top[n][e] = next;
+                sum[n][e] *= keep[n][e];
             }
-        float keep[2];
+        float rescaled = 1.0f;      // of acc, behind what the rows' maxima say
+        moved = __any_sync(0xffffffffu, moved);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 1));
-            most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 2));
-            const float next = fmaxf(top[h], most[h]);
-            keep[h] = next == top[h] ? 1.0f : qa_exp2(top[h] - next);
-            top[h] = next;
-        }
-        uint4 hi_part, lo_part;
-        {
-            float w[2][4], add[2] = {0.0f, 0.0f};
+            uint2 hi_part[NT], lo_part[NT];
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int n = 0; n < NT; ++n) {
+                float w[4];
+                const float base[2] = {top[n][0] == -INFINITY ? 0.0f : top[n][0] - QA_LIFT, top[n][1] == -INFINITY ? 0.0f : top[n][1] - QA_LIFT};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float base = top[i >> 1] == -INFINITY ? 0.0f : top[i >> 1] - QA_LIFT;
-                    w[t][i] = qa_exp2(s[t][i] - base);
-                    add[i >> 1] += w[t][i];
-                }
+                for (int i = 0; i < 4; ++i) w[i] = qa_exp2(s[h][n][i] - base[i & 1]);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) sum[h] = sum[h] * keep[h] + add[h];
-            uint32_t hi[4], lo[4];      // fragment words: row g of tile 0, row g + 8 of tile 0, row g of tile 1, row g + 8 of tile 1
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const float x = w[n >> 1][(n & 1) * 2], y = w[n >> 1][(n & 1) * 2 + 1];
-                hi[n] = qa_pack(x, y);
-                const float2 r = qa_unpack(hi[n]);
-                lo[n] = qa_pack(x - r.x, y - r.y);
+                for (int e = 0; e < 2; ++e) sum[n][e] += w[e] + w[2 + e];
+                const uint32_t a0 = qa_pack(w[0], w[1]), a1 = qa_pack(w[2], w[3]);
+                const float2 r0 = qa_unpack(a0), r1 = qa_unpack(a1);
+                hi_part[n] = make_uint2(qa_turn(a0), qa_turn(a1));
+                lo_part[n] = make_uint2(qa_turn(qa_pack(w[0] - r0.x, w[1] - r0.y)), qa_turn(qa_pack(w[2] - r1.x, w[3] - r1.y)));
             }
-            hi_part = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            lo_part = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
-        // a block whose scale is NaN makes the rows NaN that see one of its keys here, and no others
-        float times[2] = {value_scale, value_scale};
-        if (value_scale != value_scale) {
+            // Products of bf16 and f16 rows are added to acc by the tensor cores where its unit is, or can be made, the block's scale. Others, of f32 rows, of scales that are 0,
+            // NaN or too far from the last one, are added in f32 with the unit 1.
+            const float value_scale = scales[2 * h + 1], scale_now = value_scale * LOWER, ratio = unit * cache_inverse(scale_now);
+            const bool direct = PARTS == 1 && scale_now > 0.0f && (unit == 0.0f || (ratio >= 0x1p-60f && ratio <= 0x1p40f));
+            rescaled = direct ? ratio : unit;
+            if ((h == 0 && moved) || rescaled != 1.0f) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                bool any = all;
-                for (uint32_t k = 0; k < QA_STEP; ++k) any |= row[h].sees(key0 + k, steps.end, a.window, a.keep_first);
-                if (!any) times[h] = 0.0f;
-            }
-        }
-        const bool moved = __any_sync(0xffffffffu, keep[0] != 1.0f || keep[1] != 1.0f);
+                for (int n = 0; n < NT; ++n) {
+                    const float times[2] = {h ? rescaled : keep[n][0] * rescaled, h ? rescaled : keep[n][1] * rescaled};
 #pragma unroll
-        for (int u = 0; u < (int)S::V_UNITS; ++u) {
-            uint32_t v[4][S::V_UNIT / 4];      // key, word
+                    for (int m = 0; m < DP / 16; ++m)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t v_at = at + 16 * DP + (u * 4 + k) * (32 * S::V_UNIT) + lane * S::V_UNIT;
-                if (S::V_UNIT == 16) {
-                    const uint4 x = qa_lds16(v_at);
-                    v[k][0] = x.x; v[k][1] = x.y;
-                    v[k][S::V_UNIT / 4 - 2] = x.z; v[k][S::V_UNIT / 4 - 1] = x.w;
-                } else {
-                    const uint2 x = qa_lds8(v_at);
-                    v[k][0] = x.x; v[k][1] = x.y;
+                        for (int i = 0; i < 4; ++i) acc[n][m][i] *= times[i & 1];
                 }
             }
+            unit = direct ? scale_now : 1.0f;
+            // the values' products: rows of operand A are channels, two of a lane's each time
+            auto products = [&](auto add) {
 #pragma unroll
-            for (int w = 0; w < (int)S::V_UNIT / 4; ++w) {
-                uint32_t b[4][2];      // channel, pair of keys
+                for (int u = 0; u < (int)S::V_UNITS; ++u) {
+                    uint32_t v[4][S::V_UNIT / 4];      // key, word
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    uint32_t x = v[2 * k][w], y = v[2 * k + 1][w];
-                    if (CODE == UZU_CACHE_CODE_I8) { x ^= 0x80808080u; y ^= 0x80808080u; }
-                    const uint32_t lo = __byte_perm(x, y, 0x5140), hi = __byte_perm(x, y, 0x7362);
-                    if (CODE == UZU_CACHE_CODE_I8) {
-                        b[0][k] = qa_i8_f16x2(__byte_perm(lo, 0x64646464u, 0x4140));
-                        b[1][k] = qa_i8_f16x2(__byte_perm(lo, 0x64646464u, 0x4342));
-                        b[2][k] = qa_i8_f16x2(__byte_perm(hi, 0x64646464u, 0x4140));
-                        b[3][k] = qa_i8_f16x2(__byte_perm(hi, 0x64646464u, 0x4342));
-                    } else {
-                        b[0][k] = cache_e4m3x2_f16x2(lo);
-                        b[1][k] = cache_e4m3x2_f16x2(lo >> 16);
-                        b[2][k] = cache_e4m3x2_f16x2(hi);
-                        b[3][k] = cache_e4m3x2_f16x2(hi >> 16);
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    qa_mma(d, lo_part, b[j][0], b[j][1]);
-                    qa_mma(d, hi_part, b[j][0], b[j][1]);
-                    float(&o)[4] = acc[u * 16 + w * 4 + j];
-                    if (moved) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[i] *= keep[i >> 1];
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t v_at = at + h * S::HALF_BYTES + v_to + (u * 4 + k) * (32 * S::V_UNIT);
+                        if (S::V_UNIT == 16) {
+                            const uint4 x = qa_lds16(v_at);
+                            v[k][0] = x.x; v[k][1] = x.y;
+                            v[k][S::V_UNIT / 4 - 2] = x.z; v[k][S::V_UNIT / 4 - 1] = x.w;
+                        } else {
+                            const uint2 x = qa_lds8(v_at);
+                            v[k][0] = x.x; v[k][1] = x.y;
+                        }
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[i] = fmaf(d[i], times[i >> 1], o[i]);
+                    for (int w = 0; w < (int)S::V_UNIT / 4; ++w) {
+                        uint32_t b[4][2];      // channel, pair of keys
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            uint32_t x = v[2 * k][w], y = v[2 * k + 1][w];
+                            if (CODE == UZU_CACHE_CODE_I8) { x ^= 0x80808080u; y ^= 0x80808080u; }
+                            const uint32_t lo = __byte_perm(x, y, 0x5140), hi = __byte_perm(x, y, 0x7362);
+                            if (CODE == UZU_CACHE_CODE_I8) {
+                                b[0][k] = qa_i8_f16x2(__byte_perm(lo, 0x64646464u, 0x4140));
+                                b[1][k] = qa_i8_f16x2(__byte_perm(lo, 0x64646464u, 0x4342));
+                                b[2][k] = qa_i8_f16x2(__byte_perm(hi, 0x64646464u, 0x4140));
+                                b[3][k] = qa_i8_f16x2(__byte_perm(hi, 0x64646464u, 0x4342));
+                            } else {
+                                b[0][k] = cache_e4m3x2_f16x2(lo);
+                                b[1][k] = cache_e4m3x2_f16x2(lo >> 16);
+                                b[2][k] = cache_e4m3x2_f16x2(hi);
+                                b[3][k] = cache_e4m3x2_f16x2(hi >> 16);
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) add((u * (int)S::V_UNIT + w * 4) / 2 + j, make_uint4(b[2 * j][0], b[2 * j + 1][0], b[2 * j][1], b[2 * j + 1][1]));
+                    }
                 }
+            };
+            if (PARTS == 1 && direct)
+                products([&](int m, const uint4& f) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        qa_mma(acc[n][m], f, lo_part[n].x, lo_part[n].y);
+                        qa_mma(acc[n][m], f, hi_part[n].x, hi_part[n].y);
+                    }
+                });
+            else {
+                float times[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        times[n][e] = scale_now;
+                        // a block whose scale is NaN makes the rows NaN that see one of its keys here, and no others
+                        if (value_scale != value_scale) {
+                            bool any = all;
+                            for (uint32_t k = 0; k < QA_HALF; ++k) any |= (there >> h & 1u) && row[n][e].sees(key0 + h * QA_HALF + k, steps.end, a.window, a.keep_first);
+                            if (!any) times[n][e] = 0.0f;
+                        }
+                    }
+                products([&](int m, const uint4& f) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        qa_mma(d, f, lo_part[n].x, lo_part[n].y);
+                        qa_mma(d, f, hi_part[n].x, hi_part[n].y);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[n][m][i] = fmaf(d[i], times[n][i & 1], acc[n][m][i]);
+                    }
+                });
             }
         }
         __syncwarp();      // (the scales are read before the slot is filled again)
@@ -388,37 +526,40 @@ __global__ void __launch_bounds__(QA_THREADS) quantized_cache_attention_kernel(c
 
     // ---- the warps' sums: [row][channel] each, in the place of the rings ----
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-        if (quad == 0) {
-            tops[warp][g + 8 * h] = top[h];
-            sums[warp][g + 8 * h] = sum[h];
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            sum[n][h] += __shfl_xor_sync(0xffffffffu, sum[n][h], 4);
+            sum[n][h] += __shfl_xor_sync(0xffffffffu, sum[n][h], 8);
+            sum[n][h] += __shfl_xor_sync(0xffffffffu, sum[n][h], 16);
+            if (g == 0) {
+                tops[warp][n * 8 + 2 * quad + h] = top[n][h];
+                sums[warp][n * 8 + 2 * quad + h] = sum[n][h];
+            }
         }
-    }
     __syncthreads();
     float* const all_sums = reinterpret_cast<float*>(qa_raw);
-    float whole[2];      // the largest score of the row over the warps
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        whole[h] = -INFINITY;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int w = 0; w < (int)QA_WARPS; ++w) whole[h] = fmaxf(whole[h], tops[w][g + 8 * h]);
-        const float f = top[h] == whole[h] ? 1.0f : qa_exp2(top[h] - whole[h]);
-        float* out = all_sums + (size_t)warp * (QA_ROWS * DP) + (g + 8 * h) * DP;
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t r = n * 8 + 2 * quad + h;
+            float whole = -INFINITY;      // the largest score of the row over the warps
 #pragma unroll
-        for (int u = 0; u < (int)S::V_UNITS; ++u)
+            for (int w = 0; w < (int)QA_WARPS; ++w) whole = fmaxf(whole, tops[w][r]);
+            const float f = (top[n][h] == whole ? 1.0f : qa_exp2(top[n][h] - whole)) * unit;
+            float* out = all_sums + (size_t)warp * (ROWS * DP) + r * DP;
+            // (channels of a unit: 2 m and 2 m + 1 are rows g and g + 8 of product m)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int u = 0; u < (int)S::V_UNITS; ++u)
 #pragma unroll
-                for (int n = 0; n < (int)S::V_UNIT; n += 4) {
-                    const int at = u * 16 + n;
-                    *reinterpret_cast<float4*>(out + (2 * quad + j + 8 * u) * S::V_UNIT + n) =
-                        make_float4(acc[at][2 * h + j] * f, acc[at + 1][2 * h + j] * f, acc[at + 2][2 * h + j] * f, acc[at + 3][2 * h + j] * f);
+                for (int k = 0; k < (int)S::V_UNIT; k += 4) {
+                    const int m = (u * (int)S::V_UNIT + k) / 2;
+                    *reinterpret_cast<float4*>(out + (g + 8 * u) * S::V_UNIT + k) = make_float4(acc[n][m][h] * f, acc[n][m][2 + h] * f, acc[n][m + 1][h] * f, acc[n][m + 1][2 + h] * f);
                 }
-    }
+        }
     __syncthreads();
-    const uint32_t rows = min(QA_ROWS, pairs - pair0), quads = dim / 4;
+    const uint32_t rows = min(ROWS, pairs - pair0), quads = dim / 4;
     auto row_top = [&](uint32_t r) {
         float m = tops[0][r];
 #pragma unroll
@@ -435,7 +576,7 @@ __global__ void __launch_bounds__(QA_THREADS) quantized_cache_attention_kernel(c
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int w = 0; w < (int)QA_WARPS; ++w) {
-            const float4 x = *reinterpret_cast<const float4*>(all_sums + (size_t)w * (QA_ROWS * DP) + r * DP + n * 4);
+            const float4 x = *reinterpret_cast<const float4*>(all_sums + (size_t)w * (ROWS * DP) + r * DP + n * 4);
             o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
         }
         return o;
@@ -450,7 +591,7 @@ __global__ void __launch_bounds__(QA_THREADS) quantized_cache_attention_kernel(c
             f = m == base ? 1.0f : qa_exp2(m - base);
             l = l * f + qa_exp2(sink - base + QA_LIFT);
         }
-        const float inv = l != 0.0f ? f / l : 0.0f;
+        const float inv = l != 0.0f ? f * (float)(1 << (int)QA_LIFT) / l : 0.0f;      // (the sum of the weights is lifted, the sums of values are not)
         if (p.stats && n == 0) *reinterpret_cast<float2*>(p.stats + ((size_t)t * a.heads + h) * 2) = make_float2(base, l != 0.0f ? exp2f(QA_LIFT) / l : 0.0f);
         T* out = reinterpret_cast<T*>(a.out) + (size_t)t * a.out_stride + (size_t)h * dim + n * 4;
         const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
@@ -471,13 +612,13 @@ __global__ void __launch_bounds__(QA_THREADS) quantized_cache_attention_kernel(c
     }
     // ---- several CTAs: the last to be ready adds up what each has left, in their order ----
     const size_t place = ((size_t)sequence * gridDim.y + head) * p.tiles + tile;
-    float* const mine = p.partials + (place * p.splits + split) * (QA_ROWS * (dim + 2));
+    float* const mine = p.partials + (place * p.splits + split) * (ROWS * (dim + 2));
     for (uint32_t i = tid; i < rows * quads; i += QA_THREADS) {
         const uint32_t r = i / quads, n = i % quads;
         reinterpret_cast<float4*>(mine)[r * quads + n] = row_quad(r, n);
         if (n == 0) {
             const float m = row_top(r);
-            *reinterpret_cast<float2*>(mine + QA_ROWS * dim + r * 2) = make_float2(m, row_sum(r, m));
+            *reinterpret_cast<float2*>(mine + ROWS * dim + r * 2) = make_float2(m, row_sum(r, m));
         }
     }
     __threadfence();
@@ -490,15 +631,15 @@ __global__ void __launch_bounds__(QA_THREADS) quantized_cache_attention_kernel(c
     __syncthreads();
     if (!last_of_all) return;
     __threadfence();
-    const float* const theirs = p.partials + place * p.splits * (QA_ROWS * (dim + 2));
+    const float* const theirs = p.partials + place * p.splits * (ROWS * (dim + 2));
     for (uint32_t i = tid; i < rows * quads; i += QA_THREADS) {
         const uint32_t r = i / quads, n = i % quads;
         float m = -INFINITY, l = 0.0f;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
         for (uint32_t z = 0; z < p.splits; ++z) {
-            const float* part = theirs + (size_t)z * (QA_ROWS * (dim + 2));
-            const float2 ml = *reinterpret_cast<const float2*>(part + QA_ROWS * dim + r * 2);
+            const float* part = theirs + (size_t)z * (ROWS * (dim + 2));
+            const float2 ml = *reinterpret_cast<const float2*>(part + ROWS * dim + r * 2);
             const float4 x = reinterpret_cast<const float4*>(part)[r * quads + n];
             const float next = fmaxf(m, ml.x), keep = m == next ? 1.0f : qa_exp2(m - next), f = ml.x == next ? 1.0f : qa_exp2(ml.x - next);
             l = l * keep + ml.y * f;
@@ -509,40 +650,80 @@ __global__ void __launch_bounds__(QA_THREADS) quantized_cache_attention_kernel(c
     }
 }
 
-// The weight of each key, summed over the last rows of its sequence and the heads of its key head, in the order of the pairs: scores once more, with the rows' maxima and sums.
-template <typename T, int CODE, int DP>
-__global__ void __launch_bounds__(QA_THREADS) quantized_cache_weights_kernel(const __grid_constant__ QaParams p) {
-    using S = QaShape<DP>;
-    constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
-    extern __shared__ __align__(128) uint8_t qa_raw[];
-    __shared__ float factors[QA_ROWS];
+// The weight of each key, summed over the last rows of its sequence and the heads of its key head, in the order of the pairs, from the scores that the kernel above has kept (4 bytes
+// a key and pair, where the keys' codes are head_dim a key): a thread a key.
+__global__ void __launch_bounds__(QA_SUM) quantized_cache_sum_kernel(const __grid_constant__ QaParams p) {
+    __shared__ float2 rows[64];
+    pdl_launch_dependents();
+    pdl_wait();
     const uzu_quantized_cache_attention_args& a = p.a;
     const uzu_quantized_cache& c = a.cache;
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, quad = lane & 3u, query = qa_smem(qa_raw);
+    const uint32_t sequence = blockIdx.z, head = blockIdx.y;
+    const CacheSequence q = cache_sequence(a.sequences, p.capacity, sequence);
+    const uint32_t pairs = q.rows * p.group, first = (q.rows - min(q.rows, a.weight_rows)) * p.group;
+    if (pairs > p.score_pairs || !pairs) return;
+    const QaSteps steps(q.length, q.length + q.rows - 1u, a.window, a.keep_first, p.capacity);      // (what some row sees)
+    const float* const scores = p.scores + ((size_t)sequence * c.kv_heads + head) * p.score_pairs * p.score_stride;
+    for (uint32_t r = threadIdx.x; r < pairs; r += QA_SUM) {
+        const float2 st = *reinterpret_cast<const float2*>(p.stats + ((size_t)(q.row + r / p.group) * a.heads + head * p.group + r % p.group) * 2);
+        rows[r] = make_float2(st.x == -INFINITY ? 0.0f : st.x, st.y);
+    }
+    __syncthreads();
+    const uint32_t keys = steps.steps * QA_STEP;
+    for (uint32_t i = blockIdx.x * QA_SUM + threadIdx.x; i < keys; i += gridDim.x * QA_SUM) {
+        const uint32_t key = steps.key(i / QA_STEP) + i % QA_STEP;
+        if (key >= steps.end) continue;
+        const uint32_t block = reinterpret_cast<const uint32_t*>(a.sequences.tables)[(size_t)sequence * a.sequences.table_stride + (key >> p.shift)];
+        if (block >= c.blocks) continue;
+        float x = 0.0f;
+        // (a tile of rows stores the steps that one of its rows sees: of others of these keys it may not, so a row's own tile's are asked)
+        for (uint32_t r = first; r < pairs; ++r) {
+            const uint32_t pair0 = r / p.tile_rows * p.tile_rows, token0 = q.length + pair0 / p.group, token1 = q.length + min(pair0 + p.tile_rows - 1u, pairs - 1u) / p.group;
+            if (!(key <= token1 && (!a.window || token0 < a.window || key >= ((token0 - a.window + 1u) & ~(QA_STEP - 1u)) || key / QA_STEP * QA_STEP < a.keep_first))) continue;
+            x += qa_exp2(scores[(size_t)r * p.score_stride + key] - rows[r].x) * rows[r].y;
+        }
+        float* at = reinterpret_cast<float*>(c.key_weights) + (((size_t)block * c.kv_heads + head) << p.shift) + (key & (c.block_tokens - 1u));
+        *at += x;
+    }
+}
+
+// The same with the scores once more, for the rows of prompts, or where they would take too much memory.
+template <typename T, int CODE, int DP, int NT>
+__global__ void __launch_bounds__(QA_THREADS) quantized_cache_weights_kernel(const __grid_constant__ QaParams p) {
+    using S = QaShape<DP, NT>;
+    constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
+    __shared__ float factors[S::ROWS];
+    __shared__ uint32_t mosts[S::ROWS];
+    const uzu_quantized_cache_attention_args& a = p.a;
+    const uzu_quantized_cache& c = a.cache;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, quad = lane & 3u, query = 0;
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t sequence = blockIdx.z, head = blockIdx.y;
     const CacheSequence q = cache_sequence(a.sequences, p.capacity, sequence);
     const uint32_t pairs = q.rows * p.group, dim = c.head_dim, bt = c.block_tokens;
+    if (p.scores && pairs <= p.score_pairs) return;      // (the kernel above's)
     const uint32_t* table = reinterpret_cast<const uint32_t*>(a.sequences.tables) + (size_t)sequence * a.sequences.table_stride;
-    for (uint32_t pair0 = (q.rows - min(q.rows, a.weight_rows)) * p.group; pair0 < pairs; pair0 += QA_ROWS) {
+    for (uint32_t pair0 = (q.rows - min(q.rows, a.weight_rows)) * p.group; pair0 < pairs; pair0 += S::ROWS) {
         __syncthreads();
-        qa_query<T, DP>(p, q, head * p.group, pair0, pairs, query, factors);
-        __syncthreads();
-        const uint32_t token0 = q.length + pair0 / p.group, token1 = q.length + min(pair0 + QA_ROWS - 1u, pairs - 1u) / p.group;
+        qa_query<T, DP, NT>(p, q, head * p.group, pair0, pairs, query, factors, mosts);
+        const uint32_t token0 = q.length + pair0 / p.group, token1 = q.length + min(pair0 + S::ROWS - 1u, pairs - 1u) / p.group;
         const QaSteps steps(token0, token1, a.window, a.keep_first, p.capacity);
-        QaRow row[2];
-        float factor[2], base[2], times[2];
+        QaRow row[NT][2];
+        float factor[NT][2], base[NT][2], times[NT][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t r = pair0 + g + 8 * h, pair = r < pairs ? r : pairs - 1u;
-            row[h].live = r < pairs;
-            row[h].index = q.length + pair / p.group;
-            factor[h] = factors[g + 8 * h];
-            const float2 st = *reinterpret_cast<const float2*>(p.stats + ((size_t)(q.row + pair / p.group) * a.heads + head * p.group + pair % p.group) * 2);
-            base[h] = st.x == -INFINITY ? 0.0f : st.x;
-            times[h] = st.y;
-        }
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t r = pair0 + n * 8 + 2 * quad + h, pair = r < pairs ? r : pairs - 1u;
+                row[n][h].live = r < pairs;
+                row[n][h].index = q.length + pair / p.group;
+                factor[n][h] = factors[n * 8 + 2 * quad + h];
+                const float2 st = *reinterpret_cast<const float2*>(p.stats + ((size_t)(q.row + pair / p.group) * a.heads + head * p.group + pair % p.group) * 2);
+                base[n][h] = st.x == -INFINITY ? 0.0f : st.x;
+                times[n][h] = st.y;
+            }
+        const QaQuery<DP, NT, PARTS, S::KEPT> fragments(query, lane);
         // a key is always the same warp's, whatever the tile of rows: steps are named by their first key
         const uint32_t stride = gridDim.x * QA_WARPS, mine = blockIdx.x * QA_WARPS + warp;
         for (uint32_t step = 0; step < steps.steps; ++step) {
@@ -554,79 +735,81 @@ __global__ void __launch_bounds__(QA_THREADS) quantized_cache_weights_kernel(con
                 step += min(ahead, run) - 1u;
                 continue;
             }
-            const uint32_t block = table[key0 / bt];
-            if (block >= c.blocks) continue;
-            const size_t pair = (size_t)block * c.kv_heads + head;
-            const uint32_t in_block = key0 % bt, left = steps.end - key0;
-            const uint8_t* keys = reinterpret_cast<const uint8_t*>(c.key_codes) + (pair * bt + in_block) * dim;
-            const float key_scale = reinterpret_cast<const float*>(c.key_scales)[pair];
-            uint4 w[S::K_LOADS];
+#pragma unroll 2
+            for (uint32_t at = key0; at < min(key0 + QA_STEP, steps.end); at += QA_HALF) {
+                const uint32_t block = table[at >> p.shift];
+                if (block >= c.blocks) continue;
+                const size_t pair = (size_t)block * c.kv_heads + head;
+                const uint32_t in_block = at & (bt - 1u), left = steps.end - at;
+                const uint8_t* keys = reinterpret_cast<const uint8_t*>(c.key_codes) + (pair * bt + in_block) * dim;
+                const float key_scale = reinterpret_cast<const float*>(c.key_scales)[pair];
+                uint4 w[S::K_LOADS];
 #pragma unroll
-            for (uint32_t n = 0; n < S::K_LOADS; ++n) {
-                const uint32_t key = (n & 1u) * 8 + g, d = (n >> 1) * 64 + quad * 16;
-                w[n] = key < left && d < dim ? *reinterpret_cast<const uint4*>(keys + key * dim + d) : make_uint4(0, 0, 0, 0);
-            }
-            float s[2][4];
+                for (uint32_t n = 0; n < S::K_LOADS; ++n) {
+                    const uint32_t key = (n & 1u) * 8 + g, d = (n >> 1) * 64 + quad * 16;
+                    w[n] = key < left && d < dim ? *reinterpret_cast<const uint4*>(keys + key * dim + d) : make_uint4(0, 0, 0, 0);
+                }
+                float s[NT][4];
+                qa_scores<CODE, DP, NT, PARTS>(fragments, [&](int n) { return w[n]; }, factor, key_scale, a.softcap, s);
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[t][i] = 0.0f;
-#pragma unroll
-            for (int b = 0; b < DP / 64; ++b)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-#pragma unroll
-                    for (int part = PARTS - 1; part >= 0; --part) {
-                        const uint4 f = qa_lds16(query + part * S::QUERY + (b * 4 + k) * 512 + lane * 16);
-#pragma unroll
-                        for (int t = 0; t < 2; ++t) {
-                            uint32_t lo, hi;
-                            qa_pairs<CODE>(reinterpret_cast<const uint32_t*>(&w[2 * b + t])[k], lo, hi);
-                            qa_mma(s[t], f, lo, hi);
-                        }
-                    }
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const uint32_t key = key0 + 8 * t + 2 * quad + j;
+                for (int t = 0; t < 2; ++t) {
+                    const uint32_t key = at + g + 8 * t;
                     float x = 0.0f;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        if (row[h].sees(key, steps.end, a.window, a.keep_first)) x += qa_exp2(qa_score(s[t][2 * h + j], factor[h] * key_scale, a.softcap) - base[h]) * times[h];
-                    x += __shfl_xor_sync(0xffffffffu, x, 4);
-                    x += __shfl_xor_sync(0xffffffffu, x, 8);
-                    x += __shfl_xor_sync(0xffffffffu, x, 16);
-                    if (g == 0 && key < steps.end) reinterpret_cast<float*>(c.key_weights)[pair * bt + in_block + 8 * t + 2 * quad + j] += x;
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            if (row[n][h].sees(key, steps.end, a.window, a.keep_first)) x += qa_exp2(s[n][2 * t + h] - base[n][h]) * times[n][h];
+                    x += __shfl_xor_sync(0xffffffffu, x, 1);
+                    x += __shfl_xor_sync(0xffffffffu, x, 2);
+                    if (quad == 0 && key < steps.end) reinterpret_cast<float*>(c.key_weights)[pair * bt + in_block + g + 8 * t] += x;
                 }
+            }
         }
     }
 }
 
 struct QaPlan {
-    uint32_t group, tiles, splits, most_rows;
-    uint64_t partial_bytes, stats_bytes;
+    uint32_t group, tiles, splits, few, eights;      // eights: of pairs, a tile's
+    uint32_t score_pairs, score_stride;      // 0: scores are not kept
+    uint64_t partial_bytes, stats_bytes, score_bytes;
 };
 QaPlan qa_plan(uint32_t sm_count, const uzu_quantized_cache_attention_args& a) {
     QaPlan p{};
     const uzu_cache_sequences& s = a.sequences;
     const uint32_t capacity = cache_capacity(s, a.cache.block_tokens);
     p.group = a.heads / a.cache.kv_heads;
-    p.most_rows = std::min(s.max_rows, s.rows);
-    p.tiles = (uint32_t)(((uint64_t)p.most_rows * p.group + QA_ROWS - 1) / QA_ROWS);
+    const uint32_t most_rows = std::min(s.max_rows, s.rows);
+    const uint64_t most_pairs = (uint64_t)most_rows * p.group;
+    p.few = quantized_cache_umma_applicable(a) ? kCacheFewPairs : 0xffffffffu;
+    // tiles as wide as registers allow: a tile reads its keys once
+    const uint64_t pairs = std::min<uint64_t>(most_pairs, p.few);
+    p.eights = pairs <= 8 ? 1 : a.cache.head_dim <= 64 && pairs > 16 ? 4 : 2;
+    p.tiles = (uint32_t)((pairs + p.eights * 8 - 1) / (p.eights * 8));
     const uint64_t ctas = (uint64_t)s.count * a.cache.kv_heads * p.tiles;
-    const uint64_t keys = a.window ? std::min<uint64_t>(capacity, (uint64_t)a.window + p.most_rows + a.keep_first + 32) : capacity, steps = (keys + QA_STEP - 1) / QA_STEP;
+    const uint64_t keys = a.window ? std::min<uint64_t>(capacity, (uint64_t)a.window + most_rows + a.keep_first + 32) : capacity, steps = (keys + QA_STEP - 1) / QA_STEP;
     p.splits = 1;
     if (ctas && ctas <= QA_TICKETS) {
-        const uint64_t wanted = ((uint64_t)sm_count * 3 + ctas - 1) / ctas;
-        p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({wanted, (steps + 2 * QA_WARPS - 1) / (2 * QA_WARPS), 64}));
+        // one wave where the tiles are few (a CTA too many would double the time), else parts short enough for lengths that differ
+        const uint64_t slots = (uint64_t)sm_count * (a.cache.head_dim > 128 ? 1 : 3), wanted = ctas <= slots ? slots / ctas : (2 * slots + ctas - 1) / ctas;
+        p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({wanted, (steps + QA_WARPS - 1) / QA_WARPS, 128}));
     }
-    if (p.splits > 1) p.partial_bytes = ctas * p.splits * QA_ROWS * (a.cache.head_dim + 2) * 4;
-    if (a.weight_rows) p.stats_bytes = (uint64_t)s.rows * a.heads * 8;
+    if (p.splits > 1) p.partial_bytes = ctas * p.splits * p.eights * 8 * (a.cache.head_dim + 2) * 4;
+    if (a.weight_rows) {
+        p.stats_bytes = (uint64_t)s.rows * a.heads * 8;
+        const uint64_t stride = ((uint64_t)capacity + 63) & ~63ull, most = std::min<uint64_t>(most_pairs, kCacheFewPairs), bytes = (uint64_t)s.count * a.cache.kv_heads * most * stride * 4;
+        if (most_pairs <= kCacheFewPairs || p.few == kCacheFewPairs) {
+            if (bytes <= QA_SCORES) {
+                p.score_pairs = (uint32_t)most;
+                p.score_stride = (uint32_t)stride;
+                p.score_bytes = bytes;
+            }
+        }
+    }
     return p;
 }
 uint64_t qa_align(uint64_t v) { return (v + 255) & ~255ull; }
-uint64_t qa_scratch(const QaPlan& p) { return QA_TICKETS * 4 + qa_align(p.partial_bytes) + qa_align(p.stats_bytes); }
+uint64_t qa_scratch(const QaPlan& p) { return QA_TICKETS * 4 + qa_align(p.partial_bytes) + qa_align(p.stats_bytes) + p.score_bytes; }
 
 const char* attention_check(const uzu_quantized_cache_attention_args* a) {
     if (!a) return "null arguments";
@@ -659,11 +842,16 @@ const char* attention_check(const uzu_quantized_cache_attention_args* a) {
 }
 
 template <typename F>
-void qa_instance(const uzu_quantized_cache_attention_args& a, F f) {
+void qa_instance(const uzu_quantized_cache_attention_args& a, uint32_t eights, F f) {
+    auto tiles = [&](auto t, auto code, auto dp) {
+        if (eights == 1) f(t, code, dp, std::integral_constant<int, 1>());
+        else if constexpr (decltype(dp)::value == 64) eights == 4 ? f(t, code, dp, std::integral_constant<int, 4>()) : f(t, code, dp, std::integral_constant<int, 2>());
+        else f(t, code, dp, std::integral_constant<int, 2>());
+    };
     auto dims = [&](auto t, auto code) {
-        if (a.cache.head_dim <= 64) f(t, code, std::integral_constant<int, 64>());
-        else if (a.cache.head_dim <= 128) f(t, code, std::integral_constant<int, 128>());
-        else f(t, code, std::integral_constant<int, 256>());
+        if (a.cache.head_dim <= 64) tiles(t, code, std::integral_constant<int, 64>());
+        else if (a.cache.head_dim <= 128) tiles(t, code, std::integral_constant<int, 128>());
+        else tiles(t, code, std::integral_constant<int, 256>());
     };
     auto codes = [&](auto t) {
         if (a.cache.code_type == UZU_CACHE_CODE_I8) dims(t, std::integral_constant<int, UZU_CACHE_CODE_I8>());
@@ -673,19 +861,19 @@ void qa_instance(const uzu_quantized_cache_attention_args& a, F f) {
     else codes(uint16_t());
 }
 
-template <typename T, int CODE, int DP>
+template <typename T, int CODE, int DP, int NT>
 void qa_attend(uzu_command_buffer* cmd, const QaParams& p) {
-    using S = QaShape<DP>;
+    using S = QaShape<DP, NT>;
     static std::atomic<uint64_t> opted{0};
-    const uint32_t parts = sizeof(T) == 4 ? 2 : 1, sums = QA_WARPS * QA_ROWS * DP * 4, smem = std::max(S::RING + parts * S::QUERY, sums);
-    opt_in_dynamic_smem(cmd, quantized_cache_attention_kernel<T, CODE, DP>, (int)smem, opted);
-    launch(cmd, "quantized_cache_attention_kernel", quantized_cache_attention_kernel<T, CODE, DP>, dim3(p.tiles * p.splits, p.a.cache.kv_heads, p.a.sequences.count), dim3(QA_THREADS), smem, p);
+    const uint32_t parts = sizeof(T) == 4 ? 2 : 1, sums = QA_WARPS * S::ROWS * DP * 4, smem = std::max(S::RING + parts * S::QUERY, sums);
+    opt_in_dynamic_smem(cmd, quantized_cache_attention_kernel<T, CODE, DP, NT>, (int)smem, opted);
+    launch(cmd, "quantized_cache_attention_kernel", quantized_cache_attention_kernel<T, CODE, DP, NT>, dim3(p.tiles * p.splits, p.a.cache.kv_heads, p.a.sequences.count), dim3(QA_THREADS), smem, p);
 }
-template <typename T, int CODE, int DP>
+template <typename T, int CODE, int DP, int NT>
 void qa_weigh(uzu_command_buffer* cmd, const QaParams& p) {
     const uint32_t parts = sizeof(T) == 4 ? 2 : 1, ctas = p.a.sequences.count * p.a.cache.kv_heads, steps = (p.capacity + QA_STEP - 1) / QA_STEP;
     const uint32_t parts_of_keys = std::max(1u, std::min((steps + QA_WARPS - 1) / QA_WARPS, ((uint32_t)cmd->ctx->sm_count * 8 + ctas - 1) / ctas));
-    launch(cmd, "quantized_cache_weights_kernel", quantized_cache_weights_kernel<T, CODE, DP>, dim3(parts_of_keys, p.a.cache.kv_heads, p.a.sequences.count), dim3(QA_THREADS), parts * QaShape<DP>::QUERY, p);
+    launch(cmd, "quantized_cache_weights_kernel", quantized_cache_weights_kernel<T, CODE, DP, NT>, dim3(parts_of_keys, p.a.cache.kv_heads, p.a.sequences.count), dim3(QA_THREADS), parts * QaShape<DP, NT>::QUERY, p);
 }
 
 }  // namespace
@@ -723,13 +911,25 @@ void uzu_quantized_cache_attention_encode(uzu_command_buffer* cmd, const uzu_qua
     p.group = plan.group;
     p.tiles = plan.tiles;
     p.splits = plan.splits;
+    p.few = plan.few;
+    p.shift = a->cache.block_tokens == 16 ? 4 : a->cache.block_tokens == 32 ? 5 : 6;
     p.tickets = reinterpret_cast<uint32_t*>(a->scratch);
     p.partials = reinterpret_cast<float*>(a->scratch + QA_TICKETS * 4);
     p.stats = a->weight_rows ? reinterpret_cast<float*>(a->scratch + QA_TICKETS * 4 + qa_align(plan.partial_bytes)) : nullptr;
-    qa_instance(*a, [&](auto t, auto code, auto dim) {
-        qa_attend<decltype(t), decltype(code)::value, decltype(dim)::value>(cmd, p);
-        if (a->weight_rows) qa_weigh<decltype(t), decltype(code)::value, decltype(dim)::value>(cmd, p);
+    if (plan.score_pairs) p.scores = reinterpret_cast<float*>(a->scratch + QA_TICKETS * 4 + qa_align(plan.partial_bytes) + qa_align(plan.stats_bytes));
+    p.score_pairs = plan.score_pairs;
+    p.score_stride = plan.score_stride;
+    p.tile_rows = plan.eights * 8;
+    // prompts, then sequences of few rows (a pass may have both), then the weights of both
+    if (plan.few == kCacheFewPairs) encode_quantized_cache_umma(cmd, *a, reinterpret_cast<uint64_t>(p.stats));
+    qa_instance(*a, plan.eights, [&](auto t, auto code, auto dim, auto eights) {
+        qa_attend<decltype(t), decltype(code)::value, decltype(dim)::value, decltype(eights)::value>(cmd, p);
+        if (a->weight_rows && (!p.scores || plan.few == kCacheFewPairs)) qa_weigh<decltype(t), decltype(code)::value, decltype(dim)::value, decltype(eights)::value>(cmd, p);
     });
+    if (p.scores) {
+        const uint32_t ctas = a->sequences.count * a->cache.kv_heads, most = (p.capacity + QA_SUM - 1) / QA_SUM;
+        launch(cmd, "quantized_cache_sum_kernel", quantized_cache_sum_kernel, dim3(std::max(1u, std::min(most, ((uint32_t)cmd->ctx->sm_count * 16 + ctas - 1) / ctas)), a->cache.kv_heads, a->sequences.count), dim3(QA_SUM), 0, p);
+    }
 }
 
 }  // extern "C"
