@@ -144,8 +144,8 @@ class Cache:
                     out[t, h] = w @ vv
                     # A small weight's second f16 part ends at the subnormal spacing: off by 2^-25 of what is at most 2^15 for the row's largest weight, 2^-40 of that one
                     bound[t, h] = (w * (part + (len(js) / 16 + 60) * 2.0 ** -23) + 2.0 ** -40 * w.max(initial=0)) @ np.abs(vv)
-                    # On tcgen05 a weight is one f16 number: half a step of 11 bits, and below the normal ones half of 2^-24, lifted by 2^7 and lowered by 2^8 at most
-                    bound[t, h] += ((w * 2.0 ** -12 + 2.0 ** -24 * w.max(initial=0)) @ np.abs(vv)) if tensor else 0.0
+                    # On tcgen05 a weight is one f16 number: half a step of 11 bits, and below the normal ones half of 2^-24, lifted by 2^1 and lowered by 2^4 at most (its group's value scale over the unit)
+                    bound[t, h] += ((w * 2.0 ** -12 + 2.0 ** -22 * w.max(initial=0)) @ np.abs(vv)) if tensor else 0.0
                 if t >= n - min(weight_rows, n):
                     grow[js, g] += w
                     grow_bound[js, g] += w * (part + (per * n + 4) * 2.0 ** -23)
