@@ -10,7 +10,6 @@ namespace uzu {
 namespace {
 
 constexpr uint32_t QC_THREADS = 256;
-constexpr int QC_UNITS = 4;      // of 16 numbers a thread: 64 tokens of 256 numbers
 
 template <typename T> __device__ __forceinline__ float qc_f(T v);
 template <> __device__ __forceinline__ float qc_f(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -50,7 +49,8 @@ struct QcAppendParams {
     uint32_t capacity;
 };
 
-template <typename T, int CODE, bool WIDE>
+// UNITS: of 16 numbers a thread
+template <typename T, int CODE, bool WIDE, int UNITS>
 __global__ void __launch_bounds__(QC_THREADS) quantized_cache_append_kernel(const __grid_constant__ QcAppendParams p) {
     __shared__ uint32_t most_of[QC_THREADS / 32];
     pdl_launch_dependents();
@@ -73,16 +73,16 @@ __global__ void __launch_bounds__(QC_THREADS) quantized_cache_append_kernel(cons
     float* scale_at = reinterpret_cast<float*>(values ? c.value_scales : c.key_scales) + pair;
     const float was = old ? *scale_at : 0.0f;
 
-    QcUnit<T, WIDE> x[QC_UNITS];
+    QcUnit<T, WIDE> x[UNITS];
     uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < QC_UNITS; ++i) {
+    for (int i = 0; i < UNITS; ++i) {
         const uint32_t u = tid + i * QC_THREADS, token = u / chunks;
         if (u >= units || token < old) continue;
         x[i].load(rows + (size_t)((uint32_t)first + token - begin) * stride + (u - token * chunks) * 16);
     }
 #pragma unroll
-    for (int i = 0; i < QC_UNITS; ++i) {
+    for (int i = 0; i < UNITS; ++i) {
         const uint32_t u = tid + i * QC_THREADS;
         if (u >= units || u / chunks < old) continue;
 #pragma unroll
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(QC_THREADS) quantized_cache_append_kernel(cons
     if (tid == 0) *scale_at = scale;
     const float again = was * inverse;      // (NaN is not asked for below)
 #pragma unroll
-    for (int i = 0; i < QC_UNITS; ++i) {
+    for (int i = 0; i < UNITS; ++i) {
         const uint32_t u = tid + i * QC_THREADS, token = u / chunks;
         if (u >= units) continue;
         uint4* at = reinterpret_cast<uint4*>(codes + (size_t)u * 16);
@@ -249,13 +249,20 @@ void uzu_quantized_cache_append_encode(uzu_command_buffer* cmd, const uzu_quanti
     // blocks that a sequence's rows can touch
     const uint32_t bt = a->cache.block_tokens, most = std::min(std::min(s.max_rows, s.rows), p.capacity), blocks = std::min((most + 2 * bt - 2) / bt, s.table_stride);
     const dim3 grid(std::max(blocks, 1u) * 2, a->cache.kv_heads, s.count);
+    const uint32_t units = bt * (a->cache.head_dim / 16);      // of a whole block
     const uint64_t size = qc_size(a->data_type);
     const bool wide = ((a->keys | a->values) & 15u) == 0 && a->key_stride * size % 16 == 0 && a->value_stride * size % 16 == 0;
     by_type(a->data_type, [&](auto t) {
         using T = decltype(t);
         auto go = [&](auto kernel) { launch(cmd, "quantized_cache_append_kernel", kernel, grid, dim3(QC_THREADS), 0, p); };
-        if (a->cache.code_type == UZU_CACHE_CODE_I8) wide ? go(quantized_cache_append_kernel<T, UZU_CACHE_CODE_I8, true>) : go(quantized_cache_append_kernel<T, UZU_CACHE_CODE_I8, false>);
-        else wide ? go(quantized_cache_append_kernel<T, UZU_CACHE_CODE_E4M3, true>) : go(quantized_cache_append_kernel<T, UZU_CACHE_CODE_E4M3, false>);
+        auto by_units = [&](auto code) {
+            constexpr int CODE = decltype(code)::value;
+            if (units <= QC_THREADS) wide ? go(quantized_cache_append_kernel<T, CODE, true, 1>) : go(quantized_cache_append_kernel<T, CODE, false, 1>);
+            else if (units <= 2 * QC_THREADS) wide ? go(quantized_cache_append_kernel<T, CODE, true, 2>) : go(quantized_cache_append_kernel<T, CODE, false, 2>);
+            else wide ? go(quantized_cache_append_kernel<T, CODE, true, 4>) : go(quantized_cache_append_kernel<T, CODE, false, 4>);
+        };
+        if (a->cache.code_type == UZU_CACHE_CODE_I8) by_units(std::integral_constant<int, UZU_CACHE_CODE_I8>());
+        else by_units(std::integral_constant<int, UZU_CACHE_CODE_E4M3>());
     });
 }
 

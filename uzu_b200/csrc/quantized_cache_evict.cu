@@ -12,7 +12,6 @@ namespace uzu {
 namespace {
 
 constexpr uint32_t QE_CHOICE = 1024, QE_ITEMS = 4, QE_MOVE = 256;
-constexpr int QE_UNITS = 4;                        // of 16 codes a thread
 constexpr uint32_t QE_CACHED = 40960;              // weights of a sequence that are kept in shared memory
 
 struct QeParams {
@@ -149,8 +148,9 @@ __device__ __forceinline__ uint32_t qe_acquire(const uint32_t* p) {
     return v;
 }
 
-template <int CODE>
-__global__ void __launch_bounds__(QE_MOVE) quantized_cache_move_kernel(const __grid_constant__ QeParams p) {
+// UNITS: of 16 codes a thread
+template <int CODE, int UNITS>
+__global__ void __launch_bounds__(QE_MOVE, UNITS == 4 ? 2 : 5) quantized_cache_move_kernel(const __grid_constant__ QeParams p) {
     __shared__ uint32_t most_of[QE_MOVE / 32], item_at, late;
     pdl_launch_dependents();
     pdl_wait();
@@ -173,28 +173,32 @@ __global__ void __launch_bounds__(QE_MOVE) quantized_cache_move_kernel(const __g
     uint8_t* codes = reinterpret_cast<uint8_t*>(values ? c.value_codes : c.key_codes);
     float* scales = reinterpret_cast<float*>(values ? c.value_scales : c.key_scales);
 
-    uint4 x[QE_UNITS];
-    float from[QE_UNITS];
+    // (asked for early: what says who reads this block, and where it is)
+    const uint32_t* starts = p.starts + (size_t)(chain >> 1) * (p.blocks + 1);
+    const uint32_t at[2] = {starts[b], (uint64_t)(b + 1) * bt < length ? starts[b + 1] : a.budget}, block = table[b];
+
+    uint4 x[UNITS];
+    float from[UNITS];
     uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < QE_UNITS; ++i) {
+    for (int i = 0; i < UNITS; ++i) {
         const uint32_t u = tid + i * QE_MOVE, token = u / chunks;
         x[i] = make_uint4(0, 0, 0, 0);
         from[i] = 0.0f;
         if (u >= units) continue;
-        const uint32_t j = indices[first + token], block = table[j / bt];
-        if (block >= c.blocks) continue;      // (a token without a block: zeros)
-        const size_t pair = (size_t)block * c.kv_heads + head;
+        const uint32_t j = indices[first + token], its = table[j / bt];
+        if (its >= c.blocks) continue;      // (a token without a block: zeros)
+        const size_t pair = (size_t)its * c.kv_heads + head;
         from[i] = scales[pair];
         x[i] = *reinterpret_cast<const uint4*>(codes + (pair * bt + j % bt) * dim + (u - token * chunks) * 16);
     }
     float weight = 0.0f;
     if (!values && tid < tokens) {
-        const uint32_t j = indices[first + tid], block = table[j / bt];
-        if (block < c.blocks) weight = reinterpret_cast<const float*>(c.key_weights)[((size_t)block * c.kv_heads + head) * bt + j % bt];
+        const uint32_t j = indices[first + tid], its = table[j / bt];
+        if (its < c.blocks) weight = reinterpret_cast<const float*>(c.key_weights)[((size_t)its * c.kv_heads + head) * bt + j % bt];
     }
 #pragma unroll
-    for (int i = 0; i < QE_UNITS; ++i) {
+    for (int i = 0; i < UNITS; ++i) {
         const uint32_t* ws = reinterpret_cast<const uint32_t*>(&x[i]);
         if (from[i] != from[i]) most = 0x7fc00000u;
 #pragma unroll
@@ -215,8 +219,6 @@ __global__ void __launch_bounds__(QE_MOVE) quantized_cache_move_kernel(const __g
 
     // who reads block b: the blocks of the kept tokens [lo, hi) that are in it, all of them at or before b
     if (tid < 32) {
-        const uint32_t* starts = p.starts + (size_t)(chain >> 1) * (p.blocks + 1);
-        const uint32_t at[2] = {starts[b], (uint64_t)(b + 1) * bt < length ? starts[b + 1] : a.budget};
         if (at[1] > at[0]) {
             const uint32_t last = min((at[1] - 1) / bt, b);      // (b itself has)
             uint64_t t0, t1;
@@ -236,12 +238,11 @@ __global__ void __launch_bounds__(QE_MOVE) quantized_cache_move_kernel(const __g
     }
     __syncthreads();
     if (late) return;      // (nothing is written over what may still be read)
-    const uint32_t block = table[b];
     if (block >= c.blocks) return;
     const size_t pair = (size_t)block * c.kv_heads + head;
     const float scale = cache_scale<CODE>(most), inverse = cache_inverse(scale);
 #pragma unroll
-    for (int i = 0; i < QE_UNITS; ++i) {
+    for (int i = 0; i < UNITS; ++i) {
         const uint32_t u = tid + i * QE_MOVE;
         if (u >= units) continue;
         uint32_t* ws = reinterpret_cast<uint32_t*>(&x[i]);
@@ -351,8 +352,16 @@ void uzu_quantized_cache_evict_encode(uzu_command_buffer* cmd, const uzu_quantiz
     launch(cmd, "quantized_cache_choice_kernel", quantized_cache_choice_kernel, dim3(a->cache.kv_heads, s.count), dim3(QE_CHOICE), p.cached * 4, p);
     if (p.capacity <= a->budget) return;      // (no sequence can be longer)
     const dim3 grid(plan.blocks * s.count * a->cache.kv_heads * 2);
-    if (a->cache.code_type == UZU_CACHE_CODE_I8) launch(cmd, "quantized_cache_move_kernel", quantized_cache_move_kernel<UZU_CACHE_CODE_I8>, grid, dim3(QE_MOVE), 0, p);
-    else launch(cmd, "quantized_cache_move_kernel", quantized_cache_move_kernel<UZU_CACHE_CODE_E4M3>, grid, dim3(QE_MOVE), 0, p);
+    const uint32_t units = a->cache.block_tokens * a->cache.head_dim / 16;
+    auto go = [&](auto kernel) { launch(cmd, "quantized_cache_move_kernel", kernel, grid, dim3(QE_MOVE), 0, p); };
+    auto by_units = [&](auto code) {
+        constexpr int CODE = decltype(code)::value;
+        if (units <= QE_MOVE) go(quantized_cache_move_kernel<CODE, 1>);
+        else if (units <= 2 * QE_MOVE) go(quantized_cache_move_kernel<CODE, 2>);
+        else go(quantized_cache_move_kernel<CODE, 4>);
+    };
+    if (a->cache.code_type == UZU_CACHE_CODE_I8) by_units(std::integral_constant<int, UZU_CACHE_CODE_I8>());
+    else by_units(std::integral_constant<int, UZU_CACHE_CODE_E4M3>());
 }
 
 }  // extern "C"
