@@ -123,7 +123,7 @@ class Served:
             mine = P.of_kept(P.to_kept(x[at:at + n], dt), dt).reshape(n, heads, p.dim)
             capn = self.capacity(max_length)
             ref, bound, grow, gb = p.attend(self.table[i], self.lengths[i], mine, capn, float(scale), window, first, cap, sinks, weight_rows, 2.0 ** -22 if dt == P.F32 else 0.0,
-                                                tensor and n * heads // p.heads > 64)
+                                                tensor and n * heads // p.heads > 64, dt != P.F32)
             mine_got = got[at:at + n].reshape(n, heads, p.dim)
             assert np.array_equal(np.isnan(mine_got), np.isnan(ref)), (i, np.argwhere(np.isnan(mine_got) != np.isnan(ref))[:4])
             with np.errstate(invalid="ignore"):

@@ -106,8 +106,8 @@ class Cache:
                     self.weights[b, :, lo - first:hi - first] = 0
         return min(length + len(rows[0]), capacity)
 
-    def attend(self, table, length, q, capacity, scale, window=0, first=0, cap=0.0, sinks=None, weight_rows=0, q_error=0.0, tensor=False):
-        """q [rows, query heads, dim]; tensor: on tcgen05. (out, bound of its error before the last rounding), and the same of what the weights of each key grow by: [tokens, heads]"""
+    def attend(self, table, length, q, capacity, scale, window=0, first=0, cap=0.0, sinks=None, weight_rows=0, q_error=0.0, tensor=False, fast_cap=False):
+        """q [rows, query heads, dim]; tensor: on tcgen05; fast_cap: of 16-bit rows. (out, bound of its error before the last rounding), and the same of what the weights of each key grow by: [tokens, heads]"""
         n, hq, d = q.shape
         per = hq // self.heads
         end = min(length + n, capacity)
@@ -132,7 +132,7 @@ class Cache:
                 err = mag * ((d / 16 + 3) * 2.0 ** -22 + q_error)
                 if cap:
                     s = cap * np.tanh(s / cap)
-                    err = err + (cap * 2.0 ** -21 if tensor else 0.0)      # 1 - 2 / (1 + e^2x): roundings of numbers of up to 2
+                    err = err + (cap * 2.0 ** -21 if fast_cap else 0.0)      # 1 - 2 / (1 + e^2x): roundings of numbers of up to 2
                 err = err + (np.abs(s) + np.abs(s).max()) * 2.0 ** -22
                 with np.errstate(invalid="ignore"):
                     top = s.max() if sinks is None else max(s.max(), sinks[h])

@@ -194,6 +194,25 @@ def test_a_block_that_is_no_number(ctx, which, rows):
 
 
 @pytest.mark.parametrize("dt", TYPES)
+def test_weights_of_a_row_that_is_no_number(ctx, dt):
+    """keys that such a row does not see get theirs from the others: behind it, and before its window"""
+    for kv, heads, rows in ((1, 2, [6]), (1, 4, [40])):
+        s = Served(ctx, Q.I8, 16, kv, 64, [100], room=200)
+        s.append(rows, P.F32)
+        x = s.rng.standard_normal((rows[0], heads * 64))
+        x[2, 7] = np.nan
+        y = np.delete(x, 2, 0)
+        before = s.device_weights()
+        got, grown = s.attend(rows, heads, dt, tail=0, query=x, window=20, weight_rows=ALL, check=False)
+        assert np.isnan(got[2, :64]).all() and np.isfinite(np.delete(got, 2, 0)).all()
+        tokens = np.arange(100 + rows[0])
+        seen = (tokens <= 102) & (102 - tokens < 20)
+        of = grown[s.table[0][tokens // 16], 0, tokens % 16]
+        assert np.array_equal(np.isnan(of), seen), np.flatnonzero(np.isnan(of) != seen)
+        assert len(y) and np.isfinite(before).all()
+
+
+@pytest.mark.parametrize("dt", TYPES)
 def test_queries_at_the_ends(ctx, dt):
     """queries that are zero, tiny, huge or not finite"""
     s = Served(ctx, Q.I8, 32, 1, 64, [50], room=100)

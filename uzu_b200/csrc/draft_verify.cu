@@ -110,7 +110,7 @@ struct DvShared {
 };
 
 template <typename T, bool WIDE, uint32_t WARPS, uint32_t CLUSTER>
-__global__ void __launch_bounds__(WARPS * 32) draft_verify_kernel(const __grid_constant__ DvParams p) {
+__global__ void __launch_bounds__(WARPS * 32, WARPS == 8 ? 4 : 1) draft_verify_kernel(const __grid_constant__ DvParams p) {
     namespace cg = cooperative_groups;
     static_assert(WARPS <= 32 && CLUSTER <= 32, "a lane for each");
     __shared__ DvShared<WARPS> s;

@@ -188,6 +188,9 @@ struct QaRow {
     }
 };
 
+// tanh(x) = 1 - 2 / (1 + e^2x), within 2^-22
+__device__ __forceinline__ float qa_tanh(float x) { return 1.0f - 2.0f * __frcp_rn(1.0f + qa_exp2(2.8853900817779268f * x)); }
+
 // the queries' fragments, from shared memory or, once read, from registers
 template <int DP, int NT, int PARTS, bool KEPT>
 struct QaQuery {
@@ -237,7 +240,7 @@ __device__ __forceinline__ void qa_scores(const Query& query, Word word, const f
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][i] = cap * tanhf(s[n][i]);
+            for (int i = 0; i < 4; ++i) s[n][i] = cap * (PARTS == 1 ? qa_tanh(s[n][i]) : tanhf(s[n][i]));      // (of 16-bit rows within 2^-22 of the cap, for a fifth of the instructions)
     }
 }
 
@@ -654,6 +657,7 @@ __global__ void __launch_bounds__(QA_THREADS, QaShape<DP, NT>::CTAS) quantized_c
 // a key and pair, where the keys' codes are head_dim a key): a thread a key.
 __global__ void __launch_bounds__(QA_SUM) quantized_cache_sum_kernel(const __grid_constant__ QaParams p) {
     __shared__ float2 rows[64];
+    __shared__ uint2 spans[64];      // keys that a row's tile has scores of: from .x (or the first kept ones) to .y
     pdl_launch_dependents();
     pdl_wait();
     const uzu_quantized_cache_attention_args& a = p.a;
@@ -667,6 +671,8 @@ __global__ void __launch_bounds__(QA_SUM) quantized_cache_sum_kernel(const __gri
     for (uint32_t r = threadIdx.x; r < pairs; r += QA_SUM) {
         const float2 st = *reinterpret_cast<const float2*>(p.stats + ((size_t)(q.row + r / p.group) * a.heads + head * p.group + r % p.group) * 2);
         rows[r] = make_float2(st.x == -INFINITY ? 0.0f : st.x, st.y);
+        const uint32_t pair0 = r / p.tile_rows * p.tile_rows, token0 = q.length + pair0 / p.group, token1 = q.length + min(pair0 + p.tile_rows - 1u, pairs - 1u) / p.group;
+        spans[r] = make_uint2(a.window && token0 >= a.window ? (token0 - a.window + 1u) & ~(QA_STEP - 1u) : 0u, token1);
     }
     __syncthreads();
     const uint32_t keys = steps.steps * QA_STEP;
@@ -676,11 +682,12 @@ __global__ void __launch_bounds__(QA_SUM) quantized_cache_sum_kernel(const __gri
         const uint32_t block = reinterpret_cast<const uint32_t*>(a.sequences.tables)[(size_t)sequence * a.sequences.table_stride + (key >> p.shift)];
         if (block >= c.blocks) continue;
         float x = 0.0f;
-        // (a tile of rows stores the steps that one of its rows sees: of others of these keys it may not, so a row's own tile's are asked)
+        const bool kept = (key & ~(QA_STEP - 1u)) < a.keep_first;
+#pragma unroll 4
         for (uint32_t r = first; r < pairs; ++r) {
-            const uint32_t pair0 = r / p.tile_rows * p.tile_rows, token0 = q.length + pair0 / p.group, token1 = q.length + min(pair0 + p.tile_rows - 1u, pairs - 1u) / p.group;
-            if (!(key <= token1 && (!a.window || token0 < a.window || key >= ((token0 - a.window + 1u) & ~(QA_STEP - 1u)) || key / QA_STEP * QA_STEP < a.keep_first))) continue;
-            x += qa_exp2(scores[(size_t)r * p.score_stride + key] - rows[r].x) * rows[r].y;
+            const uint2 span = spans[r];
+            const float score = (key >= span.x || kept) && key <= span.y ? scores[(size_t)r * p.score_stride + key] : -INFINITY;
+            if (score != -INFINITY) x += qa_exp2(score - rows[r].x) * rows[r].y;      // (a row that is NaN gives so to the keys that it sees)
         }
         float* at = reinterpret_cast<float*>(c.key_weights) + (((size_t)block * c.kv_heads + head) << p.shift) + (key & (c.block_tokens - 1u));
         *at += x;
@@ -784,7 +791,7 @@ QaPlan qa_plan(uint32_t sm_count, const uzu_quantized_cache_attention_args& a) {
     p.few = quantized_cache_umma_applicable(a) ? kCacheFewPairs : 0xffffffffu;
     // tiles as wide as registers allow: a tile reads its keys once
     const uint64_t pairs = std::min<uint64_t>(most_pairs, p.few);
-    p.eights = pairs <= 8 ? 1 : a.cache.head_dim <= 64 && pairs > 16 ? 4 : 2;
+    p.eights = pairs <= 8 ? 1 : a.cache.head_dim <= 64 && pairs > 16 ? (pairs <= 24 ? 3 : 4) : 2;
     p.tiles = (uint32_t)((pairs + p.eights * 8 - 1) / (p.eights * 8));
     const uint64_t ctas = (uint64_t)s.count * a.cache.kv_heads * p.tiles;
     const uint64_t keys = a.window ? std::min<uint64_t>(capacity, (uint64_t)a.window + most_rows + a.keep_first + 32) : capacity, steps = (keys + QA_STEP - 1) / QA_STEP;
@@ -845,8 +852,11 @@ template <typename F>
 void qa_instance(const uzu_quantized_cache_attention_args& a, uint32_t eights, F f) {
     auto tiles = [&](auto t, auto code, auto dp) {
         if (eights == 1) f(t, code, dp, std::integral_constant<int, 1>());
-        else if constexpr (decltype(dp)::value == 64) eights == 4 ? f(t, code, dp, std::integral_constant<int, 4>()) : f(t, code, dp, std::integral_constant<int, 2>());
-        else f(t, code, dp, std::integral_constant<int, 2>());
+        else if constexpr (decltype(dp)::value == 64) {
+            if (eights == 2) f(t, code, dp, std::integral_constant<int, 2>());
+            else if (eights == 3) f(t, code, dp, std::integral_constant<int, 3>());
+            else f(t, code, dp, std::integral_constant<int, 4>());
+        } else f(t, code, dp, std::integral_constant<int, 2>());
     };
     auto dims = [&](auto t, auto code) {
         if (a.cache.head_dim <= 64) tiles(t, code, std::integral_constant<int, 64>());
