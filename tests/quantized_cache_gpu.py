@@ -116,14 +116,14 @@ class Served:
         self.last = a
         if not check:
             return got, self.device_weights() - weights
-        # f32 queries are two f16 parts of 11 bits: 22, each product's half step 2^-23. bf16 rows of more than 64 pairs go to the tensor cores' kernel
+        # f32 queries are two f16 parts of 11 bits: 22, each product's half step 2^-23. more than 8 bf16 rows of more than 64 pairs go to the tensor cores' kernel
         tensor = dt == P.BF16 and p.dim <= 128 and scale > 0 and not shift and (stride or 8) % 8 == 0
         at, grown, grown_bound = 0, np.zeros_like(weights), np.zeros_like(weights)
         for i, n in enumerate(rows):
             mine = P.of_kept(P.to_kept(x[at:at + n], dt), dt).reshape(n, heads, p.dim)
             capn = self.capacity(max_length)
             ref, bound, grow, gb = p.attend(self.table[i], self.lengths[i], mine, capn, float(scale), window, first, cap, sinks, weight_rows, 2.0 ** -22 if dt == P.F32 else 0.0,
-                                                tensor and n * heads // p.heads > 64, dt != P.F32)
+                                                tensor and n > 8 and n * heads // p.heads > 64, dt != P.F32)
             mine_got = got[at:at + n].reshape(n, heads, p.dim)
             assert np.array_equal(np.isnan(mine_got), np.isnan(ref)), (i, np.argwhere(np.isnan(mine_got) != np.isnan(ref))[:4])
             with np.errstate(invalid="ignore"):

@@ -130,7 +130,7 @@ def test_drafted_tokens_and_prompts(ctx, code, dt, window, first, cap, sink):
 
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("rows", [[300], [129, 77], [128, 1, 64]])
-@pytest.mark.parametrize("block,kv,heads,dim", [(64, 2, 8, 128), (16, 2, 4, 64), (32, 1, 2, 256), (32, 2, 6, 96)])
+@pytest.mark.parametrize("block,kv,heads,dim", [(64, 2, 8, 128), (16, 2, 4, 64), (32, 1, 2, 256), (32, 2, 6, 96), (16, 1, 8, 16), (32, 1, 3, 80)])
 def test_prompts(ctx, dt, rows, block, kv, heads, dim):
     s = Served(ctx, Q.I8 if dim != 64 else Q.E4M3, block, kv, dim, [int(7 + 61 * i) for i in range(len(rows))], room=500)
     s.append(rows, P.F32)
@@ -231,6 +231,16 @@ def test_queries_at_the_ends(ctx, dt):
     y = x.copy()
     y[3:5] = 0
     s.attend([8], 1, dt, tail=0, query=y)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rows", [[1, 8], [9, 3]])
+def test_many_heads_of_one(ctx, dt, rows):
+    """heads of one key head: few rows of many pairs, beside a sequence whose rows are not few"""
+    s = Served(ctx, Q.E4M3, 32, 1, 64, [200, 77], room=300)
+    s.append(rows, P.F32)
+    s.attend(rows, 100, dt, weight_rows=ALL)
+    s.attend(rows, 100, dt, window=40, first=3, weight_rows=2)
 
 
 def test_long_and_many(ctx):
@@ -471,6 +481,15 @@ def test_verify_rows_without_a_distribution(ctx):
         for d in (draft, None):
             accepted, tokens, clear = verify(ctx, target, d, drafted, u, temperature, 1.0, P.BF16)
             assert clear >= 7 and accepted[2] == 0 and tokens[2, 0] == NONE
+
+
+def test_verify_a_certain_draft_with_all_of_p(ctx):
+    """nothing is left beside it: it comes as the token behind if it is not kept"""
+    target = np.full((2, 2, 300), -np.inf)
+    target[:, 0, 7], target[0, 1, 9], target[1, 1] = 1.0, 0.0, 0.0
+    u = np.array([[1.0, 0.5], [0.25, 0.999]])      # (the first is outside the range: the draft is not kept)
+    got = verify(ctx, target, None, np.full((2, 1), 7), u, 1.0, 1.0, P.F32)
+    assert got[1][0].tolist() == [7, NONE] and got[0].tolist() == [0, 1] and got[1][1, 0] == 7
 
 
 def test_verify_draws_the_target(ctx):

@@ -12,7 +12,9 @@ namespace uzu {
 constexpr uint32_t kCacheHugeBits = 0x6f800000u;      // 2^96
 constexpr int kCacheLeastExponent = -100;
 constexpr uint32_t kNoIndex = 0xffffffffu;
-constexpr uint32_t kCacheFewPairs = 64;      // (row, head) pairs of a sequence and a key head that the kernel for few rows takes where the tcgen05 kernel takes the others
+// What the kernel for few rows takes where the tcgen05 kernel takes the others: sequences of so many (row, head) pairs of a key head, or of so few rows. The latter has no split of the
+// keys, so one CTA would read a long cache for a few rows of many heads.
+constexpr uint32_t kCacheFewPairs = 64, kCacheFewRows = 8;
 
 // tokens that a sequence can have: what the host bounds and its table holds
 inline uint32_t cache_capacity(const uzu_cache_sequences& s, uint32_t block_tokens) {

@@ -9,6 +9,9 @@
 // scale, and rescaled where it changes; scales of keys multiply scores.
 // Queries are brought to 2^14 .. 2^15 by a power of two for each row, which is exact; f32 ones are two f16 parts. A weight, up to 2^15, is two f16 parts: with one, every
 // eighth bf16 result or so would be the neighbour of the right one.
+// What bounds it: instructions and their latency, not memory: schedulers issue in 40 % of the cycles at 11 warps an SM, DRAM is busy for 43 % of the time, the tensor pipe for 15 %. One row
+// behind 131071 tokens of 8 heads of 128 (i8): 75 us, 3.6 TB/s. On the way there: 134 us first, 122 with wide loads of the queries, 82 with pairs as columns of a product, 75 with 32 keys a
+// step. 64 sequences of 4096 tokens on average 170 us, the weights' sums from kept scores 34. Before that last step four CTAs an SM took 100 us, five with a ring of two 106, three 113. A grid of 448 CTAs where 444 fit at once doubled the time, so splits fill one wave.
 #include "quantized_cache.cuh"
 
 namespace uzu {
@@ -23,7 +26,7 @@ constexpr float QA_LIFT = 15.0f;            // weights are relative to 2^-15 of 
 
 struct QaParams {
     uzu_quantized_cache_attention_args a;
-    uint32_t capacity, group, tiles, splits, shift, few;      // shift: log2 of a block's tokens; few: sequences with more pairs than that are another kernel's
+    uint32_t capacity, group, tiles, splits, shift, few;      // shift: log2 of a block's tokens; few: sequences of more pairs, and more than kCacheFewRows rows, are another kernel's
     uint32_t* tickets;
     float *partials, *stats;      // stats: of every row and head, the largest score (in units of ln 2) and what a weight is multiplied by; null: not asked for
     float* scores;                // of the sequences of few pairs: [sequence, key head, pair, score_stride]; null: not kept
@@ -260,7 +263,7 @@ __global__ void __launch_bounds__(QA_THREADS, QaShape<DP, NT>::CTAS) quantized_c
     const uint32_t sequence = blockIdx.z, head = blockIdx.y, split = blockIdx.x % p.splits, tile = blockIdx.x / p.splits;
     const CacheSequence q = cache_sequence(a.sequences, p.capacity, sequence);
     const uint32_t pairs = q.rows * p.group, pair0 = tile * ROWS;
-    if (pair0 >= pairs || pairs > p.few) return;
+    if (pair0 >= pairs || (pairs > p.few && q.rows > kCacheFewRows)) return;
     const uint32_t dim = c.head_dim, bt = c.block_tokens;
     const uint32_t token0 = q.length + pair0 / p.group, token1 = q.length + min(pair0 + ROWS - 1u, pairs - 1u) / p.group;
     const QaSteps steps(token0, token1, a.window, a.keep_first, p.capacity);
@@ -382,7 +385,7 @@ __global__ void __launch_bounds__(QA_THREADS, QaShape<DP, NT>::CTAS) quantized_c
                     for (int i = 0; i < 4; ++i)
                         if (!(there >> h & 1u) || !row[n][i & 1].sees(key0 + h * QA_HALF + g + 8 * (i >> 1), steps.end, a.window, a.keep_first)) s[h][n][i] = -INFINITY;
         }
-        if (p.scores) {      // (for the weights' sums)
+        if (p.scores && pairs <= p.score_pairs) {      // (for the weights' sums)
             float* const mine = p.scores + (((size_t)sequence * c.kv_heads + head) * p.score_pairs + pair0) * p.score_stride + key0;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -790,7 +793,7 @@ QaPlan qa_plan(uint32_t sm_count, const uzu_quantized_cache_attention_args& a) {
     const uint64_t most_pairs = (uint64_t)most_rows * p.group;
     p.few = quantized_cache_umma_applicable(a) ? kCacheFewPairs : 0xffffffffu;
     // tiles as wide as registers allow: a tile reads its keys once
-    const uint64_t pairs = std::min<uint64_t>(most_pairs, p.few);
+    const uint64_t pairs = std::min<uint64_t>(most_pairs, std::max<uint64_t>(p.few, (uint64_t)std::min(most_rows, kCacheFewRows) * p.group));
     p.eights = pairs <= 8 ? 1 : a.cache.head_dim <= 64 && pairs > 16 ? (pairs <= 24 ? 3 : 4) : 2;
     p.tiles = (uint32_t)((pairs + p.eights * 8 - 1) / (p.eights * 8));
     const uint64_t ctas = (uint64_t)s.count * a.cache.kv_heads * p.tiles;

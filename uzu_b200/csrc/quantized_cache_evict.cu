@@ -5,6 +5,8 @@
 // Move (a CTA for each block to be filled, keys or values): a block's new numbers come from blocks at or behind it, so it may be written once those who read it have. CTAs take their
 // blocks from a counter in ascending order, load first, say so, and wait only for earlier ones' loads, which wait for nothing: no order of CTAs can stop it. Nothing goes
 // through memory twice and no second copy of the cache is needed.
+// What bounds it: latency, a CTA's way through counter, indices, table, scales and codes. 16 sequences of 16000 tokens cut to 8000, 8 heads of 128 (e4m3): choice 55 us, move 240 (524 MB of
+// codes read and written, 2.2 TB/s; 408 with registers for blocks of 64 x 256), reading the kept tokens back 145 (786 MB, 5.4 TB/s). One sequence of 9001 to 4096: 26, 16 and 8 us.
 #include "quantized_cache.cuh"
 
 namespace uzu {

@@ -10,6 +10,10 @@
 // below the largest of its tile would bring its weights below f16's range: such groups of keys take a pass of their own, the others masked. The unit moves where the largest has left it
 // by more than 2^2; it stays within 2^80 of the largest that the row has seen, so that O neither over- nor underflows.
 // Queries are brought to 2^14 .. 2^15 by a power of two for each row, as in the kernel for few rows.
+// What bounds it: a tile of 256 rows and 128 keys takes about 5000 cycles; the softmax of a half's rows takes 2700 of them, its scores and products follow one another (1450). The tensor
+// pipe is busy for 35 % of the time, schedulers issue in 47 % of the cycles. 6144 rows of three sequences that hold 12000 tokens together, 32 heads of 128 (i8): 655 to 710 us, 712 to 772
+// TFLOP/s. On the way there: O in registers, added tile by tile 1180 us; masks and maxima apart for whole tiles 819; codes asked for ahead 745; O in tensor memory 702. With a part left
+// out for measuring: without the conversion of codes 649, without weights 551. Slower: weights made before the largest score is known 936, two threads a row 842, codes through registers 927.
 // Every barrier wait is bounded (wait_errors.h).
 #include <type_traits>
 
@@ -141,7 +145,7 @@ __global__ void __launch_bounds__(QU_THREADS, 1) quantized_cache_umma_kernel(con
     const uint32_t sequence = blockIdx.z, head = blockIdx.y, G = p.group, dim = c.head_dim, bt = c.block_tokens;
     const CacheSequence q = cache_sequence(a.sequences, p.capacity, sequence);
     const uint32_t pairs = q.rows * G, tiles = (pairs + 2 * QU_ROWS - 1) / (2 * QU_ROWS);
-    const bool mine = pairs > kCacheFewPairs && blockIdx.x < tiles;
+    const bool mine = pairs > kCacheFewPairs && q.rows > kCacheFewRows && blockIdx.x < tiles;
     const uint32_t pair0 = mine ? (tiles - 1u - blockIdx.x) * 2 * QU_ROWS : 0u;      // the rows with the most keys first
     const uint32_t row_tiles = pair0 + QU_ROWS < pairs ? 2u : 1u;
     const uint32_t token0 = q.length + pair0 / G, token1 = q.length + (min(pair0 + 2 * QU_ROWS, pairs) - 1u) / G;
@@ -533,10 +537,10 @@ void qu_launch(uzu_command_buffer* cmd, const QuParams& p, dim3 grid) {
 
 bool quantized_cache_umma_applicable(const uzu_quantized_cache_attention_args& a) {
     return a.data_type == UZU_DT_BF16 && a.cache.head_dim <= 128 && a.scale > 0.0f && ((a.query | a.out) & 15u) == 0 && a.query_row_stride % 8 == 0 && a.query_head_stride % 8 == 0 && a.out_stride % 8 == 0 &&
-           (uint64_t)std::min(a.sequences.max_rows, a.sequences.rows) * (a.heads / a.cache.kv_heads) > kCacheFewPairs;
+           std::min(a.sequences.max_rows, a.sequences.rows) > kCacheFewRows && (uint64_t)std::min(a.sequences.max_rows, a.sequences.rows) * (a.heads / a.cache.kv_heads) > kCacheFewPairs;
 }
 
-// sequences with more than kCacheFewPairs pairs of a row and a head of a key head's group
+// sequences of more than kCacheFewRows rows and kCacheFewPairs pairs of a row and a head of a key head's group
 void encode_quantized_cache_umma(uzu_command_buffer* cmd, const uzu_quantized_cache_attention_args& a, uint64_t row_stats) {
     QuParams p{};
     p.a = a;
