@@ -1016,8 +1016,8 @@ UZU_API size_t uzu_expert_layer_scratch_bytes(const uzu_expert_layer_args* args)
  * Which sequences a pass has is read on the device, so a captured call follows it: their block numbers, how many tokens they have, where their rows are.
  * Token j of sequence i is at tables[i, j / block_tokens]. A block number that is not below `blocks` is no block: its tokens are seen by nobody and rows
  * for it are dropped. Rows that belong to no sequence, and tokens behind a sequence's last, keep what they hold. max_length and max_rows bound what the
- * device may find (they size launches and scratch); tokens and rows behind them are left out. Blocks that a call writes belong to one of its sequences
- * only; read-only ones may be shared. Buffers of one call do not overlap; arrays are aligned to their elements, codes to 16 bytes. The _validate calls
+ * device may find (they size launches and scratch); tokens and rows behind them are left out. Blocks that a call writes (with weight_rows,
+ * all that a sequence sees) belong to one of its sequences only and stand once in its table; read-only ones may be shared. Buffers of one call do not overlap; arrays are aligned to their elements, codes to 16 bytes. The _validate calls
  * make the checks of the _encode ones (UZU_ERROR_INVALID_ARGUMENT) and need no device. */
 typedef enum uzu_cache_code { UZU_CACHE_CODE_I8 = 0, UZU_CACHE_CODE_E4M3 = 1 } uzu_cache_code;
 typedef struct uzu_quantized_cache {

@@ -413,6 +413,49 @@ def test_captured_calls_follow_the_device(ctx):
         assert np.array_equal(P.of_kept(out.numpy(np.uint16, (4, heads * dim)), P.BF16), want)
 
 
+@pytest.mark.parametrize("code", CODES)
+def test_captured_evictions(ctx, code):
+    """what a call counts and waits for begins anew in every replay, and the lengths are those that the device holds then"""
+    from tests.test_state_space_gpu import _captured
+    s = Served(ctx, code, 32, 2, 64, [190, 77, 64], room=200, seed=4)
+    s.evict(64, 4, 16)      # (a kernel's first launch sets its shared memory, which is not captured)
+    args = s.last
+    replay = _captured(ctx, lambda cmd: ctx.lib.uzu_quantized_cache_evict_encode(cmd, C.byref(args)))
+    for lengths in ([150, 3, 200], [64, 65, 0], [199, 199, 199]):
+        C.memmove(s.length_buffer.cpu_ptr, np.array(lengths + [0], np.uint32).ctypes.data, 16)
+        replay()
+        after = [s.plain.evict(s.table[i], min(n, s.capacity()), 64, 4, 16)[1] for i, n in enumerate(lengths)]
+        assert s.new_lengths.numpy(np.uint32, (4,)).tolist() == after + [77]
+        assert s.same()
+        assert np.array_equal(s.device_weights(), s.plain.weights)
+
+
+def test_captured_prompts(ctx):
+    """both kernels of a pass of prompts and single tokens: a replay gives what a call gives"""
+    from tests.test_state_space_gpu import _captured
+    heads = 8
+    s = Served(ctx, Q.I8, 32, 2, 64, [40, 99], room=300, seed=5)
+    s.append([90, 90], P.BF16)
+    q = s.rng.standard_normal((180, heads * 64))
+    kw = dict(query=q, tail=0, max_rows=170)
+    s.attend([90, 90], heads, P.BF16, **kw)
+    args, out, offsets, lengths = s.last, s.kept[-3], s.kept[-6], s.length_buffer
+    assert offsets.ptr == args.sequences.row_offsets and out.ptr == args.out
+    replay = _captured(ctx, lambda cmd: ctx.lib.uzu_quantized_cache_attention_encode(cmd, C.byref(args)))
+    for held, rows in (([40, 99], [90, 90]), ([100, 20], [10, 170]), ([10, 128], [179, 1])):
+        C.memmove(lengths.cpu_ptr, np.array(held + [0], np.uint32).ctypes.data, 12)
+        C.memmove(offsets.cpu_ptr, np.cumsum([0] + rows).astype(np.uint32).ctypes.data, 12)
+        replay()
+        got = out.get()[0]
+        s.set_lengths(held)
+        n = min(rows[0], 170)      # (rows behind max_rows are left out)
+        if n < rows[0]:
+            want = s.attend(rows, heads, P.BF16, check=False, **kw)[0]
+            assert np.array_equal(got[:n], want[:n]) and np.array_equal(got[rows[0]:], want[rows[0]:])
+        else:
+            assert np.array_equal(got, s.attend(rows, heads, P.BF16, **kw))
+
+
 def test_refused_calls_are_errors_of_their_buffer(ctx):
     s = Served(ctx, Q.I8, 32, 2, 64, [40], room=100)
     s.attend([1], 8, P.BF16)
@@ -490,6 +533,30 @@ def test_verify_a_certain_draft_with_all_of_p(ctx):
     u = np.array([[1.0, 0.5], [0.25, 0.999]])      # (the first is outside the range: the draft is not kept)
     got = verify(ctx, target, None, np.full((2, 1), 7), u, 1.0, 1.0, P.F32)
     assert got[1][0].tolist() == [7, NONE] and got[0].tolist() == [0, 1] and got[1][1, 0] == 7
+
+
+def test_captured_verification(ctx):
+    """a replay reads the drafts and uniform numbers that the device holds then"""
+    from tests.test_state_space_gpu import _captured
+    n, k, vocab = 3, 4, 5000
+    rng = np.random.default_rng(11)
+    target, draft, drafted, u = _case(rng, n, k, vocab)
+    t, d = (ctx.upload(x.reshape(-1, vocab).astype(np.float32)) for x in (target, draft))
+    dr, un = ctx.upload(drafted.astype(np.uint32)), ctx.upload(u.astype(np.float32))
+    tokens, accepted = ctx.upload(np.zeros((n, k + 1), np.uint32)), ctx.upload(np.zeros(n, np.uint32))
+    verify(ctx, target, draft, drafted, u, 1.0, 1.0, P.F32)
+    a = B.DraftVerifyArgs(target_logits=t.ptr, draft_logits=d.ptr, drafted=dr.ptr, uniforms=un.ptr, tokens=tokens.ptr, accepted=accepted.ptr, sequences=n, drafts=k, vocab=vocab, target_stride=vocab,
+                          draft_stride=vocab, temperature=1.0, draft_temperature=1.0, data_type=P.F32)
+    replay = _captured(ctx, lambda cmd: ctx.lib.uzu_draft_verify_encode(cmd, C.byref(a)))
+    for _ in range(3):
+        drafted, u = rng.integers(0, vocab, (n, k)), rng.random((n, k + 1))
+        drafted[0] = draft[0].argmax(1)
+        held = [np.ascontiguousarray(drafted, np.uint32), np.ascontiguousarray(u, np.float32)]
+        for buffer, x in zip((dr, un), held):
+            C.memmove(buffer.cpu_ptr, x.ctypes.data, x.nbytes)
+        replay()
+        acc, tok, _ = verify(ctx, target, draft, drafted, u, 1.0, 1.0, P.F32)
+        assert np.array_equal(accepted.numpy(np.uint32, (n,)), acc) and np.array_equal(tokens.numpy(np.uint32, (n, k + 1)), tok)
 
 
 def test_verify_draws_the_target(ctx):
