@@ -6,8 +6,8 @@
 // known from the f32 sums but for those where both are alike to 2^-22 or so, which have next to no weight either way; so the weights of the others are summed before their
 // divisors are known, numerators and denominators by themselves. Then the warp's run where the sum passes the aim is looked through by its whole CTA.
 // What bounds it: instructions (0.63 a cycle and scheduler) for exponentials of all rows and, at half rate, of two rows in f64; 74 million numbers and 16 million of them again. 64 sequences
-// of four drafts, vocabulary of 128256 (148 MB): 91 to 92 us; 427 with a row after another and the library's exponential in f64 three times, 212 with rows ahead and the series here, 112 with one
-// pass in f64 and sums by warps, 91 with registers for four CTAs an SM (one wave). One sequence: 85 -> 29 to 31 us.
+// of four drafts, vocabulary of 128256 (148 MB): 91 to 93 us; 427 with a row after another and the library's exponential in f64 three times, 212 with rows ahead and the series here, 112 with one
+// pass in f64 and sums by warps, 91 with registers for four CTAs an SM (one wave). One sequence: 85 -> 29 to 33 us.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
