@@ -72,12 +72,13 @@ __device__ __forceinline__ double dv_power(double y) {
     v = fma(v, f, 1.0);
     return __hiloint2double(__double2hiint(v) + (__double2loint(t) << 20), __double2loint(v));
 }
-// weights exp((x - most) / temperature) of a row whose largest number is `most`
+// weights exp((x - most) / temperature) of a row whose largest number is `most`. The difference first: x * k - most * k, most * k rounded, would be off by what a cold row's or large
+// numbers' k * most has of roundings, and the largest number's weight, 1, would be any other
 struct DvHeat {
-    double k, b;      // x k + b: the exponent of 2
-    __device__ __forceinline__ DvHeat(float most, float temperature) : k(1.4426950408889634074 / (double)temperature), b(-(double)most * k) {}
+    double most, k;      // (x - most) k: the exponent of 2
+    __device__ __forceinline__ DvHeat(float most, float temperature) : most((double)most), k(1.4426950408889634074 / (double)temperature) {}
     __device__ __forceinline__ double operator()(float x) const {
-        const double y = fma((double)x, k, b);
+        const double y = ((double)x - most) * k;
         return y >= -1000.0 ? dv_power(y) : 0.0;
     }
 };
