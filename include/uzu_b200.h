@@ -1114,13 +1114,13 @@ UZU_API size_t uzu_quantized_cache_evict_scratch_bytes(uzu_context* ctx, const u
 /* Verification of drafted tokens: which of a sequence's drafts the target model keeps, and the token behind them, so that the result is distributed as the
  * target's own samples are. With p_k = softmax(target_logits[i, k] / temperature), q_k = softmax(draft_logits[i, k] / draft_temperature):
  *   draft k = 0, 1, .. is kept while uniforms[i, k] * q_k(draft) < p_k(draft); behind the first that is not kept, the token is drawn from max(p_k - q_k, 0),
- *   behind the last draft from p (and from p where that difference is zero everywhere): the smallest token whose cumulative weight is more than
+ *   behind the last draft from p (and from p where that difference is 2^-44 or less in all): the smallest token whose cumulative weight is more than
  *   uniforms[i, drafts] times the sum of all.
  * Without draft_logits the drafts are certain (q = 1 at the draft). temperature 0: a draft is kept if it is the largest target logit (the lowest index of several),
  * and the token behind is that logit's; uniforms and draft_logits are not read then. draft_counts (optional, u32 [sequences], DEVICE): drafts of a sequence, at most `drafts`.
  * accepted u32 [sequences]; tokens u32 [sequences, drafts + 1]: the kept drafts, the token behind them, UZU_NO_TOKEN in the rest. Logits of -infinity have no
  * weight; rows without a distribution (a NaN or +infinity among the logits, or nothing above -infinity) keep no draft and give UZU_NO_TOKEN as the token behind;
- * a drafted token that is not below vocab is not kept. Sums that decide a token are f64. uniforms are in [0, 1); temperatures other than 0 at least 2^-60. */
+ * a drafted token that is not below vocab is not kept. Weights and sums that decide a token, a draft's too, are f64 (a weight within 2^-37 of itself). uniforms are in [0, 1); temperatures other than 0 at least 2^-60. */
 #define UZU_NO_TOKEN 0xFFFFFFFFu
 typedef struct uzu_draft_verify_args {
     uint64_t target_logits;        /* data_type [sequences * (drafts + 1), vocab], rows target_stride apart */

@@ -2,12 +2,13 @@
 //
 // A cluster of CTAs has a sequence; a warp has the same run of the vocabulary in every row, and asks for the next row's numbers before it sums up one's. One reading of all rows
 // gives each row's maximum and sum (f32 in a warp, f64 from there on); the CTAs exchange them and all come to the same first refusal. Only the row that a token is drawn from is read
-// again (it lies in L2), in f64, as is the draft's: where a sum of weights passes its aim must not depend on f32 roundings. One pass gives all its sums: which tokens have p > q is
-// known from the f32 sums but for those where both are alike to 2^-22 or so, which have next to no weight either way; so the weights of the others are summed before their
-// divisors are known, numerators and denominators by themselves. Then the warp's run where the sum passes the aim is looked through by its whole CTA.
+// again (it lies in L2), in f64, as is the draft's: where a sum of weights passes its aim must not depend on f32 roundings, nor must whether a draft is kept: one that the f32 sums leave open has its row read in
+// f64 as well. One pass gives all its sums: which tokens have p > q is known from the f32 sums but for those where both are alike to 2^-22 or so; so the weights of the others are summed before their
+// divisors are known, numerators and denominators by themselves, and once more, with the divisors, only where those few could matter. Then the warp's run where the sum passes the aim is looked through by its
+// whole CTA.
 // What bounds it: instructions (0.63 a cycle and scheduler) for exponentials of all rows and, at half rate, of two rows in f64; 74 million numbers and 16 million of them again. 64 sequences
-// of four drafts, vocabulary of 128256 (148 MB): 91 to 93 us; 427 with a row after another and the library's exponential in f64 three times, 212 with rows ahead and the series here, 112 with one
-// pass in f64 and sums by warps, 91 with registers for four CTAs an SM (one wave). One sequence: 85 -> 29 to 33 us.
+// of four drafts, vocabulary of 128256 (148 MB): 95 to 97 us; 427 with a row after another and the library's exponential in f64 three times, 212 with rows ahead and the series here, 112 with one
+// pass in f64 and sums by warps, 91 to 93 with registers for four CTAs an SM (one wave) and without the decisions in f64, which spill 44 bytes. One sequence: 85 -> 29 to 34 us.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -109,8 +110,8 @@ struct DvShared {
     DvRow part[DV_ROWS], row[DV_ROWS];      // this CTA's run; the whole vocabulary
     float row_most[DV_ROWS][WARPS], row_sum[DV_ROWS][WARPS];
     uint32_t row_index[DV_ROWS][WARPS];
-    double sums[4][WARPS], cta[4];
-    uint32_t accepted, token;
+    double sums[5][WARPS], cta[5];
+    uint32_t accepted, close, token;
 };
 
 template <typename T, bool WIDE, uint32_t WARPS, uint32_t CLUSTER>
@@ -218,89 +219,125 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 8 ? 4 : 1) draft_verify_k
     }
     __syncthreads();
 
-    // ---- the first draft that is not kept ----
-    if (warp == 0) {
-        bool kept = false;
-        if (lane < count) {
-            const uint32_t token = drafted[lane];
-            const DvRow& t = s.row[lane];
-            if (token < vocab && t.most == t.most) {
-                if (greedy) kept = token == t.index;
-                else {
-                    const double pt = DvHeat(t.most, a.temperature)(dv_f(row_of(lane)[token])) / t.sum;
-                    double qt = 1.0;
-                    if (with_draft) {
-                        const DvRow& d = s.row[count + 1 + lane];
-                        qt = d.most == d.most ? DvHeat(d.most, a.draft_temperature)(dv_f(row_of(count + 1 + lane)[token])) / d.sum : INFINITY;
-                    }
-                    kept = (double)uniforms[lane] * qt < pt;
-                }
-            }
-        }
-        const uint32_t refused = __ballot_sync(0xffffffffu, lane < count && !kept);
-        if (lane == 0) s.accepted = refused ? __ffs(refused) - 1 : count;
-    }
-    __syncthreads();
-    const uint32_t at_row = s.accepted;
-    const DvRow target = s.row[at_row];
-    const bool residual = at_row < count, against = residual && with_draft;
-    const DvRow other = against ? s.row[count + 1 + at_row] : target;
-    const bool valid = target.most == target.most && other.most == other.most;
+    // ---- the first draft that is not kept, and one row in f64: sums of p's and q's weights, and of both where p is above q ----
+    // The f32 sums say which drafts are kept, but for those whose u q is as near p as the sums may be off: by 2^-17 of themselves for exponents of 2^6 and their factor in 32 bits, and by what a group's additions
+    // and a new maximum's factor round, below 2^-21 a group. (A factor below f32's normal numbers has fewer bits: all drafts with p above a half of u q, then.) For such a draft the f64 sums of its row, which the
+    // token behind needs where it is refused, say whether it is kept.
+    const double margin = fminf(per_target, per_draft) < 0x1p-120f ? 1.0 : 0x1p-15 + 0x1p-20 * (double)((p.tiles + DV_GROUP - 1) / DV_GROUP);
+    uint32_t at_row = 0;
+    double parts[5], all[5];              // of CTA `lane`, of the whole vocabulary: p's weights, q's, both again where p is above q, p's where the two are alike within the margin
     auto answer = [&](uint32_t token) {
         if (tid < k1) reinterpret_cast<uint32_t*>(a.tokens)[(size_t)sequence * k1 + tid] = tid < at_row ? drafted[tid] : tid == at_row ? token : UZU_NO_TOKEN;
         if (tid == 0) reinterpret_cast<uint32_t*>(a.accepted)[sequence] = at_row;
     };
-    if (!valid || greedy) {      // (alike in all CTAs)
-        if (rank == 0) answer(valid ? target.index : UZU_NO_TOKEN);
-        cluster.sync();      // (nobody leaves while its parts are read)
-        return;
-    }
-    // ---- one row in f64: sums of p's and q's weights, and of both where p is above q ----
-    const T *row = row_of(at_row), *draft = against ? row_of(count + 1 + at_row) : row;
-    const DvHeat heat(target.most, a.temperature), draft_heat(other.most, against ? a.draft_temperature : a.temperature);
-    const uint32_t without = residual && !with_draft ? drafted[at_row] : UZU_NO_TOKEN;      // a certain draft has all of q
-    {
-        double sum[4] = {0.0, 0.0, 0.0, 0.0};
-        for (uint32_t t = 0; t < p.tiles; ++t) {
-            const uint32_t at = first + t * DV_TILE + lane * 8;
-            if (at >= vocab) break;
-            alignas(16) T x[8], y[8];
-            dv_load<T, WIDE>(row, at, vocab, x);
-            if (against) dv_load<T, WIDE>(draft, at, vocab, y);
-#pragma unroll 4
-            for (int i = 0; i < 8; ++i) {
-                const double w = at + i == without ? 0.0 : heat(dv_f(x[i]));
-                sum[0] += w;
-                if (!against) continue;
-                const double v = draft_heat(dv_f(y[i]));
-                sum[1] += v;
-                if (w * other.sum > v * target.sum) {
-                    sum[2] += w;
-                    sum[3] += v;
+#pragma unroll 1
+    for (uint32_t from = 0;; from = at_row + 1) {      // (alike in all CTAs; from: drafts before it are kept)
+        if (warp == 0) {
+            bool kept = false, close = false;
+            if (lane >= from && lane < count) {
+                const uint32_t token = drafted[lane];
+                const DvRow& t = s.row[lane];
+                if (token < vocab && t.most == t.most) {
+                    if (greedy) kept = token == t.index;
+                    else {
+                        const double pt = DvHeat(t.most, a.temperature)(dv_f(row_of(lane)[token])) / t.sum;
+                        double qt = 1.0;
+                        if (with_draft) {
+                            const DvRow& d = s.row[count + 1 + lane];
+                            qt = d.most == d.most ? DvHeat(d.most, a.draft_temperature)(dv_f(row_of(count + 1 + lane)[token])) / d.sum : INFINITY;
+                        }
+                        const double uq = (double)uniforms[lane] * qt;
+                        kept = uq < pt;
+                        close = pt > 0.0 && fabs(uq - pt) <= margin * pt;
+                    }
                 }
             }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (i && !against) break;
-            sum[i] = dv_warp_sum(sum[i]);
-            if (lane == 0) s.sums[i][warp] = sum[i];
+            const uint32_t open = __ballot_sync(0xffffffffu, lane >= from && lane < count && (!kept || close)), closes = __ballot_sync(0xffffffffu, close);
+            if (lane == 0) {
+                s.accepted = open ? __ffs(open) - 1 : count;
+                s.close = open & (0u - open) & closes;
+            }
         }
         __syncthreads();
-        if (warp < 4 && (warp == 0 || against)) {
-            const double v = dv_warp_sum(lane < WARPS ? s.sums[warp][lane] : 0.0);
-            if (lane == 0) s.cta[warp] = v;
+        at_row = s.accepted;
+        const bool close = s.close != 0;
+        const DvRow target = s.row[at_row];
+        const bool residual = at_row < count, against = residual && with_draft;
+        const DvRow other = against ? s.row[count + 1 + at_row] : target;
+        const bool valid = target.most == target.most && other.most == other.most;
+        if (!valid || greedy) {
+            if (rank == 0) answer(valid ? target.index : UZU_NO_TOKEN);
+            cluster.sync();      // (nobody leaves while its parts are read)
+            return;
         }
-        cluster.sync();
-    }
-    double parts[4] = {0.0, 0.0, 0.0, 0.0}, all[4] = {0.0, 0.0, 0.0, 0.0};      // of CTA `lane`, of the whole vocabulary
+        const T *row = row_of(at_row), *draft = against ? row_of(count + 1 + at_row) : row;
+        const DvHeat heat(target.most, a.temperature), draft_heat(other.most, against ? a.draft_temperature : a.temperature);
+        const uint32_t without = residual && !with_draft ? drafted[at_row] : UZU_NO_TOKEN;      // a certain draft has all of q
+        bool kept = false;
+        double per_w = other.sum, per_v = target.sum;      // p is above q where w / target.sum is above v / other.sum
+#pragma unroll 1
+        for (bool again = false;; again = true) {
+            double sum[5] = {0.0, 0.0, 0.0, 0.0, 0.0};
+            for (uint32_t t = 0; t < p.tiles; ++t) {
+                const uint32_t at = first + t * DV_TILE + lane * 8;
+                if (at >= vocab) break;
+                alignas(16) T x[8], y[8];
+                dv_load<T, WIDE>(row, at, vocab, x);
+                if (against) dv_load<T, WIDE>(draft, at, vocab, y);
+#pragma unroll 4
+                for (int i = 0; i < 8; ++i) {
+                    const double w = at + i == without ? 0.0 : heat(dv_f(x[i]));
+                    sum[0] += w;
+                    if (!against) continue;
+                    const double v = draft_heat(dv_f(y[i])), much = w * per_w, more = fma(-v, per_v, much);
+                    sum[1] += v;
+                    if (more > 0.0) {
+                        sum[2] += w;
+                        sum[3] += v;
+                    }
+                    if (fabs(more) <= margin * much) sum[4] += w;
+                }
+            }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (i && !against) break;
-        if (lane < CLUSTER) parts[i] = *cluster.map_shared_rank(&s.cta[i], lane);
-        all[i] = dv_warp_sum(parts[i]);
+            for (int i = 0; i < 5; ++i) {
+                if (i && !against) break;
+                sum[i] = dv_warp_sum(sum[i]);
+                if (lane == 0) s.sums[i][warp] = sum[i];
+            }
+            __syncthreads();
+            if (warp < 5 && (warp == 0 || against)) {
+                const double v = dv_warp_sum(lane < WARPS ? s.sums[warp][lane] : 0.0);
+                if (lane == 0) s.cta[warp] = v;
+            }
+            cluster.sync();
+#pragma unroll
+            for (int i = 0; i < 5; ++i) {
+                parts[i] = all[i] = 0.0;
+                if (i && !against) continue;
+                if (lane < CLUSTER) parts[i] = *cluster.map_shared_rank(&s.cta[i], lane);
+                all[i] = dv_warp_sum(parts[i]);
+            }
+            cluster.sync();      // (from here on, or until it sums up again, nobody reads another CTA's shared memory)
+            if (close && !again) {
+                const double w = heat(dv_f(row[drafted[at_row]]));
+                const double pt = w / (against ? all[0] : all[0] + w), qt = against ? draft_heat(dv_f(draft[drafted[at_row]])) / all[1] : 1.0;
+                kept = (double)uniforms[at_row] * qt < pt;
+                if (kept) break;
+            }
+            if (!against || again) break;
+            // How far the f32 sums' quotient was off, times p's share that is as near q as that: what the border between p and q may have moved. More than 2^-32 of the difference, as with a draft
+            // model that is nearly the target: once more with the sums of 64 bits.
+            const double off = fabs(other.sum * all[0] - target.sum * all[1]) / (target.sum * all[1]);
+            if (off <= margin && off * all[4] <= 0x1p-32 * (all[2] - all[3] * (all[0] / all[1]))) break;
+            per_w = all[1];
+            per_v = all[0];
+        }
+        if (!kept) break;
     }
-    cluster.sync();      // (from here on nobody reads another CTA's shared memory)
+    const bool residual = at_row < count, against = residual && with_draft;
+    const T *row = row_of(at_row), *draft = against ? row_of(count + 1 + at_row) : row;
+    const DvHeat heat(s.row[at_row].most, a.temperature), draft_heat(s.row[against ? count + 1 + at_row : at_row].most, against ? a.draft_temperature : a.temperature);
+    const uint32_t without = residual && !with_draft ? drafted[at_row] : UZU_NO_TOKEN;
     const double inv = against ? 1.0 / all[0] : 1.0, draft_inv = against ? 1.0 / all[1] : 0.0;
     double whole = against ? all[2] * inv - all[3] * draft_inv : all[0];
     const bool plain = !against || !(whole > 0x1p-44);      // (nothing is left of the difference but roundings: the target's own weights)
