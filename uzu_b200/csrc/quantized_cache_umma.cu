@@ -31,13 +31,13 @@ constexpr uint32_t QU_BLOCK = 128 * 128;               // bytes of 128 rows of 6
 constexpr uint32_t QU_SOFT_REGS = 184, QU_CONVERT_REGS = 72;
 static_assert(2 * QU_SOFT_REGS + 2 * QU_CONVERT_REGS == 4 * 128, "a warpgroup that asks for more than there are waits for good");
 
-constexpr float QU_NONE = 1000.0f;      // no unit yet; no largest scale of groups among which one has none
+constexpr float QU_NONE = 1000.0f;      // no unit yet; less than any (-): no largest scale, of groups among which one's is NaN
 struct alignas(16) QuGroup {
-    float key_scale, value_log, value_inverse, pad;              // log2 of the value scale, and 1 / it (of a scale that is 0, whose numbers are zeros in any unit: as if it were the largest)
+    float key_scale, value_log, value_inverse, none;             // log2 of the value scale, and 1 / it (of a scale that is 0, whose numbers are zeros in any unit, or NaN: as if it were the largest); NaN or 0
 };
 struct alignas(16) QuItem {
     uint32_t key0, groups, more;                                 // first key, which groups of 16 count, 0: no tile, the end
-    float largest;                                               // of value_log; QU_NONE where a scale is NaN
+    float largest;                                               // of value_log; -QU_NONE where a value scale is NaN
     QuGroup group[QU_GROUPS];
 };
 struct QuParams {
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(QU_THREADS, 1) quantized_cache_umma_kernel(con
                 const uint32_t group_bits = (groups & 1u ? 0xffffu : 0u) | (groups & 2u ? 0xffff0000u : 0u);
                 return live ? below(min(index + 1u, end)) & (~below(lowest) | below(a.keep_first)) & group_bits : 0u;
             };
-            float top = -INFINITY, sum = 0.0f, unit = QU_NONE, top_unit = -QU_NONE, unit_scale = 1.0f;      // (the unit's logarithm, and itself)
+            float top = -INFINITY, sum = 0.0f, unit = QU_NONE, top_unit = -QU_NONE, unit_scale = 1.0f, none = 0.0f;      // (the unit's logarithm, and itself; NaN: a value that the row sees is)
             auto capped = [&](float x) { return cap - 2.0f * cap * __frcp_rn(1.0f + qu_exp2(x)); };      // cap * tanh: within 2^-22 of the cap
             const uint32_t my_s = tm + r * 128u, my_o = tm + S::O_COL + r * 128u;
             for (uint32_t i = 0;; ++i) {
@@ -245,10 +245,15 @@ __global__ void __launch_bounds__(QU_THREADS, 1) quantized_cache_umma_kernel(con
                     sum *= times;
                 }
                 if (const float away = item.largest - unit; !whole || !(away <= 2.0f && away >= -2.0f)) {
+                    if (item.largest == -QU_NONE) {      // (weights are of scores alone and stay numbers: the output is not)
+#pragma unroll
+                        for (int g = 0; g < (int)QU_GROUPS; ++g)
+                            if (bits[g / 2] >> (16 * (g & 1)) & 0xffffu) none += item.group[g].none;
+                    }
                     float largest = -QU_NONE;      // of the groups that the row sees
 #pragma unroll
                     for (int g = 0; g < (int)QU_GROUPS; ++g)
-                        if (bits[g / 2] >> (16 * (g & 1)) & 0xffffu) largest = fmaxf(largest, item.group[g].value_log);      // (not NaN)
+                        if (bits[g / 2] >> (16 * (g & 1)) & 0xffffu) largest = fmaxf(largest, item.group[g].value_log);
                     if (largest > -QU_NONE && (unit == QU_NONE || largest > unit + 2.0f || largest < unit - 2.0f)) {
                         top_unit = fmaxf(top_unit, largest);
                         const float next = fmaxf(largest, top_unit - 80.0f);
@@ -315,7 +320,7 @@ __global__ void __launch_bounds__(QU_THREADS, 1) quantized_cache_umma_kernel(con
                     sum = sum * f + qu_exp2(sink - high + QU_LIFT);
                     scale *= f;
                 }
-                const float inv = sum != 0.0f ? scale / sum : 0.0f;      // (both sums are lifted)
+                const float inv = none != 0.0f ? none : sum != 0.0f ? scale / sum : 0.0f;      // (both sums are lifted)
                 if (p.stats && live) *reinterpret_cast<float2*>(p.stats + ((size_t)(q.row + token) * a.heads + h) * 2) = make_float2(high, sum != 0.0f ? (float)(1 << (int)QU_LIFT) / sum : 0.0f);
                 __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (live ? (size_t)(q.row + token) * a.out_stride + (size_t)h * dim : 0);
                 for (uint32_t n = 0; n < dim; n += 16) {      // (by whole warps; a row without weights has no products to read, or none of its own)
@@ -402,15 +407,15 @@ __global__ void __launch_bounds__(QU_THREADS, 1) quantized_cache_umma_kernel(con
                 QuItem& item = items[n % QU_ITEMS];
                 const uint32_t among = vs > 0.0f && (take >> lane & 1u) ? __float_as_uint(vs) : 0u, largest = __reduce_max_sync(0xffffffffu, among);
                 const bool nan = __any_sync(0xffffffffu, (take >> lane & 1u) && vs != vs);
-                // (a scale of 0 goes as the largest; so do groups that do not count)
+                // (a scale of 0 or NaN goes as the largest; so do groups that do not count)
                 const uint32_t as = among ? among : largest ? largest : 0x3f800000u;
                 const float log = (float)((int)(as >> 23) - 127);
-                if (lane < QU_GROUPS) item.group[lane] = QuGroup{ks, vs != vs && (take >> lane & 1u) ? vs : log, cache_inverse(__uint_as_float(as)), 0.0f};
+                if (lane < QU_GROUPS) item.group[lane] = QuGroup{ks, log, cache_inverse(__uint_as_float(as)), vs != vs && (take >> lane & 1u) ? vs : 0.0f};
                 if (lane == 0) {
                     item.key0 = key0;
                     item.groups = take;
                     item.more = 1;
-                    item.largest = nan ? QU_NONE : (float)((int)((largest ? largest : 0x3f800000u) >> 23) - 127);
+                    item.largest = nan ? -QU_NONE : (float)((int)((largest ? largest : 0x3f800000u) >> 23) - 127);
                 }
             }
             const uint32_t s = n % QU_STAGES, to = stage0 + s * S::KV;
