@@ -1,4 +1,4 @@
-"""The 8-bit cache's attention at the ends of its range: values that are no numbers beside weights that are summed."""
+"""The 8-bit cache's attention at the ends of its range: values that are no numbers beside weights that are summed, queries of any size."""
 import numpy as np
 import pytest
 
@@ -29,3 +29,14 @@ def test_weights_beside_values_that_are_no_numbers(ctx, dt, apart, lengths, rows
         assert np.isnan(got).any() and not np.isnan(got).all()
         s.attend(rows, 4, dt, window=30, weight_rows=ALL)
         s.attend(rows, 4, dt, window=50, first=8, cap=20.0, sinks=[0.5, -1.0, 0.0, 3.0], weight_rows=5)
+
+
+@pytest.mark.parametrize("dt,power", [(P.F32, 123), (P.BF16, 123), (P.F32, 116), (P.BF16, 116), (P.F32, -121), (P.BF16, -121), (P.F32, -100), (P.BF16, -100)])
+@pytest.mark.parametrize("rows", [[3], [40]])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_queries_of_any_size(ctx, dt, power, rows, cap):
+    """finite queries from one end of the type to the other, with a scale that makes scores of them"""
+    s = Served(ctx, Q.I8, 32, 1, 64, [70], room=200)
+    s.append(rows, P.F32)
+    x = np.clip(s.rng.standard_normal((rows[0] + 2, 4 * 64)), -7, 7) * 2.0 ** power
+    s.attend(rows, 4, dt, query=x, scale=2.0 ** -(power + 3), cap=cap, weight_rows=2)

@@ -12,6 +12,8 @@ namespace uzu {
 constexpr uint32_t kCacheHugeBits = 0x6f800000u;      // 2^96
 constexpr int kCacheLeastExponent = -100;
 constexpr uint32_t kNoIndex = 0xffffffffu;
+// A row of queries is brought to 2^14 .. 2^15 by a power of two, from 2^-113 for the largest numbers on up to this: 2^-126, its inverse, is still a normal number. Rows below 2^-112 stay below 2^14.
+constexpr int kCacheMostPower = 126;
 // What the kernel for few rows takes where the tcgen05 kernel takes the others: sequences of so many (row, head) pairs of a key head, or of so few rows. The latter has no split of the
 // keys, so one CTA would read a long cache for a few rows of many heads.
 constexpr uint32_t kCacheFewPairs = 64, kCacheFewRows = 8;

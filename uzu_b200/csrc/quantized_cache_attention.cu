@@ -160,9 +160,9 @@ __device__ __forceinline__ void qa_query(const QaParams& p, const CacheSequence&
         const uint32_t u = warp + e * QA_WARPS, n = u % NT, s = u / NT;
         if (u >= UNITS) continue;
         const uint32_t most = most_of[n * 8 + g];
-        const int power = most ? max(-100, min(100, 14 + 127 - (int)(most >> 23))) : 0;
+        const int power = most ? min(kCacheMostPower, 14 + 127 - (int)(most >> 23)) : 0;
         const float up = __uint_as_float((uint32_t)(power + 127) << 23), down = __uint_as_float((uint32_t)(127 - power) << 23);
-        if (s == 0 && c == 0) factor[n * 8 + g] = most >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : a.softcap > 0.0f ? a.scale / a.softcap * down : a.scale * 1.4426950408889634f * down;
+        if (s == 0 && c == 0) factor[n * 8 + g] = most >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : a.softcap > 0.0f ? a.scale * down / a.softcap : a.scale * down * 1.4426950408889634f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             float y[4];

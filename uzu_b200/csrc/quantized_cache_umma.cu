@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(QU_THREADS, 1) quantized_cache_umma_kernel(con
                 for (int k = 0; k < 4; ++k) most_bits = max(most_bits, max(ws[k] & 0x7fffu, ws[k] >> 16 & 0x7fffu));
             }
             most_bits <<= 16;
-            const int e = most_bits ? max(-100, min(100, 14 + 127 - (int)(most_bits >> 23))) : 0;
+            const int e = most_bits ? min(kCacheMostPower, 14 + 127 - (int)(most_bits >> 23)) : 0;
             const float up = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
             const uint32_t my_q = q0 + r * S::Q + lr * 128u;
             for (uint32_t i = 0; i < dim / 8; ++i) {
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(QU_THREADS, 1) quantized_cache_umma_kernel(con
             um_fence_proxy();
             um_arrive(q_full(r));
             // of a score in units of ln 2, or (capped) of a fraction of the cap, doubled and in units of ln 2 as the exponential takes it
-            const float factor = most_bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : (CAP ? 2.0f * a.scale / a.softcap : a.scale) * 1.4426950408889634f * down;
+            const float factor = most_bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : (CAP ? 2.0f * (a.scale * down) / a.softcap : a.scale * down) * 1.4426950408889634f;
             const float cap = a.softcap * 1.4426950408889634f;
             const uint32_t index = q.length + token, lowest = a.window && index >= a.window ? index - a.window + 1u : 0u, tm = tmem + ((warp & 3u) << 21);
             // bits of the keys [first, first + 32) that the row sees
