@@ -1075,7 +1075,8 @@ UZU_API uzu_status uzu_quantized_cache_read_validate(const uzu_quantized_cache_r
  * query and out are whole 16-byte groups: weights are one f16 number there (11 bits, or within 2^-22 of the row's largest).
  * Sums run in an order that the shapes, the lengths and max_length set.
  * scratch: of uzu_quantized_cache_attention_scratch_bytes() bytes, 256-byte aligned, its first 64 KB zero before the first use; every call leaves it ready for the next,
- * of any sizes. Calls that may run at the same time do not share it. */
+ * of any sizes. The size is enough for all calls with at most these count, rows, max_rows and max_length of a cache of these heads and channels, with the same heads, window and keep_first, and any
+ * weight_rows if it is not 0 here; pointers, strides, types and scale may be any then (and need not be there yet). Calls that may run at the same time do not share it. */
 typedef struct uzu_quantized_cache_attention_args {
     uzu_quantized_cache cache;
     uzu_cache_sequences sequences;

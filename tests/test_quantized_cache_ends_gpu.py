@@ -1,14 +1,18 @@
-"""The 8-bit cache's attention at the ends of its range: values that are no numbers beside weights that are summed, queries of any size."""
+"""The 8-bit cache's attention at the ends of its range: values that are no numbers beside weights that are summed, queries of any size, one scratch for calls of many sizes."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 from tests import quantized_cache_plain as Q
 from tests import state_space_plain as P
 from tests.quantized_cache_gpu import Served
+from uzu_b200 import binding as B
 
 pytestmark = pytest.mark.gpu
 
 ALL = 0xFFFFFFFF
+TYPES = [P.BF16, P.F32, P.F16]
 
 
 @pytest.mark.parametrize("dt,apart", [(P.BF16, False), (P.F32, False), (P.F16, False), (P.BF16, True), (P.F32, True)])      # (values of 2^40 are no f16 numbers)
@@ -40,3 +44,29 @@ def test_queries_of_any_size(ctx, dt, power, rows, cap):
     s.append(rows, P.F32)
     x = np.clip(s.rng.standard_normal((rows[0] + 2, 4 * 64)), -7, 7) * 2.0 ** power
     s.attend(rows, 4, dt, query=x, scale=2.0 ** -(power + 3), cap=cap, weight_rows=2)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("dim,heads", [(64, 8), (128, 8), (64, 2), (256, 4)])
+def test_one_scratch_for_many_calls(ctx, dt, dim, heads):
+    """what is asked for before there are pointers, for the largest pass, is enough for every smaller one, wherever its rows are"""
+    s = Served(ctx, Q.I8, 32, 2, dim, [300, 280, 5], room=420)
+    most = [70, 9, 70]
+    s.append(most, P.F32)
+    a = B.QuantizedCacheAttentionArgs(cache=s.cache(), sequences=s.sequences(most, sum(most) + 2), heads=heads, query_row_stride=heads * dim, query_head_stride=dim, out_stride=heads * dim, weight_rows=ALL,
+                                      scale=0.125, data_type=dt)
+    size = ctx.lib.uzu_quantized_cache_attention_scratch_bytes(ctx.h, C.byref(a))
+    scratch = ctx.upload(np.zeros(size, np.uint8))
+    before = s.device_weights()
+    for rows, kw in (([70, 9, 70], dict()), ([70, 9, 70], dict(shift=1, stride=heads * dim + 3)), ([17, 9, 3], dict(shift=1)), ([17, 9, 3], dict()), ([9, 8, 9], dict(scale=-0.125)), ([1, 1, 1], dict(window=40, first=3)),
+                     ([5, 4, 5], dict(weight_rows=0)), ([33, 0, 0], dict(max_length=333)), ([0, 5, 1], dict(cap=30.0))):
+        kw = dict(dict(weight_rows=ALL), **kw)
+        query = s.rng.standard_normal((sum(rows) + 2, heads * dim))
+        want, _ = s.attend(rows, heads, dt, query=query, check=False, **kw)
+        b, out = B.QuantizedCacheAttentionArgs.from_buffer_copy(s.last), s.kept[-3]
+        assert out.ptr == b.out and b.scratch_bytes <= size, (rows, kw, b.scratch_bytes, size)
+        # the same call once more in the large scratch: the same bits
+        b.scratch, b.scratch_bytes = scratch.ptr, size
+        s.run("attention", ("uzu_quantized_cache_attention_encode", b))
+        assert np.array_equal(out.get()[0], want)
+    assert np.isfinite(before).all()

@@ -784,42 +784,81 @@ struct QaPlan {
     uint32_t score_pairs, score_stride;      // 0: scores are not kept
     uint64_t partial_bytes, stats_bytes, score_bytes;
 };
+// how so many pairs of a key head of each sequence would be taken
+struct QaWays {
+    uint32_t eights, tiles;
+    uint64_t ctas, slots, most_splits;
+};
+QaWays qa_ways(uint32_t sm_count, const uzu_quantized_cache_attention_args& a, uint64_t pairs) {
+    QaWays w{};
+    const uzu_cache_sequences& s = a.sequences;
+    const uint32_t capacity = cache_capacity(s, a.cache.block_tokens);
+    // tiles as wide as registers allow: a tile reads its keys once
+    w.eights = pairs <= 8 ? 1 : a.cache.head_dim <= 64 && pairs > 16 ? (pairs <= 24 ? 3 : 4) : 2;
+    w.tiles = (uint32_t)((pairs + w.eights * 8 - 1) / (w.eights * 8));
+    w.ctas = (uint64_t)s.count * a.cache.kv_heads * w.tiles;
+    w.slots = (uint64_t)sm_count * (a.cache.head_dim > 128 ? 1 : 3);
+    const uint64_t keys = a.window ? std::min<uint64_t>(capacity, (uint64_t)a.window + std::min(s.max_rows, s.rows) + a.keep_first + 32) : capacity, steps = (keys + QA_STEP - 1) / QA_STEP;
+    w.most_splits = std::min<uint64_t>((steps + QA_WARPS - 1) / QA_WARPS, 128);
+    return w;
+}
+uint64_t qa_partial_bytes(const uzu_quantized_cache_attention_args& a, uint64_t parts, uint32_t eights) { return parts * eights * 8 * (a.cache.head_dim + 2) * 4; }
+uint64_t qa_stats_bytes(const uzu_quantized_cache_attention_args& a) { return (uint64_t)a.sequences.rows * a.heads * 8; }
+uint64_t qa_score_pairs(const uzu_quantized_cache_attention_args& a) {
+    return std::min<uint64_t>((uint64_t)std::min(a.sequences.max_rows, a.sequences.rows) * (a.heads / a.cache.kv_heads), kCacheFewPairs);
+}
+uint64_t qa_score_stride(const uzu_quantized_cache_attention_args& a) { return ((uint64_t)cache_capacity(a.sequences, a.cache.block_tokens) + 63) & ~63ull; }
+// (more than QA_SCORES: any number above it, so that nothing overflows)
+uint64_t qa_score_bytes(const uzu_quantized_cache_attention_args& a) {
+    const uint64_t rows = (uint64_t)a.sequences.count * a.cache.kv_heads * qa_score_pairs(a), row = qa_score_stride(a) * 4;
+    return rows && row > QA_SCORES / rows ? QA_SCORES + 1 : rows * row;
+}
+
 QaPlan qa_plan(uint32_t sm_count, const uzu_quantized_cache_attention_args& a) {
     QaPlan p{};
     const uzu_cache_sequences& s = a.sequences;
-    const uint32_t capacity = cache_capacity(s, a.cache.block_tokens);
     p.group = a.heads / a.cache.kv_heads;
     const uint32_t most_rows = std::min(s.max_rows, s.rows);
     const uint64_t most_pairs = (uint64_t)most_rows * p.group;
     p.few = quantized_cache_umma_applicable(a) ? kCacheFewPairs : 0xffffffffu;
-    // tiles as wide as registers allow: a tile reads its keys once
-    const uint64_t pairs = std::min<uint64_t>(most_pairs, std::max<uint64_t>(p.few, (uint64_t)std::min(most_rows, kCacheFewRows) * p.group));
-    p.eights = pairs <= 8 ? 1 : a.cache.head_dim <= 64 && pairs > 16 ? (pairs <= 24 ? 3 : 4) : 2;
-    p.tiles = (uint32_t)((pairs + p.eights * 8 - 1) / (p.eights * 8));
-    const uint64_t ctas = (uint64_t)s.count * a.cache.kv_heads * p.tiles;
-    const uint64_t keys = a.window ? std::min<uint64_t>(capacity, (uint64_t)a.window + most_rows + a.keep_first + 32) : capacity, steps = (keys + QA_STEP - 1) / QA_STEP;
+    const QaWays w = qa_ways(sm_count, a, std::min<uint64_t>(most_pairs, std::max<uint64_t>(p.few, (uint64_t)std::min(most_rows, kCacheFewRows) * p.group)));
+    p.eights = w.eights;
+    p.tiles = w.tiles;
     p.splits = 1;
-    if (ctas && ctas <= QA_TICKETS) {
+    if (w.ctas && w.ctas <= QA_TICKETS) {
         // one wave where the tiles are few (a CTA too many would double the time), else parts short enough for lengths that differ
-        const uint64_t slots = (uint64_t)sm_count * (a.cache.head_dim > 128 ? 1 : 3), wanted = ctas <= slots ? slots / ctas : (2 * slots + ctas - 1) / ctas;
-        p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({wanted, (steps + QA_WARPS - 1) / QA_WARPS, 128}));
+        const uint64_t wanted = w.ctas <= w.slots ? w.slots / w.ctas : (2 * w.slots + w.ctas - 1) / w.ctas;
+        p.splits = (uint32_t)std::max<uint64_t>(1, std::min(wanted, w.most_splits));
     }
-    if (p.splits > 1) p.partial_bytes = ctas * p.splits * p.eights * 8 * (a.cache.head_dim + 2) * 4;
+    if (p.splits > 1) p.partial_bytes = qa_partial_bytes(a, w.ctas * p.splits, p.eights);
     if (a.weight_rows) {
-        p.stats_bytes = (uint64_t)s.rows * a.heads * 8;
-        const uint64_t stride = ((uint64_t)capacity + 63) & ~63ull, most = std::min<uint64_t>(most_pairs, kCacheFewPairs), bytes = (uint64_t)s.count * a.cache.kv_heads * most * stride * 4;
-        if (most_pairs <= kCacheFewPairs || p.few == kCacheFewPairs) {
-            if (bytes <= QA_SCORES) {
-                p.score_pairs = (uint32_t)most;
-                p.score_stride = (uint32_t)stride;
-                p.score_bytes = bytes;
-            }
+        p.stats_bytes = qa_stats_bytes(a);
+        const uint64_t bytes = qa_score_bytes(a);
+        if ((most_pairs <= kCacheFewPairs || p.few == kCacheFewPairs) && bytes <= QA_SCORES) {
+            p.score_pairs = (uint32_t)qa_score_pairs(a);
+            p.score_stride = (uint32_t)qa_score_stride(a);
+            p.score_bytes = bytes;
         }
     }
     return p;
 }
 uint64_t qa_align(uint64_t v) { return (v + 255) & ~255ull; }
 uint64_t qa_scratch(const QaPlan& p) { return QA_TICKETS * 4 + qa_align(p.partial_bytes) + qa_align(p.stats_bytes) + p.score_bytes; }
+// Enough for the plans of all calls with at most these sequences, rows and lengths, wherever rows are and whatever the scale is. Which kernel has a sequence, and with it the pairs here, hangs on those; and fewer
+// tiles have more splits: their product is at most one wave, or with more tiles than that two waves and the tiles, as long as there are splits at all.
+uint64_t qa_scratch_of_all(uint32_t sm_count, const uzu_quantized_cache_attention_args& a) {
+    const QaWays w = qa_ways(sm_count, a, (uint64_t)std::min(a.sequences.max_rows, a.sequences.rows) * (a.heads / a.cache.kv_heads));
+    QaPlan p{};
+    if (w.most_splits > 1) {
+        const uint64_t ctas = std::min(w.ctas, 4 * w.slots), parts = std::min(ctas * w.most_splits, ctas <= w.slots ? w.slots : std::min(4 * w.slots, 2 * w.slots + ctas));
+        p.partial_bytes = qa_partial_bytes(a, parts, w.eights);
+    }
+    if (a.weight_rows) {
+        p.stats_bytes = qa_stats_bytes(a);
+        p.score_bytes = std::min(qa_score_bytes(a), QA_SCORES);
+    }
+    return qa_scratch(p);
+}
 
 const char* attention_check(const uzu_quantized_cache_attention_args* a) {
     if (!a) return "null arguments";
@@ -898,7 +937,7 @@ extern "C" {
 
 size_t uzu_quantized_cache_attention_scratch_bytes(uzu_context* ctx, const uzu_quantized_cache_attention_args* a) {
     if (!ctx || !a || check_cache(a->cache) || check_cache_sequences(a->sequences, true) || !a->heads || a->heads % a->cache.kv_heads) return 0;
-    return qa_scratch(qa_plan(ctx->sm_count, *a));
+    return qa_scratch_of_all(ctx->sm_count, *a);
 }
 
 uzu_status uzu_quantized_cache_attention_validate(const uzu_quantized_cache_attention_args* a) {
