@@ -1070,13 +1070,13 @@ UZU_API uzu_status uzu_quantized_cache_read_validate(const uzu_quantized_cache_r
  *   out[t, h, :] = sum_j w_j value_j      (zeros for a row that sees nothing)
  *   weight_rows > 0: key_weights[j, g] += sum of w_j over the last weight_rows rows of a sequence and the heads of group g (0xffffffff: all its rows)
  * A query that is not finite makes its row NaN. Scores, weights and sums are f32. bf16 and f16 queries enter the products as they are, f32 ones as two f16
- * parts (22 bits, relative to the row's largest), capped scores of 16-bit rows are within 2^-22 of the cap; weights as two f16 parts (22 bits, or within 2^-40 of the row's largest weight). A sequence's
- * bf16 rows of up to 128 channels run on tcgen05 (csrc/quantized_cache_umma.cu) where they are more than 8 and more than 64 pairs of a row and a head of a key head's group, scale is above 0 and
+ * parts (22 bits, relative to the row's largest, from 2^-112 on), capped scores of 16-bit rows are within 2^-22 of caps of up to 64; weights as two f16 parts (22 bits, or within 2^-40 of the row's largest weight). A sequence's
+ * bf16 rows of up to 128 channels run on tcgen05 (csrc/quantized_cache_umma.cu) where they are more than 8 and more than 64 pairs of a row and a head of a key head's group, scale is above 0, the cap at most 64 and
  * query and out are whole 16-byte groups: weights are one f16 number there (11 bits, or within 2^-22 of the row's largest).
  * Sums run in an order that the shapes, the lengths and max_length set.
  * scratch: of uzu_quantized_cache_attention_scratch_bytes() bytes, 256-byte aligned, its first 64 KB zero before the first use; every call leaves it ready for the next,
  * of any sizes. The size is enough for all calls with at most these count, rows, max_rows and max_length of a cache of these heads and channels, with the same heads, window and keep_first, and any
- * weight_rows if it is not 0 here; pointers, strides, types and scale may be any then (and need not be there yet). Calls that may run at the same time do not share it. */
+ * weight_rows if it is not 0 here; pointers, strides, types, scale and cap may be any then (and need not be there yet). Calls that may run at the same time do not share it. */
 typedef struct uzu_quantized_cache_attention_args {
     uzu_quantized_cache cache;
     uzu_cache_sequences sequences;

@@ -1,4 +1,4 @@
-"""The 8-bit cache's attention at the ends of its range: values that are no numbers beside weights that are summed, queries of any size, one scratch for calls of many sizes."""
+"""The 8-bit cache's attention at the ends of its range: values that are no numbers beside weights that are summed, queries and caps of any size, one scratch for calls of many sizes."""
 import ctypes as C
 
 import numpy as np
@@ -70,3 +70,38 @@ def test_one_scratch_for_many_calls(ctx, dt, dim, heads):
         s.run("attention", ("uzu_quantized_cache_attention_encode", b))
         assert np.array_equal(out.get()[0], want)
     assert np.isfinite(before).all()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("cap", [1e-38, 1e-12, 1e-3, 60.0, 1e3, 1e5, 1e9, 3e38])
+@pytest.mark.parametrize("rows,heads", [([3, 1], 4), ([40, 50], 4), ([90, 20], 8)])
+def test_caps_of_any_size(ctx, dt, cap, rows, heads):
+    """a cap far above the scores leaves them as they are, one far below makes them alike"""
+    s = Served(ctx, Q.I8, 32, 2, 64, [70, 130], room=260)
+    s.append(rows, P.F32)
+    cap = float(np.float32(cap))
+    query = s.rng.standard_normal((sum(rows) + 2, heads * 64))
+    before = s.device_weights()
+    got, grown = s.attend(rows, heads, dt, query=query, cap=cap, weight_rows=ALL, check=False)
+    assert np.isfinite(got).all()
+    at, want_weights = 0, before.copy()
+    slack = np.zeros_like(before)
+    for i, n in enumerate(rows):
+        mine = P.of_kept(P.to_kept(query[at:at + n], dt), dt).reshape(n, heads, 64)
+        tensor = dt == P.BF16 and n > 8 and n * heads // 2 > 64
+        ref, bound, grow, grow_bound = s.plain.attend(s.table[i], s.lengths[i], mine, s.capacity(), float(np.float32(0.125)), cap=cap, weight_rows=ALL, q_error=2.0 ** -22 if dt == P.F32 else 0.0, tensor=tensor)
+        # Capped scores of 16-bit rows may be off by 2^-21 of caps of up to 64, with larger ones by two units in the last place of themselves, as f32 rows' are: each weight by twice that, scores' and the largest's
+        off = 2 * (2.0 ** -21 * cap if dt != P.F32 and cap <= 64 else 2.0 ** -21 * min(cap, 40.0))
+        bound += off * 2 * np.abs(s.plain.numbers(1, s.table[i], np.arange(s.lengths[i] + n))[0]).max()
+        grow_bound += off * 2 * grow
+        assert np.abs(ref).max() > 0.01
+        tol = P.HALF_STEP[dt] * (np.abs(ref) + bound) + P.TINY[dt] + bound
+        worst = np.abs(got[at:at + n].reshape(ref.shape) - ref) / tol
+        assert worst.max() <= 1, (i, float(worst.max()))
+        tokens = np.arange(len(grow))
+        b = s.table[i][tokens // 32]
+        want_weights[b, :, tokens % 32] += grow
+        slack[b, :, tokens % 32] += grow_bound
+        at += n
+    after = s.device_weights()
+    assert (np.abs(after - want_weights) <= slack + 2.0 ** -24 * (1 + max(rows) * heads / 16) * np.abs(want_weights) + 1e-30).all()

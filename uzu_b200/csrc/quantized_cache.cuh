@@ -14,6 +14,9 @@ constexpr int kCacheLeastExponent = -100;
 constexpr uint32_t kNoIndex = 0xffffffffu;
 // A row of queries is brought to 2^14 .. 2^15 by a power of two, from 2^-113 for the largest numbers on up to this: 2^-126, its inverse, is still a normal number. Rows below 2^-112 stay below 2^14.
 constexpr int kCacheMostPower = 126;
+// Capped scores of 16-bit rows come of 1 - 2 / (1 + e^2x), which is off by 2^-22 of the cap whatever the score: up to this cap 2^-16, an eighth of what an f16 output's rounding moves. Above it tanhf, in the kernel for
+// few rows. Caps are brought between the other two, where 1 / cap and its products stay normal numbers: below 2^-40 all weights are alike, and above 2^80 scores of up to 2^68 are left as they are, in f32.
+constexpr float kCacheFastCap = 64.0f, kCacheLeastCap = 0x1p-40f, kCacheMostCap = 0x1p80f;
 // What the kernel for few rows takes where the tcgen05 kernel takes the others: sequences of so many (row, head) pairs of a key head, or of so few rows. The latter has no split of the
 // keys, so one CTA would read a long cache for a few rows of many heads.
 constexpr uint32_t kCacheFewPairs = 64, kCacheFewRows = 8;

@@ -240,10 +240,17 @@ __device__ __forceinline__ void qa_scores(const Query& query, Word word, const f
     }
     if (softcap > 0.0f) {
         const float cap = softcap * 1.4426950408889634f;
+        if (PARTS == 1 && softcap <= kCacheFastCap) {      // (within 2^-22 of the cap, for a fifth of the instructions)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][i] = cap * (PARTS == 1 ? qa_tanh(s[n][i]) : tanhf(s[n][i]));      // (of 16-bit rows within 2^-22 of the cap, for a fifth of the instructions)
+                for (int i = 0; i < 4; ++i) s[n][i] = cap * qa_tanh(s[n][i]);
+        } else {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[n][i] = cap * tanhf(s[n][i]);
+        }
     }
 }
 
@@ -945,12 +952,15 @@ uzu_status uzu_quantized_cache_attention_validate(const uzu_quantized_cache_atte
     return e ? fail(UZU_ERROR_INVALID_ARGUMENT, std::string("quantized_cache_attention: ") + e) : UZU_OK;
 }
 
-void uzu_quantized_cache_attention_encode(uzu_command_buffer* cmd, const uzu_quantized_cache_attention_args* a) {
+void uzu_quantized_cache_attention_encode(uzu_command_buffer* cmd, const uzu_quantized_cache_attention_args* args) {
     if (!encodable(cmd, "quantized_cache_attention")) return;
-    if (const char* e = attention_check(a)) {
+    if (const char* e = attention_check(args)) {
         cmd->record_error(UZU_ERROR_INVALID_ARGUMENT, std::string("quantized_cache_attention: ") + e);
         return;
     }
+    uzu_quantized_cache_attention_args within = *args;
+    if (within.softcap > 0.0f) within.softcap = std::min(std::max(within.softcap, kCacheLeastCap), kCacheMostCap);
+    const uzu_quantized_cache_attention_args* const a = &within;
     if (!a->sequences.count || !a->sequences.rows || !a->sequences.max_rows) return;
     const QaPlan plan = qa_plan(cmd->ctx->sm_count, *a);
     if (a->scratch_bytes < qa_scratch(plan)) {

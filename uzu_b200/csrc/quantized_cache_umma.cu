@@ -541,7 +541,7 @@ void qu_launch(uzu_command_buffer* cmd, const QuParams& p, dim3 grid) {
 }  // namespace
 
 bool quantized_cache_umma_applicable(const uzu_quantized_cache_attention_args& a) {
-    return a.data_type == UZU_DT_BF16 && a.cache.head_dim <= 128 && a.scale > 0.0f && ((a.query | a.out) & 15u) == 0 && a.query_row_stride % 8 == 0 && a.query_head_stride % 8 == 0 && a.out_stride % 8 == 0 &&
+    return a.data_type == UZU_DT_BF16 && a.cache.head_dim <= 128 && a.scale > 0.0f && a.softcap <= kCacheFastCap && ((a.query | a.out) & 15u) == 0 && a.query_row_stride % 8 == 0 && a.query_head_stride % 8 == 0 && a.out_stride % 8 == 0 &&
            std::min(a.sequences.max_rows, a.sequences.rows) > kCacheFewRows && (uint64_t)std::min(a.sequences.max_rows, a.sequences.rows) * (a.heads / a.cache.kv_heads) > kCacheFewPairs;
 }
 
