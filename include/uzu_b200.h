@@ -1095,7 +1095,8 @@ UZU_API size_t uzu_quantized_cache_attention_scratch_bytes(uzu_context* ctx, con
 /* Sequences of more than `budget` tokens cut down to `budget`, each key head by itself: the first keep_first tokens, the last keep_last, and of those between
  * the ones with the largest key_weights (the lower index wins a tie, NaN comes last). They move up in their order to tokens 0 .. budget - 1 of the same
  * table, blocks are coded anew as if their tokens had been appended to begun-anew blocks in one pass, and key_weights move along. Sequences of at most `budget` tokens
- * are left as they are. Tables stay; the blocks behind budget are the caller's to use again. sequences.row_offsets, rows and max_rows are not used.
+ * are left as they are. Tables stay; the blocks behind budget are the caller's to use again. From then on a token is counted by its new place, another one in each key head: attention's window and keep_first go by
+ * places, while rotations and other positions of new rows go on from the true ones. sequences.row_offsets, rows and max_rows are not used.
  * new_lengths u32 [count]: min(length, budget), not the same array as lengths. indices (optional, u32 [count, kv_heads, budget]): the token that each kept
  * one was, 0xffffffff behind the last.
  * scratch: of uzu_quantized_cache_evict_scratch_bytes() bytes, 256-byte aligned, content free before and after. Calls that may run at the same time do not
