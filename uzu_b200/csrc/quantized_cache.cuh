@@ -18,7 +18,9 @@ constexpr int kCacheMostPower = 126;
 // few rows. Caps are brought between the other two, where 1 / cap and its products stay normal numbers: below 2^-40 all weights are alike, and above 2^80 scores of up to 2^68 are left as they are, in f32.
 constexpr float kCacheFastCap = 64.0f, kCacheLeastCap = 0x1p-40f, kCacheMostCap = 0x1p80f;
 // What the kernel for few rows takes where the tcgen05 kernel takes the others: sequences of so many (row, head) pairs of a key head, or of so few rows. The latter has no split of the
-// keys, so one CTA would read a long cache for a few rows of many heads.
+// keys, so one CTA would read a long cache for a few rows of many heads. The border is where the other kernel needs a second tile of pairs; for one sequence alone the two cross later.
+// One sequence, 32 heads of 128 on 8 (i8), us on tcgen05 / in the other kernel, behind 4096 tokens: 17 rows 78 / 30, 64 rows 94 / 66, 128 rows 95 / 125; behind 131072: 17 rows 2275 / 467, 64 rows 2676 / 1608, 128
+// rows 2605 / 3655. 6144 rows of three sequences: 655 to 710 / 5083.
 constexpr uint32_t kCacheFewPairs = 64, kCacheFewRows = 8;
 
 // tokens that a sequence can have: what the host bounds and its table holds

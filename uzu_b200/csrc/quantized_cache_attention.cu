@@ -9,9 +9,10 @@
 // scale, and rescaled where it changes; scales of keys multiply scores.
 // Queries are brought to 2^14 .. 2^15 by a power of two for each row, which is exact; f32 ones are two f16 parts. A weight, up to 2^15, is two f16 parts: with one, every
 // eighth bf16 result or so would be the neighbour of the right one.
-// What bounds it: instructions and their latency, not memory: schedulers issue in 40 % of the cycles at 11 warps an SM, DRAM is busy for 43 % of the time, the tensor pipe for 15 %. One row
-// behind 131071 tokens of 8 heads of 128 (i8): 75 us, 3.6 TB/s. On the way there: 134 us first, 122 with wide loads of the queries, 82 with pairs as columns of a product, 75 with 32 keys a
-// step. 64 sequences of 4096 tokens on average 170 us, the weights' sums from kept scores 34. Before that last step four CTAs an SM took 100 us, five with a ring of two 106, three 113. A grid of 448 CTAs where 444 fit at once doubled the time, so splits fill one wave.
+// What bounds it: instructions and their latency, not memory: schedulers issue in 40 % of the cycles at 11 warps an SM, DRAM is busy for 43 % of the time, the tensor pipe for 15 % (capped drafted rows: 39 %, 10 warps,
+// 13 % and 13 %). One row behind 131071 tokens of 8 heads of 128 (i8): 75 to 77 us, 3.6 TB/s. On the way there: 134 us first, 122 with wide loads of the queries, 82 with pairs as columns of a product, 75 with 32 keys a
+// step. 64 sequences of 4096 tokens on average 170 us, the weights' sums from kept scores 34. With 16 keys a step four CTAs an SM took 100 us, five with a ring of two 106, three 113; the rings of 32 keys of heads of 128
+// leave room for three, and of heads of 64 four are slower too (16 x 5 rows 65 against 55 us, registers of four spill). A grid of 448 CTAs where 444 fit at once doubled the time, so splits fill one wave.
 #include "quantized_cache.cuh"
 
 namespace uzu {
@@ -800,7 +801,7 @@ QaWays qa_ways(uint32_t sm_count, const uzu_quantized_cache_attention_args& a, u
     QaWays w{};
     const uzu_cache_sequences& s = a.sequences;
     const uint32_t capacity = cache_capacity(s, a.cache.block_tokens);
-    // tiles as wide as registers allow: a tile reads its keys once
+    // tiles as wide as registers allow: a tile reads its keys once. (24 pairs: 55 us where 32 for the same 20 or 24 take 72, 16 sequences of 6000 tokens)
     w.eights = pairs <= 8 ? 1 : a.cache.head_dim <= 64 && pairs > 16 ? (pairs <= 24 ? 3 : 4) : 2;
     w.tiles = (uint32_t)((pairs + w.eights * 8 - 1) / (w.eights * 8));
     w.ctas = (uint64_t)s.count * a.cache.kv_heads * w.tiles;
