@@ -1,4 +1,4 @@
-"""The 8-bit cache's attention at the ends of its range: values that are no numbers beside weights that are summed, queries and caps of any size, one scratch for calls of many sizes."""
+"""The 8-bit cache's attention at the ends of its range: values that are no numbers beside weights that are summed, queries and caps of any size, one scratch for calls of many sizes, sequences longer than was said."""
 import ctypes as C
 
 import numpy as np
@@ -105,3 +105,40 @@ def test_caps_of_any_size(ctx, dt, cap, rows, heads):
         at += n
     after = s.device_weights()
     assert (np.abs(after - want_weights) <= slack + 2.0 ** -24 * (1 + max(rows) * heads / 16) * np.abs(want_weights) + 1e-30).all()
+
+
+def _held(s, rows, heads, dt, max_length, window, first):
+    """attention with weights against the definition"""
+    query = s.rng.standard_normal((sum(rows) + 2, heads * 64))
+    before = s.device_weights()
+    got, _ = s.attend(rows, heads, dt, query=query, max_length=max_length, window=window, first=first, weight_rows=ALL, check=False)
+    want, slack, at = before.copy(), np.zeros_like(before), 0
+    for i, n in enumerate(rows):
+        mine = P.of_kept(P.to_kept(query[at:at + n], dt), dt).reshape(n, heads, 64)
+        given = (s.table[i], s.lengths[i], mine, s.capacity(max_length), float(np.float32(0.125)), window, first, 0.0, None, ALL, 2.0 ** -22 if dt == P.F32 else 0.0)
+        ref, bound, grow, grow_bound = s.plain.attend(*given)
+        if dt == P.BF16 and n > 8 and n * heads // 2 > 64:
+            # Weights are one f16 number there. F16 numbers are 2^-10 apart from 1 to 2: a rounding is off by up to 2^-11 of the value, which is twice what the form's bound takes for it
+            bound = bound + 2 * (s.plain.attend(*given, tensor=True)[1] - bound)
+        mine_got = got[at:at + n].reshape(ref.shape)
+        tol = P.HALF_STEP[dt] * (np.abs(ref) + bound) + P.TINY[dt] + bound
+        assert (np.abs(mine_got - ref) <= tol).all(), (i, float((np.abs(mine_got - ref) / tol).max()))
+        tokens = np.arange(len(grow))
+        b = s.table[i][tokens // s.plain.block]
+        want[b, :, tokens % s.plain.block] += grow
+        slack[b, :, tokens % s.plain.block] += grow_bound
+        at += n
+    # (an addition for each tile of 16 pairs)
+    assert (np.abs(s.device_weights() - want) <= slack + 2.0 ** -24 * (1 + max(rows) * heads / 16) * np.abs(want) + 1e-30).all()
+    s.plain.weights = s.device_weights()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("rows", [[1, 1, 1], [3, 20, 9], [70, 40, 50]])
+@pytest.mark.parametrize("window,first", [(0, 0), (7, 0), (40, 5), (100, 20)])
+def test_sequences_behind_max_length(ctx, dt, rows, window, first):
+    """keys behind max_length are left out, and rows stay the tokens that they are: windows that begin behind it are empty"""
+    s = Served(ctx, Q.I8, 16, 2, 64, [60, 20, 150], room=240)
+    s.append(rows, P.F32)
+    for max_length in (50, 64, 23):
+        _held(s, rows, 8, dt, max_length, window, first)

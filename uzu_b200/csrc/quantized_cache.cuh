@@ -12,6 +12,8 @@ namespace uzu {
 constexpr uint32_t kCacheHugeBits = 0x6f800000u;      // 2^96
 constexpr int kCacheLeastExponent = -100;
 constexpr uint32_t kNoIndex = 0xffffffffu;
+// Attention's rows are the tokens that they are, of a sequence that has grown behind max_length as well (its keys there are left out, windows and kept first tokens stay); row numbers added, 32 bits hold them.
+constexpr uint32_t kCacheAnyLength = 0x7fffffffu;
 // A row of queries is brought to 2^14 .. 2^15 by a power of two, from 2^-113 for the largest numbers on up to this: 2^-126, its inverse, is still a normal number. Rows below 2^-112 stay below 2^14.
 constexpr int kCacheMostPower = 126;
 // Capped scores of 16-bit rows come of 1 - 2 / (1 + e^2x), which is off by 2^-22 of the cap whatever the score: up to this cap 2^-16, an eighth of what an f16 output's rounding moves. Above it tanhf, in the kernel for

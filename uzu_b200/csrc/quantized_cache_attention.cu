@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(QA_THREADS, QaShape<DP, NT>::CTAS) quantized_c
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t sequence = blockIdx.z, head = blockIdx.y, split = blockIdx.x % p.splits, tile = blockIdx.x / p.splits;
-    const CacheSequence q = cache_sequence(a.sequences, p.capacity, sequence);
+    const CacheSequence q = cache_sequence(a.sequences, kCacheAnyLength, sequence);
     const uint32_t pairs = q.rows * p.group, pair0 = tile * ROWS;
     if (pair0 >= pairs || (pairs > p.few && q.rows > kCacheFewRows)) return;
     const uint32_t dim = c.head_dim, bt = c.block_tokens;
@@ -674,7 +674,7 @@ __global__ void __launch_bounds__(QA_SUM) quantized_cache_sum_kernel(const __gri
     const uzu_quantized_cache_attention_args& a = p.a;
     const uzu_quantized_cache& c = a.cache;
     const uint32_t sequence = blockIdx.z, head = blockIdx.y;
-    const CacheSequence q = cache_sequence(a.sequences, p.capacity, sequence);
+    const CacheSequence q = cache_sequence(a.sequences, kCacheAnyLength, sequence);
     const uint32_t pairs = q.rows * p.group, first = (q.rows - min(q.rows, a.weight_rows)) * p.group;
     if (pairs > p.score_pairs || !pairs) return;
     const QaSteps steps(q.length, q.length + q.rows - 1u, a.window, a.keep_first, p.capacity);      // (what some row sees)
@@ -718,7 +718,7 @@ __global__ void __launch_bounds__(QA_THREADS) quantized_cache_weights_kernel(con
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t sequence = blockIdx.z, head = blockIdx.y;
-    const CacheSequence q = cache_sequence(a.sequences, p.capacity, sequence);
+    const CacheSequence q = cache_sequence(a.sequences, kCacheAnyLength, sequence);
     const uint32_t pairs = q.rows * p.group, dim = c.head_dim, bt = c.block_tokens;
     if (p.scores && pairs <= p.score_pairs) return;      // (the kernel above's)
     const uint32_t* table = reinterpret_cast<const uint32_t*>(a.sequences.tables) + (size_t)sequence * a.sequences.table_stride;

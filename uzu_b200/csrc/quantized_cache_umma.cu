@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(QU_THREADS, 1) quantized_cache_umma_kernel(con
     pdl_wait();
 
     const uint32_t sequence = blockIdx.z, head = blockIdx.y, G = p.group, dim = c.head_dim, bt = c.block_tokens;
-    const CacheSequence q = cache_sequence(a.sequences, p.capacity, sequence);
+    const CacheSequence q = cache_sequence(a.sequences, kCacheAnyLength, sequence);
     const uint32_t pairs = q.rows * G, tiles = (pairs + 2 * QU_ROWS - 1) / (2 * QU_ROWS);
     const bool mine = pairs > kCacheFewPairs && q.rows > kCacheFewRows && blockIdx.x < tiles;
     const uint32_t pair0 = mine ? (tiles - 1u - blockIdx.x) * 2 * QU_ROWS : 0u;      // the rows with the most keys first
